@@ -541,6 +541,60 @@ enum { TDGS_IMAGE_RGB = 0, TDGS_IMAGE_TRANSMITTANCE = 1, TDGS_IMAGE_DEPTH = 2 };
 int tdgs_image_to_rgb8(void* stream, int32_t kind, const float* src, int32_t width, int32_t height,
                        float min_depth, float max_depth, uint8_t* dst);
 
+/* ---- operators of a learned decoder of rendered images ---------------------------------
+ * No counterpart in the reference: what a network that turns rendered features into images (an
+ * appearance model of a photo collection, a refiner, a codebook of Gaussian attributes) needs
+ * besides matrix products. Element types are TDGS_F32, TDGS_BF16 and TDGS_F16; sums, softmax and
+ * norm statistics are held in 32 bits. Results do not depend on the order in which workgroups run.
+ * Scratch needs no initialisation and holds nothing between calls, except that a gradient call
+ * may be given the forward call's. Calls allocate nothing and do not synchronise. */
+enum { TDGS_F32 = 0, TDGS_BF16 = 1, TDGS_F16 = 2 };
+enum { TDGS_ACT_IDENTITY = 0, TDGS_ACT_SILU = 1, TDGS_ACT_GELU = 2, TDGS_ACT_RELU = 3 };
+
+/* A (batch, length, heads, head_dim) tensor: strides in elements, the last dimension contiguous. */
+typedef struct tdgs_heads {
+    void* data;
+    int64_t stride_b;
+    int64_t stride_l;
+    int64_t stride_h;
+} tdgs_heads;
+
+/* Cross attention: query (b, i, h) attends the kv_len keys of kv head h / (heads / kv_heads) of batch
+ * b, or of the only batch where kv_batch is 1 (one encoder's states for every query batch).
+ * Key j is allowed where j < kv_lengths[kb] (null: kv_len) and kv_mask[kb * kv_mask_stride + j] != 0
+ * (null: all); kb is the key's batch. Keys that are not allowed contribute nothing, whatever k and v
+ * hold there. s_ij = scale q_i . k_j, p_ij = exp(s_ij - lse_i) over the allowed keys,
+ * out_i = sum_j p_ij v_j, lse_i = log sum_j exp(s_ij). Without any allowed key out is 0 and lse -inf. */
+typedef struct tdgs_attention {
+    int32_t dtype;              /* of q, k, v, out and their gradients */
+    int32_t batch, kv_batch;    /* kv_batch is batch or 1 */
+    int32_t q_len, kv_len;
+    int32_t heads, kv_heads;    /* heads a multiple of kv_heads */
+    int32_t head_dim;           /* 1 to 128 */
+    float scale;                /* positive */
+    int32_t reserved;
+    tdgs_heads q, k, v, out;
+    const int32_t* kv_lengths;  /* kv_batch entries, clamped to [0, kv_len]; may be null */
+    const uint8_t* kv_mask;     /* kv_batch rows of kv_len bytes; may be null */
+    int64_t kv_mask_stride;     /* bytes between its rows */
+    float* lse;                 /* batch x heads x q_len; may be null in the forward call */
+    void* temp;                 /* scratch of tdgs_cross_attention_temp_bytes() bytes */
+    size_t temp_bytes;
+} tdgs_attention;
+
+/* The gradients' tensors: dout as q's shape; dq, dk, dv as q's, k's and v's (dk and dv summed over the
+ * query heads and, where kv_batch is 1, over the batches that share a key). */
+typedef struct tdgs_attention_grads {
+    tdgs_heads dout, dq, dk, dv;
+} tdgs_attention_grads;
+
+/* Scratch of tdgs_cross_attention (grad 0) or of that and tdgs_cross_attention_grad (grad 1). */
+size_t tdgs_cross_attention_temp_bytes(const tdgs_attention* a, int32_t grad);
+int tdgs_cross_attention(void* stream, const tdgs_attention* a);
+/* The gradients of sum(dout * out), from the forward call's out and lse. A query without allowed
+ * keys has zero gradient and gives none; so does a key that is not allowed. */
+int tdgs_cross_attention_grad(void* stream, const tdgs_attention* a, const tdgs_attention_grads* g);
+
 #ifdef __cplusplus
 }
 #endif

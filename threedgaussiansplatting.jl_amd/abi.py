@@ -26,6 +26,14 @@ TDGS_IMAGE_RGB = 0
 TDGS_IMAGE_TRANSMITTANCE = 1
 TDGS_IMAGE_DEPTH = 2
 
+TDGS_F32 = 0
+TDGS_BF16 = 1
+TDGS_F16 = 2
+TDGS_ACT_IDENTITY = 0
+TDGS_ACT_SILU = 1
+TDGS_ACT_GELU = 2
+TDGS_ACT_RELU = 3
+
 fp = C.POINTER(C.c_float)
 i32p = C.POINTER(C.c_int32)
 i64p = C.POINTER(C.c_int64)
@@ -93,6 +101,22 @@ class AdcBuffersC(C.Structure):
                 ("prune", C.c_void_p), ("densify", C.c_void_p), ("clone", C.c_void_p),
                 ("new_counts_cs", C.c_void_p), ("ngidx_to_gidx", C.c_void_p),
                 ("temp", C.c_void_p), ("temp_bytes", C.c_size_t)]
+
+
+class HeadsC(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_l", C.c_int64), ("stride_h", C.c_int64)]
+
+
+class AttentionC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("batch", C.c_int32), ("kv_batch", C.c_int32), ("q_len", C.c_int32),
+                ("kv_len", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("scale", C.c_float), ("reserved", C.c_int32), ("q", HeadsC), ("k", HeadsC), ("v", HeadsC),
+                ("out", HeadsC), ("kv_lengths", C.c_void_p), ("kv_mask", C.c_void_p), ("kv_mask_stride", C.c_int64),
+                ("lse", C.c_void_p), ("temp", C.c_void_p), ("temp_bytes", C.c_size_t)]
+
+
+class AttentionGradsC(C.Structure):
+    _fields_ = [("dout", HeadsC), ("dq", HeadsC), ("dk", HeadsC), ("dv", HeadsC)]
 
 
 def sh_coeffs_per_channel(degree: int) -> int:

@@ -1,0 +1,829 @@
+// attention.hip — cross attention of a decoder's queries to an encoder's states, forward and
+// backward, on the matrix cores.
+//
+// The query heads that share a kv head, and the query batches that share an encoder's states, are
+// stacked into the rows of one problem per kv head and kv batch: row r is query
+// (r / (q_len G)) of the sharing batches, r / G % q_len of its queries and r % G of the G heads. A tile
+// of keys is so staged once for all of them, and a single query token of G heads fills G rows.
+//
+// Products are 32x32 blocks (elem.hpp). Scores are taken as S^T = K Q^T in the forward pass and for
+// dQ: a lane then holds 16 keys of one row, the softmax's maximum and sum are in-lane but for one
+// swap of the halves, and P^T is in place as the next product's B operand (O^T = V^T P^T,
+// dQ^T = K^T dS^T), V^T and K^T coming from LDS by the transposing reads. For dK and dV the block is
+// S = Q K^T, a lane holding 16 rows of one key, and dV^T = dO^T P, dK^T = Q^T dS follow likewise.
+// P and dS are rounded to the inputs' type for their products (the matrix cores take no wider
+// operand at that rate); maxima, sums, exponentials and every accumulator stay in 32 bits.
+#include "internal.hpp"
+#include "elem.hpp"
+
+namespace tdgs {
+
+constexpr int kAtThreads = 256;
+constexpr int kAtWaves = kAtThreads / kWave;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct AtHeads {
+    int64_t b, l, h;   // strides in elements
+};
+
+struct AtArgs {
+    const void *q, *k, *v, *dout, *o;
+    void *out, *dq, *dk, *dv;
+    AtHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
+    const int32_t* lengths;
+    const uint8_t* mask;
+    int64_t mask_stride;
+    float* lse;       // batch x heads x q_len, natural logarithm
+    float* delta;     // the same shape: dout . out
+    float *part, *part_ml;
+    int32_t q_len, kv_len, heads, kv_heads, d;
+    int32_t rows;     // per kv head and kv batch
+    int32_t group_batches, splits, blocks;
+    float c, scale;   // scale log2(e), scale
+    FastDiv by_g, by_lg;
+    bool vec, vec_out;
+};
+
+struct AtRow {
+    int32_t b, i, h;   // batch, query, head
+};
+
+__device__ __forceinline__ AtRow at_row(const AtArgs& a, int kb, int hk, int r) {
+    const uint32_t bb = a.by_lg.div(r), rest = r - bb * a.by_lg.d, i = a.by_g.div(rest);
+    return {kb * a.group_batches + (int32_t)bb, (int32_t)i, hk * (int32_t)a.by_g.d + (int32_t)(rest - i * a.by_g.d)};
+}
+__device__ __forceinline__ int64_t at_offset(const AtHeads& s, const AtRow& r) {
+    return r.b * s.b + r.i * s.l + r.h * s.h;
+}
+__device__ __forceinline__ int64_t at_stat(const AtArgs& a, const AtRow& r) {
+    return ((int64_t)r.b * a.heads + r.h) * a.q_len + r.i;
+}
+
+// Bit j: key t0 + j is allowed (the KT keys from t0 on). The same in every wavefront.
+__device__ __forceinline__ uint64_t at_allowed(const AtArgs& a, int kb, int len, int t0, int kt) {
+    const int j = t0 + (int)__lane_id();
+    bool ok = (int)__lane_id() < kt && j < len;
+    if (a.mask && ok) ok = a.mask[kb * a.mask_stride + j] != 0;
+    return __ballot(ok);
+}
+__device__ __forceinline__ int at_length(const AtArgs& a, int kb) {
+    if (!a.lengths) return a.kv_len;
+    const int n = a.lengths[kb];
+    return n < 0 ? 0 : (n < a.kv_len ? n : a.kv_len);
+}
+
+// Keys per tile of the forward and dQ kernels, and rows per tile of the dK, dV kernel. LDS rows are
+// padded by 16 bytes: for every DP, a b128 read of one depth chunk of 16 rows then covers the 64
+// banks exactly once.
+template <class T>
+constexpr int at_tile() { return sizeof(T) == 4 ? 32 : 64; }
+template <class T, int DP>
+constexpr int at_pitch() { return DP + 16 / (int)sizeof(T); }
+
+// One tile of N rows x DP elements in registers on its way to LDS.
+template <class T, int DP, int N>
+struct AtTile {
+    static constexpr int kChunks = N * (DP / 8);
+    static constexpr int kPer = (kChunks + kAtThreads - 1) / kAtThreads;
+    typename Elem<T>::V8 r[kPer];
+    // row(j) gives row j's pointer, or null for a row of zeros
+    template <class Row>
+    __device__ __forceinline__ void load(int d, bool vec, Row&& row) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int c = (int)threadIdx.x + k * kAtThreads, j = c / (DP / 8), e = (c % (DP / 8)) * 8;
+            const T* p = (kChunks % kAtThreads == 0 || c < kChunks) ? row(j) : nullptr;
+            r[k] = p ? load8<T>(p + e, d - e, vec) : zero8<T>();
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int c = (int)threadIdx.x + k * kAtThreads, j = c / (DP / 8), e = (c % (DP / 8)) * 8;
+            if (kChunks % kAtThreads == 0 || c < kChunks)
+                *reinterpret_cast<typename Elem<T>::V8a*>(lds + j * at_pitch<T, DP>() + e) = r[k];
+        }
+    }
+};
+
+// A operand: rows base.. of the tile, depth chunk c (slot (l / 32) * 8 + i is element 16 c + that).
+template <class T, int DP>
+__device__ __forceinline__ typename Elem<T>::V8 at_rows(const T* lds, int base, int c) {
+    const int l = (int)__lane_id();
+    return *reinterpret_cast<const typename Elem<T>::V8a*>(lds + (base + (l & 31)) * at_pitch<T, DP>() + c * 16 +
+                                                           (l >> 5) * 8);
+}
+// A operand of the transposed tile: its rows are the tile's columns db * 32.., its depth the 16 tile
+// rows from base on, in the order the registers of a block of results hold them: slot (h, i) is row
+// base + (i / 4) * 8 + h * 4 + i % 4. For 16-bit types two transposing reads: 16 lanes give the
+// addresses of 4 rows x 16 columns and each gets one column.
+template <class T, int DP>
+__device__ __forceinline__ typename Elem<T>::V8 at_cols(const T* lds, int base, int db) {
+    const int l = (int)__lane_id();
+    typename Elem<T>::V8 r;
+    if constexpr (sizeof(T) == 4) {
+        const T* p = lds + (base + (l >> 5) * 4) * at_pitch<T, DP>() + db * 32 + (l & 31);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = p[((i >> 2) * 8 + (i & 3)) * at_pitch<T, DP>()];
+    } else {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        const T* p = lds + (base + (l >> 5) * 4 + ((l & 15) >> 2)) * at_pitch<T, DP>() + db * 32 + ((l >> 4) & 1) * 16 +
+                     (l & 3) * 4;
+        typedef __attribute__((address_space(3))) s4* lp;
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 8 * at_pitch<T, DP>()));
+        r = __builtin_bit_cast(typename Elem<T>::V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return r;
+}
+
+// Eight registers of a block of results as an operand, rounded to T.
+template <class T>
+__device__ __forceinline__ typename Elem<T>::V8 at_pack(const f32x16& s, int half) {
+    typename Elem<T>::V8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)s[half * 8 + i];
+    return r;
+}
+
+// Row r's elements in the order of a B operand's lanes (row l % 32 of the block): chunk c of DP / 16.
+template <class T, int DP>
+__device__ __forceinline__ void at_load_row(typename Elem<T>::V8 (&f)[DP / 16], const T* p, int d, bool vec) {
+    const int h = (int)__lane_id() >> 5;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        const int e = c * 16 + h * 8;
+        f[c] = p ? load8<T>(p + e, d - e, vec) : zero8<T>();
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void at_store4(T* p, f32x4 x, int n, bool vec) {
+    if (vec && n >= 4) {
+        typedef T V4a __attribute__((ext_vector_type(4), aligned(8)));
+        V4a r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (T)x[i];
+        *reinterpret_cast<V4a*>(p) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) p[i] = (T)x[i];
+    }
+}
+
+// A block column of results (d x 32 lanes' rows, DP / 32 blocks) times f to a row of T.
+template <class T, int DP>
+__device__ __forceinline__ void at_store_row(T* p, const f32x16 (&o)[DP / 32], float f, int d, bool vec) {
+    const int h = (int)__lane_id() >> 5;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int e = db * 32 + k * 8 + h * 4;
+            f32x4 x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = o[db][k * 4 + i] * f;
+            at_store4<T>(p + e, x, d - e, vec);
+        }
+}
+
+// ---- forward -------------------------------------------------------------------------------
+
+// Workgroup: 4 wavefronts of QB * 32 rows each of one kv head, the keys of one split. Online softmax in
+// base 2: m is the running maximum of c s, O and l are relative to it.
+template <class T, int DP, int QB>
+__global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
+    constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
+    __shared__ __attribute__((aligned(16))) T s_k[KT * P];
+    __shared__ __attribute__((aligned(16))) T s_v[KT * P];
+    const int item = xcd_band_item(blockIdx.x, gridDim.x);
+    const int blk = item % a.blocks, sp = item / a.blocks % a.splits, kvh = item / a.blocks / a.splits;
+    const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
+    const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
+    const int row0 = (blk * kAtWaves + wave) * (QB * 32) + (lane & 31);
+
+    typename Elem<T>::V8 qf[QB][NC];
+    f32x16 o[QB][NB];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int r = row0 + qb * 32;
+        const T* p = nullptr;
+        if (r < a.rows) p = (const T*)a.q + at_offset(a.sq, at_row(a, kb, hk, r));
+        at_load_row<T, DP>(qf[qb], p, a.d, a.vec);
+        m[qb] = -INFINITY;
+        l[qb] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[qb][db][i] = 0.0f;
+    }
+    const int len = at_length(a, kb);
+    const int tiles = (len + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
+    const int t_end = min(tiles, (sp + 1) * per);
+    const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
+    const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
+    AtTile<T, DP, KT> tk, tv;
+    uint64_t next = 0;
+    auto fetch = [&](int t) {
+        next = at_allowed(a, kb, len, t * KT, KT);
+        tk.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? kbase + (int64_t)(t * KT + j) * a.sk.l : nullptr; });
+        tv.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? vbase + (int64_t)(t * KT + j) * a.sv.l : nullptr; });
+    };
+    if (sp * per < t_end) fetch(sp * per);
+    for (int t = sp * per; t < t_end; ++t) {
+        const uint64_t allowed = next;
+        __syncthreads();
+        tk.store(s_k);
+        tv.store(s_v);
+        __syncthreads();
+        if (t + 1 < t_end) fetch(t + 1);
+        if (allowed == 0) continue;
+        f32x16 s[QB][KT / 32];
+#pragma unroll
+        for (int kk = 0; kk < KT / 32; ++kk) {
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[qb][kk][i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const auto f = at_rows<T, DP>(s_k, kk * 32, c);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) s[qb][kk] = mma(f, qf[qb][c], s[qb][kk]);
+            }
+        }
+        if (allowed != (KT == 64 ? ~0ull : 0xffffffffull)) {
+            const uint64_t mine = allowed >> (h * 4);
+#pragma unroll
+            for (int kk = 0; kk < KT / 32; ++kk)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const bool ok = (mine >> (kk * 32 + (i >> 2) * 8 + (i & 3))) & 1;
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb) s[qb][kk][i] = ok ? s[qb][kk][i] : -INFINITY;
+                }
+        }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+            float top = s[qb][0][0];
+#pragma unroll
+            for (int kk = 0; kk < KT / 32; ++kk)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[qb][kk][i]);
+            top = fmaxf(m[qb], max_halves(top) * a.c);
+            const float base = top == -INFINITY ? 0.0f : top;
+            if (wave_any(top > m[qb])) {
+                const float f = __builtin_amdgcn_exp2f(m[qb] - base);
+                l[qb] *= f;
+#pragma unroll
+                for (int db = 0; db < NB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[qb][db][i] *= f;
+                m[qb] = top;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < KT / 32; ++kk)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[qb][kk][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kk][i], a.c, -base));
+                    sum += s[qb][kk][i];
+                }
+            l[qb] += sum;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KT / 16; ++ks) {
+            typename Elem<T>::V8 p[QB];
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) p[qb] = at_pack<T>(s[qb][ks / 2], ks % 2);
+#pragma unroll
+            for (int db = 0; db < NB; ++db) {
+                const auto f = at_cols<T, DP>(s_v, ks * 16, db);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) o[qb][db] = mma(f, p[qb], o[qb][db]);
+            }
+        }
+    }
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+        const int r = row0 + qb * 32;
+        const float sum = sum_halves(l[qb]);
+        if (r >= a.rows) continue;
+        if (a.splits == 1) {
+            const AtRow row = at_row(a, kb, hk, r);
+            at_store_row<T, DP>((T*)a.out + at_offset(a.so, row), o[qb], sum > 0.0f ? 1.0f / sum : 0.0f, a.d, a.vec_out);
+            if (a.lse && h == 0) a.lse[at_stat(a, row)] = (m[qb] + __builtin_amdgcn_logf(sum)) * kLn2;
+        } else {
+            const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
+            at_store_row<float, DP>(a.part + pr * DP, o[qb], 1.0f, DP, true);
+            if (h == 0) {
+                a.part_ml[2 * pr] = m[qb];
+                a.part_ml[2 * pr + 1] = sum;
+            }
+        }
+    }
+}
+
+// Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. One wavefront per row.
+template <class T>
+__global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, int64_t all_rows) {
+    const int64_t pr0 = (int64_t)blockIdx.x * kAtWaves + threadIdx.x / kWave;
+    if (pr0 >= all_rows) return;
+    const int lane = (int)__lane_id();
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * all_rows + pr0)]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
+    for (int s = 0; s < a.splits; ++s) {
+        const int64_t pr = s * all_rows + pr0;
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - base);
+        sum = __builtin_fmaf(f, a.part_ml[2 * pr + 1], sum);
+        if (lane < a.d) x0 = __builtin_fmaf(f, a.part[pr * dp + lane], x0);
+        if (lane + 64 < a.d) x1 = __builtin_fmaf(f, a.part[pr * dp + lane + 64], x1);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const int kvh = (int)(pr0 / a.rows);
+    const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr0 % a.rows));
+    T* const out = (T*)a.out + at_offset(a.so, row);
+    if (lane < a.d) out[lane] = (T)(x0 * inv);
+    if (lane + 64 < a.d) out[lane + 64] = (T)(x1 * inv);
+    if (a.lse && lane == 0) a.lse[at_stat(a, row)] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// ---- backward ------------------------------------------------------------------------------
+
+// The base-2 logarithm of a row's sum, from lse; +inf (all its p are 0) for a row without allowed keys.
+__device__ __forceinline__ float at_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+
+// dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split.
+template <class T, int DP>
+__global__ __launch_bounds__(kAtThreads) void k_attend_dq(AtArgs a) {
+    constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
+    __shared__ __attribute__((aligned(16))) T s_k[KT * P];
+    __shared__ __attribute__((aligned(16))) T s_v[KT * P];
+    const int item = xcd_band_item(blockIdx.x, gridDim.x);
+    const int blk = item % a.blocks, sp = item / a.blocks % a.splits, kvh = item / a.blocks / a.splits;
+    const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
+    const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
+    const int r = (blk * kAtWaves + wave) * 32 + (lane & 31);
+    AtRow row = {0, 0, 0};
+    if (r < a.rows) row = at_row(a, kb, hk, r);
+
+    typename Elem<T>::V8 qf[NC], df[NC];
+    at_load_row<T, DP>(qf, r < a.rows ? (const T*)a.q + at_offset(a.sq, row) : nullptr, a.d, a.vec);
+    at_load_row<T, DP>(df, r < a.rows ? (const T*)a.dout + at_offset(a.sdo, row) : nullptr, a.d, a.vec);
+    float lse2 = INFINITY, delta = 0.0f;
+    {
+        typename Elem<T>::V8 of[NC];
+        at_load_row<T, DP>(of, r < a.rows ? (const T*)a.o + at_offset(a.so, row) : nullptr, a.d, a.vec);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)df[c][i], (float)of[c][i], delta);
+        delta = sum_halves(delta);
+        if (r < a.rows) {
+            lse2 = at_lse2(a.lse[at_stat(a, row)]);
+            if (sp == 0 && h == 0) a.delta[at_stat(a, row)] = delta;
+        }
+    }
+    f32x16 o[NB];
+#pragma unroll
+    for (int db = 0; db < NB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
+    const int len = at_length(a, kb);
+    const int tiles = (len + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
+    const int t_end = min(tiles, (sp + 1) * per);
+    const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
+    const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
+    AtTile<T, DP, KT> tk, tv;
+    uint64_t next = 0;
+    auto fetch = [&](int t) {
+        next = at_allowed(a, kb, len, t * KT, KT);
+        tk.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? kbase + (int64_t)(t * KT + j) * a.sk.l : nullptr; });
+        tv.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? vbase + (int64_t)(t * KT + j) * a.sv.l : nullptr; });
+    };
+    if (sp * per < t_end) fetch(sp * per);
+    for (int t = sp * per; t < t_end; ++t) {
+        const uint64_t allowed = next;
+        __syncthreads();
+        tk.store(s_k);
+        tv.store(s_v);
+        __syncthreads();
+        if (t + 1 < t_end) fetch(t + 1);
+        if (allowed == 0) continue;
+        const uint64_t mine = allowed >> (h * 4);
+#pragma unroll
+        for (int kk = 0; kk < KT / 32; ++kk) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                s = mma(at_rows<T, DP>(s_k, kk * 32, c), qf[c], s);
+                dp = mma(at_rows<T, DP>(s_v, kk * 32, c), df[c], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool ok = (mine >> (kk * 32 + (i >> 2) * 8 + (i & 3))) & 1;
+                const float p = ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse2)) : 0.0f;
+                s[i] = p * (dp[i] - delta);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const auto b = at_pack<T>(s, ks);
+#pragma unroll
+                for (int db = 0; db < NB; ++db) o[db] = mma(at_cols<T, DP>(s_k, kk * 32 + ks * 16, db), b, o[db]);
+            }
+        }
+    }
+    if (r >= a.rows) return;
+    if (a.splits == 1) {
+        at_store_row<T, DP>((T*)a.dq + at_offset(a.sdq, row), o, a.scale, a.d, a.vec_out);
+    } else {
+        const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
+        at_store_row<float, DP>(a.part + pr * DP, o, 1.0f, DP, true);
+    }
+}
+
+// dK and dV. Workgroup: 4 wavefronts of 32 keys each, the rows of one split.
+template <class T, int DP>
+__global__ __launch_bounds__(kAtThreads) void k_attend_dkv(AtArgs a) {
+    constexpr int RT = 32, P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
+    __shared__ __attribute__((aligned(16))) T s_q[RT * P];
+    __shared__ __attribute__((aligned(16))) T s_d[RT * P];
+    __shared__ __attribute__((aligned(16))) float s_lse[RT];
+    __shared__ __attribute__((aligned(16))) float s_delta[RT];
+    const int item = xcd_band_item(blockIdx.x, gridDim.x);
+    const int sp = item % a.splits, blk = item / a.splits % a.blocks, kvh = item / a.splits / a.blocks;
+    const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
+    const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
+    const int j = (blk * kAtWaves + wave) * 32 + (lane & 31);
+    const int len = at_length(a, kb);
+    bool ok = j < len;
+    if (a.mask && ok) ok = a.mask[kb * a.mask_stride + j] != 0;
+
+    typename Elem<T>::V8 kf[NC], vf[NC];
+    at_load_row<T, DP>(kf, ok ? (const T*)a.k + kb * a.sk.b + hk * a.sk.h + j * a.sk.l : nullptr, a.d, a.vec);
+    at_load_row<T, DP>(vf, ok ? (const T*)a.v + kb * a.sv.b + hk * a.sv.h + j * a.sv.l : nullptr, a.d, a.vec);
+    f32x16 gk[NB], gv[NB];
+#pragma unroll
+    for (int db = 0; db < NB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) gk[db][i] = gv[db][i] = 0.0f;
+    const int tiles = (a.rows + RT - 1) / RT, per = (tiles + a.splits - 1) / a.splits;
+    const int t_end = blk * kAtWaves * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
+    AtTile<T, DP, RT> tq, td;
+    float st = 0.0f;
+    auto fetch = [&](int t) {
+        tq.load(a.d, a.vec, [&](int i) {
+            const int r = t * RT + i;
+            return r < a.rows ? (const T*)a.q + at_offset(a.sq, at_row(a, kb, hk, r)) : nullptr;
+        });
+        td.load(a.d, a.vec, [&](int i) {
+            const int r = t * RT + i;
+            return r < a.rows ? (const T*)a.dout + at_offset(a.sdo, at_row(a, kb, hk, r)) : nullptr;
+        });
+        if (threadIdx.x < 2 * RT) {   // lse of the tile's rows, then delta
+            const int r = t * RT + (threadIdx.x & (RT - 1));
+            st = threadIdx.x < RT ? INFINITY : 0.0f;
+            if (r < a.rows) {
+                const int64_t at = at_stat(a, at_row(a, kb, hk, r));
+                st = threadIdx.x < RT ? at_lse2(a.lse[at]) : a.delta[at];
+            }
+        }
+    };
+    if (sp * per < t_end) fetch(sp * per);
+    for (int t = sp * per; t < t_end; ++t) {
+        __syncthreads();
+        tq.store(s_q);
+        td.store(s_d);
+        if (threadIdx.x < RT) s_lse[threadIdx.x] = st;
+        else if (threadIdx.x < 2 * RT) s_delta[threadIdx.x - RT] = st;
+        __syncthreads();
+        if (t + 1 < t_end) fetch(t + 1);
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            s = mma(at_rows<T, DP>(s_q, 0, c), kf[c], s);
+            dp = mma(at_rows<T, DP>(s_d, 0, c), vf[c], dp);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const f32x4 ls = *reinterpret_cast<const f32x4*>(s_lse + k * 8 + h * 4);
+            const f32x4 de = *reinterpret_cast<const f32x4*>(s_delta + k * 8 + h * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[k * 4 + i], a.c, -ls[i])) : 0.0f;
+                s[k * 4 + i] = p;
+                dp[k * 4 + i] = p * (dp[k * 4 + i] - de[i]);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const auto p = at_pack<T>(s, ks), ds = at_pack<T>(dp, ks);
+#pragma unroll
+            for (int db = 0; db < NB; ++db) {
+                gv[db] = mma(at_cols<T, DP>(s_d, ks * 16, db), p, gv[db]);
+                gk[db] = mma(at_cols<T, DP>(s_q, ks * 16, db), ds, gk[db]);
+            }
+        }
+    }
+    if (j >= a.kv_len) return;
+    if (!ok) {   // (0 P would be NaN for a dout that is not finite)
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) gk[db][i] = gv[db][i] = 0.0f;
+    }
+    if (a.splits == 1) {
+        at_store_row<T, DP>((T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + j * a.sdk.l, gk, a.scale, a.d, a.vec_out);
+        at_store_row<T, DP>((T*)a.dv + kb * a.sdv.b + hk * a.sdv.h + j * a.sdv.l, gv, 1.0f, a.d, a.vec_out);
+    } else {
+        const int64_t all = (int64_t)(gridDim.x / (a.blocks * a.splits)) * a.kv_len;
+        const int64_t pr = (2 * sp * all) + (int64_t)kvh * a.kv_len + j;
+        at_store_row<float, DP>(a.part + pr * DP, gk, 1.0f, DP, true);
+        at_store_row<float, DP>(a.part + (pr + all) * DP, gv, 1.0f, DP, true);
+    }
+}
+
+// Sums the splits' partial gradients, in order: dQ's rows (what 0), or dK's and dV's (what 1). One thread
+// per four elements.
+template <class T>
+__global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int64_t all, int what) {
+    const int64_t id = (int64_t)blockIdx.x * kAtThreads + threadIdx.x;
+    const int quads = dp / 4;
+    const int64_t n = (what ? 2 : 1) * all;
+    const int64_t pr = id / quads;
+    const int e = (int)(id % quads) * 4;
+    if (pr >= n || e >= a.d) return;
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < a.splits; ++s) x += *reinterpret_cast<const f32x4*>(a.part + (s * n + pr) * dp + e);
+    if (what == 0) {
+        const int kvh = (int)(pr / a.rows);
+        const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr % a.rows));
+        at_store4<T>((T*)a.dq + at_offset(a.sdq, row) + e, x * a.scale, a.d - e, a.vec_out);
+    } else {
+        const bool is_v = pr >= all;
+        const int64_t rest = is_v ? pr - all : pr;
+        const int j = (int)(rest % a.kv_len), kvh = (int)(rest / a.kv_len);
+        const AtHeads& st = is_v ? a.sdv : a.sdk;
+        T* const p = (T*)(is_v ? a.dv : a.dk) + kvh / a.kv_heads * st.b + kvh % a.kv_heads * st.h + j * st.l;
+        at_store4<T>(p + e, is_v ? x : x * a.scale, a.d - e, a.vec_out);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+// Workgroups that a launch should have at least, two per CU, and the most parts its long axis is
+// split into to reach them.
+constexpr int64_t kAtWorkgroups = 512;
+constexpr int kAtSplits = 64;
+
+static int at_splits(int64_t workgroups, int64_t tiles) {
+    int64_t s = workgroups > 0 ? ceil_div(kAtWorkgroups, workgroups) : 1;
+    if (workgroups >= kAtWorkgroups / 2) s = 1;   // (a second pass over the partial results costs more)
+    if (s > kAtSplits) s = kAtSplits;
+    if (s > tiles) s = tiles;
+    return (int)(s > 1 ? s : 1);
+}
+
+static int at_padded(int d) { return (d + 31) / 32 * 32; }
+
+// How the three launches are cut, from the sizes alone.
+struct AtPlan {
+    int64_t kvh, rows;   // kv heads over all kv batches; rows of each
+    int dp, qb, tile;
+    int blocks_f, splits_f, blocks_q, splits_q, blocks_k, splits_k;
+    size_t delta_bytes, forward_bytes, grad_bytes;
+};
+
+static AtPlan at_plan(const tdgs_attention* a) {
+    AtPlan p;
+    p.kvh = (int64_t)a->kv_batch * a->kv_heads;
+    p.rows = (int64_t)(a->kv_batch > 0 ? a->batch / a->kv_batch : 0) * a->q_len * (a->heads / a->kv_heads);
+    p.dp = at_padded(a->head_dim);
+    p.tile = a->dtype == TDGS_F32 ? 32 : 64;
+    p.qb = a->dtype != TDGS_F32 && p.dp <= 64 ? 2 : 1;
+    const int64_t key_tiles = ceil_div(a->kv_len, p.tile), row_tiles = ceil_div(p.rows, 32);
+    p.blocks_f = (int)ceil_div(p.rows, kAtWaves * 32 * p.qb);
+    p.splits_f = at_splits(p.blocks_f * p.kvh, key_tiles);
+    p.blocks_q = (int)ceil_div(p.rows, kAtWaves * 32);
+    p.splits_q = at_splits(p.blocks_q * p.kvh, key_tiles);
+    p.blocks_k = (int)ceil_div(a->kv_len, kAtWaves * 32);
+    p.splits_k = at_splits(p.blocks_k * p.kvh, row_tiles);
+    const size_t all_rows = (size_t)(p.kvh * p.rows), all_keys = (size_t)(p.kvh * a->kv_len);
+    p.delta_bytes = align_up(all_rows * sizeof(float));
+    p.forward_bytes = p.splits_f > 1 ? p.splits_f * (align_up(all_rows * p.dp * sizeof(float)) + align_up(all_rows * 2 * sizeof(float))) : 0;
+    const size_t q = p.splits_q > 1 ? p.splits_q * all_rows * p.dp * sizeof(float) : 0;
+    const size_t k = p.splits_k > 1 ? p.splits_k * 2 * all_keys * p.dp * sizeof(float) : 0;
+    p.grad_bytes = p.delta_bytes + align_up(q > k ? q : k);
+    return p;
+}
+
+static int at_check_view(const tdgs_heads* v, const char* name, const tdgs_attention* a, bool keys, bool written) {
+    TDGS_REQUIRE(v->data != nullptr, "attention: %s is null", name);
+    const size_t e = (size_t)dtype_size(a->dtype);
+    TDGS_REQUIRE(aligned_to(v->data, e), "attention: %s is not aligned to its element type", name);
+    const int64_t nb = keys ? a->kv_batch : a->batch, nl = keys ? a->kv_len : a->q_len, nh = keys ? a->kv_heads : a->heads;
+    TDGS_REQUIRE(v->stride_b >= 0 && v->stride_l >= 0 && v->stride_h >= 0, "attention: %s has a negative stride", name);
+    if (written)
+        TDGS_REQUIRE((nb <= 1 || v->stride_b >= a->head_dim) && (nl <= 1 || v->stride_l >= a->head_dim) &&
+                         (nh <= 1 || v->stride_h >= a->head_dim),
+                     "attention: rows of %s overlap", name);
+    return TDGS_OK;
+}
+
+static int at_check(const tdgs_attention* a) {
+    TDGS_REQUIRE(a != nullptr, "attention: null arguments");
+    TDGS_REQUIRE(known_dtype(a->dtype), "attention: unknown element type %d", a->dtype);
+    TDGS_REQUIRE(a->batch >= 0 && a->q_len >= 0 && a->kv_len >= 0, "attention: negative size");
+    TDGS_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0,
+                 "attention: %d query heads do not divide among %d kv heads", a->heads, a->kv_heads);
+    TDGS_REQUIRE(a->kv_batch == a->batch || a->kv_batch == 1, "attention: kv batch %d is neither the batch %d nor 1",
+                 a->kv_batch, a->batch);
+    TDGS_REQUIRE(a->head_dim >= 1 && a->head_dim <= 128, "attention: head dimension %d is not in 1 to 128", a->head_dim);
+    TDGS_REQUIRE(a->scale > 0.0f && a->scale < INFINITY, "attention: the scale must be positive and finite");
+    const int64_t g = a->heads / a->kv_heads;
+    TDGS_REQUIRE((int64_t)a->batch * a->q_len <= INT32_MAX / g - 256, "attention: too many queries for one kv head");
+    TDGS_REQUIRE((int64_t)a->batch * a->heads <= INT32_MAX / (a->q_len / 128 + 1) / kAtSplits, "attention: too many heads");
+    TDGS_REQUIRE(a->kv_len <= INT32_MAX - 256, "attention: too many keys");
+    TDGS_REQUIRE((int64_t)a->kv_batch * a->kv_heads <= INT32_MAX / (a->kv_len / 128 + 1) / kAtSplits, "attention: too many kv heads");
+    return TDGS_OK;
+}
+
+static AtHeads at_strides(const tdgs_heads& v) { return {v.stride_b, v.stride_l, v.stride_h}; }
+
+// Whether rows of the view start on 16 bytes.
+static bool at_rows_aligned(const tdgs_heads& v, int64_t e) {
+    return aligned_to(v.data, 16) && v.stride_b * e % 16 == 0 && v.stride_l * e % 16 == 0 && v.stride_h * e % 16 == 0;
+}
+
+static AtArgs at_args(const tdgs_attention* a, const AtPlan& p) {
+    AtArgs r = {};
+    const int64_t e = dtype_size(a->dtype);
+    r.q = a->q.data;
+    r.k = a->k.data;
+    r.v = a->v.data;
+    r.o = r.out = a->out.data;
+    r.sq = at_strides(a->q);
+    r.sk = at_strides(a->k);
+    r.sv = at_strides(a->v);
+    r.so = at_strides(a->out);
+    r.lengths = a->kv_lengths;
+    r.mask = a->kv_mask;
+    r.mask_stride = a->kv_mask_stride;
+    r.lse = a->lse;
+    r.q_len = a->q_len;
+    r.kv_len = a->kv_len;
+    r.heads = a->heads;
+    r.kv_heads = a->kv_heads;
+    r.d = a->head_dim;
+    r.rows = (int32_t)p.rows;
+    r.group_batches = a->batch / a->kv_batch;
+    r.scale = a->scale;
+    r.c = a->scale * kLog2e;
+    const uint32_t g = (uint32_t)(a->heads / a->kv_heads);
+    r.by_g = FastDiv(g);
+    r.by_lg = FastDiv(g * (uint32_t)(a->q_len > 0 ? a->q_len : 1));
+    r.vec = a->head_dim % 8 == 0 && at_rows_aligned(a->q, e) && at_rows_aligned(a->k, e) && at_rows_aligned(a->v, e);
+    r.vec_out = a->head_dim % 8 == 0 && at_rows_aligned(a->out, e);
+    return r;
+}
+
+// f(integral constant) for the padded head dimension.
+template <class F>
+static int with_padded(int dp, F&& f) {
+    switch (dp) {
+        case 32: return f(std::integral_constant<int, 32>{});
+        case 64: return f(std::integral_constant<int, 64>{});
+        case 96: return f(std::integral_constant<int, 96>{});
+        default: return f(std::integral_constant<int, 128>{});
+    }
+}
+
+}  // namespace tdgs
+
+using namespace tdgs;
+
+extern "C" {
+
+size_t tdgs_cross_attention_temp_bytes(const tdgs_attention* a, int32_t grad) {
+    if (at_check(a) != TDGS_OK || a->batch == 0) return 0;
+    const AtPlan p = at_plan(a);
+    return grad && p.grad_bytes > p.forward_bytes ? p.grad_bytes : p.forward_bytes;
+}
+
+int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
+    TDGS_TRY(at_check(a));
+    if (a->batch == 0 || a->q_len == 0) return TDGS_OK;
+    TDGS_TRY(at_check_view(&a->q, "q", a, false, false));
+    TDGS_TRY(at_check_view(&a->out, "out", a, false, true));
+    if (a->kv_len > 0) {
+        TDGS_TRY(at_check_view(&a->k, "k", a, true, false));
+        TDGS_TRY(at_check_view(&a->v, "v", a, true, false));
+    }
+    const AtPlan p = at_plan(a);
+    TDGS_REQUIRE(p.forward_bytes == 0 || (a->temp && a->temp_bytes >= p.forward_bytes && aligned_to(a->temp, 16)),
+                 "attention: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, p.forward_bytes);
+    hipStream_t stream = (hipStream_t)stream_;
+    AtArgs r = at_args(a, p);
+    r.blocks = p.blocks_f;
+    r.splits = p.splits_f;
+    const int64_t all = p.kvh * p.rows;
+    if (p.splits_f > 1) {
+        r.part = (float*)a->temp;
+        r.part_ml = r.part + p.splits_f * all * p.dp;
+    }
+    const unsigned grid = (unsigned)(p.kvh * p.splits_f * p.blocks_f);
+    return with_dtype(a->dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        TDGS_TRY(with_padded(p.dp, [&](auto dp) -> int {
+            constexpr int DP = decltype(dp)::value;
+            constexpr int QB = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+            k_attend<T, DP, QB><<<grid, kAtThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
+            return TDGS_OK;
+        }));
+        if (p.splits_f > 1) {
+            k_attend_join<T><<<(unsigned)ceil_div(all, kAtWaves), kAtThreads, 0, stream>>>(r, p.dp, all);
+            TDGS_LAUNCHED();
+        }
+        return TDGS_OK;
+    });
+}
+
+int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs_attention_grads* g) {
+    TDGS_TRY(at_check(a));
+    TDGS_REQUIRE(g != nullptr, "attention: null gradients");
+    if (a->batch == 0 || (a->q_len == 0 && a->kv_len == 0)) return TDGS_OK;
+    if (a->q_len > 0) {
+        TDGS_TRY(at_check_view(&a->q, "q", a, false, false));
+        TDGS_TRY(at_check_view(&a->out, "out", a, false, false));
+        TDGS_TRY(at_check_view(&g->dout, "dout", a, false, false));
+        TDGS_TRY(at_check_view(&g->dq, "dq", a, false, true));
+        TDGS_REQUIRE(a->lse != nullptr, "attention: the gradient needs the forward call's lse");
+    }
+    if (a->kv_len > 0) {
+        TDGS_TRY(at_check_view(&a->k, "k", a, true, false));
+        TDGS_TRY(at_check_view(&a->v, "v", a, true, false));
+        TDGS_TRY(at_check_view(&g->dk, "dk", a, true, true));
+        TDGS_TRY(at_check_view(&g->dv, "dv", a, true, true));
+    }
+    const AtPlan p = at_plan(a);
+    TDGS_REQUIRE(a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16),
+                 "attention: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0,
+                 p.grad_bytes);
+    hipStream_t stream = (hipStream_t)stream_;
+    AtArgs r = at_args(a, p);
+    const int64_t e = dtype_size(a->dtype);
+    r.dout = g->dout.data;
+    r.dq = g->dq.data;
+    r.dk = g->dk.data;
+    r.dv = g->dv.data;
+    r.sdo = at_strides(g->dout);
+    r.sdq = at_strides(g->dq);
+    r.sdk = at_strides(g->dk);
+    r.sdv = at_strides(g->dv);
+    r.vec = r.vec && r.vec_out && at_rows_aligned(g->dout, e);
+    r.vec_out = a->head_dim % 8 == 0 && at_rows_aligned(g->dq, e) && at_rows_aligned(g->dk, e) && at_rows_aligned(g->dv, e);
+    r.delta = (float*)a->temp;
+    r.part = (float*)((char*)a->temp + p.delta_bytes);
+    const int64_t all_rows = p.kvh * p.rows, all_keys = p.kvh * a->kv_len;
+    return with_dtype(a->dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        return with_padded(p.dp, [&](auto dp) -> int {
+            constexpr int DP = decltype(dp)::value;
+            if (a->q_len > 0) {
+                r.blocks = p.blocks_q;
+                r.splits = p.splits_q;
+                k_attend_dq<T, DP><<<(unsigned)(p.kvh * p.splits_q * p.blocks_q), kAtThreads, 0, stream>>>(r);
+                TDGS_LAUNCHED();
+                if (p.splits_q > 1) {
+                    k_attend_sum<T><<<(unsigned)ceil_div(all_rows * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
+                        r, DP, all_rows, 0);
+                    TDGS_LAUNCHED();
+                }
+            }
+            if (a->kv_len > 0) {
+                r.blocks = p.blocks_k;
+                r.splits = p.splits_k;
+                k_attend_dkv<T, DP><<<(unsigned)(p.kvh * p.splits_k * p.blocks_k), kAtThreads, 0, stream>>>(r);
+                TDGS_LAUNCHED();
+                if (p.splits_k > 1) {
+                    k_attend_sum<T><<<(unsigned)ceil_div(2 * all_keys * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
+                        r, DP, all_keys, 1);
+                    TDGS_LAUNCHED();
+                }
+            }
+            return TDGS_OK;
+        });
+    });
+}
+
+}  // extern "C"
