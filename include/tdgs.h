@@ -595,6 +595,62 @@ int tdgs_cross_attention(void* stream, const tdgs_attention* a);
  * keys has zero gradient and gives none; so does a key that is not allowed. */
 int tdgs_cross_attention_grad(void* stream, const tdgs_attention* a, const tdgs_attention_grads* g);
 
+/* A (n, pixels, channels) image: strides in elements, the channels contiguous. */
+typedef struct tdgs_pixels {
+    void* data;
+    int64_t stride_n;
+    int64_t stride_p;
+} tdgs_pixels;
+
+/* Group norm with an activation, channels last: per image and group of channels / groups neighbouring
+ * channels, with the mean m and the (biased) variance over its pixels,
+ * out = act((x - m) / sqrt(variance + eps) weight_c + bias_c). act: identity, SiLU, GELU (by the error
+ * function) or ReLU. */
+typedef struct tdgs_norm {
+    int32_t dtype;          /* of x, out, dout and dx */
+    int32_t param_dtype;    /* of weight, bias and their gradients: TDGS_F32 or dtype */
+    int32_t n;              /* images, at most 65535 */
+    int32_t channels, groups;
+    int32_t activation;
+    float eps;
+    int32_t reserved;
+    int64_t pixels;         /* per image */
+    tdgs_pixels x, out;     /* out is not read by the gradient */
+    const void* weight;     /* channels; null: 1 */
+    const void* bias;       /* channels; null: 0 */
+    float* stats;           /* 2 x groups x n: mean, 1 / sqrt(variance + eps); written by the forward call
+                               (where not null), read by the gradient */
+    void* temp;             /* scratch of tdgs_group_norm_temp_bytes() bytes */
+    size_t temp_bytes;
+} tdgs_norm;
+
+typedef struct tdgs_norm_grads {
+    tdgs_pixels dout, dx;
+    void* dweight;          /* channels; null: not wanted */
+    void* dbias;            /* channels; null: not wanted */
+} tdgs_norm_grads;
+
+/* Scratch of tdgs_group_norm (grad 0) or of that and tdgs_group_norm_grad (grad 1). */
+size_t tdgs_group_norm_temp_bytes(const tdgs_norm* a, int32_t grad);
+int tdgs_group_norm(void* stream, const tdgs_norm* a);
+/* The gradients of sum(dout * out). dx may be dout. */
+int tdgs_group_norm_grad(void* stream, const tdgs_norm* a, const tdgs_norm_grads* g);
+
+/* Embedding: out_i = scale table[tokens_i] for n tokens of index_bytes (4 or 8) bytes each; rows of
+ * dim elements, table_stride and out_stride elements apart. A token outside [0, vocab) gives a row of zeros
+ * and raises an error on ctx (tdgs_ctx_check). */
+int tdgs_embedding_lookup(tdgs_ctx* ctx, void* stream, int32_t dtype, const void* table, int64_t table_stride,
+                          int64_t vocab, int32_t dim, const void* tokens, int32_t index_bytes, int64_t n,
+                          float scale, void* out, int64_t out_stride);
+/* The gradient of sum(dout * out) for the table: dtable_v = scale * the sum, in 32 bits, of the dout_i
+ * with tokens_i = v; every row of dtable is written. The token `padding` (-1: none) gives no gradient.
+ * The tokens are sorted and added up in order, so that the result is the same every time. */
+size_t tdgs_embedding_grad_temp_bytes(int64_t n, int64_t vocab, int32_t dim);
+int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream, int32_t dtype, const void* dout, int64_t dout_stride,
+                        const void* tokens, int32_t index_bytes, int64_t n, int64_t padding, float scale,
+                        void* dtable, int64_t dtable_stride, int64_t vocab, int32_t dim, void* temp,
+                        size_t temp_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -119,5 +119,20 @@ class AttentionGradsC(C.Structure):
     _fields_ = [("dout", HeadsC), ("dq", HeadsC), ("dk", HeadsC), ("dv", HeadsC)]
 
 
+class PixelsC(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_n", C.c_int64), ("stride_p", C.c_int64)]
+
+
+class NormC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("param_dtype", C.c_int32), ("n", C.c_int32), ("channels", C.c_int32),
+                ("groups", C.c_int32), ("activation", C.c_int32), ("eps", C.c_float), ("reserved", C.c_int32),
+                ("pixels", C.c_int64), ("x", PixelsC), ("out", PixelsC), ("weight", C.c_void_p),
+                ("bias", C.c_void_p), ("stats", C.c_void_p), ("temp", C.c_void_p), ("temp_bytes", C.c_size_t)]
+
+
+class NormGradsC(C.Structure):
+    _fields_ = [("dout", PixelsC), ("dx", PixelsC), ("dweight", C.c_void_p), ("dbias", C.c_void_p)]
+
+
 def sh_coeffs_per_channel(degree: int) -> int:
     return (int(degree) + 1) ** 2

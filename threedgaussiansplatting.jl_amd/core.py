@@ -47,7 +47,8 @@ def lib():
         L = C.CDLL(LIB_PATH)
         L.tdgs_last_error.restype = C.c_char_p
         for name in ("tdgs_scan_temp_bytes", "tdgs_sort_pairs_temp_bytes", "tdgs_render_temp_bytes",
-                     "tdgs_loss_temp_bytes", "tdgs_cross_attention_temp_bytes"):
+                     "tdgs_loss_temp_bytes", "tdgs_cross_attention_temp_bytes", "tdgs_group_norm_temp_bytes",
+                     "tdgs_embedding_grad_temp_bytes"):
             getattr(L, name).restype = C.c_size_t
         L.tdgs_loss_temp_bytes.argtypes = [C.c_int32, C.c_int32]
         L.tdgs_scan_temp_bytes.argtypes = [C.c_int64]
@@ -66,6 +67,16 @@ def lib():
         L.tdgs_cross_attention_temp_bytes.argtypes = [C.c_void_p, C.c_int32]
         L.tdgs_cross_attention.argtypes = [C.c_void_p, C.c_void_p]
         L.tdgs_cross_attention_grad.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.tdgs_group_norm_temp_bytes.argtypes = [C.c_void_p, C.c_int32]
+        L.tdgs_group_norm.argtypes = [C.c_void_p, C.c_void_p]
+        L.tdgs_group_norm_grad.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.tdgs_embedding_lookup.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_int64,
+                                            C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_void_p,
+                                            C.c_int64]
+        L.tdgs_embedding_grad_temp_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int32]
+        L.tdgs_embedding_grad.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                          C.c_int32, C.c_int64, C.c_int64, C.c_float, C.c_void_p, C.c_int64,
+                                          C.c_int64, C.c_int32, C.c_void_p, C.c_size_t]
         _LIB = L
     return _LIB
 

@@ -34,6 +34,9 @@ int read_counters(tdgs_ctx* ctx, hipStream_t stream) {
         if (flags & kErrSortCounts)
             set_error("a radix sort on this context found counts that disagree with its keys; the sorted "
                       "lists of that call are incomplete (device flags 0x%x)", flags);
+        else if (flags & kErrTokenRange)
+            set_error("an embedding call on this context was given a token outside its table; it took it for a "
+                      "row of zeros (device flags 0x%x)", flags);
         else
             set_error("device error flags 0x%x raised on this context", flags);
         return TDGS_ERR_DEVICE;

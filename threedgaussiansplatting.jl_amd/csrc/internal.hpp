@@ -25,6 +25,7 @@ constexpr int kMonitor = 5;
 // kErr* bits into it; every host synchronisation through read_counters reports and clears it.
 constexpr int kErrSlot = 7;
 constexpr uint32_t kErrSortCounts = 1u;   // radix-sort counts disagreed with the keys
+constexpr uint32_t kErrTokenRange = 2u;   // an embedding token outside the table
 
 inline uint32_t* ctx_error_word(tdgs_ctx* ctx) { return reinterpret_cast<uint32_t*>(ctx->d_counters + kErrSlot); }
 

@@ -1,0 +1,668 @@
+// norm.hip — group norm with an activation over channels-last images, forward and backward.
+//
+// A workgroup takes a run of pixels and all channels (or 256 vectors of them): thread t holds VW
+// neighbouring channels, 16 bytes where the tensors allow it, of every (256 / vectors)th pixel, so
+// its channels' statistics, weights and sums live in its registers and a pixel's channels are read
+// as one contiguous piece. The kernels are bound by memory.
+//
+// Statistics are Welford's running mean and sum of squared deviations in 32 bits, per channel, and
+// are joined between threads, workgroups and a group's channels by the exact rule for two parts
+// (Chan, Golub & LeVeque 1979): M2 = M2_a + M2_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b). A sum of
+// squares minus the squared mean would lose the variance of a channel whose mean is large.
+#include "internal.hpp"
+#include "elem.hpp"
+
+namespace tdgs {
+
+constexpr int kGnThreads = 256;
+
+struct GnArgs {
+    const void *x, *dout, *weight, *bias;
+    void *out, *dx, *dweight, *dbias;
+    int64_t xn, xp, on, op, dn, dp, gn, gp;   // strides of x, out, dout, dx between images and pixels
+    float* stats;                             // mean and 1 / deviation per image and group
+    float *part, *chan;
+    int64_t pixels, per;                      // per: pixels per workgroup
+    int32_t n, channels, groups, group_size, blocks, vectors;
+    float eps;
+    bool param_f32;
+};
+
+// Channel c's weight or bias (null: none given).
+template <class T>
+__device__ __forceinline__ float gn_param(const void* p, bool f32, int c, float none) {
+    if (!p) return none;
+    return f32 ? ((const float*)p)[c] : (float)((const T*)p)[c];
+}
+template <class T>
+__device__ __forceinline__ void gn_set_param(void* p, bool f32, int c, float v) {
+    if (f32) ((float*)p)[c] = v;
+    else ((T*)p)[c] = (T)v;
+}
+
+template <class T, int VW>
+struct GnVec {
+    typedef T V __attribute__((ext_vector_type(VW)));
+    float f[VW];
+    __device__ __forceinline__ void load(const T* __restrict__ p) {
+        if constexpr (VW == 1) {
+            f[0] = (float)*p;
+        } else {
+            const V v = *reinterpret_cast<const V*>(p);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) f[i] = (float)v[i];
+        }
+    }
+    __device__ __forceinline__ void store(T* __restrict__ p) const {
+        if constexpr (VW == 1) {
+            *p = (T)f[0];
+        } else {
+            V v;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) v[i] = (T)f[i];
+            *reinterpret_cast<V*>(p) = v;
+        }
+    }
+};
+
+// act(z), and its derivative in *slope where wanted. SiLU: z s, s + y (1 - s) with s = 1 / (1 + e^-z).
+// GELU: z cdf(z), cdf + z e^(-z^2 / 2) / sqrt(2 pi); the normal distribution's tail is
+// erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most (Abramowitz & Stegun
+// 7.1.26), which takes the exponential that the derivative needs anyway: 0.8e-7 in cdf, one rounding.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float gn_act(float z, float* slope) {
+    if constexpr (ACT == TDGS_ACT_IDENTITY) {
+        if (SLOPE) *slope = 1.0f;
+        return z;
+    } else if constexpr (ACT == TDGS_ACT_RELU) {
+        if (SLOPE) *slope = z > 0.0f ? 1.0f : 0.0f;
+        return z < 0.0f ? 0.0f : z;   // (NaN stays)
+    } else if constexpr (ACT == TDGS_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
+        const float y = z * s;
+        if (SLOPE) *slope = __builtin_fmaf(y, 1.0f - s, s);
+        return y;
+    } else {
+        const float ax = fabsf(z) * 0.70710678118654752f;
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, ax, 1.0f));
+        const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
+        float a = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+        a = __builtin_fmaf(a, t, 1.421413741f);
+        a = __builtin_fmaf(a, t, -0.284496736f);
+        a = __builtin_fmaf(a, t, 0.254829592f);
+        const float tail = 0.5f * a * t * e;
+        const float cdf = z < 0.0f ? tail : 1.0f - tail;
+        if (SLOPE) *slope = __builtin_fmaf(z * 0.39894228040143268f, e, cdf);
+        return z * cdf;
+    }
+}
+
+// Joins (nb, mb, sb) into (n, m, s): counts, means, sums of squared deviations.
+__device__ __forceinline__ void gn_join(float& n, float& m, float& s, float nb, float mb, float sb) {
+    const float all = n + nb;
+    if (nb <= 0.0f) return;
+    const float d = mb - m, share = nb / all;
+    m = __builtin_fmaf(d, share, m);
+    s += sb + d * d * (n * share);
+    n = all;
+}
+
+// Where a thread of a workgroup of `vectors` channel vectors stands.
+struct GnPlace {
+    int cv, pl, lanes;   // channel vector, first pixel, pixels apart
+    bool on;
+    __device__ __forceinline__ explicit GnPlace(int vectors) {
+        lanes = kGnThreads / vectors;
+        cv = (int)threadIdx.x % vectors;
+        pl = (int)threadIdx.x / vectors;
+        on = pl < lanes;
+    }
+};
+
+// Per-channel statistics of pixels [p0, p1) of the channels from x on, joined over the workgroup: thread
+// c < vectors * VW gets channel c's mean and sum of squared deviations.
+template <class T, int VW>
+__device__ __forceinline__ void gn_stats(const T* __restrict__ x, int64_t xp, int64_t p0, int64_t p1, int vectors,
+                                         float* s_mean, float* s_m2, float* mean_out, float* m2_out) {
+    const GnPlace at(vectors);
+    float mean[VW], m2[VW];
+#pragma unroll
+    for (int i = 0; i < VW; ++i) mean[i] = m2[i] = 0.0f;
+    if (at.on) {
+        float count = 0.0f;
+        constexpr int U = 4;
+        int64_t p = p0 + at.pl;
+        auto add = [&](const GnVec<T, VW>& v) {
+            count += 1.0f;
+            const float r = __builtin_amdgcn_rcpf(count);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                const float d = v.f[i] - mean[i];
+                mean[i] = __builtin_fmaf(d, r, mean[i]);
+                m2[i] = __builtin_fmaf(d, v.f[i] - mean[i], m2[i]);
+            }
+        };
+        for (; p + (U - 1) * at.lanes < p1; p += U * at.lanes) {
+            GnVec<T, VW> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u].load(x + (p + u * at.lanes) * xp + at.cv * VW);
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(v[u]);
+        }
+        for (; p < p1; p += at.lanes) {
+            GnVec<T, VW> v;
+            v.load(x + p * xp + at.cv * VW);
+            add(v);
+        }
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            s_mean[threadIdx.x * VW + i] = mean[i];
+            s_m2[threadIdx.x * VW + i] = m2[i];
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) {
+        float n = 0.0f, m = 0.0f, s = 0.0f;
+        for (int l = 0; l < at.lanes; ++l) {
+            const int64_t left = p1 - p0 - l;
+            const float nb = left > 0 ? (float)((left + at.lanes - 1) / at.lanes) : 0.0f;
+            gn_join(n, m, s, nb, s_mean[l * vectors * VW + c], s_m2[l * vectors * VW + c]);
+        }
+        mean_out[c] = m;
+        m2_out[c] = s;
+    }
+}
+
+// Workgroup (b, y, n): statistics of run b of image n's pixels, channel block y.
+template <class T, int VW>
+__global__ __launch_bounds__(kGnThreads) void k_norm_stats(GnArgs a) {
+    __shared__ float s_mean[kGnThreads * VW];
+    __shared__ float s_m2[kGnThreads * VW];
+    __shared__ float s_o1[kGnThreads * VW];
+    __shared__ float s_o2[kGnThreads * VW];
+    const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads;
+    const int vectors = min(a.vectors - v0, kGnThreads), c0 = v0 * VW;
+    const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
+    gn_stats<T, VW>((const T*)a.x + n * a.xn + c0, a.xp, p0, p1, vectors, s_mean, s_m2, s_o1, s_o2);
+    __syncthreads();
+    float2* const out = (float2*)a.part + ((int64_t)n * a.blocks + b) * a.channels + c0;
+    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) out[c] = make_float2(s_o1[c], s_o2[c]);
+}
+
+// Workgroup n * groups + g: joins the runs and the channels of a group.
+static __global__ __launch_bounds__(kGnThreads) void k_norm_join(GnArgs a) {
+    __shared__ float s_n[kGnThreads], s_m[kGnThreads], s_s[kGnThreads];
+    const int n = blockIdx.x / a.groups, g = blockIdx.x % a.groups, t = threadIdx.x;
+    const float2* const part = (const float2*)a.part + (int64_t)n * a.blocks * a.channels + g * a.group_size;
+    float cnt = 0.0f, m = 0.0f, s = 0.0f;
+    const int64_t items = (int64_t)a.blocks * a.group_size;
+    for (int64_t i = t; i < items; i += kGnThreads) {
+        const int b = (int)(i / a.group_size), c = (int)(i % a.group_size);
+        const float2 v = part[(int64_t)b * a.channels + c];
+        gn_join(cnt, m, s, (float)(min(a.pixels, (b + 1) * a.per) - b * a.per), v.x, v.y);
+    }
+    s_n[t] = cnt;
+    s_m[t] = m;
+    s_s[t] = s;
+    for (int w = kGnThreads / 2; w > 0; w >>= 1) {
+        __syncthreads();
+        if (t < w) {
+            gn_join(s_n[t], s_m[t], s_s[t], s_n[t + w], s_m[t + w], s_s[t + w]);
+        }
+    }
+    if (t == 0) {
+        a.stats[2 * blockIdx.x] = s_m[0];
+        a.stats[2 * blockIdx.x + 1] = 1.0f / sqrtf(s_s[0] / s_n[0] + a.eps);
+    }
+}
+
+// What a thread needs of its channels: xhat = (x - mean) r, z = xhat w + b.
+template <class T, int VW>
+struct GnChannels {
+    float mean[VW], r[VW], w[VW], b[VW];
+    __device__ __forceinline__ void load(const GnArgs& a, const float* stats, int c0) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            const int g = (c0 + i) / a.group_size;
+            mean[i] = stats[2 * g];
+            r[i] = stats[2 * g + 1];
+            w[i] = gn_param<T>(a.weight, a.param_f32, c0 + i, 1.0f);
+            b[i] = gn_param<T>(a.bias, a.param_f32, c0 + i, 0.0f);
+        }
+    }
+};
+
+template <class T, int VW, int ACT>
+__device__ __forceinline__ void gn_apply(const GnArgs& a, const T* __restrict__ x, T* __restrict__ out,
+                                         const GnChannels<T, VW>& ch, int64_t p0, int64_t p1, const GnPlace& at) {
+    float rw[VW];
+#pragma unroll
+    for (int i = 0; i < VW; ++i) rw[i] = ch.r[i] * ch.w[i];
+    auto one = [&](GnVec<T, VW>& v) {
+        float none;
+#pragma unroll
+        for (int i = 0; i < VW; ++i)
+            v.f[i] = gn_act<ACT, false>(__builtin_fmaf(v.f[i] - ch.mean[i], rw[i], ch.b[i]), &none);
+    };
+    constexpr int U = 4;
+    int64_t p = p0 + at.pl;
+    for (; p + (U - 1) * at.lanes < p1; p += U * at.lanes) {
+        GnVec<T, VW> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].load(x + (p + u * at.lanes) * a.xp + at.cv * VW);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            one(v[u]);
+            v[u].store(out + (p + u * at.lanes) * a.op + at.cv * VW);
+        }
+    }
+    for (; p < p1; p += at.lanes) {
+        GnVec<T, VW> v;
+        v.load(x + p * a.xp + at.cv * VW);
+        one(v);
+        v.store(out + p * a.op + at.cv * VW);
+    }
+}
+
+template <class T, int VW, int ACT>
+__global__ __launch_bounds__(kGnThreads) void k_norm_apply(GnArgs a) {
+    const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads, c0 = v0 * VW;
+    const GnPlace at(min(a.vectors - v0, kGnThreads));
+    if (!at.on) return;
+    GnChannels<T, VW> ch;
+    ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
+    const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
+    gn_apply<T, VW, ACT>(a, (const T*)a.x + n * a.xn + c0, (T*)a.out + n * a.on + c0, ch, p0, p1, at);
+}
+
+// ---- backward ------------------------------------------------------------------------------
+
+// e = dout act'(z) and xhat of one vector.
+template <class T, int VW, int ACT>
+__device__ __forceinline__ void gn_slope(const GnChannels<T, VW>& ch, const GnVec<T, VW>& x, const GnVec<T, VW>& d,
+                                         float (&e)[VW], float (&xhat)[VW]) {
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+        float slope;
+        xhat[i] = (x.f[i] - ch.mean[i]) * ch.r[i];
+        gn_act<ACT, true>(__builtin_fmaf(xhat[i], ch.w[i], ch.b[i]), &slope);
+        e[i] = d.f[i] * slope;
+    }
+}
+
+// Sums of e and e xhat over pixels [p0, p1), per channel, joined over the workgroup into o1 and o2.
+template <class T, int VW, int ACT>
+__device__ __forceinline__ void gn_sums(const GnArgs& a, const T* __restrict__ x, const T* __restrict__ dout,
+                                        const GnChannels<T, VW>& ch, int64_t p0, int64_t p1, const GnPlace& at,
+                                        int vectors, float* s_1, float* s_2, float* o1, float* o2) {
+    if (at.on) {
+        float s1[VW], s2[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) s1[i] = s2[i] = 0.0f;
+        auto add = [&](const GnVec<T, VW>& vx, const GnVec<T, VW>& vd) {
+            float e[VW], xhat[VW];
+            gn_slope<T, VW, ACT>(ch, vx, vd, e, xhat);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) {
+                s1[i] += e[i];
+                s2[i] = __builtin_fmaf(e[i], xhat[i], s2[i]);
+            }
+        };
+        constexpr int U = 2;
+        int64_t p = p0 + at.pl;
+        for (; p + (U - 1) * at.lanes < p1; p += U * at.lanes) {
+            GnVec<T, VW> vx[U], vd[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                vx[u].load(x + (p + u * at.lanes) * a.xp + at.cv * VW);
+                vd[u].load(dout + (p + u * at.lanes) * a.dp + at.cv * VW);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(vx[u], vd[u]);
+        }
+        for (; p < p1; p += at.lanes) {
+            GnVec<T, VW> vx, vd;
+            vx.load(x + p * a.xp + at.cv * VW);
+            vd.load(dout + p * a.dp + at.cv * VW);
+            add(vx, vd);
+        }
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            s_1[threadIdx.x * VW + i] = s1[i];
+            s_2[threadIdx.x * VW + i] = s2[i];
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) {
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int l = 0; l < at.lanes; ++l) {
+            s1 += s_1[l * vectors * VW + c];
+            s2 += s_2[l * vectors * VW + c];
+        }
+        o1[c] = s1;
+        o2[c] = s2;
+    }
+}
+
+template <class T, int VW, int ACT>
+__global__ __launch_bounds__(kGnThreads) void k_norm_sums(GnArgs a) {
+    __shared__ float s_1[kGnThreads * VW];
+    __shared__ float s_2[kGnThreads * VW];
+    __shared__ float s_o1[kGnThreads * VW];
+    __shared__ float s_o2[kGnThreads * VW];
+    const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads, c0 = v0 * VW;
+    const int vectors = min(a.vectors - v0, kGnThreads);
+    const GnPlace at(vectors);
+    GnChannels<T, VW> ch;
+    ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
+    const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
+    gn_sums<T, VW, ACT>(a, (const T*)a.x + n * a.xn + c0, (const T*)a.dout + n * a.dn + c0, ch, p0, p1, at, vectors, s_1,
+                        s_2, s_o1, s_o2);
+    __syncthreads();
+    float2* const out = (float2*)a.part + ((int64_t)n * a.blocks + b) * a.channels + c0;
+    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) out[c] = make_float2(s_o1[c], s_o2[c]);
+}
+
+// Workgroup: 16 channels; joins the runs of each image (sums per image and channel to chan) and the images
+// (dweight, dbias).
+template <class T>
+__global__ __launch_bounds__(kGnThreads) void k_norm_sums_join(GnArgs a) {
+    __shared__ float2 s[kGnThreads];
+    const int c = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
+    float dw = 0.0f, db = 0.0f;
+    for (int n = 0; n < a.n; ++n) {
+        float2 v = make_float2(0.0f, 0.0f);
+        if (c < a.channels)
+            for (int b = lane; b < a.blocks; b += 16) {
+                const float2 p = ((const float2*)a.part)[((int64_t)n * a.blocks + b) * a.channels + c];
+                v.x += p.x;
+                v.y += p.y;
+            }
+        __syncthreads();
+        s[threadIdx.x] = v;
+        __syncthreads();
+        if (lane == 0 && c < a.channels) {
+            float2 sum = make_float2(0.0f, 0.0f);
+            for (int l = 0; l < 16; ++l) {
+                sum.x += s[l * 16 + threadIdx.x].x;
+                sum.y += s[l * 16 + threadIdx.x].y;
+            }
+            ((float2*)a.chan)[(int64_t)n * a.channels + c] = sum;
+            db += sum.x;
+            dw += sum.y;
+        }
+    }
+    if (lane == 0 && c < a.channels) {
+        if (a.dweight) gn_set_param<T>(a.dweight, a.param_f32, c, dw);
+        if (a.dbias) gn_set_param<T>(a.dbias, a.param_f32, c, db);
+    }
+}
+
+// dx of pixels [p0, p1): r (w e - m1 - xhat m2), m1 and m2 the group's means of w e and w e xhat.
+template <class T, int VW, int ACT>
+__device__ __forceinline__ void gn_dx(const GnArgs& a, const T* __restrict__ x, const T* __restrict__ dout,
+                                      T* __restrict__ dx, const GnChannels<T, VW>& ch, const float (&m1)[VW],
+                                      const float (&m2)[VW], int64_t p0, int64_t p1, const GnPlace& at) {
+    auto one = [&](const GnVec<T, VW>& vx, GnVec<T, VW>& vd) {
+        float e[VW], xhat[VW];
+        gn_slope<T, VW, ACT>(ch, vx, vd, e, xhat);
+#pragma unroll
+        for (int i = 0; i < VW; ++i)
+            vd.f[i] = ch.r[i] * __builtin_fmaf(-xhat[i], m2[i], __builtin_fmaf(ch.w[i], e[i], -m1[i]));
+    };
+    constexpr int U = 2;
+    int64_t p = p0 + at.pl;
+    for (; p + (U - 1) * at.lanes < p1; p += U * at.lanes) {
+        GnVec<T, VW> vx[U], vd[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            vx[u].load(x + (p + u * at.lanes) * a.xp + at.cv * VW);
+            vd[u].load(dout + (p + u * at.lanes) * a.dp + at.cv * VW);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            one(vx[u], vd[u]);
+            vd[u].store(dx + (p + u * at.lanes) * a.gp + at.cv * VW);
+        }
+    }
+    for (; p < p1; p += at.lanes) {
+        GnVec<T, VW> vx, vd;
+        vx.load(x + p * a.xp + at.cv * VW);
+        vd.load(dout + p * a.dp + at.cv * VW);
+        one(vx, vd);
+        vd.store(dx + p * a.gp + at.cv * VW);
+    }
+}
+
+template <class T, int VW, int ACT>
+__global__ __launch_bounds__(kGnThreads) void k_norm_dx(GnArgs a) {
+    const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads, c0 = v0 * VW;
+    const GnPlace at(min(a.vectors - v0, kGnThreads));
+    if (!at.on) return;
+    GnChannels<T, VW> ch;
+    ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
+    float m1[VW], m2[VW];
+    const float count = (float)a.pixels * (float)a.group_size;
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+        const int g = (c0 + at.cv * VW + i) / a.group_size;
+        if (i > 0 && g == last) {
+            m1[i] = m1[i - 1];
+            m2[i] = m2[i - 1];
+            continue;
+        }
+        last = g;
+        float s1 = 0.0f, s2 = 0.0f;
+        const float2* const chan = (const float2*)a.chan + (int64_t)n * a.channels;
+        for (int c = g * a.group_size; c < (g + 1) * a.group_size; ++c) {
+            const float w = gn_param<T>(a.weight, a.param_f32, c, 1.0f);
+            const float2 v = chan[c];
+            s1 = __builtin_fmaf(w, v.x, s1);
+            s2 = __builtin_fmaf(w, v.y, s2);
+        }
+        m1[i] = s1 / count;
+        m2[i] = s2 / count;
+    }
+    const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
+    gn_dx<T, VW, ACT>(a, (const T*)a.x + n * a.xn + c0, (const T*)a.dout + n * a.dn + c0, (T*)a.dx + n * a.gn + c0, ch, m1,
+                      m2, p0, p1, at);
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+struct GnPlan {
+    int vw, vectors, blocks;
+    int64_t per;
+    size_t stats_bytes, part_bytes, chan_bytes;
+    size_t forward_bytes, grad_bytes;
+};
+
+// Workgroups of one pass over all images, and the least pixels a thread takes: the runs' joining costs
+// as much as they are many.
+constexpr int64_t kGnWorkgroups = 1024;
+constexpr int64_t kGnPixels = 8;
+
+// Scratch sized for either vector width (the tensors' alignment may differ between calls).
+static GnPlan gn_plan(const tdgs_norm* a, bool vec) {
+    GnPlan p;
+    p.vw = vec ? (a->dtype == TDGS_F32 ? 4 : 8) : 1;
+    p.vectors = a->channels / p.vw;
+    const int64_t lanes = p.vectors < kGnThreads ? kGnThreads / p.vectors : 1;
+    int64_t blocks = ceil_div(a->pixels, lanes * kGnPixels);
+    const int64_t most = ceil_div(kGnWorkgroups, (a->n > 0 ? a->n : 1) * ceil_div(p.vectors, kGnThreads));
+    if (blocks > most) blocks = most;
+    p.per = ceil_div(a->pixels, blocks > 0 ? blocks : 1);
+    p.blocks = (int)ceil_div(a->pixels, p.per > 0 ? p.per : 1);
+    p.stats_bytes = align_up((size_t)a->n * a->groups * 2 * sizeof(float));
+    p.part_bytes = align_up((size_t)a->n * p.blocks * a->channels * 2 * sizeof(float));
+    p.chan_bytes = align_up((size_t)a->n * a->channels * 2 * sizeof(float));
+    p.forward_bytes = p.stats_bytes + p.part_bytes;
+    p.grad_bytes = p.chan_bytes + p.part_bytes;
+    return p;
+}
+
+static int gn_check(const tdgs_norm* a) {
+    TDGS_REQUIRE(a != nullptr, "group norm: null arguments");
+    TDGS_REQUIRE(known_dtype(a->dtype), "group norm: unknown element type %d", a->dtype);
+    TDGS_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == TDGS_F32,
+                 "group norm: weight and bias must be float32 or of the input's type");
+    TDGS_REQUIRE(a->n >= 0 && a->pixels >= 0 && a->n <= 65535, "group norm: %d images of %lld pixels", a->n,
+                 (long long)a->pixels);
+    TDGS_REQUIRE(a->channels > 0 && a->channels <= (1 << 20) && a->groups > 0 && a->channels % a->groups == 0,
+                 "group norm: %d channels do not divide into %d groups", a->channels, a->groups);
+    TDGS_REQUIRE((int64_t)a->n * a->groups <= INT32_MAX, "group norm: %d groups in each of %d images", a->groups, a->n);
+    TDGS_REQUIRE(a->activation >= TDGS_ACT_IDENTITY && a->activation <= TDGS_ACT_RELU, "group norm: unknown activation %d",
+                 a->activation);
+    TDGS_REQUIRE(a->eps >= 0.0f && a->eps < INFINITY, "group norm: eps must be finite and not negative");
+    return TDGS_OK;
+}
+
+static int gn_check_view(const tdgs_pixels* v, const char* name, const tdgs_norm* a, bool written) {
+    TDGS_REQUIRE(v->data != nullptr, "group norm: %s is null", name);
+    TDGS_REQUIRE(aligned_to(v->data, (size_t)dtype_size(a->dtype)), "group norm: %s is not aligned to its element type", name);
+    TDGS_REQUIRE(v->stride_n >= 0 && v->stride_p >= 0, "group norm: %s has a negative stride", name);
+    if (written)
+        TDGS_REQUIRE((a->n <= 1 || v->stride_n >= a->channels) && (a->pixels <= 1 || v->stride_p >= a->channels),
+                     "group norm: pixels of %s overlap", name);
+    return TDGS_OK;
+}
+
+static bool gn_vec(const tdgs_pixels& v, const tdgs_norm* a) {
+    const int64_t e = dtype_size(a->dtype);
+    return a->channels * e % 16 == 0 && aligned_to(v.data, 16) && v.stride_n * e % 16 == 0 && v.stride_p * e % 16 == 0;
+}
+
+static GnArgs gn_args(const tdgs_norm* a, const GnPlan& p) {
+    GnArgs r = {};
+    r.x = a->x.data;
+    r.xn = a->x.stride_n;
+    r.xp = a->x.stride_p;
+    r.weight = a->weight;
+    r.bias = a->bias;
+    r.stats = a->stats;
+    r.pixels = a->pixels;
+    r.per = p.per;
+    r.n = a->n;
+    r.channels = a->channels;
+    r.groups = a->groups;
+    r.group_size = a->channels / a->groups;
+    r.blocks = p.blocks;
+    r.vectors = p.vectors;
+    r.eps = a->eps;
+    r.param_f32 = a->param_dtype == TDGS_F32;
+    return r;
+}
+
+// f(T{}, vector width, activation) for the call's kernels.
+template <class F>
+static int gn_dispatch(const tdgs_norm* a, int vw, F&& f) {
+    return with_dtype(a->dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        auto with_act = [&](auto w) -> int {
+            switch (a->activation) {
+                case TDGS_ACT_IDENTITY: return f(t, w, std::integral_constant<int, TDGS_ACT_IDENTITY>{});
+                case TDGS_ACT_SILU: return f(t, w, std::integral_constant<int, TDGS_ACT_SILU>{});
+                case TDGS_ACT_GELU: return f(t, w, std::integral_constant<int, TDGS_ACT_GELU>{});
+                default: return f(t, w, std::integral_constant<int, TDGS_ACT_RELU>{});
+            }
+        };
+        return vw == 1 ? with_act(std::integral_constant<int, 1>{}) : with_act(std::integral_constant<int, 16 / (int)sizeof(T)>{});
+    });
+}
+
+}  // namespace tdgs
+
+using namespace tdgs;
+
+extern "C" {
+
+size_t tdgs_group_norm_temp_bytes(const tdgs_norm* a, int32_t grad) {
+    if (gn_check(a) != TDGS_OK) return 0;
+    size_t bytes = 0;
+    for (int vec = 0; vec < 2; ++vec) {
+        if (vec && a->channels * dtype_size(a->dtype) % 16 != 0) continue;
+        const GnPlan p = gn_plan(a, vec != 0);
+        const size_t b = grad && p.grad_bytes > p.forward_bytes ? p.grad_bytes : p.forward_bytes;
+        if (b > bytes) bytes = b;
+    }
+    return bytes;
+}
+
+int tdgs_group_norm(void* stream_, const tdgs_norm* a) {
+    TDGS_TRY(gn_check(a));
+    if (a->n == 0 || a->pixels == 0) return TDGS_OK;
+    TDGS_TRY(gn_check_view(&a->x, "x", a, false));
+    TDGS_TRY(gn_check_view(&a->out, "out", a, true));
+    const bool vec = gn_vec(a->x, a) && gn_vec(a->out, a);
+    const GnPlan p = gn_plan(a, vec);
+    TDGS_REQUIRE(a->temp && a->temp_bytes >= p.forward_bytes && aligned_to(a->temp, 16),
+                 "group norm: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, p.forward_bytes);
+    hipStream_t stream = (hipStream_t)stream_;
+    GnArgs r = gn_args(a, p);
+    r.out = a->out.data;
+    r.on = a->out.stride_n;
+    r.op = a->out.stride_p;
+    if (!r.stats) r.stats = (float*)a->temp;
+    r.part = (float*)((char*)a->temp + p.stats_bytes);
+    const dim3 grid((unsigned)p.blocks, (unsigned)ceil_div(p.vectors, kGnThreads), (unsigned)a->n);
+    return gn_dispatch(a, p.vw, [&](auto t, auto w, auto act) -> int {
+        using T = decltype(t);
+        constexpr int VW = decltype(w)::value, ACT = decltype(act)::value;
+        k_norm_stats<T, VW><<<grid, kGnThreads, 0, stream>>>(r);
+        TDGS_LAUNCHED();
+        k_norm_join<<<(unsigned)((int64_t)a->n * a->groups), kGnThreads, 0, stream>>>(r);
+        TDGS_LAUNCHED();
+        k_norm_apply<T, VW, ACT><<<grid, kGnThreads, 0, stream>>>(r);
+        TDGS_LAUNCHED();
+        return TDGS_OK;
+    });
+}
+
+int tdgs_group_norm_grad(void* stream_, const tdgs_norm* a, const tdgs_norm_grads* g) {
+    TDGS_TRY(gn_check(a));
+    TDGS_REQUIRE(g != nullptr, "group norm: null gradients");
+    TDGS_REQUIRE(a->stats != nullptr, "group norm: the gradient needs the forward call's stats");
+    const bool empty = a->n == 0 || a->pixels == 0;
+    if (!empty) {
+        TDGS_TRY(gn_check_view(&a->x, "x", a, false));
+        TDGS_TRY(gn_check_view(&g->dout, "dout", a, false));
+        TDGS_TRY(gn_check_view(&g->dx, "dx", a, true));
+    }
+    const bool vec = !empty && gn_vec(a->x, a) && gn_vec(g->dout, a) && gn_vec(g->dx, a);
+    GnPlan p = gn_plan(a, vec);
+    if (empty) p.blocks = 0;   // (dweight and dbias are zero)
+    TDGS_REQUIRE(a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16),
+                 "group norm: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0,
+                 p.grad_bytes);
+    hipStream_t stream = (hipStream_t)stream_;
+    GnArgs r = gn_args(a, p);
+    r.dout = g->dout.data;
+    r.dn = g->dout.stride_n;
+    r.dp = g->dout.stride_p;
+    r.dx = g->dx.data;
+    r.gn = g->dx.stride_n;
+    r.gp = g->dx.stride_p;
+    r.dweight = g->dweight;
+    r.dbias = g->dbias;
+    r.chan = (float*)a->temp;
+    r.part = (float*)((char*)a->temp + p.chan_bytes);
+    const dim3 grid((unsigned)p.blocks, (unsigned)ceil_div(p.vectors, kGnThreads), (unsigned)a->n);
+    return gn_dispatch(a, p.vw, [&](auto t, auto w, auto act) -> int {
+        using T = decltype(t);
+        constexpr int VW = decltype(w)::value, ACT = decltype(act)::value;
+        if (!empty) {
+            k_norm_sums<T, VW, ACT><<<grid, kGnThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
+        }
+        k_norm_sums_join<T><<<(unsigned)ceil_div(a->channels, 16), kGnThreads, 0, stream>>>(r);
+        TDGS_LAUNCHED();
+        if (!empty) {
+            k_norm_dx<T, VW, ACT><<<grid, kGnThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
+        }
+        return TDGS_OK;
+    });
+}
+
+}  // extern "C"

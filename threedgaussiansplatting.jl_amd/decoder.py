@@ -1,8 +1,9 @@
 """Operators of a learned decoder of rendered images over libtdgs.so: cross attention to an
-encoder's states, with the gradient of each operand.
+encoder's states, group norm with an activation (channels last) and embedding lookup, each with
+its gradients.
 
 What a network that turns rendered features into images needs besides matrix products (an
-appearance model of a photo collection, a refiner). The reference has no counterpart. Tensors are
+appearance model of a photo collection, a refiner, a codebook of Gaussian attributes). The reference has no counterpart. Tensors are
 float32, bfloat16 or float16 on the GPU; outputs and gradients are written into the tensors given,
 on the current stream, without synchronisation. temp is scratch of the size its function's
 *_temp() gives: with None a call allocates its own.
@@ -14,9 +15,12 @@ import ctypes as C
 import torch
 
 from . import abi
-from .core import check, dptr, lib, stream_ptr
+from .core import _handle, check, dptr, lib, stream_ptr
 
 DTYPES = {torch.float32: abi.TDGS_F32, torch.bfloat16: abi.TDGS_BF16, torch.float16: abi.TDGS_F16}
+
+ACTIVATIONS = {"identity": abi.TDGS_ACT_IDENTITY, "silu": abi.TDGS_ACT_SILU, "gelu": abi.TDGS_ACT_GELU,
+               "relu": abi.TDGS_ACT_RELU}
 
 
 def _require(cond, message):
@@ -85,18 +89,14 @@ def _temp(temp, like):
     _require(temp.dtype == torch.uint8 and temp.is_contiguous(), "temp must be contiguous uint8")
 
 
-def _own_temp(a, grad, like):
-    n = lib().tdgs_cross_attention_temp_bytes(C.byref(a), grad)
-    temp = torch.empty(max(n, 1), dtype=torch.uint8, device=like.device)
-    a.temp, a.temp_bytes = temp.data_ptr(), temp.numel()
-    return temp
+def _new_temp(size, a, grad, like):
+    return torch.empty(max(size(C.byref(a), int(grad)), 1), dtype=torch.uint8, device=like.device)
 
 
 def cross_attention_temp(q, k, grad=False):
     """Scratch for cross_attention_ (with grad also cross_attention_grad_) on tensors of these sizes."""
     a = _attention(q, k, None, None, None, None, None, None, None)
-    n = lib().tdgs_cross_attention_temp_bytes(C.byref(a), int(grad))
-    return torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+    return _new_temp(lib().tdgs_cross_attention_temp_bytes, a, grad, q)
 
 
 def cross_attention_(out, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None, lse=None, temp=None):
@@ -111,7 +111,8 @@ def cross_attention_(out, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None,
     receives the logarithm of each softmax's sum, which the gradient needs."""
     a = _attention(q, k, v, out, lse, scale, kv_lengths, kv_mask, temp)
     if temp is None:
-        temp = _own_temp(a, 0, q)
+        temp = _new_temp(lib().tdgs_cross_attention_temp_bytes, a, False, q)
+        a.temp, a.temp_bytes = temp.data_ptr(), temp.numel()
     check(lib().tdgs_cross_attention(stream_ptr(q.device), C.byref(a)))
     return out
 
@@ -123,7 +124,8 @@ def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv
     a = _attention(q, k, v, out, lse, scale, kv_lengths, kv_mask, temp)
     _require(lse is not None, "the gradient needs the forward call's lse")
     if temp is None:
-        temp = _own_temp(a, 1, q)
+        temp = _new_temp(lib().tdgs_cross_attention_temp_bytes, a, True, q)
+        a.temp, a.temp_bytes = temp.data_ptr(), temp.numel()
     g = abi.AttentionGradsC()
     g.dout = _heads(dout, "dout", tuple(q.shape), q)
     g.dq = _heads(dq, "dq", tuple(q.shape), q)
@@ -131,3 +133,164 @@ def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv
     g.dv = _heads(dv, "dv", tuple(k.shape), q)
     check(lib().tdgs_cross_attention_grad(stream_ptr(q.device), C.byref(a), C.byref(g)))
     return dq, dk, dv
+
+
+# ------------------------------------------------------------------------------------
+# Group norm with an activation
+# ------------------------------------------------------------------------------------
+
+def _pixels(t, name, like):
+    """The tdgs_pixels of a (n, .., channels) tensor whose middle dimensions are evenly strided."""
+    _tensor(t, name, like)
+    _require(t.dtype == like.dtype, f"{name} is {t.dtype}, not {like.dtype}")
+    _require(t.shape == like.shape, f"{name} has shape {tuple(t.shape)}, not {tuple(like.shape)}")
+    s, n = t.stride(), t.shape
+    _require(s[-1] == 1 or n[-1] <= 1, f"the channels of {name} must be contiguous")
+    step, count = 0, 1
+    for i in range(t.dim() - 2, 0, -1):
+        if n[i] > 1:
+            _require(count == 1 or s[i] == step * count, f"the pixels of {name} must be evenly strided")
+            if count == 1:
+                step = s[i]
+            count *= n[i]
+    return abi.PixelsC(t.data_ptr(), s[0], step if count > 1 else n[-1])
+
+
+def _norm(x, out, groups, weight, bias, eps, activation, stats, temp):
+    _tensor(x, "x", x)
+    _require(x.dtype in DTYPES, f"x is {x.dtype}: float32, bfloat16 and float16 are supported")
+    _require(x.dim() >= 2, "x must be (n, .., channels)")
+    _require(activation in ACTIVATIONS, f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
+    a = abi.NormC()
+    n, c = x.shape[0], x.shape[-1]
+    a.dtype = a.param_dtype = DTYPES[x.dtype]
+    a.n, a.channels, a.groups, a.activation, a.eps = n, c, groups, ACTIVATIONS[activation], eps
+    a.pixels = x.numel() // (n * c) if n * c else 0
+    a.x = _pixels(x, "x", x)
+    if out is not None:
+        a.out = _pixels(out, "out", x)
+    params = [p for p in (weight, bias) if p is not None]
+    for p in params:
+        _param(p, "weight and bias", x, params[0].dtype)
+    if params:
+        a.param_dtype = DTYPES[params[0].dtype]
+    a.weight, a.bias = dptr(weight), dptr(bias)
+    if stats is not None:
+        _tensor(stats, "stats", x)
+        _require(stats.dtype == torch.float32 and tuple(stats.shape) == (n, groups, 2) and stats.is_contiguous(),
+                 f"stats must be contiguous float32, ({n}, {groups}, 2)")
+        a.stats = stats.data_ptr()
+    if temp is not None:
+        _temp(temp, x)
+        a.temp, a.temp_bytes = temp.data_ptr(), temp.numel()
+    return a
+
+
+def _param(p, name, x, dtype):
+    _tensor(p, name, x)
+    _require(p.dtype == dtype and dtype in (torch.float32, x.dtype),
+             f"{name} must be of one type, float32 or {x.dtype}")
+    _require(tuple(p.shape) == (x.shape[-1],) and p.is_contiguous(), f"{name} must be {x.shape[-1]} contiguous values")
+
+
+def group_norm_temp(x, groups, grad=False):
+    """Scratch for group_norm_ (with grad also group_norm_grad_) on images of this size."""
+    a = _norm(x, None, groups, None, None, 0.0, "identity", None, None)
+    return _new_temp(lib().tdgs_group_norm_temp_bytes, a, grad, x)
+
+
+def group_norm_(out, x, groups, weight=None, bias=None, *, eps=1e-5, activation="silu", stats=None, temp=None):
+    """out = act(group norm of x * weight + bias), channels last (tdgs_group_norm).
+
+    x and out are (n, .., channels): the dimensions between are the pixels, evenly strided, the
+    channels contiguous; (width, height, channels) images as they are rendered, with a leading dimension. Mean and
+    variance are taken per image and group of channels / groups neighbouring channels. weight and bias are
+    float32 or of x's type; activation is identity, silu, gelu or relu. stats (n, groups, 2; float32),
+    where given, receives mean and 1 / deviation, which the gradient needs. out may be x."""
+    a = _norm(x, out, groups, weight, bias, eps, activation, stats, temp)
+    if temp is None:
+        temp = _new_temp(lib().tdgs_group_norm_temp_bytes, a, False, x)
+        a.temp, a.temp_bytes = temp.data_ptr(), temp.numel()
+    check(lib().tdgs_group_norm(stream_ptr(x.device), C.byref(a)))
+    return out
+
+
+def group_norm_grad_(dx, dweight, dbias, dout, x, stats, groups, weight=None, bias=None, *, activation="silu",
+                     temp=None):
+    """The gradients of sum(dout * out) for group_norm_'s operands (tdgs_group_norm_grad), from its stats.
+    dweight and dbias (of weight's and bias's type, float32 without them) may be None; dx may be dout."""
+    _require(stats is not None, "the gradient needs the forward call's stats")
+    a = _norm(x, None, groups, weight, bias, 0.0, activation, stats, temp)
+    param = next((p.dtype for p in (weight, bias) if p is not None), torch.float32)
+    a.param_dtype = DTYPES[param]
+    g = abi.NormGradsC(_pixels(dout, "dout", x), _pixels(dx, "dx", x))
+    for p, name in ((dweight, "dweight"), (dbias, "dbias")):
+        if p is not None:
+            _param(p, name, x, param)
+    g.dweight, g.dbias = dptr(dweight), dptr(dbias)
+    if temp is None:
+        temp = _new_temp(lib().tdgs_group_norm_temp_bytes, a, True, x)
+        a.temp, a.temp_bytes = temp.data_ptr(), temp.numel()
+    check(lib().tdgs_group_norm_grad(stream_ptr(x.device), C.byref(a), C.byref(g)))
+    return dx, dweight, dbias
+
+
+# ------------------------------------------------------------------------------------
+# Embedding
+# ------------------------------------------------------------------------------------
+
+def _tokens(tokens, like):
+    _tensor(tokens, "tokens", like)
+    _require(tokens.dtype in (torch.int32, torch.int64) and tokens.is_contiguous(),
+             "tokens must be contiguous int32 or int64")
+    return tokens.element_size()
+
+
+def _rows(t, name, rows, dim, like):
+    """(pointer, row stride) of a tensor of `rows` rows of dim contiguous elements."""
+    _tensor(t, name, like)
+    _require(t.dtype == like.dtype and t.dtype in DTYPES, f"{name} is {t.dtype}: one of float32, bfloat16 and float16")
+    _require(t.dim() >= 2 and t.shape[-1] == dim and t.numel() == rows * dim,
+             f"{name} has shape {tuple(t.shape)}, not {rows} rows of {dim}")
+    if t.dim() > 2:
+        _require(t.is_contiguous(), f"{name} must be contiguous, or two-dimensional")
+        return t.data_ptr(), dim
+    _require(t.stride(1) == 1 or dim <= 1, f"the rows of {name} must be contiguous")
+    return t.data_ptr(), t.stride(0) if rows > 1 else dim
+
+
+def embedding_lookup_(out, table, tokens, *, scale=1.0, ctx=None):
+    """out[i] = scale table[tokens[i]] (tdgs_embedding_lookup). table is (vocab, dim), tokens int32 or int64
+    of any shape, out their shape with dim behind. A token outside the table gives a row of zeros and an
+    error at the next ctx_check of the context (by default the device's)."""
+    size = _tokens(tokens, table)
+    _require(table.dim() == 2, "table must be (vocab, dim)")
+    vocab, dim = table.shape
+    t, ts = _rows(table, "table", vocab, dim, table)
+    o, os = _rows(out, "out", tokens.numel(), dim, table)
+    check(lib().tdgs_embedding_lookup(_handle(ctx, table.device.index), stream_ptr(table.device), DTYPES[table.dtype], t,
+                                      ts, vocab, dim, tokens.data_ptr(), size, tokens.numel(), scale, o, os))
+    return out
+
+
+def embedding_temp(table, tokens):
+    """Scratch for embedding_grad_ with a table and tokens of these sizes."""
+    n = lib().tdgs_embedding_grad_temp_bytes(tokens.numel(), table.shape[0], table.shape[1])
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=table.device)
+
+
+def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None, ctx=None):
+    """dtable[v] = scale times the sum of the dout rows whose token is v, in 32 bits and in the tokens'
+    order (tdgs_embedding_grad); every row is written. The token `padding` gives no gradient."""
+    size = _tokens(tokens, dtable)
+    _require(dtable.dim() == 2, "dtable must be (vocab, dim)")
+    vocab, dim = dtable.shape
+    t, ts = _rows(dtable, "dtable", vocab, dim, dtable)
+    d, ds = _rows(dout, "dout", tokens.numel(), dim, dtable)
+    if temp is None:
+        temp = embedding_temp(dtable, tokens)
+    _temp(temp, dtable)
+    check(lib().tdgs_embedding_grad(_handle(ctx, dtable.device.index), stream_ptr(dtable.device), DTYPES[dtable.dtype], d,
+                                    ds, tokens.data_ptr(), size, tokens.numel(), -1 if padding is None else padding,
+                                    scale, t, ts, vocab, dim, temp.data_ptr(), temp.numel()))
+    return dtable
