@@ -185,6 +185,7 @@ def test_refusals(gpu):
     table = torch.zeros((20, 8), device="cuda")
     tokens = torch.zeros((5,), dtype=torch.int64, device="cuda")
     out = torch.empty((5, 8), device="cuda")
+    many = torch.zeros((5000,), dtype=torch.int64, device="cuda")
     decoder.embedding_lookup_(out, table, tokens)
     for bad in (
         lambda: decoder.embedding_lookup_(out[:4], table, tokens),
@@ -202,7 +203,8 @@ def test_refusals(gpu):
     for bad in (
         lambda: decoder.embedding_lookup_(out[:1].expand(5, 8), table, tokens),
         lambda: decoder.embedding_grad_(table[:1].expand(20, 8), out, tokens),
-        lambda: decoder.embedding_grad_(table, out, tokens, temp=torch.empty(5, dtype=torch.uint8, device="cuda")),
+        lambda: decoder.embedding_grad_(table, torch.zeros((5000, 8), device="cuda"), many,
+                                        temp=torch.empty(5, dtype=torch.uint8, device="cuda")),
     ):
         with pytest.raises(core.TdgsError):
             bad()

@@ -256,6 +256,7 @@ def test_graph_replays(gpu):
 def test_refusals(gpu):
     x = torch.zeros((2, 10, 16), device="cuda")
     out, stats, w = torch.empty_like(x), torch.zeros((2, 4, 2), device="cuda"), torch.zeros(16, device="cuda")
+    large = torch.zeros((2, 100000, 16), device="cuda")
     decoder.group_norm_(out, x, 4, w, w, stats=stats)
     for bad in (
         lambda: decoder.group_norm_(out[:, :5], x, 4),
@@ -279,7 +280,7 @@ def test_refusals(gpu):
         lambda: decoder.group_norm_(out, x, 4, eps=-1.0),
         lambda: decoder.group_norm_(out, x, 4, eps=math.nan),
         lambda: decoder.group_norm_(out[:1].expand(2, 10, 16), x, 4),
-        lambda: decoder.group_norm_(out, x, 4, temp=torch.empty(8, dtype=torch.uint8, device="cuda")),
+        lambda: decoder.group_norm_(torch.empty_like(large), large, 4, temp=torch.empty(8, dtype=torch.uint8, device="cuda")),
     ):
         with pytest.raises(core.TdgsError):
             bad()

@@ -2,9 +2,11 @@
 //
 // The gradient adds up the rows of dout that hold the same token. The tokens are sorted (stably, by the
 // radix sort of sort.hpp, on the bits the table's size needs) with their positions, so that a
-// token's rows follow each other; runs of kEmRows sorted positions are summed in registers by a few lanes each,
-// and a token whose rows lie in several runs is joined afterwards from their partial sums, in order. No
-// float is added atomically: the result does not depend on which workgroup runs first.
+// token's rows follow each other. A workgroup takes a block of sorted positions, a group of lanes (as many as a row
+// has 16-byte vectors) each a run of it, summing in registers; tokens that span runs are joined in LDS,
+// tokens that span blocks afterwards from the blocks' partial sums, in order. No float is added
+// atomically: the result does not depend on which workgroup runs first. A few tokens (kEmFew) take one
+// launch instead: every workgroup picks, and sorts, those of its own rows of the table.
 #include "internal.hpp"
 #include "elem.hpp"
 #include "sort.hpp"
@@ -12,20 +14,23 @@
 namespace tdgs {
 
 constexpr int kEmThreads = 256;
-constexpr int kEmRows = 32;   // sorted positions per run
+constexpr int kEmBlock = 2048;   // the most sorted positions of a workgroup
+constexpr int kEmRun = 32;       // and of one of its runs
+constexpr int kEmFew = 1024;     // tokens up to which one launch is taken
 
 struct EmArgs {
     const void *table, *dout, *tokens;
     void *out, *dtable;
-    int64_t table_stride, out_stride, dout_stride, dtable_stride, n, vocab, padding, runs;
+    int64_t table_stride, out_stride, dout_stride, dtable_stride, n, vocab, padding, blocks;
     const uint32_t* keys;    // sorted tokens; vocab where there is nothing to add
     const int32_t* order;    // their positions
     uint8_t* present;        // whether a token occurs
-    float* part;             // 2 rows per run: of the token it begins within, of the token it ends within
-    int32_t *list, *count;   // runs that a token starts in and goes on past; their number
+    float* part;             // 2 rows per block: of the token it begins within, of the token it ends within
+    int32_t *list, *count;   // blocks that a token starts in and goes on past; their number
     uint32_t* err;
     float scale;
     int32_t dim, vectors, lanes;   // elements, vectors and lanes per row
+    int32_t run, rows;             // positions per run; table rows per workgroup (one launch)
     bool tokens64;
 };
 
@@ -97,72 +102,136 @@ static __global__ __launch_bounds__(kEmThreads) void k_embed_keys(EmArgs a, uint
     values[i] = (int32_t)i;
 }
 
-// The first workgroups: a few lanes per run of sorted positions, adding its rows token by token; the
-// others: rows of the table that no token names become zero.
+// Sums a block of sorted positions, `count` of them from LDS (their tokens, and rows of dout): group g of
+// the workgroup's lane groups takes `run` of them from g * run on. A token's sum goes to its row of the table;
+// that of the token `before` the block, and of one that goes on `after` it, to part (row 0 and row 1).
+// Every thread of the workgroup calls it. Returns whether a token starts here and goes on.
 template <class T, int VW>
-__global__ __launch_bounds__(kEmThreads) void k_embed_sums(EmArgs a, int run_blocks) {
-    const int lane = (int)__lane_id(), wave = threadIdx.x / kWave;
-    const int per_wave = kWave / a.lanes, sub = lane / a.lanes;
-    const int vec = blockIdx.y * kWave + lane % a.lanes, e = vec * VW;
-    const bool on = sub < per_wave && vec < a.vectors;
-    if ((int)blockIdx.x >= run_blocks) {
-        const int64_t rows = (int64_t)(gridDim.x - run_blocks) * (kEmThreads / kWave) * per_wave;
-        EmVec<T, VW> z;
-        z.zero();
-        if (on)
-            for (int64_t v = ((int64_t)(blockIdx.x - run_blocks) * (kEmThreads / kWave) + wave) * per_wave + sub; v < a.vocab;
-                 v += rows)
-                if (!a.present[v]) z.store((T*)a.dtable + v * a.dtable_stride + e, 0.0f);
-        return;
-    }
-    const int64_t run = ((int64_t)blockIdx.x * (kEmThreads / kWave) + wave) * per_wave + sub;
-    if (!on || run >= a.runs) return;
-    const int64_t i0 = run * kEmRows, i1 = min(a.n, i0 + kEmRows);
+__device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key, const int32_t* s_row, int count, int run,
+                                         uint32_t before, uint32_t after, float* part, float* s_head, float* s_tail,
+                                         uint32_t* s_flag) {
+    const int groups = kEmThreads / a.lanes, sub = (int)threadIdx.x / a.lanes, col = (int)threadIdx.x % a.lanes;
+    const int vec = blockIdx.y * kWave + col, e = vec * VW;
+    const bool on = sub < groups && vec < a.vectors;
     const uint32_t none = (uint32_t)a.vocab;
-    const uint32_t before = i0 > 0 ? a.keys[i0 - 1] : none, after = i1 < a.n ? a.keys[i1] : none;
-    EmVec<T, VW> sum;
-    sum.zero();
-    uint32_t cur = a.keys[i0];
-    bool first = cur == before;   // the run begins within a token
-    auto flush = [&](bool last) {
-        if (cur == none) return;
-        if (first || (last && cur == after)) {
-            float* const p = a.part + (2 * run + (first ? 0 : 1)) * ((int64_t)a.vectors * VW) + e;
+    const int i0 = sub * run, i1 = min(count, i0 + run);
+    constexpr uint32_t kHead = 1u, kThrough = 2u, kTail = 4u;
+    auto keep = [&](float* s, const EmVec<T, VW>& v) {
 #pragma unroll
-            for (int i = 0; i < VW; ++i) p[i] = sum.f[i];
-            if (!first && vec == 0) a.list[atomicAdd(a.count, 1)] = (int32_t)run;
-        } else {
-            sum.store((T*)a.dtable + (int64_t)cur * a.dtable_stride + e, a.scale);
-        }
+        for (int i = 0; i < VW; ++i) s[i * kEmThreads + threadIdx.x] = v.f[i];
     };
-    constexpr int U = 4;
-    for (int64_t i = i0; i < i1; i += U) {
-        EmVec<T, VW> v[U];
-        uint32_t key[U];
+    if (on && i0 < i1) {
+        EmVec<T, VW> sum;
+        sum.zero();
+        uint32_t cur = s_key[i0], flag = 0;
+        bool first = cur == (i0 > 0 ? s_key[i0 - 1] : before);
+        const uint32_t next = i1 < count ? s_key[i1] : after;
+        auto flush = [&](bool last) {
+            if (cur == none) return;
+            const bool on_past = last && cur == next;
+            if (first) {
+                keep(s_head, sum);
+                flag |= kHead | (on_past ? kThrough : 0u);
+            } else if (on_past) {
+                keep(s_tail, sum);
+                flag |= kTail;
+            } else {
+                sum.store((T*)a.dtable + (int64_t)cur * a.dtable_stride + e, a.scale);
+            }
+        };
+        constexpr int U = VW == 1 ? 8 : 4;
+        for (int i = i0; i < i1; i += U) {
+            EmVec<T, VW> v[U];
+            uint32_t key[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = i + u < i1;
-            key[u] = in ? a.keys[i + u] : none;
-            v[u].zero();
-            if (key[u] != none) v[u].load((const T*)a.dout + (int64_t)a.order[i + u] * a.dout_stride + e);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i + u >= i1) break;
-            if (key[u] != cur) {
-                flush(false);
-                cur = key[u];
-                first = false;
-                sum.zero();
+            for (int u = 0; u < U; ++u) {
+                key[u] = i + u < i1 ? s_key[i + u] : none;
+                v[u].zero();
+                if (key[u] != none) v[u].load((const T*)a.dout + (int64_t)s_row[i + u] * a.dout_stride + e);
             }
 #pragma unroll
-            for (int k = 0; k < VW; ++k) sum.f[k] += v[u].f[k];
+            for (int u = 0; u < U; ++u) {
+                if (i + u < i1 && key[u] != cur) {
+                    flush(false);
+                    cur = key[u];
+                    first = false;
+                    sum.zero();
+                }
+#pragma unroll
+                for (int k = 0; k < VW; ++k) sum.f[k] += v[u].f[k];
+            }
         }
+        flush(true);
+        if (col == 0) s_flag[sub] = flag;
+    } else if (sub < groups && col == 0) {
+        s_flag[sub] = 0;
     }
-    flush(true);
+    __syncthreads();
+    bool starts = false;
+    if (on && i0 < i1) {
+        // chains of runs: from a token's start to the run that it ends in, or the block's end
+        const uint32_t flag = s_flag[sub];
+        auto chain = [&](const float* s, bool through, bool outside) {
+            EmVec<T, VW> v;
+#pragma unroll
+            for (int i = 0; i < VW; ++i) v.f[i] = s[i * kEmThreads + threadIdx.x];
+            int g = sub + 1;
+            for (; through && g < groups && (s_flag[g] & kHead); ++g) {
+#pragma unroll
+                for (int i = 0; i < VW; ++i) v.f[i] += s_head[i * kEmThreads + g * a.lanes + col];
+                through = (s_flag[g] & kThrough) != 0;
+            }
+            const uint32_t key = s_key[i1 - 1];   // (of a tail; a head's that ends here is not stored to its row)
+            if (outside || through) {
+                float* const p = part + (outside ? 0 : (int64_t)a.vectors * VW) + e;
+#pragma unroll
+                for (int i = 0; i < VW; ++i) p[i] = v.f[i];
+                return !outside;
+            }
+            v.store((T*)a.dtable + (int64_t)key * a.dtable_stride + e, a.scale);
+            return false;
+        };
+        if (sub == 0 && (flag & kHead)) chain(s_head, (flag & kThrough) != 0, true);
+        if (flag & kTail) starts = chain(s_tail, true, false);
+    }
+    return starts;
 }
 
-// A workgroup per token that spans runs: the end of the run it starts in, then the following runs'
+// The first workgroups: a block of sorted positions each; the others: rows of the table that no token
+// names become zero.
+template <class T, int VW>
+__global__ __launch_bounds__(kEmThreads) void k_embed_sums(EmArgs a) {
+    __shared__ uint32_t s_key[kEmBlock];
+    __shared__ int32_t s_row[kEmBlock];
+    __shared__ float s_head[kEmThreads * VW];
+    __shared__ float s_tail[kEmThreads * VW];
+    __shared__ uint32_t s_flag[kEmThreads];
+    const int groups = kEmThreads / a.lanes;
+    const uint32_t none = (uint32_t)a.vocab;
+    if ((int64_t)blockIdx.x >= a.blocks) {
+        const int sub = (int)threadIdx.x / a.lanes, vec = blockIdx.y * kWave + (int)threadIdx.x % a.lanes;
+        if (sub >= groups || vec >= a.vectors) return;
+        const int64_t step = (gridDim.x - a.blocks) * groups;
+        EmVec<T, VW> z;
+        z.zero();
+        for (int64_t v = (blockIdx.x - a.blocks) * groups + sub; v < a.vocab; v += step)
+            if (!a.present[v]) z.store((T*)a.dtable + v * a.dtable_stride + vec * VW, 0.0f);
+        return;
+    }
+    const int size = groups * a.run;
+    const int64_t i0 = (int64_t)blockIdx.x * size, i1 = min(a.n, i0 + size);
+    for (int i = threadIdx.x; i < (int)(i1 - i0); i += kEmThreads) {
+        s_key[i] = a.keys[i0 + i];
+        s_row[i] = a.order[i0 + i];
+    }
+    __syncthreads();
+    const bool starts = em_block<T, VW>(a, s_key, s_row, (int)(i1 - i0), a.run, i0 > 0 ? a.keys[i0 - 1] : none,
+                                        i1 < a.n ? a.keys[i1] : none, a.part + 2 * blockIdx.x * ((int64_t)a.vectors * VW),
+                                        s_head, s_tail, s_flag);
+    if (starts && blockIdx.y == 0 && threadIdx.x % a.lanes == 0) a.list[atomicAdd(a.count, 1)] = (int32_t)blockIdx.x;
+}
+
+// A workgroup per token that spans blocks: the end of the block it starts in, then the following blocks'
 // beginnings, each lane group adding every so manieth, in order.
 template <class T, int VW>
 __global__ __launch_bounds__(kEmThreads) void k_embed_join(EmArgs a) {
@@ -171,18 +240,18 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_join(EmArgs a) {
     const int groups = kEmThreads / a.lanes, sub = threadIdx.x / a.lanes;
     const int vec = blockIdx.y * kWave + (int)threadIdx.x % a.lanes, e = vec * VW;
     const bool on = sub < groups && vec < a.vectors;
-    const int64_t pitch = (int64_t)a.vectors * VW;
+    const int64_t pitch = (int64_t)a.vectors * VW, size = (int64_t)groups * a.run;
     const int count = *a.count;
     for (int item = blockIdx.x; item < count; item += gridDim.x) {
-        const int64_t run = a.list[item];
-        const uint32_t key = a.keys[(run + 1) * kEmRows];   // (goes on there: the list says so)
-        // the last run that begins with the token
-        int64_t last = run;
+        const int64_t block = a.list[item];
+        const uint32_t key = a.keys[(block + 1) * size];   // (goes on there: the list says so)
+        // the last block that begins with the token
+        int64_t last = block;
         for (bool more = true; more; ) {
             if (threadIdx.x == 0) s_last = kEmThreads;
             __syncthreads();
             const int64_t r = last + 1 + threadIdx.x;
-            if (r >= a.runs || a.keys[r * kEmRows] != key) atomicMin(&s_last, (int)threadIdx.x);
+            if (r >= a.blocks || a.keys[r * size] != key) atomicMin(&s_last, (int)threadIdx.x);
             __syncthreads();
             last += s_last;
             more = s_last == kEmThreads;
@@ -191,24 +260,89 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_join(EmArgs a) {
         float sum[VW];
 #pragma unroll
         for (int i = 0; i < VW; ++i) sum[i] = 0.0f;
-        if (on)
-            for (int64_t r = run + sub; r <= last; r += groups) {
-                const float* const p = a.part + (2 * r + (r == run ? 1 : 0)) * pitch + e;
+        if (on) {
+#pragma unroll 4
+            for (int64_t r = block + sub; r <= last; r += groups) {
+                const float* const p = a.part + (2 * r + (r == block ? 1 : 0)) * pitch + e;
 #pragma unroll
                 for (int i = 0; i < VW; ++i) sum[i] += p[i];
             }
+        }
 #pragma unroll
-        for (int i = 0; i < VW; ++i) s_sum[threadIdx.x * VW + i] = sum[i];
+        for (int i = 0; i < VW; ++i) s_sum[i * kEmThreads + threadIdx.x] = sum[i];
         __syncthreads();
         if (on && sub == 0) {
             EmVec<T, VW> v;
             v.zero();
-            for (int g = 0; g < groups && run + g <= last; ++g)
+            for (int g = 0; g < groups && block + g <= last; ++g)
 #pragma unroll
-                for (int i = 0; i < VW; ++i) v.f[i] += s_sum[(g * a.lanes + (int)threadIdx.x) * VW + i];
+                for (int i = 0; i < VW; ++i) v.f[i] += s_sum[i * kEmThreads + g * a.lanes + (int)threadIdx.x];
             v.store((T*)a.dtable + (int64_t)key * a.dtable_stride + e, a.scale);
         }
         __syncthreads();
+    }
+}
+
+// One launch for a few tokens: workgroup x takes a.rows rows of the table, picks the tokens that name them, ranks
+// them (by token, then position), sums, and writes zeros where no token does.
+template <class T, int VW>
+__global__ __launch_bounds__(kEmThreads) void k_embed_few(EmArgs a) {
+    __shared__ uint32_t s_tok[kEmFew], s_key[kEmFew];
+    __shared__ int32_t s_at[kEmFew], s_row[kEmFew];
+    __shared__ float s_head[kEmThreads * VW];
+    __shared__ float s_tail[kEmThreads * VW];
+    __shared__ uint32_t s_flag[kEmThreads];
+    __shared__ int s_wave[kEmThreads / kWave], s_count;
+    const int64_t v0 = (int64_t)blockIdx.x * a.rows, v1 = min(a.vocab, v0 + a.rows);
+    const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, n = (int)a.n;
+    if (threadIdx.x == 0) s_count = 0;
+    for (int i0 = 0; i0 < n; i0 += kEmThreads) {
+        const int i = i0 + threadIdx.x;
+        int64_t tok = -1;
+        if (i < n) {
+            tok = em_token(a, i);
+            if ((tok < 0 || tok >= a.vocab) && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, kErrTokenRange);
+        }
+        const bool mine = i < n && tok >= v0 && tok < v1 && tok != a.padding;
+        const uint64_t votes = __ballot(mine);
+        if (lane == 0) s_wave[wave] = __popcll(votes);
+        __syncthreads();
+        int at = s_count;
+        for (int w = 0; w < wave; ++w) at += s_wave[w];
+        at += __popcll(votes & lanemask_lt());
+        if (mine) {
+            s_tok[at] = (uint32_t)tok;
+            s_at[at] = i;
+        }
+        __syncthreads();
+        if (threadIdx.x == kEmThreads - 1) s_count = at + (mine ? 1 : 0);
+        __syncthreads();
+    }
+    __syncthreads();
+    const int count = s_count;
+    for (int i = threadIdx.x; i < count; i += kEmThreads) {
+        const uint32_t tok = s_tok[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += (s_tok[j] < tok || (s_tok[j] == tok && j < i)) ? 1 : 0;
+        s_key[rank] = tok;
+        s_row[rank] = s_at[i];
+    }
+    __syncthreads();
+    const int groups = kEmThreads / a.lanes, sub = (int)threadIdx.x / a.lanes;
+    const int vec = blockIdx.y * kWave + (int)threadIdx.x % a.lanes;
+    const uint32_t none = (uint32_t)a.vocab;
+    em_block<T, VW>(a, s_key, s_row, count, (count + groups - 1) / groups, none, none, nullptr, s_head, s_tail, s_flag);
+    if (sub >= groups || vec >= a.vectors) return;
+    EmVec<T, VW> z;
+    z.zero();
+    for (int64_t v = v0 + sub; v < v1; v += groups) {
+        int lo = 0, hi = count;   // the first rank whose token is v or above
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (s_key[mid] < (uint32_t)v) lo = mid + 1;
+            else hi = mid;
+        }
+        if (lo == count || s_key[lo] != (uint32_t)v) z.store((T*)a.dtable + v * a.dtable_stride + vec * VW, 0.0f);
     }
 }
 
@@ -220,16 +354,31 @@ static int em_bits(int64_t vocab) {
     return b;
 }
 
-static int64_t em_runs(int64_t n) { return ceil_div(n, kEmRows); }
+// Positions per run: kEmRun, fewer where a workgroup would take more than kEmBlock, or where there would
+// be less than two workgroups per CU.
+static int em_run(int64_t n, int groups) {
+    int64_t run = n / (512 * groups);
+    if (run > kEmRun) run = kEmRun;
+    if (run > kEmBlock / groups) run = kEmBlock / groups;
+    return (int)(run > 4 ? run : 4);
+}
+
+static int em_lanes(int vectors) { return vectors < kWave ? vectors : kWave; }
 
 struct EmPlan {
-    int64_t runs, group_words, clear_words;
+    int vectors, lanes, run;
+    int64_t blocks, group_words, clear_words;
     size_t sort_bytes, bytes;
 };
 
-static EmPlan em_plan(int64_t n, int64_t vocab, int32_t dim) {
-    EmPlan p;
-    p.runs = em_runs(n);
+static EmPlan em_plan(int64_t n, int64_t vocab, int32_t dim, int vw) {
+    EmPlan p = {};
+    p.vectors = dim / vw;
+    p.lanes = em_lanes(p.vectors);
+    if (n <= kEmFew) return p;
+    const int groups = kEmThreads / p.lanes;
+    p.run = em_run(n, groups);
+    p.blocks = ceil_div(n, (int64_t)groups * p.run);
     p.sort_bytes = radix_temp_bytes(n);
     p.group_words = radix_tiles<uint32_t>(n) <= RsTile<uint32_t>::kGroupedTiles
                         ? radix_group_words<uint32_t>(n, 0, em_bits(vocab)) : 0;
@@ -241,8 +390,8 @@ static EmPlan em_plan(int64_t n, int64_t vocab, int32_t dim) {
         s.take<int32_t>(n);
     }
     s.take<char>((int64_t)p.sort_bytes);
-    s.take<int32_t>(p.runs);
-    s.take<float>(2 * p.runs * dim);
+    s.take<int32_t>(p.blocks);
+    s.take<float>(2 * p.blocks * dim);
     p.bytes = s.used;
     return p;
 }
@@ -321,7 +470,13 @@ int tdgs_embedding_lookup(tdgs_ctx* ctx, void* stream_, int32_t dtype, const voi
 
 size_t tdgs_embedding_grad_temp_bytes(int64_t n, int64_t vocab, int32_t dim) {
     if (em_check(TDGS_F32, 4, vocab, dim, n) != TDGS_OK) return 0;
-    return em_plan(n, vocab, dim).bytes;
+    size_t bytes = 0;   // (for whichever vector width the tensors' alignment will allow)
+    for (int vw = 1; vw <= 8; vw *= 2) {
+        if (dim % vw != 0) break;
+        const size_t b = em_plan(n, vocab, dim, vw).bytes;
+        if (b > bytes) bytes = b;
+    }
+    return bytes;
 }
 
 int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void* dout, int64_t dout_stride,
@@ -333,24 +488,12 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     TDGS_REQUIRE(n == 0 || (tokens && aligned_to(tokens, (size_t)index_bytes)), "embedding: tokens are null or misaligned");
     TDGS_TRY(em_check_rows(dout, "dout", dtype, dout_stride, dim, n, false));
     TDGS_TRY(em_check_rows(dtable, "dtable", dtype, dtable_stride, dim, vocab, true));
-    const EmPlan p = em_plan(n, vocab, dim);
-    TDGS_REQUIRE(temp && temp_bytes >= p.bytes && aligned_to(temp, 16), "embedding: scratch of %zu bytes, %zu needed",
+    const int vw = em_vw(dtype, dim, dout, dout_stride, dtable, dtable_stride);
+    const EmPlan p = em_plan(n, vocab, dim, vw);
+    TDGS_REQUIRE(p.bytes == 0 || (temp && temp_bytes >= p.bytes && aligned_to(temp, 16)), "embedding: scratch of %zu bytes, %zu needed",
                  temp ? temp_bytes : (size_t)0, p.bytes);
     hipStream_t stream = (hipStream_t)stream_;
-    Arena ar(temp, temp_bytes);
     EmArgs a = {};
-    uint32_t* const clear = ar.take<uint32_t>(p.clear_words);
-    uint32_t* k[3];
-    int32_t* v[3];
-    for (int i = 0; i < 3; ++i) {
-        k[i] = ar.take<uint32_t>(n);
-        v[i] = ar.take<int32_t>(n);
-    }
-    void* const sort_temp = ar.take<char>((int64_t)p.sort_bytes);
-    a.list = ar.take<int32_t>(p.runs);
-    a.count = (int32_t*)clear + p.group_words;
-    a.part = ar.take<float>(2 * p.runs * dim);
-    a.present = (uint8_t*)(clear + p.group_words + 1);
     a.dout = dout;
     a.dout_stride = dout_stride;
     a.tokens = tokens;
@@ -360,37 +503,58 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     a.n = n;
     a.vocab = vocab;
     a.padding = padding;
-    a.runs = p.runs;
     a.scale = scale;
     a.dim = dim;
     a.err = ctx_error_word(ctx);
-    const int vw = em_vw(dtype, dim, dout, dout_stride, dtable, dtable_stride);
-    a.vectors = dim / vw;
-    a.lanes = a.vectors < kWave ? a.vectors : kWave;
+    a.vectors = p.vectors;
+    a.lanes = p.lanes;
+    a.run = p.run;
+    a.blocks = p.blocks;
+    const int groups = kEmThreads / a.lanes;
+    const unsigned column_blocks = (unsigned)ceil_div(a.vectors, kWave);
+    if (n <= kEmFew) {
+        // a group of lanes takes a row at a time; at least four workgroups per CU where the table has the rows
+        int64_t rows = ceil_div(vocab, 1024);
+        if (rows < groups) rows = groups;
+        a.rows = (int32_t)rows;
+        return em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
+            k_embed_few<decltype(t), decltype(w)::value>
+                <<<dim3((unsigned)ceil_div(vocab, rows), column_blocks), kEmThreads, 0, stream>>>(a);
+            TDGS_LAUNCHED();
+            return TDGS_OK;
+        });
+    }
+    Arena ar(temp, temp_bytes);
+    uint32_t* const clear = ar.take<uint32_t>(p.clear_words);
+    uint32_t* k[3];
+    int32_t* v[3];
+    for (int i = 0; i < 3; ++i) {
+        k[i] = ar.take<uint32_t>(n);
+        v[i] = ar.take<int32_t>(n);
+    }
+    void* const sort_temp = ar.take<char>((int64_t)p.sort_bytes);
+    a.list = ar.take<int32_t>(p.blocks);
+    a.count = (int32_t*)clear + p.group_words;
+    a.part = ar.take<float>(2 * p.blocks * dim);
+    a.present = (uint8_t*)(clear + p.group_words + 1);
     a.keys = k[1];
     a.order = v[1];
     k_embed_clear<<<(unsigned)ceil_div(p.clear_words, kEmThreads), kEmThreads, 0, stream>>>(clear, p.clear_words);
     TDGS_LAUNCHED();
-    if (n > 0) {
-        k_embed_keys<<<(unsigned)ceil_div(n, kEmThreads), kEmThreads, 0, stream>>>(a, k[0], v[0]);
-        TDGS_LAUNCHED();
-        TDGS_TRY(radix_sort_pairs_grouped<uint32_t>(k[0], k[1], v[0], v[1], k[2], v[2], n, 0, em_bits(vocab), sort_temp,
-                                                    p.sort_bytes, p.group_words > 0 ? clear : nullptr, p.group_words,
-                                                    stream, a.err));
-    }
-    const int per_block = kEmThreads / kWave * (kWave / a.lanes);
-    const int64_t run_blocks = ceil_div(p.runs, per_block);
-    int64_t zero_blocks = ceil_div(vocab, per_block);
+    k_embed_keys<<<(unsigned)ceil_div(n, kEmThreads), kEmThreads, 0, stream>>>(a, k[0], v[0]);
+    TDGS_LAUNCHED();
+    TDGS_TRY(radix_sort_pairs_grouped<uint32_t>(k[0], k[1], v[0], v[1], k[2], v[2], n, 0, em_bits(vocab), sort_temp,
+                                                p.sort_bytes, p.group_words > 0 ? clear : nullptr, p.group_words,
+                                                stream, a.err));
+    int64_t zero_blocks = ceil_div(vocab, groups);
     if (zero_blocks > 2048) zero_blocks = 2048;
-    const unsigned column_blocks = (unsigned)ceil_div(a.vectors, kWave);
     return em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
         using T = decltype(t);
         constexpr int VW = decltype(w)::value;
-        k_embed_sums<T, VW><<<dim3((unsigned)(run_blocks + zero_blocks), column_blocks), kEmThreads, 0, stream>>>(
-            a, (int)run_blocks);
+        k_embed_sums<T, VW><<<dim3((unsigned)(p.blocks + zero_blocks), column_blocks), kEmThreads, 0, stream>>>(a);
         TDGS_LAUNCHED();
-        if (p.runs > 1) {
-            k_embed_join<T, VW><<<dim3((unsigned)(p.runs < 1024 ? p.runs : 1024), column_blocks), kEmThreads, 0, stream>>>(a);
+        if (p.blocks > 1) {
+            k_embed_join<T, VW><<<dim3((unsigned)(p.blocks < 1024 ? p.blocks : 1024), column_blocks), kEmThreads, 0, stream>>>(a);
             TDGS_LAUNCHED();
         }
         return TDGS_OK;

@@ -7,14 +7,20 @@
 //
 // Statistics are Welford's running mean and sum of squared deviations in 32 bits, per channel, and
 // are joined between threads, workgroups and a group's channels by the exact rule for two parts
-// (Chan, Golub & LeVeque 1979): M2 = M2_a + M2_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b). A sum of
-// squares minus the squared mean would lose the variance of a channel whose mean is large.
+// (Chan, Golub & LeVeque 1979) in its form for many: mean = sum n_i mean_i / n,
+// M2 = sum M2_i + n_i (mean_i - mean)^2. A sum of squares minus the squared mean would lose the variance of
+// a channel whose mean is large.
+//
+// Three launches (runs of pixels, their joining, the result), or one for images of few pixels, a
+// workgroup then taking all pixels of a few whole groups.
 #include "internal.hpp"
 #include "elem.hpp"
 
 namespace tdgs {
 
 constexpr int kGnThreads = 256;
+constexpr int kGnSmallThreads = 512;   // of a workgroup that takes whole groups, and
+constexpr int kGnSmallVectors = 64;    // the most channel vectors it takes
 
 struct GnArgs {
     const void *x, *dout, *weight, *bias;
@@ -24,6 +30,7 @@ struct GnArgs {
     float *part, *chan;
     int64_t pixels, per;                      // per: pixels per workgroup
     int32_t n, channels, groups, group_size, blocks, vectors;
+    int32_t parts;      // partial statistics per run: one per group, or per channel
     float eps;
     bool param_f32;
 };
@@ -97,34 +104,30 @@ __device__ __forceinline__ float gn_act(float z, float* slope) {
     }
 }
 
-// Joins (nb, mb, sb) into (n, m, s): counts, means, sums of squared deviations.
-__device__ __forceinline__ void gn_join(float& n, float& m, float& s, float nb, float mb, float sb) {
-    const float all = n + nb;
-    if (nb <= 0.0f) return;
-    const float d = mb - m, share = nb / all;
-    m = __builtin_fmaf(d, share, m);
-    s += sb + d * d * (n * share);
-    n = all;
-}
-
-// Where a thread of a workgroup of `vectors` channel vectors stands.
+// Where a thread of a workgroup of THREADS stands among `vectors` channel vectors.
+template <int THREADS>
 struct GnPlace {
     int cv, pl, lanes;   // channel vector, first pixel, pixels apart
     bool on;
     __device__ __forceinline__ explicit GnPlace(int vectors) {
-        lanes = kGnThreads / vectors;
+        lanes = THREADS / vectors;
         cv = (int)threadIdx.x % vectors;
         pl = (int)threadIdx.x / vectors;
         on = pl < lanes;
     }
 };
 
-// Per-channel statistics of pixels [p0, p1) of the channels from x on, joined over the workgroup: thread
-// c < vectors * VW gets channel c's mean and sum of squared deviations.
-template <class T, int VW>
+__device__ __forceinline__ float gn_segment_sum(float x, int width) {
+    for (int w = width / 2; w > 0; w >>= 1) x += __shfl_xor(x, w, kWave);
+    return x;
+}
+
+// Per-channel statistics of pixels [p0, p1) of the channels from x on, joined over the workgroup's
+// lanes: thread c < vectors * VW leaves channel c's mean and sum of squared deviations in s_mean[c], s_m2[c].
+template <class T, int VW, int THREADS>
 __device__ __forceinline__ void gn_stats(const T* __restrict__ x, int64_t xp, int64_t p0, int64_t p1, int vectors,
-                                         float* s_mean, float* s_m2, float* mean_out, float* m2_out) {
-    const GnPlace at(vectors);
+                                         float* s_mean, float* s_m2) {
+    const GnPlace<THREADS> at(vectors);
     float mean[VW], m2[VW];
 #pragma unroll
     for (int i = 0; i < VW; ++i) mean[i] = m2[i] = 0.0f;
@@ -154,65 +157,144 @@ __device__ __forceinline__ void gn_stats(const T* __restrict__ x, int64_t xp, in
             v.load(x + p * xp + at.cv * VW);
             add(v);
         }
+    }
+    // channel-major, the lanes of a channel next to each other and padded by one
+    const int pitch = at.lanes | 1;
+    if (at.on) {
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            s_mean[threadIdx.x * VW + i] = mean[i];
-            s_m2[threadIdx.x * VW + i] = m2[i];
+            s_mean[(at.cv * VW + i) * pitch + at.pl] = mean[i];
+            s_m2[(at.cv * VW + i) * pitch + at.pl] = m2[i];
         }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) {
-        float n = 0.0f, m = 0.0f, s = 0.0f;
-        for (int l = 0; l < at.lanes; ++l) {
-            const int64_t left = p1 - p0 - l;
-            const float nb = left > 0 ? (float)((left + at.lanes - 1) / at.lanes) : 0.0f;
-            gn_join(n, m, s, nb, s_mean[l * vectors * VW + c], s_m2[l * vectors * VW + c]);
+    // `width` lanes per channel, a power of two up to a wavefront; each adds every width-th entry
+    const int channels = vectors * VW;
+    int width = 1;
+    while (width < kWave && width * 2 <= at.lanes && width * 2 * channels <= THREADS) width *= 2;
+    const int64_t pixels = p1 - p0;
+    const int whole = (int)(pixels / at.lanes), extra = (int)(pixels % at.lanes);
+    const int sub = (int)threadIdx.x & (width - 1);
+    float out_m[VW], out_s[VW];
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+        const int c = (k * THREADS + (int)threadIdx.x) / width;
+        out_m[k] = out_s[k] = 0.0f;
+        if (k * THREADS / width >= channels) continue;
+        float m = 0.0f, s2 = 0.0f;
+        if (c < channels)
+            for (int l = sub; l < at.lanes; l += width)
+                m = __builtin_fmaf((float)(whole + (l < extra)), s_mean[c * pitch + l], m);
+        m = gn_segment_sum(m, width) / (float)pixels;
+        if (c < channels)
+            for (int l = sub; l < at.lanes; l += width) {
+                const float d = s_mean[c * pitch + l] - m;
+                s2 += __builtin_fmaf((float)(whole + (l < extra)) * d, d, s_m2[c * pitch + l]);
+            }
+        out_m[k] = m;
+        out_s[k] = gn_segment_sum(s2, width);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+        const int c = (k * THREADS + (int)threadIdx.x) / width;
+        if (sub == 0 && c < channels) {
+            s_mean[c] = out_m[k];
+            s_m2[c] = out_s[k];
         }
-        mean_out[c] = m;
-        m2_out[c] = s;
+    }
+    __syncthreads();
+}
+
+// The statistics of `groups` groups of `size` channels, each channel over `pixels` pixels, from the
+// channels' in LDS: f(group, mean, sum of squared deviations) by one lane each.
+template <class F>
+__device__ __forceinline__ void gn_groups(const float* s_mean, const float* s_m2, int groups, int size, float pixels,
+                                          int threads, F&& f) {
+    int width = 1;
+    while (width < kWave && width < size) width *= 2;
+    const int sub = (int)threadIdx.x & (width - 1);
+    for (int g0 = 0; g0 < groups; g0 += threads / width) {
+        const int g = g0 + (int)threadIdx.x / width;
+        float m = 0.0f, s2 = 0.0f;
+        if (g < groups)
+            for (int c = sub; c < size; c += width) m += s_mean[g * size + c];
+        m = gn_segment_sum(m, width) / (float)size;
+        if (g < groups)
+            for (int c = sub; c < size; c += width) {
+                const float d = s_mean[g * size + c] - m;
+                s2 += __builtin_fmaf(pixels * d, d, s_m2[g * size + c]);
+            }
+        s2 = gn_segment_sum(s2, width);
+        if (g < groups && sub == 0) f(g, m, s2);
     }
 }
 
-// Workgroup (b, y, n): statistics of run b of image n's pixels, channel block y.
+__device__ __forceinline__ float gn_inverse(const GnArgs& a, float m2, float count) {
+    return 1.0f / sqrtf(m2 / count + a.eps);
+}
+
+// Floats of LDS for one array of gn_stats or gn_sums: an entry per lane and channel, a channel's entries
+// padded to an odd number (by a half at most, where there are two lanes).
+template <int VW, int THREADS>
+constexpr int gn_lds() { return VW * THREADS * 3 / 2; }
+
+// Workgroup (b, y, n): statistics of run b of image n's pixels, channel block y; per group where a
+// workgroup holds all channels.
 template <class T, int VW>
 __global__ __launch_bounds__(kGnThreads) void k_norm_stats(GnArgs a) {
-    __shared__ float s_mean[kGnThreads * VW];
-    __shared__ float s_m2[kGnThreads * VW];
-    __shared__ float s_o1[kGnThreads * VW];
-    __shared__ float s_o2[kGnThreads * VW];
+    __shared__ float s_mean[gn_lds<VW, kGnThreads>()];
+    __shared__ float s_m2[gn_lds<VW, kGnThreads>()];
     const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads;
     const int vectors = min(a.vectors - v0, kGnThreads), c0 = v0 * VW;
     const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
-    gn_stats<T, VW>((const T*)a.x + n * a.xn + c0, a.xp, p0, p1, vectors, s_mean, s_m2, s_o1, s_o2);
-    __syncthreads();
-    float2* const out = (float2*)a.part + ((int64_t)n * a.blocks + b) * a.channels + c0;
-    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) out[c] = make_float2(s_o1[c], s_o2[c]);
+    gn_stats<T, VW, kGnThreads>((const T*)a.x + n * a.xn + c0, a.xp, p0, p1, vectors, s_mean, s_m2);
+    float2* const out = (float2*)a.part + ((int64_t)n * a.blocks + b) * a.parts;
+    if (a.parts == a.groups) {
+        gn_groups(s_mean, s_m2, a.groups, a.group_size, (float)(p1 - p0), kGnThreads,
+                  [&](int g, float m, float s2) { out[g] = make_float2(m, s2); });
+    } else {
+        for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) out[c0 + c] = make_float2(s_mean[c], s_m2[c]);
+    }
 }
 
-// Workgroup n * groups + g: joins the runs and the channels of a group.
+__device__ __forceinline__ float gn_block_sum(float x, float* s) {
+    for (int w = kWave / 2; w > 0; w >>= 1) x += __shfl_xor(x, w, kWave);
+    __syncthreads();
+    if (__lane_id() == 0) s[threadIdx.x / kWave] = x;
+    __syncthreads();
+    float all = 0.0f;
+    for (int w = 0; w < kGnThreads / kWave; ++w) all += s[w];
+    return all;
+}
+
+// Workgroup n * groups + g: joins the runs (and the channels, where they came by channel) of a group.
 static __global__ __launch_bounds__(kGnThreads) void k_norm_join(GnArgs a) {
-    __shared__ float s_n[kGnThreads], s_m[kGnThreads], s_s[kGnThreads];
-    const int n = blockIdx.x / a.groups, g = blockIdx.x % a.groups, t = threadIdx.x;
-    const float2* const part = (const float2*)a.part + (int64_t)n * a.blocks * a.channels + g * a.group_size;
-    float cnt = 0.0f, m = 0.0f, s = 0.0f;
-    const int64_t items = (int64_t)a.blocks * a.group_size;
-    for (int64_t i = t; i < items; i += kGnThreads) {
-        const int b = (int)(i / a.group_size), c = (int)(i % a.group_size);
-        const float2 v = part[(int64_t)b * a.channels + c];
-        gn_join(cnt, m, s, (float)(min(a.pixels, (b + 1) * a.per) - b * a.per), v.x, v.y);
-    }
-    s_n[t] = cnt;
-    s_m[t] = m;
-    s_s[t] = s;
-    for (int w = kGnThreads / 2; w > 0; w >>= 1) {
-        __syncthreads();
-        if (t < w) {
-            gn_join(s_n[t], s_m[t], s_s[t], s_n[t + w], s_m[t + w], s_s[t + w]);
+    __shared__ float s[kGnThreads / kWave];
+    const int n = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
+    const int size = a.parts == a.groups ? 1 : a.group_size;   // entries per run
+    const float2* const part = (const float2*)a.part + (int64_t)n * a.blocks * a.parts + g * size;
+    const float share = (float)(a.group_size / size);          // channels per entry
+    const int64_t items = (int64_t)a.blocks * size;
+    const float total = (float)a.pixels * (float)a.group_size;
+    auto each = [&](auto&& f) {
+#pragma unroll 4
+        for (int64_t i = threadIdx.x; i < items; i += kGnThreads) {
+            const int b = size == 1 ? (int)i : (int)(i / size), c = size == 1 ? 0 : (int)(i % size);
+            f(part[(int64_t)b * a.parts + c], share * (float)(min(a.pixels, (b + 1) * a.per) - b * a.per));
         }
-    }
-    if (t == 0) {
-        a.stats[2 * blockIdx.x] = s_m[0];
-        a.stats[2 * blockIdx.x + 1] = 1.0f / sqrtf(s_s[0] / s_n[0] + a.eps);
+    };
+    float m = 0.0f, m2 = 0.0f;
+    each([&](const float2& v, float count) { m = __builtin_fmaf(count, v.x, m); });
+    m = gn_block_sum(m, s) / total;
+    each([&](const float2& v, float count) {
+        const float d = v.x - m;
+        m2 += __builtin_fmaf(count * d, d, v.y);
+    });
+    m2 = gn_block_sum(m2, s);
+    if (threadIdx.x == 0) {
+        a.stats[2 * blockIdx.x] = m;
+        a.stats[2 * blockIdx.x + 1] = gn_inverse(a, m2, total);
     }
 }
 
@@ -220,10 +302,11 @@ static __global__ __launch_bounds__(kGnThreads) void k_norm_join(GnArgs a) {
 template <class T, int VW>
 struct GnChannels {
     float mean[VW], r[VW], w[VW], b[VW];
-    __device__ __forceinline__ void load(const GnArgs& a, const float* stats, int c0) {
+    // stats: of the groups from g0 on
+    __device__ __forceinline__ void load(const GnArgs& a, const float* stats, int c0, int g0 = 0) {
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            const int g = (c0 + i) / a.group_size;
+            const int g = (c0 + i) / a.group_size - g0;
             mean[i] = stats[2 * g];
             r[i] = stats[2 * g + 1];
             w[i] = gn_param<T>(a.weight, a.param_f32, c0 + i, 1.0f);
@@ -232,9 +315,10 @@ struct GnChannels {
     }
 };
 
-template <class T, int VW, int ACT>
+template <class T, int VW, int ACT, int THREADS>
 __device__ __forceinline__ void gn_apply(const GnArgs& a, const T* __restrict__ x, T* __restrict__ out,
-                                         const GnChannels<T, VW>& ch, int64_t p0, int64_t p1, const GnPlace& at) {
+                                         const GnChannels<T, VW>& ch, int64_t p0, int64_t p1,
+                                         const GnPlace<THREADS>& at) {
     float rw[VW];
 #pragma unroll
     for (int i = 0; i < VW; ++i) rw[i] = ch.r[i] * ch.w[i];
@@ -267,12 +351,41 @@ __device__ __forceinline__ void gn_apply(const GnArgs& a, const T* __restrict__ 
 template <class T, int VW, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_norm_apply(GnArgs a) {
     const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads, c0 = v0 * VW;
-    const GnPlace at(min(a.vectors - v0, kGnThreads));
+    const GnPlace<kGnThreads> at(min(a.vectors - v0, kGnThreads));
     if (!at.on) return;
     GnChannels<T, VW> ch;
     ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
     const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
-    gn_apply<T, VW, ACT>(a, (const T*)a.x + n * a.xn + c0, (T*)a.out + n * a.on + c0, ch, p0, p1, at);
+    gn_apply<T, VW, ACT, kGnThreads>(a, (const T*)a.x + n * a.xn + c0, (T*)a.out + n * a.on + c0, ch, p0, p1, at);
+}
+
+// Workgroup (y, n): all pixels of channel block y, whole groups of a.vectors vectors, of image n.
+template <class T, int VW, int ACT>
+__global__ __launch_bounds__(kGnSmallThreads) void k_norm_small(GnArgs a) {
+    __shared__ float s_mean[gn_lds<VW, kGnSmallThreads>()];
+    __shared__ float s_m2[gn_lds<VW, kGnSmallThreads>()];
+    __shared__ float s_stats[2 * kGnSmallVectors * VW];
+    const int n = blockIdx.y, c0 = blockIdx.x * a.vectors * VW, g0 = c0 / a.group_size;
+    const int vectors = min(a.vectors, a.channels / VW - (int)blockIdx.x * a.vectors);
+    const T* const x = (const T*)a.x + n * a.xn + c0;
+    gn_stats<T, VW, kGnSmallThreads>(x, a.xp, 0, a.pixels, vectors, s_mean, s_m2);
+    float* const stats = a.stats ? a.stats + ((int64_t)n * a.groups + g0) * 2 : nullptr;
+    gn_groups(s_mean, s_m2, vectors * VW / a.group_size, a.group_size, (float)a.pixels, kGnSmallThreads,
+              [&](int g, float m, float s2) {
+                  const float r = gn_inverse(a, s2, (float)a.pixels * (float)a.group_size);
+                  s_stats[2 * g] = m;
+                  s_stats[2 * g + 1] = r;
+                  if (stats) {
+                      stats[2 * g] = m;
+                      stats[2 * g + 1] = r;
+                  }
+              });
+    __syncthreads();
+    const GnPlace<kGnSmallThreads> at(vectors);
+    if (!at.on) return;
+    GnChannels<T, VW> ch;
+    ch.load(a, s_stats, c0 + at.cv * VW, g0);
+    gn_apply<T, VW, ACT, kGnSmallThreads>(a, x, (T*)a.out + n * a.on + c0, ch, 0, a.pixels, at);
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -290,11 +403,13 @@ __device__ __forceinline__ void gn_slope(const GnChannels<T, VW>& ch, const GnVe
     }
 }
 
-// Sums of e and e xhat over pixels [p0, p1), per channel, joined over the workgroup into o1 and o2.
-template <class T, int VW, int ACT>
+// Sums of e and e xhat over pixels [p0, p1), per channel, joined over the workgroup's lanes into
+// s_1[channel] and s_2[channel].
+template <class T, int VW, int ACT, int THREADS>
 __device__ __forceinline__ void gn_sums(const GnArgs& a, const T* __restrict__ x, const T* __restrict__ dout,
-                                        const GnChannels<T, VW>& ch, int64_t p0, int64_t p1, const GnPlace& at,
-                                        int vectors, float* s_1, float* s_2, float* o1, float* o2) {
+                                        const GnChannels<T, VW>& ch, int64_t p0, int64_t p1,
+                                        const GnPlace<THREADS>& at, int vectors, float* s_1, float* s_2) {
+    const int pitch = at.lanes | 1;
     if (at.on) {
         float s1[VW], s2[VW];
 #pragma unroll
@@ -328,81 +443,107 @@ __device__ __forceinline__ void gn_sums(const GnArgs& a, const T* __restrict__ x
         }
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
-            s_1[threadIdx.x * VW + i] = s1[i];
-            s_2[threadIdx.x * VW + i] = s2[i];
+            s_1[(at.cv * VW + i) * pitch + at.pl] = s1[i];
+            s_2[(at.cv * VW + i) * pitch + at.pl] = s2[i];
         }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) {
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int l = 0; l < at.lanes; ++l) {
-            s1 += s_1[l * vectors * VW + c];
-            s2 += s_2[l * vectors * VW + c];
-        }
-        o1[c] = s1;
-        o2[c] = s2;
+    const int channels = vectors * VW;
+    int width = 1;
+    while (width < kWave && width * 2 <= at.lanes && width * 2 * channels <= THREADS) width *= 2;
+    const int sub = (int)threadIdx.x & (width - 1);
+    float o1[VW], o2[VW];
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+        const int c = (k * THREADS + (int)threadIdx.x) / width;
+        o1[k] = o2[k] = 0.0f;
+        if (k * THREADS / width >= channels) continue;
+        if (c < channels)
+            for (int l = sub; l < at.lanes; l += width) {
+                o1[k] += s_1[c * pitch + l];
+                o2[k] += s_2[c * pitch + l];
+            }
+        o1[k] = gn_segment_sum(o1[k], width);
+        o2[k] = gn_segment_sum(o2[k], width);
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < VW; ++k) {
+        const int c = (k * THREADS + (int)threadIdx.x) / width;
+        if (sub == 0 && c < channels) {
+            s_1[c] = o1[k];
+            s_2[c] = o2[k];
+        }
+    }
+    __syncthreads();
 }
 
 template <class T, int VW, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_norm_sums(GnArgs a) {
-    __shared__ float s_1[kGnThreads * VW];
-    __shared__ float s_2[kGnThreads * VW];
-    __shared__ float s_o1[kGnThreads * VW];
-    __shared__ float s_o2[kGnThreads * VW];
+    __shared__ float s_1[gn_lds<VW, kGnThreads>()];
+    __shared__ float s_2[gn_lds<VW, kGnThreads>()];
     const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads, c0 = v0 * VW;
     const int vectors = min(a.vectors - v0, kGnThreads);
-    const GnPlace at(vectors);
+    const GnPlace<kGnThreads> at(vectors);
     GnChannels<T, VW> ch;
     ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
     const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
-    gn_sums<T, VW, ACT>(a, (const T*)a.x + n * a.xn + c0, (const T*)a.dout + n * a.dn + c0, ch, p0, p1, at, vectors, s_1,
-                        s_2, s_o1, s_o2);
-    __syncthreads();
+    gn_sums<T, VW, ACT, kGnThreads>(a, (const T*)a.x + n * a.xn + c0, (const T*)a.dout + n * a.dn + c0, ch, p0, p1, at,
+                                    vectors, s_1, s_2);
     float2* const out = (float2*)a.part + ((int64_t)n * a.blocks + b) * a.channels + c0;
-    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) out[c] = make_float2(s_o1[c], s_o2[c]);
+    for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) out[c] = make_float2(s_1[c], s_2[c]);
 }
 
-// Workgroup: 16 channels; joins the runs of each image (sums per image and channel to chan) and the images
-// (dweight, dbias).
-template <class T>
-__global__ __launch_bounds__(kGnThreads) void k_norm_sums_join(GnArgs a) {
-    __shared__ float2 s[kGnThreads];
-    const int c = blockIdx.x * 16 + (threadIdx.x & 15), lane = threadIdx.x >> 4;
-    float dw = 0.0f, db = 0.0f;
-    for (int n = 0; n < a.n; ++n) {
-        float2 v = make_float2(0.0f, 0.0f);
-        if (c < a.channels)
-            for (int b = lane; b < a.blocks; b += 16) {
-                const float2 p = ((const float2*)a.part)[((int64_t)n * a.blocks + b) * a.channels + c];
-                v.x += p.x;
-                v.y += p.y;
-            }
-        __syncthreads();
-        s[threadIdx.x] = v;
-        __syncthreads();
-        if (lane == 0 && c < a.channels) {
-            float2 sum = make_float2(0.0f, 0.0f);
-            for (int l = 0; l < 16; ++l) {
-                sum.x += s[l * 16 + threadIdx.x].x;
-                sum.y += s[l * 16 + threadIdx.x].y;
-            }
-            ((float2*)a.chan)[(int64_t)n * a.channels + c] = sum;
-            db += sum.x;
-            dw += sum.y;
+// Workgroup (y, n): 8 channels of image n, joins the runs to chan.
+static __global__ __launch_bounds__(kGnThreads) void k_norm_sums_join(GnArgs a) {
+    constexpr int C = 8, L = kGnThreads / C;
+    __shared__ float2 s[L][C + 1];
+    const int cc = threadIdx.x % C, c = blockIdx.x * C + cc, lane = threadIdx.x / C, n = blockIdx.y;
+    float2 v = make_float2(0.0f, 0.0f);
+    if (c < a.channels) {
+        const float2* const part = (const float2*)a.part + (int64_t)n * a.blocks * a.channels + c;
+#pragma unroll 4
+        for (int b = lane; b < a.blocks; b += L) {
+            const float2 p = part[(int64_t)b * a.channels];
+            v.x += p.x;
+            v.y += p.y;
         }
     }
-    if (lane == 0 && c < a.channels) {
-        if (a.dweight) gn_set_param<T>(a.dweight, a.param_f32, c, dw);
-        if (a.dbias) gn_set_param<T>(a.dbias, a.param_f32, c, db);
+    s[lane][cc] = v;
+    for (int w = L / 2; w > 0; w >>= 1) {
+        __syncthreads();
+        if (lane < w) {
+            s[lane][cc].x += s[lane + w][cc].x;
+            s[lane][cc].y += s[lane + w][cc].y;
+        }
     }
+    if (lane == 0 && c < a.channels) ((float2*)a.chan)[(int64_t)n * a.channels + c] = s[0][cc];
+}
+
+// Thread per channel: the images' sums to dbias and dweight.
+template <class T>
+__device__ __forceinline__ void gn_params(const GnArgs& a, int c) {
+    float db = 0.0f, dw = 0.0f;
+    for (int n = 0; n < a.n; ++n) {
+        const float2 v = ((const float2*)a.chan)[(int64_t)n * a.channels + c];
+        db += v.x;
+        dw += v.y;
+    }
+    if (a.dweight) gn_set_param<T>(a.dweight, a.param_f32, c, dw);
+    if (a.dbias) gn_set_param<T>(a.dbias, a.param_f32, c, db);
+}
+
+template <class T>
+__global__ __launch_bounds__(kGnThreads) void k_norm_params(GnArgs a) {
+    const int c = blockIdx.x * kGnThreads + threadIdx.x;
+    if (c < a.channels) gn_params<T>(a, c);
 }
 
 // dx of pixels [p0, p1): r (w e - m1 - xhat m2), m1 and m2 the group's means of w e and w e xhat.
-template <class T, int VW, int ACT>
+template <class T, int VW, int ACT, int THREADS>
 __device__ __forceinline__ void gn_dx(const GnArgs& a, const T* __restrict__ x, const T* __restrict__ dout,
                                       T* __restrict__ dx, const GnChannels<T, VW>& ch, const float (&m1)[VW],
-                                      const float (&m2)[VW], int64_t p0, int64_t p1, const GnPlace& at) {
+                                      const float (&m2)[VW], int64_t p0, int64_t p1, const GnPlace<THREADS>& at) {
     auto one = [&](const GnVec<T, VW>& vx, GnVec<T, VW>& vd) {
         float e[VW], xhat[VW];
         gn_slope<T, VW, ACT>(ch, vx, vd, e, xhat);
@@ -434,47 +575,97 @@ __device__ __forceinline__ void gn_dx(const GnArgs& a, const T* __restrict__ x, 
     }
 }
 
+// A group's means of w e and w e xhat, from its channels' sums, by one wavefront.
+template <class T, class Sum>
+__device__ __forceinline__ float2 gn_group_means(const GnArgs& a, int g, Sum&& sum) {
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int c = g * a.group_size + (int)__lane_id(); c < (g + 1) * a.group_size; c += kWave) {
+        const float w = gn_param<T>(a.weight, a.param_f32, c, 1.0f);
+        const float2 v = sum(c);
+        s1 = __builtin_fmaf(w, v.x, s1);
+        s2 = __builtin_fmaf(w, v.y, s2);
+    }
+    const float count = (float)a.pixels * (float)a.group_size;
+    return make_float2(gn_segment_sum(s1, kWave) / count, gn_segment_sum(s2, kWave) / count);
+}
+
+// The first workgroups also write dbias and dweight.
 template <class T, int VW, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_norm_dx(GnArgs a) {
+    __shared__ float2 s_means[kGnThreads * VW];
     const int b = blockIdx.x, n = blockIdx.z, v0 = blockIdx.y * kGnThreads, c0 = v0 * VW;
-    const GnPlace at(min(a.vectors - v0, kGnThreads));
+    const int vectors = min(a.vectors - v0, kGnThreads);
+    if (b == 0 && n == 0)
+        for (int c = threadIdx.x; c < vectors * VW; c += kGnThreads) gn_params<T>(a, c0 + c);
+    const int g0 = c0 / a.group_size, g1 = (c0 + vectors * VW - 1) / a.group_size;
+    for (int g = g0 + threadIdx.x / kWave; g <= g1; g += kGnThreads / kWave) {
+        const float2 m = gn_group_means<T>(
+            a, g, [&](int c) { return ((const float2*)a.chan)[(int64_t)n * a.channels + c]; });
+        if (__lane_id() == 0) s_means[g - g0] = m;
+    }
+    __syncthreads();
+    const GnPlace<kGnThreads> at(vectors);
     if (!at.on) return;
     GnChannels<T, VW> ch;
     ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
     float m1[VW], m2[VW];
-    const float count = (float)a.pixels * (float)a.group_size;
-    int last = -1;
 #pragma unroll
     for (int i = 0; i < VW; ++i) {
-        const int g = (c0 + at.cv * VW + i) / a.group_size;
-        if (i > 0 && g == last) {
-            m1[i] = m1[i - 1];
-            m2[i] = m2[i - 1];
-            continue;
-        }
-        last = g;
-        float s1 = 0.0f, s2 = 0.0f;
-        const float2* const chan = (const float2*)a.chan + (int64_t)n * a.channels;
-        for (int c = g * a.group_size; c < (g + 1) * a.group_size; ++c) {
-            const float w = gn_param<T>(a.weight, a.param_f32, c, 1.0f);
-            const float2 v = chan[c];
-            s1 = __builtin_fmaf(w, v.x, s1);
-            s2 = __builtin_fmaf(w, v.y, s2);
-        }
-        m1[i] = s1 / count;
-        m2[i] = s2 / count;
+        const float2 m = s_means[(c0 + at.cv * VW + i) / a.group_size - g0];
+        m1[i] = m.x;
+        m2[i] = m.y;
     }
     const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
-    gn_dx<T, VW, ACT>(a, (const T*)a.x + n * a.xn + c0, (const T*)a.dout + n * a.dn + c0, (T*)a.dx + n * a.gn + c0, ch, m1,
-                      m2, p0, p1, at);
+    gn_dx<T, VW, ACT, kGnThreads>(a, (const T*)a.x + n * a.xn + c0, (const T*)a.dout + n * a.dn + c0,
+                                  (T*)a.dx + n * a.gn + c0, ch, m1, m2, p0, p1, at);
+}
+
+// Workgroup (y, n): all pixels of channel block y of image n. dbias and dweight too for a single image;
+// otherwise the sums go to chan.
+template <class T, int VW, int ACT>
+__global__ __launch_bounds__(kGnSmallThreads) void k_norm_small_grad(GnArgs a) {
+    __shared__ float s_1[gn_lds<VW, kGnSmallThreads>()];
+    __shared__ float s_2[gn_lds<VW, kGnSmallThreads>()];
+    __shared__ float2 s_means[kGnSmallVectors * VW];
+    const int n = blockIdx.y, c0 = blockIdx.x * a.vectors * VW, g0 = c0 / a.group_size;
+    const int vectors = min(a.vectors, a.channels / VW - (int)blockIdx.x * a.vectors);
+    const GnPlace<kGnSmallThreads> at(vectors);
+    const T* const x = (const T*)a.x + n * a.xn + c0;
+    const T* const dout = (const T*)a.dout + n * a.dn + c0;
+    GnChannels<T, VW> ch;
+    ch.load(a, a.stats + (int64_t)2 * n * a.groups, c0 + at.cv * VW);
+    gn_sums<T, VW, ACT, kGnSmallThreads>(a, x, dout, ch, 0, a.pixels, at, vectors, s_1, s_2);
+    for (int c = threadIdx.x; c < vectors * VW; c += kGnSmallThreads) {
+        if (a.n > 1) {
+            ((float2*)a.chan)[(int64_t)n * a.channels + c0 + c] = make_float2(s_1[c], s_2[c]);
+        } else {
+            if (a.dweight) gn_set_param<T>(a.dweight, a.param_f32, c0 + c, s_2[c]);
+            if (a.dbias) gn_set_param<T>(a.dbias, a.param_f32, c0 + c, s_1[c]);
+        }
+    }
+    for (int g = g0 + threadIdx.x / kWave; g * a.group_size < c0 + vectors * VW; g += kGnSmallThreads / kWave) {
+        const float2 m = gn_group_means<T>(a, g, [&](int c) { return make_float2(s_1[c - c0], s_2[c - c0]); });
+        if (__lane_id() == 0) s_means[g - g0] = m;
+    }
+    __syncthreads();
+    if (!at.on) return;
+    float m1[VW], m2[VW];
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+        const float2 m = s_means[(c0 + at.cv * VW + i) / a.group_size - g0];
+        m1[i] = m.x;
+        m2[i] = m.y;
+    }
+    gn_dx<T, VW, ACT, kGnSmallThreads>(a, x, dout, (T*)a.dx + n * a.gn + c0, ch, m1, m2, 0, a.pixels, at);
 }
 
 // ---- host ----------------------------------------------------------------------------------
 
 struct GnPlan {
-    int vw, vectors, blocks;
+    int vw, vectors, blocks, parts;
     int64_t per;
-    size_t stats_bytes, part_bytes, chan_bytes;
+    bool small;            // one launch, a workgroup per `vectors` vectors of whole groups
+    size_t stats_bytes, chan_bytes;
     size_t forward_bytes, grad_bytes;
 };
 
@@ -482,23 +673,42 @@ struct GnPlan {
 // as much as they are many.
 constexpr int64_t kGnWorkgroups = 1024;
 constexpr int64_t kGnPixels = 8;
+// Pixels per thread up to which one launch is taken.
+constexpr int64_t kGnSmallPixels = 16;
 
-// Scratch sized for either vector width (the tensors' alignment may differ between calls).
 static GnPlan gn_plan(const tdgs_norm* a, bool vec) {
     GnPlan p;
     p.vw = vec ? (a->dtype == TDGS_F32 ? 4 : 8) : 1;
     p.vectors = a->channels / p.vw;
+    p.stats_bytes = align_up((size_t)a->n * a->groups * 2 * sizeof(float));
+    p.chan_bytes = align_up((size_t)a->n * a->channels * 2 * sizeof(float));
+    // whole groups in whole vectors, 64 bytes of a pixel or more
+    const int size = a->channels / a->groups;
+    int unit = size;
+    while (unit % p.vw != 0) unit += size;
+    unit /= p.vw;
+    const int least = vec ? 4 : (int)(64 / dtype_size(a->dtype));
+    int few = (least + unit - 1) / unit * unit;
+    if (few > p.vectors) few = p.vectors;
+    p.small = few <= kGnSmallVectors && a->pixels <= kGnSmallPixels * (kGnSmallThreads / few);
+    if (p.small) {
+        p.vectors = few;
+        p.blocks = 1;
+        p.parts = 0;
+        p.per = a->pixels;
+        p.forward_bytes = 0;
+        p.grad_bytes = p.chan_bytes;
+        return p;
+    }
     const int64_t lanes = p.vectors < kGnThreads ? kGnThreads / p.vectors : 1;
     int64_t blocks = ceil_div(a->pixels, lanes * kGnPixels);
     const int64_t most = ceil_div(kGnWorkgroups, (a->n > 0 ? a->n : 1) * ceil_div(p.vectors, kGnThreads));
     if (blocks > most) blocks = most;
     p.per = ceil_div(a->pixels, blocks > 0 ? blocks : 1);
     p.blocks = (int)ceil_div(a->pixels, p.per > 0 ? p.per : 1);
-    p.stats_bytes = align_up((size_t)a->n * a->groups * 2 * sizeof(float));
-    p.part_bytes = align_up((size_t)a->n * p.blocks * a->channels * 2 * sizeof(float));
-    p.chan_bytes = align_up((size_t)a->n * a->channels * 2 * sizeof(float));
-    p.forward_bytes = p.stats_bytes + p.part_bytes;
-    p.grad_bytes = p.chan_bytes + p.part_bytes;
+    p.parts = p.vectors <= kGnThreads ? a->groups : a->channels;
+    p.forward_bytes = p.stats_bytes + align_up((size_t)a->n * p.blocks * p.parts * 2 * sizeof(float));
+    p.grad_bytes = p.chan_bytes + align_up((size_t)a->n * p.blocks * a->channels * 2 * sizeof(float));
     return p;
 }
 
@@ -549,6 +759,7 @@ static GnArgs gn_args(const tdgs_norm* a, const GnPlan& p) {
     r.group_size = a->channels / a->groups;
     r.blocks = p.blocks;
     r.vectors = p.vectors;
+    r.parts = p.parts;
     r.eps = a->eps;
     r.param_f32 = a->param_dtype == TDGS_F32;
     return r;
@@ -596,19 +807,27 @@ int tdgs_group_norm(void* stream_, const tdgs_norm* a) {
     TDGS_TRY(gn_check_view(&a->out, "out", a, true));
     const bool vec = gn_vec(a->x, a) && gn_vec(a->out, a);
     const GnPlan p = gn_plan(a, vec);
-    TDGS_REQUIRE(a->temp && a->temp_bytes >= p.forward_bytes && aligned_to(a->temp, 16),
+    TDGS_REQUIRE(p.forward_bytes == 0 || (a->temp && a->temp_bytes >= p.forward_bytes && aligned_to(a->temp, 16)),
                  "group norm: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, p.forward_bytes);
     hipStream_t stream = (hipStream_t)stream_;
     GnArgs r = gn_args(a, p);
     r.out = a->out.data;
     r.on = a->out.stride_n;
     r.op = a->out.stride_p;
-    if (!r.stats) r.stats = (float*)a->temp;
-    r.part = (float*)((char*)a->temp + p.stats_bytes);
+    const dim3 small_grid((unsigned)ceil_div(a->channels / p.vw, p.vectors), (unsigned)a->n);
+    if (!p.small) {
+        if (!r.stats) r.stats = (float*)a->temp;
+        r.part = (float*)((char*)a->temp + p.stats_bytes);
+    }
     const dim3 grid((unsigned)p.blocks, (unsigned)ceil_div(p.vectors, kGnThreads), (unsigned)a->n);
     return gn_dispatch(a, p.vw, [&](auto t, auto w, auto act) -> int {
         using T = decltype(t);
         constexpr int VW = decltype(w)::value, ACT = decltype(act)::value;
+        if (p.small) {
+            k_norm_small<T, VW, ACT><<<small_grid, kGnSmallThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
+            return TDGS_OK;
+        }
         k_norm_stats<T, VW><<<grid, kGnThreads, 0, stream>>>(r);
         TDGS_LAUNCHED();
         k_norm_join<<<(unsigned)((int64_t)a->n * a->groups), kGnThreads, 0, stream>>>(r);
@@ -630,8 +849,7 @@ int tdgs_group_norm_grad(void* stream_, const tdgs_norm* a, const tdgs_norm_grad
         TDGS_TRY(gn_check_view(&g->dx, "dx", a, true));
     }
     const bool vec = !empty && gn_vec(a->x, a) && gn_vec(g->dout, a) && gn_vec(g->dx, a);
-    GnPlan p = gn_plan(a, vec);
-    if (empty) p.blocks = 0;   // (dweight and dbias are zero)
+    const GnPlan p = gn_plan(a, vec);
     TDGS_REQUIRE(a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16),
                  "group norm: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0,
                  p.grad_bytes);
@@ -647,17 +865,28 @@ int tdgs_group_norm_grad(void* stream_, const tdgs_norm* a, const tdgs_norm_grad
     r.dbias = g->dbias;
     r.chan = (float*)a->temp;
     r.part = (float*)((char*)a->temp + p.chan_bytes);
+    const dim3 small_grid((unsigned)ceil_div(a->channels / p.vw, p.vectors), (unsigned)a->n);
     const dim3 grid((unsigned)p.blocks, (unsigned)ceil_div(p.vectors, kGnThreads), (unsigned)a->n);
     return gn_dispatch(a, p.vw, [&](auto t, auto w, auto act) -> int {
         using T = decltype(t);
         constexpr int VW = decltype(w)::value, ACT = decltype(act)::value;
-        if (!empty) {
+        const unsigned channel_blocks = (unsigned)ceil_div(a->channels, kGnThreads);
+        if (empty) {
+            r.n = 0;   // (dweight and dbias are zero)
+            k_norm_params<T><<<channel_blocks, kGnThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
+        } else if (p.small) {
+            k_norm_small_grad<T, VW, ACT><<<small_grid, kGnSmallThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
+            if (a->n > 1) {
+                k_norm_params<T><<<channel_blocks, kGnThreads, 0, stream>>>(r);
+                TDGS_LAUNCHED();
+            }
+        } else {
             k_norm_sums<T, VW, ACT><<<grid, kGnThreads, 0, stream>>>(r);
             TDGS_LAUNCHED();
-        }
-        k_norm_sums_join<T><<<(unsigned)ceil_div(a->channels, 16), kGnThreads, 0, stream>>>(r);
-        TDGS_LAUNCHED();
-        if (!empty) {
+            k_norm_sums_join<<<dim3((unsigned)ceil_div(a->channels, 8), (unsigned)a->n), kGnThreads, 0, stream>>>(r);
+            TDGS_LAUNCHED();
             k_norm_dx<T, VW, ACT><<<grid, kGnThreads, 0, stream>>>(r);
             TDGS_LAUNCHED();
         }
