@@ -41,7 +41,7 @@ struct AtArgs {
     int32_t group_batches, splits, blocks;
     float c, scale;   // scale log2(e), scale
     FastDiv by_g, by_lg;
-    bool vec, vec_out;
+    bool vec_out;
 };
 
 struct AtRow {
@@ -61,6 +61,7 @@ __device__ __forceinline__ int64_t at_stat(const AtArgs& a, const AtRow& r) {
 
 // Bit j: key t0 + j is allowed (the KT keys from t0 on). The same in every wavefront.
 __device__ __forceinline__ uint64_t at_allowed(const AtArgs& a, int kb, int len, int t0, int kt) {
+    if (!a.mask && t0 + kt <= len) return kt == 64 ? ~0ull : (1ull << kt) - 1;
     const int j = t0 + (int)__lane_id();
     bool ok = (int)__lane_id() < kt && j < len;
     if (a.mask && ok) ok = a.mask[kb * a.mask_stride + j] != 0;
@@ -80,28 +81,42 @@ constexpr int at_tile() { return sizeof(T) == 4 ? 32 : 64; }
 template <class T, int DP>
 constexpr int at_pitch() { return DP + 16 / (int)sizeof(T); }
 
-// One tile of N rows x DP elements in registers on its way to LDS.
-template <class T, int DP, int N>
+// One tile of N rows x DP elements in registers on its way to LDS, thread t of TH taking chunks of eight
+// elements t, t + TH, .. VEC: rows start on 16 bytes and d is a multiple of 8. Such chunks are loaded
+// without a condition, from an element that exists, and replaced by zeros on their way to LDS where they
+// should not count: a load behind a branch is waited for at its end, not where it is used.
+template <class T, int DP, int N, int TH, bool VEC>
 struct AtTile {
     static constexpr int kChunks = N * (DP / 8);
-    static constexpr int kPer = (kChunks + kAtThreads - 1) / kAtThreads;
+    static constexpr int kPer = (kChunks + TH - 1) / TH;
     typename Elem<T>::V8 r[kPer];
-    // row(j) gives row j's pointer, or null for a row of zeros
-    template <class Row>
-    __device__ __forceinline__ void load(int d, bool vec, Row&& row) {
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int c = (int)threadIdx.x + k * kAtThreads, j = c / (DP / 8), e = (c % (DP / 8)) * 8;
-            const T* p = (kChunks % kAtThreads == 0 || c < kChunks) ? row(j) : nullptr;
-            r[k] = p ? load8<T>(p + e, d - e, vec) : zero8<T>();
-        }
+    __device__ __forceinline__ static int chunk(int k) { return (int)threadIdx.x + k * TH; }
+    __device__ __forceinline__ static bool inside(int k) { return kChunks % TH == 0 || chunk(k) < kChunks; }
+    __device__ __forceinline__ static int row(int k) { return chunk(k) / (DP / 8); }
+    __device__ __forceinline__ static int col(int k) { return chunk(k) % (DP / 8) * 8; }
+    // Chunk k from the row at p (any readable row for one that does not count).
+    __device__ __forceinline__ void load_row(int k, const T* p, int d) {
+        if constexpr (VEC) r[k] = *reinterpret_cast<const typename Elem<T>::V8a*>(p + (col(k) < d ? col(k) : 0));
+        else r[k] = load8<T>(p + col(k), d - col(k), false);
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    // Rows base + j * stride, of which `rows` > 0 exist.
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int d) {
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int c = (int)threadIdx.x + k * kAtThreads, j = c / (DP / 8), e = (c % (DP / 8)) * 8;
-            if (kChunks % kAtThreads == 0 || c < kChunks)
-                *reinterpret_cast<typename Elem<T>::V8a*>(lds + j * at_pitch<T, DP>() + e) = r[k];
+        for (int k = 0; k < kPer; ++k) load_row(k, base + min(inside(k) ? row(k) : 0, rows - 1) * stride, d);
+    }
+    // To LDS, zeros for rows whose bit in `counts` is clear.
+    __device__ __forceinline__ void store(T* lds, uint64_t counts, int d) const {
+        auto at = [&](int k) {
+            return reinterpret_cast<typename Elem<T>::V8a*>(lds + row(k) * at_pitch<T, DP>() + col(k));
+        };
+        if (counts == (N == 64 ? ~0ull : (1ull << (N & 63)) - 1) && d == DP) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+                if (inside(k)) *at(k) = r[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k)
+                if (inside(k)) *at(k) = ((counts >> row(k)) & 1) && col(k) < d ? r[k] : zero8<T>();
         }
     }
 };
@@ -148,13 +163,18 @@ __device__ __forceinline__ typename Elem<T>::V8 at_pack(const f32x16& s, int hal
 }
 
 // Row r's elements in the order of a B operand's lanes (row l % 32 of the block): chunk c of DP / 16.
-template <class T, int DP>
-__device__ __forceinline__ void at_load_row(typename Elem<T>::V8 (&f)[DP / 16], const T* p, int d, bool vec) {
+template <class T, int DP, bool VEC>
+__device__ __forceinline__ void at_load_row(typename Elem<T>::V8 (&f)[DP / 16], const T* p, int d) {
     const int h = (int)__lane_id() >> 5;
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
         const int e = c * 16 + h * 8;
-        f[c] = p ? load8<T>(p + e, d - e, vec) : zero8<T>();
+        if constexpr (VEC) {
+            if (p && e < d) f[c] = *reinterpret_cast<const typename Elem<T>::V8a*>(p + e);
+            else f[c] = zero8<T>();
+        } else {
+            f[c] = p ? load8<T>(p + e, d - e, false) : zero8<T>();
+        }
     }
 }
 
@@ -191,10 +211,25 @@ __device__ __forceinline__ void at_store_row(T* p, const f32x16 (&o)[DP / 32], f
 
 // ---- forward -------------------------------------------------------------------------------
 
-// Workgroup: 4 wavefronts of QB * 32 rows each of one kv head, the keys of one split. Online softmax in
-// base 2: m is the running maximum of c s, O and l are relative to it.
-template <class T, int DP, int QB>
-__global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
+// How far a score may exceed the reference m of its row, in powers of two, before O and l are brought to a new one:
+// p then reaches 2^8, which every type holds, and few tiles after the first rescale anything.
+constexpr float kAtSlack = 8.0f;
+
+// The forward kernel's workgroup: threads, row blocks per wavefront, and wavefronts per SIMD that its
+// registers leave room for.
+template <class T, int DP>
+struct AtForward {
+    static constexpr int kThreads = sizeof(T) == 2 && DP <= 64 ? 512 : 256;
+    static constexpr int kBlocks = 1;
+    static constexpr int kPerSimd = sizeof(T) == 2 && DP <= 64 ? 4 : 2;
+    static constexpr int kRows = kThreads / kWave * kBlocks * 32;
+};
+
+// Workgroup: wavefronts of QB * 32 rows each of one kv head, the keys of one split. Online softmax in
+// base 2: O and l are relative to m, the largest c s so far to within kAtSlack.
+template <class T, int DP, bool VEC>
+__global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kPerSimd)) void k_attend(AtArgs a) {
+    constexpr int TH = AtForward<T, DP>::kThreads, QB = AtForward<T, DP>::kBlocks;
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
     __shared__ __attribute__((aligned(16))) T s_v[KT * P];
@@ -202,7 +237,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
     const int blk = item % a.blocks, sp = item / a.blocks % a.splits, kvh = item / a.blocks / a.splits;
     const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
-    const int row0 = (blk * kAtWaves + wave) * (QB * 32) + (lane & 31);
+    const int row0 = blk * AtForward<T, DP>::kRows + wave * (QB * 32) + (lane & 31);
 
     typename Elem<T>::V8 qf[QB][NC];
     f32x16 o[QB][NB];
@@ -212,7 +247,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
         const int r = row0 + qb * 32;
         const T* p = nullptr;
         if (r < a.rows) p = (const T*)a.q + at_offset(a.sq, at_row(a, kb, hk, r));
-        at_load_row<T, DP>(qf[qb], p, a.d, a.vec);
+        at_load_row<T, DP, VEC>(qf[qb], p, a.d);
         m[qb] = -INFINITY;
         l[qb] = 0.0f;
 #pragma unroll
@@ -225,19 +260,19 @@ __global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
     const int t_end = min(tiles, (sp + 1) * per);
     const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
     const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
-    AtTile<T, DP, KT> tk, tv;
+    AtTile<T, DP, KT, TH, VEC> tk, tv;
     uint64_t next = 0;
     auto fetch = [&](int t) {
         next = at_allowed(a, kb, len, t * KT, KT);
-        tk.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? kbase + (int64_t)(t * KT + j) * a.sk.l : nullptr; });
-        tv.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? vbase + (int64_t)(t * KT + j) * a.sv.l : nullptr; });
+        tk.load(kbase + (int64_t)t * KT * a.sk.l, a.sk.l, a.kv_len - t * KT, a.d);
+        tv.load(vbase + (int64_t)t * KT * a.sv.l, a.sv.l, a.kv_len - t * KT, a.d);
     };
     if (sp * per < t_end) fetch(sp * per);
     for (int t = sp * per; t < t_end; ++t) {
         const uint64_t allowed = next;
         __syncthreads();
-        tk.store(s_k);
-        tv.store(s_v);
+        tk.store(s_k, allowed, a.d);
+        tv.store(s_v, allowed, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
         if (allowed == 0) continue;
@@ -273,10 +308,10 @@ __global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
             for (int kk = 0; kk < KT / 32; ++kk)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) top = fmaxf(top, s[qb][kk][i]);
-            top = fmaxf(m[qb], max_halves(top) * a.c);
-            const float base = top == -INFINITY ? 0.0f : top;
-            if (wave_any(top > m[qb])) {
-                const float f = __builtin_amdgcn_exp2f(m[qb] - base);
+            top = max_halves(top) * a.c;
+            if (wave_any(top > m[qb] + kAtSlack)) {
+                top = fmaxf(top, m[qb]);
+                const float f = __builtin_amdgcn_exp2f(m[qb] - (top == -INFINITY ? 0.0f : top));
                 l[qb] *= f;
 #pragma unroll
                 for (int db = 0; db < NB; ++db)
@@ -284,6 +319,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend(AtArgs a) {
                     for (int i = 0; i < 16; ++i) o[qb][db][i] *= f;
                 m[qb] = top;
             }
+            const float base = m[qb] == -INFINITY ? 0.0f : m[qb];
             float sum = 0.0f;
 #pragma unroll
             for (int kk = 0; kk < KT / 32; ++kk)
@@ -359,8 +395,8 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, in
 __device__ __forceinline__ float at_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 // dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split.
-template <class T, int DP>
-__global__ __launch_bounds__(kAtThreads) void k_attend_dq(AtArgs a) {
+template <class T, int DP, bool VEC>
+__global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
     __shared__ __attribute__((aligned(16))) T s_v[KT * P];
@@ -373,12 +409,12 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dq(AtArgs a) {
     if (r < a.rows) row = at_row(a, kb, hk, r);
 
     typename Elem<T>::V8 qf[NC], df[NC];
-    at_load_row<T, DP>(qf, r < a.rows ? (const T*)a.q + at_offset(a.sq, row) : nullptr, a.d, a.vec);
-    at_load_row<T, DP>(df, r < a.rows ? (const T*)a.dout + at_offset(a.sdo, row) : nullptr, a.d, a.vec);
+    at_load_row<T, DP, VEC>(qf, r < a.rows ? (const T*)a.q + at_offset(a.sq, row) : nullptr, a.d);
+    at_load_row<T, DP, VEC>(df, r < a.rows ? (const T*)a.dout + at_offset(a.sdo, row) : nullptr, a.d);
     float lse2 = INFINITY, delta = 0.0f;
     {
         typename Elem<T>::V8 of[NC];
-        at_load_row<T, DP>(of, r < a.rows ? (const T*)a.o + at_offset(a.so, row) : nullptr, a.d, a.vec);
+        at_load_row<T, DP, VEC>(of, r < a.rows ? (const T*)a.o + at_offset(a.so, row) : nullptr, a.d);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -399,23 +435,24 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dq(AtArgs a) {
     const int t_end = min(tiles, (sp + 1) * per);
     const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
     const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
-    AtTile<T, DP, KT> tk, tv;
+    AtTile<T, DP, KT, kAtThreads, VEC> tk, tv;
     uint64_t next = 0;
     auto fetch = [&](int t) {
         next = at_allowed(a, kb, len, t * KT, KT);
-        tk.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? kbase + (int64_t)(t * KT + j) * a.sk.l : nullptr; });
-        tv.load(a.d, a.vec, [&](int j) { return (next >> j) & 1 ? vbase + (int64_t)(t * KT + j) * a.sv.l : nullptr; });
+        tk.load(kbase + (int64_t)t * KT * a.sk.l, a.sk.l, a.kv_len - t * KT, a.d);
+        tv.load(vbase + (int64_t)t * KT * a.sv.l, a.sv.l, a.kv_len - t * KT, a.d);
     };
     if (sp * per < t_end) fetch(sp * per);
     for (int t = sp * per; t < t_end; ++t) {
         const uint64_t allowed = next;
         __syncthreads();
-        tk.store(s_k);
-        tv.store(s_v);
+        tk.store(s_k, allowed, a.d);
+        tv.store(s_v, allowed, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
         if (allowed == 0) continue;
         const uint64_t mine = allowed >> (h * 4);
+        const bool all = allowed == (KT == 64 ? ~0ull : 0xffffffffull);
 #pragma unroll
         for (int kk = 0; kk < KT / 32; ++kk) {
             f32x16 s, dp;
@@ -426,12 +463,14 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dq(AtArgs a) {
                 s = mma(at_rows<T, DP>(s_k, kk * 32, c), qf[c], s);
                 dp = mma(at_rows<T, DP>(s_v, kk * 32, c), df[c], dp);
             }
+            if (!all) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const bool ok = (mine >> (kk * 32 + (i >> 2) * 8 + (i & 3))) & 1;
-                const float p = ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse2)) : 0.0f;
-                s[i] = p * (dp[i] - delta);
+                for (int i = 0; i < 16; ++i)
+                    if (!((mine >> (kk * 32 + (i >> 2) * 8 + (i & 3))) & 1)) s[i] = -INFINITY;
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse2)) * (dp[i] - delta);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 const auto b = at_pack<T>(s, ks);
@@ -449,9 +488,15 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dq(AtArgs a) {
     }
 }
 
-// dK and dV. Workgroup: 4 wavefronts of 32 keys each, the rows of one split.
+// Two wavefronts per SIMD, though heads of 97 to 128 elements then keep some registers in memory: without,
+// and one wavefront, 16-bit types take 1145 us for 64800 rows, 1024 keys and 8 heads where two take 1061.
+// Only float's 187 registers cost more than the second wavefront gives (5548 us, 4477 with one).
 template <class T, int DP>
-__global__ __launch_bounds__(kAtThreads) void k_attend_dkv(AtArgs a) {
+constexpr int at_dkv_per_simd() { return sizeof(T) == 4 && DP > 96 ? 1 : 2; }
+
+// dK and dV. Workgroup: 4 wavefronts of 32 keys each, the rows of one split.
+template <class T, int DP, bool VEC>
+__global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(AtArgs a) {
     constexpr int RT = 32, P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_q[RT * P];
     __shared__ __attribute__((aligned(16))) T s_d[RT * P];
@@ -467,26 +512,24 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dkv(AtArgs a) {
     if (a.mask && ok) ok = a.mask[kb * a.mask_stride + j] != 0;
 
     typename Elem<T>::V8 kf[NC], vf[NC];
-    at_load_row<T, DP>(kf, ok ? (const T*)a.k + kb * a.sk.b + hk * a.sk.h + j * a.sk.l : nullptr, a.d, a.vec);
-    at_load_row<T, DP>(vf, ok ? (const T*)a.v + kb * a.sv.b + hk * a.sv.h + j * a.sv.l : nullptr, a.d, a.vec);
+    at_load_row<T, DP, VEC>(kf, ok ? (const T*)a.k + kb * a.sk.b + hk * a.sk.h + j * a.sk.l : nullptr, a.d);
+    at_load_row<T, DP, VEC>(vf, ok ? (const T*)a.v + kb * a.sv.b + hk * a.sv.h + j * a.sv.l : nullptr, a.d);
     f32x16 gk[NB], gv[NB];
 #pragma unroll
     for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) gk[db][i] = gv[db][i] = 0.0f;
     const int tiles = (a.rows + RT - 1) / RT, per = (tiles + a.splits - 1) / a.splits;
-    const int t_end = blk * kAtWaves * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
-    AtTile<T, DP, RT> tq, td;
+    const int t_end = __syncthreads_or(ok) ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
+    AtTile<T, DP, RT, kAtThreads, VEC> tq, td;
     float st = 0.0f;
     auto fetch = [&](int t) {
-        tq.load(a.d, a.vec, [&](int i) {
-            const int r = t * RT + i;
-            return r < a.rows ? (const T*)a.q + at_offset(a.sq, at_row(a, kb, hk, r)) : nullptr;
-        });
-        td.load(a.d, a.vec, [&](int i) {
-            const int r = t * RT + i;
-            return r < a.rows ? (const T*)a.dout + at_offset(a.sdo, at_row(a, kb, hk, r)) : nullptr;
-        });
+#pragma unroll
+        for (int k = 0; k < tq.kPer; ++k) {
+            const AtRow at = at_row(a, kb, hk, min(t * RT + (tq.inside(k) ? tq.row(k) : 0), a.rows - 1));
+            tq.load_row(k, (const T*)a.q + at_offset(a.sq, at), a.d);
+            td.load_row(k, (const T*)a.dout + at_offset(a.sdo, at), a.d);
+        }
         if (threadIdx.x < 2 * RT) {   // lse of the tile's rows, then delta
             const int r = t * RT + (threadIdx.x & (RT - 1));
             st = threadIdx.x < RT ? INFINITY : 0.0f;
@@ -499,8 +542,10 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dkv(AtArgs a) {
     if (sp * per < t_end) fetch(sp * per);
     for (int t = sp * per; t < t_end; ++t) {
         __syncthreads();
-        tq.store(s_q);
-        td.store(s_d);
+        const int left = a.rows - t * RT;
+        const uint64_t in = left >= RT ? (1ull << RT) - 1 : (1ull << left) - 1;
+        tq.store(s_q, in, a.d);
+        td.store(s_d, in, a.d);
         if (threadIdx.x < RT) s_lse[threadIdx.x] = st;
         else if (threadIdx.x < 2 * RT) s_delta[threadIdx.x - RT] = st;
         __syncthreads();
@@ -519,7 +564,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dkv(AtArgs a) {
             const f32x4 de = *reinterpret_cast<const f32x4*>(s_delta + k * 8 + h * 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = ok ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[k * 4 + i], a.c, -ls[i])) : 0.0f;
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k * 4 + i], a.c, -ls[i]));
                 s[k * 4 + i] = p;
                 dp[k * 4 + i] = p * (dp[k * 4 + i] - de[i]);
             }
@@ -535,7 +580,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_dkv(AtArgs a) {
         }
     }
     if (j >= a.kv_len) return;
-    if (!ok) {   // (0 P would be NaN for a dout that is not finite)
+    if (!ok) {   // (a column of its own in every product, not masked before)
 #pragma unroll
         for (int db = 0; db < NB; ++db)
 #pragma unroll
@@ -580,14 +625,13 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
 
 // ---- host ----------------------------------------------------------------------------------
 
-// Workgroups that a launch should have at least, two per CU, and the most parts its long axis is
-// split into to reach them.
+// Workgroups that run at a time, two per CU, and the most parts that the long axis of a launch with fewer is
+// split into: as many as run together, since one more part for every workgroup would wait for a second round.
 constexpr int64_t kAtWorkgroups = 512;
 constexpr int kAtSplits = 64;
 
 static int at_splits(int64_t workgroups, int64_t tiles) {
-    int64_t s = workgroups > 0 ? ceil_div(kAtWorkgroups, workgroups) : 1;
-    if (workgroups >= kAtWorkgroups / 2) s = 1;   // (a second pass over the partial results costs more)
+    int64_t s = workgroups > 0 ? kAtWorkgroups / workgroups : 1;
     if (s > kAtSplits) s = kAtSplits;
     if (s > tiles) s = tiles;
     return (int)(s > 1 ? s : 1);
@@ -595,10 +639,27 @@ static int at_splits(int64_t workgroups, int64_t tiles) {
 
 static int at_padded(int d) { return (d + 31) / 32 * 32; }
 
+// f(integral constant) for the padded head dimension.
+template <class F>
+static int with_padded(int dp, F&& f) {
+    switch (dp) {
+        case 32: return f(std::integral_constant<int, 32>{});
+        case 64: return f(std::integral_constant<int, 64>{});
+        case 96: return f(std::integral_constant<int, 96>{});
+        default: return f(std::integral_constant<int, 128>{});
+    }
+}
+
+static int at_forward_rows(int32_t dtype, int dp) {
+    return with_dtype(dtype, [&](auto t) -> int {
+        return with_padded(dp, [&](auto d) -> int { return AtForward<decltype(t), decltype(d)::value>::kRows; });
+    });
+}
+
 // How the three launches are cut, from the sizes alone.
 struct AtPlan {
     int64_t kvh, rows;   // kv heads over all kv batches; rows of each
-    int dp, qb, tile;
+    int dp, rows_f, tile;
     int blocks_f, splits_f, blocks_q, splits_q, blocks_k, splits_k;
     size_t delta_bytes, forward_bytes, grad_bytes;
 };
@@ -609,9 +670,9 @@ static AtPlan at_plan(const tdgs_attention* a) {
     p.rows = (int64_t)(a->kv_batch > 0 ? a->batch / a->kv_batch : 0) * a->q_len * (a->heads / a->kv_heads);
     p.dp = at_padded(a->head_dim);
     p.tile = a->dtype == TDGS_F32 ? 32 : 64;
-    p.qb = a->dtype != TDGS_F32 && p.dp <= 64 ? 2 : 1;
+    p.rows_f = at_forward_rows(a->dtype, p.dp);
     const int64_t key_tiles = ceil_div(a->kv_len, p.tile), row_tiles = ceil_div(p.rows, 32);
-    p.blocks_f = (int)ceil_div(p.rows, kAtWaves * 32 * p.qb);
+    p.blocks_f = (int)ceil_div(p.rows, p.rows_f);
     p.splits_f = at_splits(p.blocks_f * p.kvh, key_tiles);
     p.blocks_q = (int)ceil_div(p.rows, kAtWaves * 32);
     p.splits_q = at_splits(p.blocks_q * p.kvh, key_tiles);
@@ -691,20 +752,8 @@ static AtArgs at_args(const tdgs_attention* a, const AtPlan& p) {
     const uint32_t g = (uint32_t)(a->heads / a->kv_heads);
     r.by_g = FastDiv(g);
     r.by_lg = FastDiv(g * (uint32_t)(a->q_len > 0 ? a->q_len : 1));
-    r.vec = a->head_dim % 8 == 0 && at_rows_aligned(a->q, e) && at_rows_aligned(a->k, e) && at_rows_aligned(a->v, e);
     r.vec_out = a->head_dim % 8 == 0 && at_rows_aligned(a->out, e);
     return r;
-}
-
-// f(integral constant) for the padded head dimension.
-template <class F>
-static int with_padded(int dp, F&& f) {
-    switch (dp) {
-        case 32: return f(std::integral_constant<int, 32>{});
-        case 64: return f(std::integral_constant<int, 64>{});
-        case 96: return f(std::integral_constant<int, 96>{});
-        default: return f(std::integral_constant<int, 128>{});
-    }
 }
 
 }  // namespace tdgs
@@ -740,13 +789,16 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
         r.part = (float*)a->temp;
         r.part_ml = r.part + p.splits_f * all * p.dp;
     }
+    const int64_t e = dtype_size(a->dtype);
+    const bool vec = a->head_dim % 8 == 0 && at_rows_aligned(a->q, e) &&
+                     (a->kv_len == 0 || (at_rows_aligned(a->k, e) && at_rows_aligned(a->v, e)));
     const unsigned grid = (unsigned)(p.kvh * p.splits_f * p.blocks_f);
     return with_dtype(a->dtype, [&](auto t) -> int {
         using T = decltype(t);
         TDGS_TRY(with_padded(p.dp, [&](auto dp) -> int {
-            constexpr int DP = decltype(dp)::value;
-            constexpr int QB = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
-            k_attend<T, DP, QB><<<grid, kAtThreads, 0, stream>>>(r);
+            constexpr int DP = decltype(dp)::value, TH = AtForward<T, DP>::kThreads;
+            if (vec) k_attend<T, DP, true><<<grid, TH, 0, stream>>>(r);
+            else k_attend<T, DP, false><<<grid, TH, 0, stream>>>(r);
             TDGS_LAUNCHED();
             return TDGS_OK;
         }));
@@ -790,7 +842,8 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
     r.sdq = at_strides(g->dq);
     r.sdk = at_strides(g->dk);
     r.sdv = at_strides(g->dv);
-    r.vec = r.vec && r.vec_out && at_rows_aligned(g->dout, e);
+    const bool vec = r.vec_out && at_rows_aligned(a->q, e) && at_rows_aligned(g->dout, e) && at_rows_aligned(a->k, e) &&
+                     at_rows_aligned(a->v, e);
     r.vec_out = a->head_dim % 8 == 0 && at_rows_aligned(g->dq, e) && at_rows_aligned(g->dk, e) && at_rows_aligned(g->dv, e);
     r.delta = (float*)a->temp;
     r.part = (float*)((char*)a->temp + p.delta_bytes);
@@ -802,7 +855,9 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
             if (a->q_len > 0) {
                 r.blocks = p.blocks_q;
                 r.splits = p.splits_q;
-                k_attend_dq<T, DP><<<(unsigned)(p.kvh * p.splits_q * p.blocks_q), kAtThreads, 0, stream>>>(r);
+                const unsigned grid = (unsigned)(p.kvh * p.splits_q * p.blocks_q);
+                if (vec) k_attend_dq<T, DP, true><<<grid, kAtThreads, 0, stream>>>(r);
+                else k_attend_dq<T, DP, false><<<grid, kAtThreads, 0, stream>>>(r);
                 TDGS_LAUNCHED();
                 if (p.splits_q > 1) {
                     k_attend_sum<T><<<(unsigned)ceil_div(all_rows * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
@@ -813,7 +868,9 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
             if (a->kv_len > 0) {
                 r.blocks = p.blocks_k;
                 r.splits = p.splits_k;
-                k_attend_dkv<T, DP><<<(unsigned)(p.kvh * p.splits_k * p.blocks_k), kAtThreads, 0, stream>>>(r);
+                const unsigned grid = (unsigned)(p.kvh * p.splits_k * p.blocks_k);
+                if (vec) k_attend_dkv<T, DP, true><<<grid, kAtThreads, 0, stream>>>(r);
+                else k_attend_dkv<T, DP, false><<<grid, kAtThreads, 0, stream>>>(r);
                 TDGS_LAUNCHED();
                 if (p.splits_k > 1) {
                     k_attend_sum<T><<<(unsigned)ceil_div(2 * all_keys * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
