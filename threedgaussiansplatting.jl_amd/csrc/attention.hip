@@ -178,6 +178,11 @@ __device__ __forceinline__ void at_load_row(typename Elem<T>::V8 (&f)[DP / 16], 
     }
 }
 
+template <class V2>
+__device__ __forceinline__ uint32_t at_bits(V2 v) {
+    return __builtin_bit_cast(uint32_t, v);
+}
+
 template <class T>
 __device__ __forceinline__ void at_store4(T* p, f32x4 x, int n, bool vec) {
     if (vec && n >= 4) {
@@ -193,10 +198,36 @@ __device__ __forceinline__ void at_store4(T* p, f32x4 x, int n, bool vec) {
     }
 }
 
-// A block column of results (d x 32 lanes' rows, DP / 32 blocks) times f to a row of T.
+// A block column of results (d x 32 lanes' rows, DP / 32 blocks) times f to a row of T. A lane holds four
+// elements in eight, its partner in the other half of the wavefront the other four: rows of a 16-bit type that
+// allow it trade two fours of theirs for one eight, and store 16 bytes (every lane of the
+// wavefront calls this; p null: nothing stored).
 template <class T, int DP>
 __device__ __forceinline__ void at_store_row(T* p, const f32x16 (&o)[DP / 32], float f, int d, bool vec) {
     const int h = (int)__lane_id() >> 5;
+    if constexpr (sizeof(T) == 2) if (vec) {
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                uint32_t x[2], y[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    typedef T V2 __attribute__((ext_vector_type(2)));
+                    const V2 lo = {(T)(o[db][k * 4 + 2 * i] * f), (T)(o[db][k * 4 + 2 * i + 1] * f)};
+                    const V2 hi = {(T)(o[db][k * 4 + 4 + 2 * i] * f), (T)(o[db][k * 4 + 5 + 2 * i] * f)};
+                    const auto r = __builtin_amdgcn_permlane32_swap(at_bits(lo), at_bits(hi), false, false);
+                    x[i] = r[0];
+                    y[i] = r[1];
+                }
+                const int e = db * 32 + (k + h) * 8;
+                typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+                const U4 v = {x[0], x[1], y[0], y[1]};
+                if (p && e < d) *reinterpret_cast<U4*>(p + e) = v;
+            }
+        return;
+    }
+    if (!p) return;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -209,7 +240,20 @@ __device__ __forceinline__ void at_store_row(T* p, const f32x16 (&o)[DP / 32], f
         }
 }
 
-// ---- forward -------------------------------------------------------------------------------
+// Kernels that share rows' heads: the workgroup of (kv head, rest), heads next to each other on one XCD. Neighbouring
+// heads of a row share its cache lines, so their workgroups should share an L2 (workgroup i runs on XCD
+// i mod 8). Keys of a head are read by many workgroups, but a band of them for each XCD gains 1 to 2% where every
+// head has much to do (32400 x 4096) and loses as much where not, and where lengths or masks differ between
+// batches leaves whole XCDs without work.
+struct AtItem {
+    int hk, rest;
+};
+__device__ __forceinline__ AtItem at_item(int i, int n, int kv_heads) {
+    const int whole = n / (kXcds * kv_heads) * (kXcds * kv_heads);
+    if (i >= whole) return {i % kv_heads, i / kv_heads};
+    const int j = i / kXcds;
+    return {j % kv_heads, j / kv_heads * kXcds + i % kXcds};
+}
 
 // How far a score may exceed the reference m of its row, in powers of two, before O and l are brought to a new one:
 // p then reaches 2^8, which every type holds, and few tiles after the first rescale anything.
@@ -233,9 +277,9 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
     __shared__ __attribute__((aligned(16))) T s_v[KT * P];
-    const int item = xcd_band_item(blockIdx.x, gridDim.x);
-    const int blk = item % a.blocks, sp = item / a.blocks % a.splits, kvh = item / a.blocks / a.splits;
-    const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
+    const AtItem item = at_item(blockIdx.x, gridDim.x, a.kv_heads);
+    const int blk = item.rest % a.blocks, sp = item.rest / a.blocks % a.splits, kb = item.rest / a.blocks / a.splits;
+    const int hk = item.hk, kvh = kb * a.kv_heads + hk;
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
     const int row0 = blk * AtForward<T, DP>::kRows + wave * (QB * 32) + (lane & 31);
 
@@ -346,13 +390,14 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
         const int r = row0 + qb * 32;
+        const bool in = r < a.rows;
         const float sum = sum_halves(l[qb]);
-        if (r >= a.rows) continue;
         if (a.splits == 1) {
-            const AtRow row = at_row(a, kb, hk, r);
-            at_store_row<T, DP>((T*)a.out + at_offset(a.so, row), o[qb], sum > 0.0f ? 1.0f / sum : 0.0f, a.d, a.vec_out);
-            if (a.lse && h == 0) a.lse[at_stat(a, row)] = (m[qb] + __builtin_amdgcn_logf(sum)) * kLn2;
-        } else {
+            const AtRow row = at_row(a, kb, hk, in ? r : 0);
+            at_store_row<T, DP>(in ? (T*)a.out + at_offset(a.so, row) : nullptr, o[qb], sum > 0.0f ? 1.0f / sum : 0.0f,
+                                a.d, a.vec_out);
+            if (in && a.lse && h == 0) a.lse[at_stat(a, row)] = (m[qb] + __builtin_amdgcn_logf(sum)) * kLn2;
+        } else if (in) {
             const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
             at_store_row<float, DP>(a.part + pr * DP, o[qb], 1.0f, DP, true);
             if (h == 0) {
@@ -363,30 +408,41 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
     }
 }
 
-// Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. One wavefront per row.
+// Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. One wavefront per row; lane s
+// holds split s's m and l (at most kAtSplits of them), then two of the row's elements.
 template <class T>
 __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, int64_t all_rows) {
     const int64_t pr0 = (int64_t)blockIdx.x * kAtWaves + threadIdx.x / kWave;
     if (pr0 >= all_rows) return;
     const int lane = (int)__lane_id();
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * all_rows + pr0)]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    if (lane < a.splits) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (lane * all_rows + pr0));
+        m = ml.x;
+        l = ml.y;
+    }
+    float top = m;
+    for (int w = kWave / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, kWave));
+    const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+    float sum = f * l;
+    for (int w = kWave / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, kWave);
+    const int e = lane * 2;
+    float x0 = 0.0f, x1 = 0.0f;
+    const float* const part = a.part + pr0 * dp + (e < dp ? e : 0);
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) {
-        const int64_t pr = s * all_rows + pr0;
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * pr] - base);
-        sum = __builtin_fmaf(f, a.part_ml[2 * pr + 1], sum);
-        if (lane < a.d) x0 = __builtin_fmaf(f, a.part[pr * dp + lane], x0);
-        if (lane + 64 < a.d) x1 = __builtin_fmaf(f, a.part[pr * dp + lane + 64], x1);
+        const float fs = __shfl(f, s, kWave);
+        const float2 v = *reinterpret_cast<const float2*>(part + s * all_rows * dp);
+        x0 = __builtin_fmaf(fs, v.x, x0);
+        x1 = __builtin_fmaf(fs, v.y, x1);
     }
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     const int kvh = (int)(pr0 / a.rows);
     const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr0 % a.rows));
     T* const out = (T*)a.out + at_offset(a.so, row);
-    if (lane < a.d) out[lane] = (T)(x0 * inv);
-    if (lane + 64 < a.d) out[lane + 64] = (T)(x1 * inv);
-    if (a.lse && lane == 0) a.lse[at_stat(a, row)] = (m + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (e < a.d) out[e] = (T)(x0 * inv);
+    if (e + 1 < a.d) out[e + 1] = (T)(x1 * inv);
+    if (a.lse && lane == 0) a.lse[at_stat(a, row)] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -400,9 +456,9 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
     __shared__ __attribute__((aligned(16))) T s_v[KT * P];
-    const int item = xcd_band_item(blockIdx.x, gridDim.x);
-    const int blk = item % a.blocks, sp = item / a.blocks % a.splits, kvh = item / a.blocks / a.splits;
-    const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
+    const AtItem item = at_item(blockIdx.x, gridDim.x, a.kv_heads);
+    const int blk = item.rest % a.blocks, sp = item.rest / a.blocks % a.splits, kb = item.rest / a.blocks / a.splits;
+    const int hk = item.hk, kvh = kb * a.kv_heads + hk;
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
     const int r = (blk * kAtWaves + wave) * 32 + (lane & 31);
     AtRow row = {0, 0, 0};
@@ -479,10 +535,9 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
             }
         }
     }
-    if (r >= a.rows) return;
     if (a.splits == 1) {
-        at_store_row<T, DP>((T*)a.dq + at_offset(a.sdq, row), o, a.scale, a.d, a.vec_out);
-    } else {
+        at_store_row<T, DP>(r < a.rows ? (T*)a.dq + at_offset(a.sdq, row) : nullptr, o, a.scale, a.d, a.vec_out);
+    } else if (r < a.rows) {
         const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
         at_store_row<float, DP>(a.part + pr * DP, o, 1.0f, DP, true);
     }
@@ -502,7 +557,7 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     __shared__ __attribute__((aligned(16))) T s_d[RT * P];
     __shared__ __attribute__((aligned(16))) float s_lse[RT];
     __shared__ __attribute__((aligned(16))) float s_delta[RT];
-    const int item = xcd_band_item(blockIdx.x, gridDim.x);
+    const int item = blockIdx.x;
     const int sp = item % a.splits, blk = item / a.splits % a.blocks, kvh = item / a.splits / a.blocks;
     const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
@@ -579,7 +634,6 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
             }
         }
     }
-    if (j >= a.kv_len) return;
     if (!ok) {   // (a column of its own in every product, not masked before)
 #pragma unroll
         for (int db = 0; db < NB; ++db)
@@ -587,9 +641,10 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
             for (int i = 0; i < 16; ++i) gk[db][i] = gv[db][i] = 0.0f;
     }
     if (a.splits == 1) {
-        at_store_row<T, DP>((T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + j * a.sdk.l, gk, a.scale, a.d, a.vec_out);
-        at_store_row<T, DP>((T*)a.dv + kb * a.sdv.b + hk * a.sdv.h + j * a.sdv.l, gv, 1.0f, a.d, a.vec_out);
-    } else {
+        const bool in = j < a.kv_len;
+        at_store_row<T, DP>(in ? (T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + j * a.sdk.l : nullptr, gk, a.scale, a.d, a.vec_out);
+        at_store_row<T, DP>(in ? (T*)a.dv + kb * a.sdv.b + hk * a.sdv.h + j * a.sdv.l : nullptr, gv, 1.0f, a.d, a.vec_out);
+    } else if (j < a.kv_len) {
         const int64_t all = (int64_t)(gridDim.x / (a.blocks * a.splits)) * a.kv_len;
         const int64_t pr = (2 * sp * all) + (int64_t)kvh * a.kv_len + j;
         at_store_row<float, DP>(a.part + pr * DP, gk, 1.0f, DP, true);
@@ -628,7 +683,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
 // Workgroups that run at a time, two per CU, and the most parts that the long axis of a launch with fewer is
 // split into: as many as run together, since one more part for every workgroup would wait for a second round.
 constexpr int64_t kAtWorkgroups = 512;
-constexpr int kAtSplits = 64;
+constexpr int kAtSplits = 64;   // (a lane each in the join)
 
 static int at_splits(int64_t workgroups, int64_t tiles) {
     int64_t s = workgroups > 0 ? kAtWorkgroups / workgroups : 1;
