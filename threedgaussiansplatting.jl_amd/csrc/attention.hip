@@ -408,41 +408,45 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
     }
 }
 
-// Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. One wavefront per row; lane s
-// holds split s's m and l (at most kAtSplits of them), then two of the row's elements.
-template <class T>
+// Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. A thread holds four
+// elements of a row; with SG > 1, for many splits of few rows, SG of them take every SG-th split and
+// are added up in LDS.
+template <class T, int SG>
 __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, int64_t all_rows) {
-    const int64_t pr0 = (int64_t)blockIdx.x * kAtWaves + threadIdx.x / kWave;
-    if (pr0 >= all_rows) return;
-    const int lane = (int)__lane_id();
-    float m = -INFINITY, l = 0.0f;
-    if (lane < a.splits) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (lane * all_rows + pr0));
-        m = ml.x;
-        l = ml.y;
-    }
-    float top = m;
-    for (int w = kWave / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, kWave));
-    const float f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
-    float sum = f * l;
-    for (int w = kWave / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, kWave);
-    const int e = lane * 2;
-    float x0 = 0.0f, x1 = 0.0f;
-    const float* const part = a.part + pr0 * dp + (e < dp ? e : 0);
+    __shared__ f32x4 s_x[SG > 1 ? kAtThreads : 1];
+    const int quads = dp / 4, q = (int)threadIdx.x % quads, slot = (int)threadIdx.x / quads;
+    const int per = kAtThreads / quads / SG, g = slot / per;   // rows per workgroup; this thread's share of the splits
+    const int64_t pr0 = (int64_t)blockIdx.x * per + slot % per;
+    const bool in = g < SG && pr0 < all_rows;
+    float top = -INFINITY, sum = 0.0f, base = 0.0f;
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (in) {
+        const float2* const ml = reinterpret_cast<const float2*>(a.part_ml) + pr0;
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) {
-        const float fs = __shfl(f, s, kWave);
-        const float2 v = *reinterpret_cast<const float2*>(part + s * all_rows * dp);
-        x0 = __builtin_fmaf(fs, v.x, x0);
-        x1 = __builtin_fmaf(fs, v.y, x1);
+        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s * all_rows].x);
+        base = top == -INFINITY ? 0.0f : top;
+        const f32x4* const part = reinterpret_cast<const f32x4*>(a.part + pr0 * dp) + q;
+#pragma unroll 4
+        for (int s = g; s < a.splits; s += SG)
+            x += *(part + s * all_rows * quads) * __builtin_amdgcn_exp2f(ml[s * all_rows].x - base);
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s) {
+            const float2 v = ml[s * all_rows];
+            sum = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x - base), v.y, sum);
+        }
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    if constexpr (SG > 1) {
+        s_x[threadIdx.x] = x;
+        __syncthreads();
+        if (g == 0)
+            for (int i = 1; i < SG; ++i) x += s_x[threadIdx.x + i * per * quads];
+    }
+    if (!in || g > 0) return;
     const int kvh = (int)(pr0 / a.rows);
     const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr0 % a.rows));
-    T* const out = (T*)a.out + at_offset(a.so, row);
-    if (e < a.d) out[e] = (T)(x0 * inv);
-    if (e + 1 < a.d) out[e + 1] = (T)(x1 * inv);
-    if (a.lse && lane == 0) a.lse[at_stat(a, row)] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (q * 4 < a.d)
+        at_store4<T>((T*)a.out + at_offset(a.so, row) + q * 4, x * (sum > 0.0f ? 1.0f / sum : 0.0f), a.d - q * 4, a.vec_out);
+    if (a.lse && q == 0) a.lse[at_stat(a, row)] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 // ---- backward ------------------------------------------------------------------------------
@@ -682,11 +686,12 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
 
 // Workgroups that run at a time, two per CU, and the most parts that the long axis of a launch with fewer is
 // split into: as many as run together, since one more part for every workgroup would wait for a second round.
+// With lengths or a mask, workgroups end at different times, and twice as many parts even that out.
 constexpr int64_t kAtWorkgroups = 512;
-constexpr int kAtSplits = 64;   // (a lane each in the join)
+constexpr int kAtSplits = 64;
 
-static int at_splits(int64_t workgroups, int64_t tiles) {
-    int64_t s = workgroups > 0 ? kAtWorkgroups / workgroups : 1;
+static int at_splits(int64_t workgroups, int64_t tiles, bool uneven) {
+    int64_t s = workgroups > 0 ? (uneven ? 2 : 1) * kAtWorkgroups / workgroups : 1;
     if (s > kAtSplits) s = kAtSplits;
     if (s > tiles) s = tiles;
     return (int)(s > 1 ? s : 1);
@@ -711,7 +716,7 @@ static int at_forward_rows(int32_t dtype, int dp) {
     });
 }
 
-// How the three launches are cut, from the sizes alone.
+// How the three launches are cut, from the sizes and whether there are lengths or a mask.
 struct AtPlan {
     int64_t kvh, rows;   // kv heads over all kv batches; rows of each
     int dp, rows_f, tile;
@@ -719,7 +724,7 @@ struct AtPlan {
     size_t delta_bytes, forward_bytes, grad_bytes;
 };
 
-static AtPlan at_plan(const tdgs_attention* a) {
+static AtPlan at_plan(const tdgs_attention* a, bool uneven) {
     AtPlan p;
     p.kvh = (int64_t)a->kv_batch * a->kv_heads;
     p.rows = (int64_t)(a->kv_batch > 0 ? a->batch / a->kv_batch : 0) * a->q_len * (a->heads / a->kv_heads);
@@ -728,11 +733,11 @@ static AtPlan at_plan(const tdgs_attention* a) {
     p.rows_f = at_forward_rows(a->dtype, p.dp);
     const int64_t key_tiles = ceil_div(a->kv_len, p.tile), row_tiles = ceil_div(p.rows, 32);
     p.blocks_f = (int)ceil_div(p.rows, p.rows_f);
-    p.splits_f = at_splits(p.blocks_f * p.kvh, key_tiles);
+    p.splits_f = at_splits(p.blocks_f * p.kvh, key_tiles, uneven);
     p.blocks_q = (int)ceil_div(p.rows, kAtWaves * 32);
-    p.splits_q = at_splits(p.blocks_q * p.kvh, key_tiles);
+    p.splits_q = at_splits(p.blocks_q * p.kvh, key_tiles, uneven);
     p.blocks_k = (int)ceil_div(a->kv_len, kAtWaves * 32);
-    p.splits_k = at_splits(p.blocks_k * p.kvh, row_tiles);
+    p.splits_k = at_splits(p.blocks_k * p.kvh, row_tiles, uneven);
     const size_t all_rows = (size_t)(p.kvh * p.rows), all_keys = (size_t)(p.kvh * a->kv_len);
     p.delta_bytes = align_up(all_rows * sizeof(float));
     p.forward_bytes = p.splits_f > 1 ? p.splits_f * (align_up(all_rows * p.dp * sizeof(float)) + align_up(all_rows * 2 * sizeof(float))) : 0;
@@ -819,8 +824,13 @@ extern "C" {
 
 size_t tdgs_cross_attention_temp_bytes(const tdgs_attention* a, int32_t grad) {
     if (at_check(a) != TDGS_OK || a->batch == 0) return 0;
-    const AtPlan p = at_plan(a);
-    return grad && p.grad_bytes > p.forward_bytes ? p.grad_bytes : p.forward_bytes;
+    size_t bytes = 0;
+    for (int uneven = 0; uneven < 2; ++uneven) {
+        const AtPlan p = at_plan(a, uneven != 0);
+        const size_t b = grad && p.grad_bytes > p.forward_bytes ? p.grad_bytes : p.forward_bytes;
+        if (b > bytes) bytes = b;
+    }
+    return bytes;
 }
 
 int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
@@ -832,7 +842,7 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
         TDGS_TRY(at_check_view(&a->k, "k", a, true, false));
         TDGS_TRY(at_check_view(&a->v, "v", a, true, false));
     }
-    const AtPlan p = at_plan(a);
+    const AtPlan p = at_plan(a, a->kv_lengths || a->kv_mask);
     TDGS_REQUIRE(p.forward_bytes == 0 || (a->temp && a->temp_bytes >= p.forward_bytes && aligned_to(a->temp, 16)),
                  "attention: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, p.forward_bytes);
     hipStream_t stream = (hipStream_t)stream_;
@@ -858,7 +868,9 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
             return TDGS_OK;
         }));
         if (p.splits_f > 1) {
-            k_attend_join<T><<<(unsigned)ceil_div(all, kAtWaves), kAtThreads, 0, stream>>>(r, p.dp, all);
+            const int per = kAtThreads / (p.dp / 4);   // rows per workgroup
+            if (p.splits_f >= 8) k_attend_join<T, 8><<<(unsigned)ceil_div(all, per / 8), kAtThreads, 0, stream>>>(r, p.dp, all);
+            else k_attend_join<T, 1><<<(unsigned)ceil_div(all, per), kAtThreads, 0, stream>>>(r, p.dp, all);
             TDGS_LAUNCHED();
         }
         return TDGS_OK;
@@ -882,7 +894,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
         TDGS_TRY(at_check_view(&g->dk, "dk", a, true, true));
         TDGS_TRY(at_check_view(&g->dv, "dv", a, true, true));
     }
-    const AtPlan p = at_plan(a);
+    const AtPlan p = at_plan(a, a->kv_lengths || a->kv_mask);
     TDGS_REQUIRE(a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16),
                  "attention: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0,
                  p.grad_bytes);
