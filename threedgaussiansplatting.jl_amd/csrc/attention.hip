@@ -11,6 +11,9 @@
 // swap of the halves, and P^T is in place as the next product's B operand (O^T = V^T P^T,
 // dQ^T = K^T dS^T), V^T and K^T coming from LDS by the transposing reads. For dK and dV the block is
 // S = Q K^T, a lane holding 16 rows of one key, and dV^T = dO^T P, dK^T = Q^T dS follow likewise.
+// A key mask is turned into a list of the allowed keys first, by which keys are then loaded and their
+// gradients stored, so that the kernels see a shorter sequence: they do no work for single keys that are not allowed,
+// and such keys, whatever they hold, are not read.
 // P and dS are rounded to the inputs' type for their products (the matrix cores take no wider
 // operand at that rate); maxima, sums, exponentials and every accumulator stay in 32 bits.
 #include "internal.hpp"
@@ -30,9 +33,8 @@ struct AtArgs {
     const void *q, *k, *v, *dout, *o;
     void *out, *dq, *dk, *dv;
     AtHeads sq, sk, sv, so, sdo, sdq, sdk, sdv;
-    const int32_t* lengths;
-    const uint8_t* mask;
-    int64_t mask_stride;
+    const int32_t* lengths;   // allowed keys of a kv batch (with a mask: of its list); null: all
+    const int32_t* index;     // with a mask: kv_len keys of each kv batch, the allowed ones first
     float* lse;       // batch x heads x q_len, natural logarithm
     float* delta;     // the same shape: dout . out
     float *part, *part_ml;
@@ -59,18 +61,57 @@ __device__ __forceinline__ int64_t at_stat(const AtArgs& a, const AtRow& r) {
     return ((int64_t)r.b * a.heads + r.h) * a.q_len + r.i;
 }
 
-// Bit j: key t0 + j is allowed (the KT keys from t0 on). The same in every wavefront.
-__device__ __forceinline__ uint64_t at_allowed(const AtArgs& a, int kb, int len, int t0, int kt) {
-    if (!a.mask && t0 + kt <= len) return kt == 64 ? ~0ull : (1ull << kt) - 1;
-    const int j = t0 + (int)__lane_id();
-    bool ok = (int)__lane_id() < kt && j < len;
-    if (a.mask && ok) ok = a.mask[kb * a.mask_stride + j] != 0;
-    return __ballot(ok);
-}
 __device__ __forceinline__ int at_length(const AtArgs& a, int kb) {
     if (!a.lengths) return a.kv_len;
     const int n = a.lengths[kb];
     return n < 0 ? 0 : (n < a.kv_len ? n : a.kv_len);
+}
+
+__device__ __forceinline__ int64_t at_key(const AtArgs& a, int kb, int j) {
+    return a.index ? a.index[(int64_t)kb * a.kv_len + j] : j;
+}
+
+// Workgroup kb: the list of kv batch kb's keys, the allowed ones first and in order, and their number.
+constexpr int kAtListThreads = 1024;
+static __global__ __launch_bounds__(kAtListThreads) void k_attend_list(const uint8_t* __restrict__ mask, int64_t stride,
+                                                                       AtArgs a, int32_t* __restrict__ index,
+                                                                       int32_t* __restrict__ counts) {
+    constexpr int PER = 4, W = kAtListThreads / kWave;
+    __shared__ int s_wave[W];
+    const int kb = blockIdx.x, lane = (int)__lane_id(), wave = threadIdx.x / kWave, len = at_length(a, kb);
+    const uint8_t* const row = mask + kb * stride;
+    int32_t* const list = index + (int64_t)kb * a.kv_len;
+    int done = 0;   // allowed keys before this round's
+    for (int r0 = 0; r0 < a.kv_len; r0 += kAtListThreads * PER) {
+        // a wavefront takes PER * 64 neighbouring keys
+        const int j0 = r0 + wave * (kWave * PER) + lane;
+        uint64_t votes[PER];
+        bool ok[PER];
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int j = j0 + i * kWave;
+            ok[i] = j < len && row[j] != 0;
+            votes[i] = __ballot(ok[i]);
+            mine += __popcll(votes[i]);
+        }
+        if (lane == 0) s_wave[wave] = mine;
+        __syncthreads();
+        int at = done;
+        for (int w = 0; w < W; ++w) {
+            const int c = s_wave[w];
+            if (w < wave) at += c;
+            done += c;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int j = j0 + i * kWave, before = at + __popcll(votes[i] & lanemask_lt());
+            if (j < a.kv_len) list[ok[i] ? before : a.kv_len - 1 - (j - before)] = j;   // (the others from the end on)
+            at += __popcll(votes[i]);
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) counts[kb] = done;
 }
 
 // Keys per tile of the forward and dQ kernels, and rows per tile of the dK, dV kernel. LDS rows are
@@ -99,24 +140,32 @@ struct AtTile {
         if constexpr (VEC) r[k] = *reinterpret_cast<const typename Elem<T>::V8a*>(p + (col(k) < d ? col(k) : 0));
         else r[k] = load8<T>(p + col(k), d - col(k), false);
     }
-    // Rows base + j * stride, of which `rows` > 0 exist.
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int d) {
+    // Rows first.. of those at base + j * stride (j from `index` where not null, with IDX), of which `rows` > 0 are
+    // left. Only the addresses are made behind branches.
+    template <bool IDX>
+    __device__ __forceinline__ void load(const T* base, int64_t stride, const int32_t* index, int first, int rows, int d) {
+        const T* p[kPer];
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) load_row(k, base + min(inside(k) ? row(k) : 0, rows - 1) * stride, d);
+        for (int k = 0; k < kPer; ++k) p[k] = base + first * stride + min(inside(k) ? row(k) : 0, rows - 1) * stride;
+        if (IDX && index) {
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) p[k] = base + index[first + min(inside(k) ? row(k) : 0, rows - 1)] * stride;
+        }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) load_row(k, p[k], d);
     }
-    // To LDS, zeros for rows whose bit in `counts` is clear.
-    __device__ __forceinline__ void store(T* lds, uint64_t counts, int d) const {
+    // To LDS; then zeros over what lies past the `rows` that are left, or past d.
+    __device__ __forceinline__ void store(T* lds, int rows, int d) const {
         auto at = [&](int k) {
             return reinterpret_cast<typename Elem<T>::V8a*>(lds + row(k) * at_pitch<T, DP>() + col(k));
         };
-        if (counts == (N == 64 ? ~0ull : (1ull << (N & 63)) - 1) && d == DP) {
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (inside(k)) *at(k) = r[k];
+        if (rows < N || d < DP) {
 #pragma unroll
             for (int k = 0; k < kPer; ++k)
-                if (inside(k)) *at(k) = r[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < kPer; ++k)
-                if (inside(k)) *at(k) = ((counts >> row(k)) & 1) && col(k) < d ? r[k] : zero8<T>();
+                if (inside(k) && (row(k) >= rows || col(k) >= d)) *at(k) = zero8<T>();
         }
     }
 };
@@ -271,7 +320,7 @@ struct AtForward {
 
 // Workgroup: wavefronts of QB * 32 rows each of one kv head, the keys of one split. Online softmax in
 // base 2: O and l are relative to m, the largest c s so far to within kAtSlack.
-template <class T, int DP, bool VEC>
+template <class T, int DP, bool VEC, bool IDX>
 __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kPerSimd)) void k_attend(AtArgs a) {
     constexpr int TH = AtForward<T, DP>::kThreads, QB = AtForward<T, DP>::kBlocks;
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
@@ -305,21 +354,19 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
     const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
     const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
     AtTile<T, DP, KT, TH, VEC> tk, tv;
-    uint64_t next = 0;
+    const int32_t* const index = IDX && a.index ? a.index + (int64_t)kb * a.kv_len : nullptr;
     auto fetch = [&](int t) {
-        next = at_allowed(a, kb, len, t * KT, KT);
-        tk.load(kbase + (int64_t)t * KT * a.sk.l, a.sk.l, a.kv_len - t * KT, a.d);
-        tv.load(vbase + (int64_t)t * KT * a.sv.l, a.sv.l, a.kv_len - t * KT, a.d);
+        tk.template load<IDX>(kbase, a.sk.l, index, t * KT, len - t * KT, a.d);
+        tv.template load<IDX>(vbase, a.sv.l, index, t * KT, len - t * KT, a.d);
     };
     if (sp * per < t_end) fetch(sp * per);
     for (int t = sp * per; t < t_end; ++t) {
-        const uint64_t allowed = next;
+        const int left = len - t * KT;
         __syncthreads();
-        tk.store(s_k, allowed, a.d);
-        tv.store(s_v, allowed, a.d);
+        tk.store(s_k, left, a.d);
+        tv.store(s_v, left, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
-        if (allowed == 0) continue;
         f32x16 s[QB][KT / 32];
 #pragma unroll
         for (int kk = 0; kk < KT / 32; ++kk) {
@@ -334,13 +381,12 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
                 for (int qb = 0; qb < QB; ++qb) s[qb][kk] = mma(f, qf[qb][c], s[qb][kk]);
             }
         }
-        if (allowed != (KT == 64 ? ~0ull : 0xffffffffull)) {
-            const uint64_t mine = allowed >> (h * 4);
+        if (left < KT) {
 #pragma unroll
             for (int kk = 0; kk < KT / 32; ++kk)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const bool ok = (mine >> (kk * 32 + (i >> 2) * 8 + (i & 3))) & 1;
+                    const bool ok = kk * 32 + (i >> 2) * 8 + (i & 3) < left - h * 4;
 #pragma unroll
                     for (int qb = 0; qb < QB; ++qb) s[qb][kk][i] = ok ? s[qb][kk][i] : -INFINITY;
                 }
@@ -455,7 +501,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, in
 __device__ __forceinline__ float at_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
 // dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split.
-template <class T, int DP, bool VEC>
+template <class T, int DP, bool VEC, bool IDX>
 __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
@@ -496,23 +542,19 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
     const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
     const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
     AtTile<T, DP, KT, kAtThreads, VEC> tk, tv;
-    uint64_t next = 0;
+    const int32_t* const index = IDX && a.index ? a.index + (int64_t)kb * a.kv_len : nullptr;
     auto fetch = [&](int t) {
-        next = at_allowed(a, kb, len, t * KT, KT);
-        tk.load(kbase + (int64_t)t * KT * a.sk.l, a.sk.l, a.kv_len - t * KT, a.d);
-        tv.load(vbase + (int64_t)t * KT * a.sv.l, a.sv.l, a.kv_len - t * KT, a.d);
+        tk.template load<IDX>(kbase, a.sk.l, index, t * KT, len - t * KT, a.d);
+        tv.template load<IDX>(vbase, a.sv.l, index, t * KT, len - t * KT, a.d);
     };
     if (sp * per < t_end) fetch(sp * per);
     for (int t = sp * per; t < t_end; ++t) {
-        const uint64_t allowed = next;
+        const int left = len - t * KT;
         __syncthreads();
-        tk.store(s_k, allowed, a.d);
-        tv.store(s_v, allowed, a.d);
+        tk.store(s_k, left, a.d);
+        tv.store(s_v, left, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
-        if (allowed == 0) continue;
-        const uint64_t mine = allowed >> (h * 4);
-        const bool all = allowed == (KT == 64 ? ~0ull : 0xffffffffull);
 #pragma unroll
         for (int kk = 0; kk < KT / 32; ++kk) {
             f32x16 s, dp;
@@ -523,10 +565,10 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
                 s = mma(at_rows<T, DP>(s_k, kk * 32, c), qf[c], s);
                 dp = mma(at_rows<T, DP>(s_v, kk * 32, c), df[c], dp);
             }
-            if (!all) {
+            if (left < KT) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (!((mine >> (kk * 32 + (i >> 2) * 8 + (i & 3))) & 1)) s[i] = -INFINITY;
+                    s[i] = kk * 32 + (i >> 2) * 8 + (i & 3) < left - h * 4 ? s[i] : -INFINITY;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -567,19 +609,19 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
     const int j = (blk * kAtWaves + wave) * 32 + (lane & 31);
     const int len = at_length(a, kb);
-    bool ok = j < len;
-    if (a.mask && ok) ok = a.mask[kb * a.mask_stride + j] != 0;
+    const bool ok = j < len;
+    const int64_t key = j < a.kv_len ? at_key(a, kb, j) : 0;
 
     typename Elem<T>::V8 kf[NC], vf[NC];
-    at_load_row<T, DP, VEC>(kf, ok ? (const T*)a.k + kb * a.sk.b + hk * a.sk.h + j * a.sk.l : nullptr, a.d);
-    at_load_row<T, DP, VEC>(vf, ok ? (const T*)a.v + kb * a.sv.b + hk * a.sv.h + j * a.sv.l : nullptr, a.d);
+    at_load_row<T, DP, VEC>(kf, ok ? (const T*)a.k + kb * a.sk.b + hk * a.sk.h + key * a.sk.l : nullptr, a.d);
+    at_load_row<T, DP, VEC>(vf, ok ? (const T*)a.v + kb * a.sv.b + hk * a.sv.h + key * a.sv.l : nullptr, a.d);
     f32x16 gk[NB], gv[NB];
 #pragma unroll
     for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) gk[db][i] = gv[db][i] = 0.0f;
     const int tiles = (a.rows + RT - 1) / RT, per = (tiles + a.splits - 1) / a.splits;
-    const int t_end = __syncthreads_or(ok) ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
+    const int t_end = blk * kAtWaves * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
     AtTile<T, DP, RT, kAtThreads, VEC> tq, td;
     float st = 0.0f;
     auto fetch = [&](int t) {
@@ -601,10 +643,8 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     if (sp * per < t_end) fetch(sp * per);
     for (int t = sp * per; t < t_end; ++t) {
         __syncthreads();
-        const int left = a.rows - t * RT;
-        const uint64_t in = left >= RT ? (1ull << RT) - 1 : (1ull << left) - 1;
-        tq.store(s_q, in, a.d);
-        td.store(s_d, in, a.d);
+        tq.store(s_q, a.rows - t * RT, a.d);
+        td.store(s_d, a.rows - t * RT, a.d);
         if (threadIdx.x < RT) s_lse[threadIdx.x] = st;
         else if (threadIdx.x < 2 * RT) s_delta[threadIdx.x - RT] = st;
         __syncthreads();
@@ -646,8 +686,8 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     }
     if (a.splits == 1) {
         const bool in = j < a.kv_len;
-        at_store_row<T, DP>(in ? (T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + j * a.sdk.l : nullptr, gk, a.scale, a.d, a.vec_out);
-        at_store_row<T, DP>(in ? (T*)a.dv + kb * a.sdv.b + hk * a.sdv.h + j * a.sdv.l : nullptr, gv, 1.0f, a.d, a.vec_out);
+        at_store_row<T, DP>(in ? (T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + key * a.sdk.l : nullptr, gk, a.scale, a.d, a.vec_out);
+        at_store_row<T, DP>(in ? (T*)a.dv + kb * a.sdv.b + hk * a.sdv.h + key * a.sdv.l : nullptr, gv, 1.0f, a.d, a.vec_out);
     } else if (j < a.kv_len) {
         const int64_t all = (int64_t)(gridDim.x / (a.blocks * a.splits)) * a.kv_len;
         const int64_t pr = (2 * sp * all) + (int64_t)kvh * a.kv_len + j;
@@ -677,7 +717,8 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
         const int64_t rest = is_v ? pr - all : pr;
         const int j = (int)(rest % a.kv_len), kvh = (int)(rest / a.kv_len);
         const AtHeads& st = is_v ? a.sdv : a.sdk;
-        T* const p = (T*)(is_v ? a.dv : a.dk) + kvh / a.kv_heads * st.b + kvh % a.kv_heads * st.h + j * st.l;
+        T* const p = (T*)(is_v ? a.dv : a.dk) + kvh / a.kv_heads * st.b + kvh % a.kv_heads * st.h +
+                     at_key(a, kvh / a.kv_heads, j) * st.l;
         at_store4<T>(p + e, is_v ? x : x * a.scale, a.d - e, a.vec_out);
     }
 }
@@ -698,6 +739,18 @@ static int at_splits(int64_t workgroups, int64_t tiles, bool uneven) {
 }
 
 static int at_padded(int d) { return (d + 31) / 32 * 32; }
+
+// Makes the list of the allowed keys in `temp` where there is a mask.
+static int at_list(const tdgs_attention* a, AtArgs* r, void* temp, hipStream_t stream) {
+    if (!a->kv_mask || a->kv_len == 0) return TDGS_OK;
+    int32_t* const index = (int32_t*)temp;
+    int32_t* const counts = index + (int64_t)a->kv_batch * a->kv_len;
+    k_attend_list<<<(unsigned)a->kv_batch, kAtListThreads, 0, stream>>>(a->kv_mask, a->kv_mask_stride, *r, index, counts);
+    TDGS_LAUNCHED();
+    r->index = index;
+    r->lengths = counts;
+    return TDGS_OK;
+}
 
 // f(integral constant) for the padded head dimension.
 template <class F>
@@ -721,7 +774,7 @@ struct AtPlan {
     int64_t kvh, rows;   // kv heads over all kv batches; rows of each
     int dp, rows_f, tile;
     int blocks_f, splits_f, blocks_q, splits_q, blocks_k, splits_k;
-    size_t delta_bytes, forward_bytes, grad_bytes;
+    size_t list_bytes, delta_bytes, forward_bytes, grad_bytes;   // (the first two within the last two)
 };
 
 static AtPlan at_plan(const tdgs_attention* a, bool uneven) {
@@ -739,11 +792,13 @@ static AtPlan at_plan(const tdgs_attention* a, bool uneven) {
     p.blocks_k = (int)ceil_div(a->kv_len, kAtWaves * 32);
     p.splits_k = at_splits(p.blocks_k * p.kvh, row_tiles, uneven);
     const size_t all_rows = (size_t)(p.kvh * p.rows), all_keys = (size_t)(p.kvh * a->kv_len);
+    p.list_bytes = align_up((size_t)a->kv_batch * ((size_t)a->kv_len + 1) * sizeof(int32_t));
     p.delta_bytes = align_up(all_rows * sizeof(float));
-    p.forward_bytes = p.splits_f > 1 ? p.splits_f * (align_up(all_rows * p.dp * sizeof(float)) + align_up(all_rows * 2 * sizeof(float))) : 0;
+    p.forward_bytes = (uneven ? p.list_bytes : 0) +
+                      (p.splits_f > 1 ? align_up(p.splits_f * all_rows * (p.dp + 2) * sizeof(float)) : 0);
     const size_t q = p.splits_q > 1 ? p.splits_q * all_rows * p.dp * sizeof(float) : 0;
     const size_t k = p.splits_k > 1 ? p.splits_k * 2 * all_keys * p.dp * sizeof(float) : 0;
-    p.grad_bytes = p.delta_bytes + align_up(q > k ? q : k);
+    p.grad_bytes = (uneven ? p.list_bytes : 0) + p.delta_bytes + align_up(q > k ? q : k);
     return p;
 }
 
@@ -797,8 +852,6 @@ static AtArgs at_args(const tdgs_attention* a, const AtPlan& p) {
     r.sv = at_strides(a->v);
     r.so = at_strides(a->out);
     r.lengths = a->kv_lengths;
-    r.mask = a->kv_mask;
-    r.mask_stride = a->kv_mask_stride;
     r.lse = a->lse;
     r.q_len = a->q_len;
     r.kv_len = a->kv_len;
@@ -842,7 +895,8 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
         TDGS_TRY(at_check_view(&a->k, "k", a, true, false));
         TDGS_TRY(at_check_view(&a->v, "v", a, true, false));
     }
-    const AtPlan p = at_plan(a, a->kv_lengths || a->kv_mask);
+    const bool uneven = a->kv_lengths || a->kv_mask;
+    const AtPlan p = at_plan(a, uneven);
     TDGS_REQUIRE(p.forward_bytes == 0 || (a->temp && a->temp_bytes >= p.forward_bytes && aligned_to(a->temp, 16)),
                  "attention: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, p.forward_bytes);
     hipStream_t stream = (hipStream_t)stream_;
@@ -850,8 +904,9 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
     r.blocks = p.blocks_f;
     r.splits = p.splits_f;
     const int64_t all = p.kvh * p.rows;
+    TDGS_TRY(at_list(a, &r, a->temp, stream));
     if (p.splits_f > 1) {
-        r.part = (float*)a->temp;
+        r.part = (float*)((char*)a->temp + (uneven ? p.list_bytes : 0));
         r.part_ml = r.part + p.splits_f * all * p.dp;
     }
     const int64_t e = dtype_size(a->dtype);
@@ -862,8 +917,9 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
         using T = decltype(t);
         TDGS_TRY(with_padded(p.dp, [&](auto dp) -> int {
             constexpr int DP = decltype(dp)::value, TH = AtForward<T, DP>::kThreads;
-            if (vec) k_attend<T, DP, true><<<grid, TH, 0, stream>>>(r);
-            else k_attend<T, DP, false><<<grid, TH, 0, stream>>>(r);
+            if (vec && !r.index) k_attend<T, DP, true, false><<<grid, TH, 0, stream>>>(r);
+            else if (vec) k_attend<T, DP, true, true><<<grid, TH, 0, stream>>>(r);
+            else k_attend<T, DP, false, true><<<grid, TH, 0, stream>>>(r);
             TDGS_LAUNCHED();
             return TDGS_OK;
         }));
@@ -894,7 +950,8 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
         TDGS_TRY(at_check_view(&g->dk, "dk", a, true, true));
         TDGS_TRY(at_check_view(&g->dv, "dv", a, true, true));
     }
-    const AtPlan p = at_plan(a, a->kv_lengths || a->kv_mask);
+    const bool uneven = a->kv_lengths || a->kv_mask;
+    const AtPlan p = at_plan(a, uneven);
     TDGS_REQUIRE(a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16),
                  "attention: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0,
                  p.grad_bytes);
@@ -912,8 +969,9 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
     const bool vec = r.vec_out && at_rows_aligned(a->q, e) && at_rows_aligned(g->dout, e) && at_rows_aligned(a->k, e) &&
                      at_rows_aligned(a->v, e);
     r.vec_out = a->head_dim % 8 == 0 && at_rows_aligned(g->dq, e) && at_rows_aligned(g->dk, e) && at_rows_aligned(g->dv, e);
-    r.delta = (float*)a->temp;
-    r.part = (float*)((char*)a->temp + p.delta_bytes);
+    TDGS_TRY(at_list(a, &r, a->temp, stream));
+    r.delta = (float*)((char*)a->temp + (uneven ? p.list_bytes : 0));
+    r.part = (float*)((char*)r.delta + p.delta_bytes);
     const int64_t all_rows = p.kvh * p.rows, all_keys = p.kvh * a->kv_len;
     return with_dtype(a->dtype, [&](auto t) -> int {
         using T = decltype(t);
@@ -923,8 +981,9 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
                 r.blocks = p.blocks_q;
                 r.splits = p.splits_q;
                 const unsigned grid = (unsigned)(p.kvh * p.splits_q * p.blocks_q);
-                if (vec) k_attend_dq<T, DP, true><<<grid, kAtThreads, 0, stream>>>(r);
-                else k_attend_dq<T, DP, false><<<grid, kAtThreads, 0, stream>>>(r);
+                if (vec && !r.index) k_attend_dq<T, DP, true, false><<<grid, kAtThreads, 0, stream>>>(r);
+                else if (vec) k_attend_dq<T, DP, true, true><<<grid, kAtThreads, 0, stream>>>(r);
+                else k_attend_dq<T, DP, false, true><<<grid, kAtThreads, 0, stream>>>(r);
                 TDGS_LAUNCHED();
                 if (p.splits_q > 1) {
                     k_attend_sum<T><<<(unsigned)ceil_div(all_rows * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
