@@ -211,6 +211,47 @@ __device__ __forceinline__ typename Elem<T>::V8 at_pack(const f32x16& s, int hal
     return r;
 }
 
+// The same as a sum of two operands of a 16-bit type: what the rounding to T leaves goes into `rest`.
+template <class T>
+__device__ __forceinline__ void at_pack2(const f32x16& s, int half, typename Elem<T>::V8& r, typename Elem<T>::V8& rest) {
+    if constexpr (std::is_same<T, bf16>::value) {   // (the upper halves as they are: what they leave is exact either way)
+        uint32_t hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float fx = s[half * 8 + 2 * i], fy = s[half * 8 + 2 * i + 1];   // (copies: this compiler casts element 0
+            const uint32_t x = __builtin_bit_cast(uint32_t, fx), y = __builtin_bit_cast(uint32_t, fy);   // of a vector only)
+            hi[i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+            rest[2 * i] = (T)(fx - __builtin_bit_cast(float, x & 0xffff0000u));
+            rest[2 * i + 1] = (T)(fy - __builtin_bit_cast(float, y & 0xffff0000u));
+        }
+        typedef uint32_t U4 __attribute__((ext_vector_type(4)));
+        const U4 v = {hi[0], hi[1], hi[2], hi[3]};
+        r = __builtin_bit_cast(typename Elem<T>::V8, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            r[i] = (T)s[half * 8 + i];
+            rest[i] = (T)(s[half * 8 + i] - (float)r[i]);
+        }
+    }
+}
+
+// Eight registers of a block of results S as an operand: acc + A S. Rounded to T, or with TWO as two operands of a 16-bit
+// type, by which S keeps 16 or more bits at the price of a second product.
+template <class T, bool TWO>
+struct AtOperand {
+    static constexpr bool kTwo = TWO && sizeof(T) == 2;
+    typename Elem<T>::V8 b, rest;
+    __device__ __forceinline__ AtOperand(const f32x16& s, int half) {
+        if constexpr (kTwo) at_pack2<T>(s, half, b, rest);
+        else b = at_pack<T>(s, half);
+    }
+    __device__ __forceinline__ f32x16 product(typename Elem<T>::V8 a, f32x16 acc) const {
+        if constexpr (kTwo) acc = mma(a, rest, acc);
+        return mma(a, b, acc);
+    }
+};
+
 // Row r's elements in the order of a B operand's lanes (row l % 32 of the block): chunk c of DP / 16.
 template <class T, int DP, bool VEC>
 __device__ __forceinline__ void at_load_row(typename Elem<T>::V8 (&f)[DP / 16], const T* p, int d) {
@@ -320,7 +361,7 @@ struct AtForward {
 
 // Workgroup: wavefronts of QB * 32 rows each of one kv head, the keys of one split. Online softmax in
 // base 2: O and l are relative to m, the largest c s so far to within kAtSlack.
-template <class T, int DP, bool VEC, bool IDX>
+template <class T, int DP, bool VEC, bool IDX, bool TWO>
 __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kPerSimd)) void k_attend(AtArgs a) {
     constexpr int TH = AtForward<T, DP>::kThreads, QB = AtForward<T, DP>::kBlocks;
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
@@ -422,14 +463,11 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
         }
 #pragma unroll
         for (int ks = 0; ks < KT / 16; ++ks) {
-            typename Elem<T>::V8 p[QB];
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) p[qb] = at_pack<T>(s[qb][ks / 2], ks % 2);
+            for (int qb = 0; qb < QB; ++qb) {
+                const AtOperand<T, TWO> p(s[qb][ks / 2], ks % 2);
 #pragma unroll
-            for (int db = 0; db < NB; ++db) {
-                const auto f = at_cols<T, DP>(s_v, ks * 16, db);
-#pragma unroll
-                for (int qb = 0; qb < QB; ++qb) o[qb][db] = mma(f, p[qb], o[qb][db]);
+                for (int db = 0; db < NB; ++db) o[qb][db] = p.product(at_cols<T, DP>(s_v, ks * 16, db), o[qb][db]);
             }
         }
     }
@@ -502,7 +540,7 @@ __device__ __forceinline__ float at_lse2(float lse) { return lse == -INFINITY ? 
 
 // dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split.
 template <class T, int DP, bool VEC, bool IDX>
-__global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
+__global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) void k_attend_dq(AtArgs a) {
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
     __shared__ __attribute__((aligned(16))) T s_v[KT * P];
@@ -526,12 +564,10 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) delta = __builtin_fmaf((float)df[c][i], (float)of[c][i], delta);
         delta = sum_halves(delta);
-        if (r < a.rows) {
-            lse2 = at_lse2(a.lse[at_stat(a, row)]);
-            if (sp == 0 && h == 0) a.delta[at_stat(a, row)] = delta;
-        }
+        if (r < a.rows) lse2 = at_lse2(a.lse[at_stat(a, row)]);
     }
     f32x16 o[NB];
+    float slip = 0.0f;   // the row's sum of dS, which an exact delta makes zero
 #pragma unroll
     for (int db = 0; db < NB; ++db)
 #pragma unroll
@@ -555,6 +591,27 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
         tv.store(s_v, left, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
+        if (sizeof(T) == 2 && len <= KT) {
+            // the row's sum of p dp instead of dout . out, whose rounding would show where few keys share a row
+            delta = 0.0f;
+#pragma unroll
+            for (int kk = 0; kk < KT / 32; ++kk) {
+                f32x16 s, dp;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    s = mma(at_rows<T, DP>(s_k, kk * 32, c), qf[c], s);
+                    dp = mma(at_rows<T, DP>(s_v, kk * 32, c), df[c], dp);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = kk * 32 + (i >> 2) * 8 + (i & 3) < left - h * 4 ? s[i] : -INFINITY;
+                    delta = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x, a.c, -lse2)), dp[i], delta);
+                }
+            }
+            delta = sum_halves(delta);
+        }
 #pragma unroll
         for (int kk = 0; kk < KT / 32; ++kk) {
             f32x16 s, dp;
@@ -571,15 +628,23 @@ __global__ __launch_bounds__(kAtThreads, 2) void k_attend_dq(AtArgs a) {
                     s[i] = kk * 32 + (i >> 2) * 8 + (i & 3) < left - h * 4 ? s[i] : -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 16; ++i) {
                 s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, -lse2)) * (dp[i] - delta);
+                slip += s[i];
+            }
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const auto b = at_pack<T>(s, ks);
+                const AtOperand<T, true> b(s, ks);
 #pragma unroll
-                for (int db = 0; db < NB; ++db) o[db] = mma(at_cols<T, DP>(s_k, kk * 32 + ks * 16, db), b, o[db]);
+                for (int db = 0; db < NB; ++db) o[db] = b.product(at_cols<T, DP>(s_k, kk * 32 + ks * 16, db), o[db]);
             }
         }
+    }
+    // dK takes delta with what the rows' sums have shown to be its error; over several splits the join adds it up
+    slip = sum_halves(slip);
+    if (h == 0 && r < a.rows) {
+        if (a.splits == 1) a.delta[at_stat(a, row)] = delta + slip;
+        else a.part_ml[((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r] = sp == 0 ? delta + slip : slip;
     }
     if (a.splits == 1) {
         at_store_row<T, DP>(r < a.rows ? (T*)a.dq + at_offset(a.sdq, row) : nullptr, o, a.scale, a.d, a.vec_out);
@@ -596,7 +661,7 @@ template <class T, int DP>
 constexpr int at_dkv_per_simd() { return sizeof(T) == 4 && DP > 96 ? 1 : 2; }
 
 // dK and dV. Workgroup: 4 wavefronts of 32 keys each, the rows of one split.
-template <class T, int DP, bool VEC>
+template <class T, int DP, bool VEC, bool TWO>
 __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(AtArgs a) {
     constexpr int RT = 32, P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_q[RT * P];
@@ -670,11 +735,11 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            const auto p = at_pack<T>(s, ks), ds = at_pack<T>(dp, ks);
+            const AtOperand<T, TWO> p(s, ks), ds(dp, ks);
 #pragma unroll
             for (int db = 0; db < NB; ++db) {
-                gv[db] = mma(at_cols<T, DP>(s_d, ks * 16, db), p, gv[db]);
-                gk[db] = mma(at_cols<T, DP>(s_q, ks * 16, db), ds, gk[db]);
+                gv[db] = p.product(at_cols<T, DP>(s_d, ks * 16, db), gv[db]);
+                gk[db] = ds.product(at_cols<T, DP>(s_q, ks * 16, db), gk[db]);
             }
         }
     }
@@ -712,6 +777,11 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
         const int kvh = (int)(pr / a.rows);
         const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr % a.rows));
         at_store4<T>((T*)a.dq + at_offset(a.sdq, row) + e, x * a.scale, a.d - e, a.vec_out);
+        if (e == 0) {
+            float delta = 0.0f;
+            for (int s = 0; s < a.splits; ++s) delta += a.part_ml[s * n + pr];
+            a.delta[at_stat(a, row)] = delta;
+        }
     } else {
         const bool is_v = pr >= all;
         const int64_t rest = is_v ? pr - all : pr;
@@ -730,6 +800,11 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
 // With lengths or a mask, workgroups end at different times, and twice as many parts even that out.
 constexpr int64_t kAtWorkgroups = 512;
 constexpr int kAtSplits = 64;
+
+// Results (elements of out; of dK) up to which P, and dS for dK, keep their bits by a second product. Rounded to a 16-bit
+// type they leave an error as large as the results' own rounding, 1.4 times that together; over a large
+// tensor it stays there, over a few results it may come to twice that.
+constexpr int64_t kAtFewResults = 1 << 16;
 
 static int at_splits(int64_t workgroups, int64_t tiles, bool uneven) {
     int64_t s = workgroups > 0 ? (uneven ? 2 : 1) * kAtWorkgroups / workgroups : 1;
@@ -796,7 +871,7 @@ static AtPlan at_plan(const tdgs_attention* a, bool uneven) {
     p.delta_bytes = align_up(all_rows * sizeof(float));
     p.forward_bytes = (uneven ? p.list_bytes : 0) +
                       (p.splits_f > 1 ? align_up(p.splits_f * all_rows * (p.dp + 2) * sizeof(float)) : 0);
-    const size_t q = p.splits_q > 1 ? p.splits_q * all_rows * p.dp * sizeof(float) : 0;
+    const size_t q = p.splits_q > 1 ? p.splits_q * all_rows * (p.dp + 1) * sizeof(float) : 0;
     const size_t k = p.splits_k > 1 ? p.splits_k * 2 * all_keys * p.dp * sizeof(float) : 0;
     p.grad_bytes = (uneven ? p.list_bytes : 0) + p.delta_bytes + align_up(q > k ? q : k);
     return p;
@@ -917,9 +992,14 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
         using T = decltype(t);
         TDGS_TRY(with_padded(p.dp, [&](auto dp) -> int {
             constexpr int DP = decltype(dp)::value, TH = AtForward<T, DP>::kThreads;
-            if (vec && !r.index) k_attend<T, DP, true, false><<<grid, TH, 0, stream>>>(r);
-            else if (vec) k_attend<T, DP, true, true><<<grid, TH, 0, stream>>>(r);
-            else k_attend<T, DP, false, true><<<grid, TH, 0, stream>>>(r);
+            auto launch = [&](auto two) {
+                constexpr bool TWO = decltype(two)::value;
+                if (vec && !r.index && !TWO) k_attend<T, DP, true, false, false><<<grid, TH, 0, stream>>>(r);
+                else if (vec) k_attend<T, DP, true, true, TWO><<<grid, TH, 0, stream>>>(r);
+                else k_attend<T, DP, false, true, TWO><<<grid, TH, 0, stream>>>(r);
+            };
+            if (sizeof(T) == 2 && all * a->head_dim <= kAtFewResults) launch(std::integral_constant<bool, sizeof(T) == 2>{});
+            else launch(std::false_type{});
             TDGS_LAUNCHED();
             return TDGS_OK;
         }));
@@ -980,6 +1060,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
             if (a->q_len > 0) {
                 r.blocks = p.blocks_q;
                 r.splits = p.splits_q;
+                r.part_ml = r.part + p.splits_q * all_rows * DP;
                 const unsigned grid = (unsigned)(p.kvh * p.splits_q * p.blocks_q);
                 if (vec && !r.index) k_attend_dq<T, DP, true, false><<<grid, kAtThreads, 0, stream>>>(r);
                 else if (vec) k_attend_dq<T, DP, true, true><<<grid, kAtThreads, 0, stream>>>(r);
@@ -995,8 +1076,13 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
                 r.blocks = p.blocks_k;
                 r.splits = p.splits_k;
                 const unsigned grid = (unsigned)(p.kvh * p.splits_k * p.blocks_k);
-                if (vec) k_attend_dkv<T, DP, true><<<grid, kAtThreads, 0, stream>>>(r);
-                else k_attend_dkv<T, DP, false><<<grid, kAtThreads, 0, stream>>>(r);
+                auto launch = [&](auto two) {
+                    constexpr bool TWO = decltype(two)::value;
+                    if (vec) k_attend_dkv<T, DP, true, TWO><<<grid, kAtThreads, 0, stream>>>(r);
+                    else k_attend_dkv<T, DP, false, TWO><<<grid, kAtThreads, 0, stream>>>(r);
+                };
+                if (sizeof(T) == 2 && all_keys * a->head_dim <= kAtFewResults) launch(std::integral_constant<bool, sizeof(T) == 2>{});
+                else launch(std::false_type{});
                 TDGS_LAUNCHED();
                 if (p.splits_k > 1) {
                     k_attend_sum<T><<<(unsigned)ceil_div(2 * all_keys * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
