@@ -40,6 +40,10 @@ SIZES = [
     (4097, 255, 512, "skewed"),
     (700, 50, 1000, "skewed"),
     (9000, 5000, 130, "any"),
+    (4096, 9, 4, "skewed"),        # the most that one launch takes, of one token nearly
+    (4096, 100000, 16, "any"),
+    (3000, 5000000, 1, "any"),     # more rows than 2^12 for each of 1024 workgroups
+    (100000, 3, 5, "skewed"),
 ]
 
 

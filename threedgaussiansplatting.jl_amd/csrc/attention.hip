@@ -389,6 +389,7 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[qb][db][i] = 0.0f;
     }
+    const bool busy = blk * AtForward<T, DP>::kRows + wave * (QB * 32) < a.rows;   // (the others only bring keys)
     const int len = at_length(a, kb);
     const int tiles = (len + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
     const int t_end = min(tiles, (sp + 1) * per);
@@ -408,6 +409,7 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
         tv.store(s_v, left, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
+        if (!busy) continue;
         f32x16 s[QB][KT / 32];
 #pragma unroll
         for (int kk = 0; kk < KT / 32; ++kk) {
@@ -572,6 +574,7 @@ __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) v
     for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
+    const bool busy = (blk * kAtWaves + wave) * 32 < a.rows;
     const int len = at_length(a, kb);
     const int tiles = (len + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
     const int t_end = min(tiles, (sp + 1) * per);
@@ -591,6 +594,7 @@ __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) v
         tv.store(s_v, left, a.d);
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
+        if (!busy) continue;
         if (sizeof(T) == 2 && len <= KT) {
             // the row's sum of p dp instead of dout . out, whose rounding would show where few keys share a row
             delta = 0.0f;
@@ -674,7 +678,7 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
     const int j = (blk * kAtWaves + wave) * 32 + (lane & 31);
     const int len = at_length(a, kb);
-    const bool ok = j < len;
+    const bool ok = j < len, busy = (blk * kAtWaves + wave) * 32 < len;
     const int64_t key = j < a.kv_len ? at_key(a, kb, j) : 0;
 
     typename Elem<T>::V8 kf[NC], vf[NC];
@@ -714,6 +718,7 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
         else if (threadIdx.x < 2 * RT) s_delta[threadIdx.x - RT] = st;
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
+        if (!busy) continue;
         f32x16 s, dp;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;

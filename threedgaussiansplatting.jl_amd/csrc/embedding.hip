@@ -5,8 +5,8 @@
 // token's rows follow each other. A workgroup takes a block of sorted positions, a group of lanes (as many as a row
 // has 16-byte vectors) each a run of it, summing in registers; tokens that span runs are joined in LDS,
 // tokens that span blocks afterwards from the blocks' partial sums, in order. No float is added
-// atomically: the result does not depend on which workgroup runs first. A few tokens (kEmFew) take one
-// launch instead: every workgroup picks, and sorts, those of its own rows of the table.
+// atomically: the result does not depend on which workgroup runs first. A few tokens take one launch
+// instead: every workgroup picks, and sorts, those of its own rows of the table.
 #include "internal.hpp"
 #include "elem.hpp"
 #include "sort.hpp"
@@ -16,7 +16,7 @@ namespace tdgs {
 constexpr int kEmThreads = 256;
 constexpr int kEmBlock = 2048;   // the most sorted positions of a workgroup
 constexpr int kEmRun = 32;       // and of one of its runs
-constexpr int kEmFew = 1024;     // tokens up to which one launch is taken
+constexpr int kEmFew = 4096;     // the most tokens that one launch is taken for
 
 struct EmArgs {
     const void *table, *dout, *tokens;
@@ -24,13 +24,12 @@ struct EmArgs {
     int64_t table_stride, out_stride, dout_stride, dtable_stride, n, vocab, padding, blocks;
     const uint32_t* keys;    // sorted tokens; vocab where there is nothing to add
     const int32_t* order;    // their positions
-    uint8_t* present;        // whether a token occurs
     float* part;             // 2 rows per block: of the token it begins within, of the token it ends within
     int32_t *list, *count;   // blocks that a token starts in and goes on past; their number
     uint32_t* err;
     float scale;
     int32_t dim, vectors, lanes;   // elements, vectors and lanes per row
-    int32_t run, rows;             // positions per run; table rows per workgroup (one launch)
+    int32_t run, rows, few;        // positions per run; of one launch: table rows per workgroup, tokens (2^k)
     bool tokens64;
 };
 
@@ -83,23 +82,29 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_lookup(EmArgs a, FastDiv b
     }
 }
 
-static __global__ __launch_bounds__(kEmThreads) void k_embed_clear(uint32_t* __restrict__ words, int64_t n) {
-    const int64_t i = (int64_t)blockIdx.x * kEmThreads + threadIdx.x;
-    if (i < n) words[i] = 0;
-}
-
-// Sort keys and values: tokens and positions; tokens to leave out sort past the table's end.
-static __global__ __launch_bounds__(kEmThreads) void k_embed_keys(EmArgs a, uint32_t* __restrict__ keys,
-                                                                  int32_t* __restrict__ values) {
-    const int64_t i = (int64_t)blockIdx.x * kEmThreads + threadIdx.x;
-    if (i >= a.n) return;
-    const int64_t tok = em_token(a, i);
-    const bool in = tok >= 0 && tok < a.vocab;
-    if (!in) atomicOr(a.err, kErrTokenRange);
-    const bool use = in && tok != a.padding;
-    if (use) a.present[tok] = 1;
-    keys[i] = use ? (uint32_t)tok : (uint32_t)a.vocab;
-    values[i] = (int32_t)i;
+// Sort keys and values: tokens and positions; tokens to leave out sort past the table's end. Also clears
+// the `words` that the sort and the list count in, and dtable, whose rows that a token names are written over
+// later: that costs less than keeping account of the others.
+template <class T, int VW>
+__global__ __launch_bounds__(kEmThreads) void k_embed_keys(EmArgs a, uint32_t* __restrict__ keys,
+                                                           int32_t* __restrict__ values, uint32_t* __restrict__ clear,
+                                                           int64_t words, FastDiv by_vectors) {
+    const int64_t id = (int64_t)blockIdx.x * kEmThreads + threadIdx.x, step = (int64_t)gridDim.x * kEmThreads;
+    for (int64_t i = id; i < a.n; i += step) {
+        const int64_t tok = em_token(a, i);
+        const bool in = tok >= 0 && tok < a.vocab;
+        if (!in) atomicOr(a.err, kErrTokenRange);
+        keys[i] = in && tok != a.padding ? (uint32_t)tok : (uint32_t)a.vocab;
+        values[i] = (int32_t)i;
+    }
+    for (int64_t i = id; i < words; i += step) clear[i] = 0;
+    EmVec<T, VW> z;
+    z.zero();
+    const int64_t total = a.vocab * a.vectors;
+    for (int64_t i = id; i < total; i += step) {
+        const int64_t row = total <= INT32_MAX ? (int64_t)by_vectors.div((uint32_t)i) : i / a.vectors;
+        z.store((T*)a.dtable + row * a.dtable_stride + (i - row * a.vectors) * VW, 0.0f);
+    }
 }
 
 // Sums a block of sorted positions, `count` of them from LDS (their tokens, and rows of dout): group g of
@@ -197,8 +202,7 @@ __device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key,
     return starts;
 }
 
-// The first workgroups: a block of sorted positions each; the others: rows of the table that no token
-// names become zero.
+// A block of sorted positions per workgroup.
 template <class T, int VW>
 __global__ __launch_bounds__(kEmThreads) void k_embed_sums(EmArgs a) {
     __shared__ uint32_t s_key[kEmBlock];
@@ -208,16 +212,6 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_sums(EmArgs a) {
     __shared__ uint32_t s_flag[kEmThreads];
     const int groups = kEmThreads / a.lanes;
     const uint32_t none = (uint32_t)a.vocab;
-    if ((int64_t)blockIdx.x >= a.blocks) {
-        const int sub = (int)threadIdx.x / a.lanes, vec = blockIdx.y * kWave + (int)threadIdx.x % a.lanes;
-        if (sub >= groups || vec >= a.vectors) return;
-        const int64_t step = (gridDim.x - a.blocks) * groups;
-        EmVec<T, VW> z;
-        z.zero();
-        for (int64_t v = (blockIdx.x - a.blocks) * groups + sub; v < a.vocab; v += step)
-            if (!a.present[v]) z.store((T*)a.dtable + v * a.dtable_stride + vec * VW, 0.0f);
-        return;
-    }
     const int size = groups * a.run;
     const int64_t i0 = (int64_t)blockIdx.x * size, i1 = min(a.n, i0 + size);
     for (int i = threadIdx.x; i < (int)(i1 - i0); i += kEmThreads) {
@@ -283,19 +277,22 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_join(EmArgs a) {
     }
 }
 
-// One launch for a few tokens: workgroup x takes a.rows rows of the table, picks the tokens that name them, ranks
-// them (by token, then position), sums, and writes zeros where no token does.
+// One launch for a few tokens: workgroup x takes a.rows <= 4096 rows of the table, picks the tokens that name them,
+// sorts them (by token, then position), sums, and writes zeros where no token does.
 template <class T, int VW>
 __global__ __launch_bounds__(kEmThreads) void k_embed_few(EmArgs a) {
-    __shared__ uint32_t s_tok[kEmFew], s_key[kEmFew];
-    __shared__ int32_t s_at[kEmFew], s_row[kEmFew];
+    extern __shared__ uint32_t s_list[];   // keys, rows and positions of a.few tokens each
     __shared__ float s_head[kEmThreads * VW];
     __shared__ float s_tail[kEmThreads * VW];
     __shared__ uint32_t s_flag[kEmThreads];
     __shared__ int s_wave[kEmThreads / kWave], s_count;
+    uint32_t* const s_key = s_list;
+    int32_t* const s_row = (int32_t*)s_list + a.few;
+    uint16_t* const s_at = (uint16_t*)(s_list + 2 * a.few);
     const int64_t v0 = (int64_t)blockIdx.x * a.rows, v1 = min(a.vocab, v0 + a.rows);
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, n = (int)a.n;
     if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
     for (int i0 = 0; i0 < n; i0 += kEmThreads) {
         const int i = i0 + threadIdx.x;
         int64_t tok = -1;
@@ -311,21 +308,35 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_few(EmArgs a) {
         for (int w = 0; w < wave; ++w) at += s_wave[w];
         at += __popcll(votes & lanemask_lt());
         if (mine) {
-            s_tok[at] = (uint32_t)tok;
-            s_at[at] = i;
+            s_key[at] = (uint32_t)(tok - v0) << 12 | (uint32_t)at;   // (at < kEmFew = 2^12)
+            s_at[at] = (uint16_t)i;
         }
         __syncthreads();
         if (threadIdx.x == kEmThreads - 1) s_count = at + (mine ? 1 : 0);
         __syncthreads();
     }
-    __syncthreads();
     const int count = s_count;
+    // sort by halves that rise and fall, padded to a power of two (at most a.few, which is one)
+    int size = 1;
+    while (size < count) size *= 2;
+    for (int i = count + threadIdx.x; i < size; i += kEmThreads) s_key[i] = 0xffffffffu;
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            __syncthreads();
+            for (int t = threadIdx.x; t < size / 2; t += kEmThreads) {
+                const int lo = (t & (j - 1)) | (t & ~(j - 1)) << 1, hi = lo | j;
+                const uint32_t x = s_key[lo], y = s_key[hi];
+                if ((x > y) == ((lo & k) == 0)) {
+                    s_key[lo] = y;
+                    s_key[hi] = x;
+                }
+            }
+        }
+    __syncthreads();
     for (int i = threadIdx.x; i < count; i += kEmThreads) {
-        const uint32_t tok = s_tok[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += (s_tok[j] < tok || (s_tok[j] == tok && j < i)) ? 1 : 0;
-        s_key[rank] = tok;
-        s_row[rank] = s_at[i];
+        const uint32_t key = s_key[i];
+        s_row[i] = s_at[key & 0xfffu];
+        s_key[i] = (uint32_t)v0 + (key >> 12);
     }
     __syncthreads();
     const int groups = kEmThreads / a.lanes, sub = (int)threadIdx.x / a.lanes;
@@ -336,7 +347,7 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_few(EmArgs a) {
     EmVec<T, VW> z;
     z.zero();
     for (int64_t v = v0 + sub; v < v1; v += groups) {
-        int lo = 0, hi = count;   // the first rank whose token is v or above
+        int lo = 0, hi = count;   // the first place whose token is v or above
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
             if (s_key[mid] < (uint32_t)v) lo = mid + 1;
@@ -365,8 +376,16 @@ static int em_run(int64_t n, int groups) {
 
 static int em_lanes(int vectors) { return vectors < kWave ? vectors : kWave; }
 
+// Whether one launch takes n tokens: a thousand, or more where a workgroup has so many lane groups that even if they
+// are all one token, a group has 64 rows to add.
+static bool em_few(int64_t n, int groups) {
+    const int64_t most = 64 * groups < kEmFew ? 64 * groups : kEmFew;
+    return n <= (most > 1024 ? most : 1024);
+}
+
 struct EmPlan {
     int vectors, lanes, run;
+    bool few;
     int64_t blocks, group_words, clear_words;
     size_t sort_bytes, bytes;
 };
@@ -375,14 +394,15 @@ static EmPlan em_plan(int64_t n, int64_t vocab, int32_t dim, int vw) {
     EmPlan p = {};
     p.vectors = dim / vw;
     p.lanes = em_lanes(p.vectors);
-    if (n <= kEmFew) return p;
     const int groups = kEmThreads / p.lanes;
+    p.few = em_few(n, groups);
+    if (p.few) return p;
     p.run = em_run(n, groups);
     p.blocks = ceil_div(n, (int64_t)groups * p.run);
     p.sort_bytes = radix_temp_bytes(n);
     p.group_words = radix_tiles<uint32_t>(n) <= RsTile<uint32_t>::kGroupedTiles
                         ? radix_group_words<uint32_t>(n, 0, em_bits(vocab)) : 0;
-    p.clear_words = p.group_words + 1 + ceil_div(vocab, 4);   // group sums, the list's count, present
+    p.clear_words = p.group_words + 1;   // group sums, the list's count
     ArenaSize s;
     s.take<uint32_t>(p.clear_words);
     for (int i = 0; i < 3; ++i) {
@@ -512,14 +532,18 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     a.blocks = p.blocks;
     const int groups = kEmThreads / a.lanes;
     const unsigned column_blocks = (unsigned)ceil_div(a.vectors, kWave);
-    if (n <= kEmFew) {
-        // a group of lanes takes a row at a time; at least four workgroups per CU where the table has the rows
+    if (p.few) {
+        // a group of lanes takes a row at a time; four workgroups per CU where the table has the rows, but
+        // no more than 2^12 of them in one
         int64_t rows = ceil_div(vocab, 1024);
         if (rows < groups) rows = groups;
+        if (rows > kEmFew) rows = kEmFew;
         a.rows = (int32_t)rows;
+        a.few = 1;
+        while (a.few < n) a.few *= 2;
         return em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
-            k_embed_few<decltype(t), decltype(w)::value>
-                <<<dim3((unsigned)ceil_div(vocab, rows), column_blocks), kEmThreads, 0, stream>>>(a);
+            k_embed_few<decltype(t), decltype(w)::value><<<dim3((unsigned)ceil_div(vocab, rows), column_blocks), kEmThreads,
+                                                           (size_t)a.few * (2 * sizeof(uint32_t) + sizeof(uint16_t)), stream>>>(a);
             TDGS_LAUNCHED();
             return TDGS_OK;
         });
@@ -536,22 +560,23 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     a.list = ar.take<int32_t>(p.blocks);
     a.count = (int32_t*)clear + p.group_words;
     a.part = ar.take<float>(2 * p.blocks * dim);
-    a.present = (uint8_t*)(clear + p.group_words + 1);
     a.keys = k[1];
     a.order = v[1];
-    k_embed_clear<<<(unsigned)ceil_div(p.clear_words, kEmThreads), kEmThreads, 0, stream>>>(clear, p.clear_words);
-    TDGS_LAUNCHED();
-    k_embed_keys<<<(unsigned)ceil_div(n, kEmThreads), kEmThreads, 0, stream>>>(a, k[0], v[0]);
-    TDGS_LAUNCHED();
+    int64_t key_blocks = ceil_div(n > vocab * a.vectors ? n : vocab * a.vectors, kEmThreads);
+    if (key_blocks > 8192) key_blocks = 8192;
+    TDGS_TRY(em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
+        k_embed_keys<decltype(t), decltype(w)::value><<<(unsigned)key_blocks, kEmThreads, 0, stream>>>(
+            a, k[0], v[0], clear, p.clear_words, FastDiv((uint32_t)a.vectors));
+        TDGS_LAUNCHED();
+        return TDGS_OK;
+    }));
     TDGS_TRY(radix_sort_pairs_grouped<uint32_t>(k[0], k[1], v[0], v[1], k[2], v[2], n, 0, em_bits(vocab), sort_temp,
                                                 p.sort_bytes, p.group_words > 0 ? clear : nullptr, p.group_words,
                                                 stream, a.err));
-    int64_t zero_blocks = ceil_div(vocab, groups);
-    if (zero_blocks > 2048) zero_blocks = 2048;
     return em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
         using T = decltype(t);
         constexpr int VW = decltype(w)::value;
-        k_embed_sums<T, VW><<<dim3((unsigned)(p.blocks + zero_blocks), column_blocks), kEmThreads, 0, stream>>>(a);
+        k_embed_sums<T, VW><<<dim3((unsigned)p.blocks, column_blocks), kEmThreads, 0, stream>>>(a);
         TDGS_LAUNCHED();
         if (p.blocks > 1) {
             k_embed_join<T, VW><<<dim3((unsigned)(p.blocks < 1024 ? p.blocks : 1024), column_blocks), kEmThreads, 0, stream>>>(a);
