@@ -60,6 +60,7 @@ struct GnVec {
             for (int i = 0; i < VW; ++i) f[i] = (float)v[i];
         }
     }
+    // Past the caches, which are to keep what an earlier pass has read for this one (960x540x128 bfloat16 101 -> 94 us).
     __device__ __forceinline__ void store(T* __restrict__ p) const {
         if constexpr (VW == 1) {
             *p = (T)f[0];
@@ -67,7 +68,7 @@ struct GnVec {
             V v;
 #pragma unroll
             for (int i = 0; i < VW; ++i) v[i] = (T)f[i];
-            *reinterpret_cast<V*>(p) = v;
+            __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
         }
     }
 };

@@ -6,7 +6,8 @@ What a network that turns rendered features into images needs besides matrix pro
 appearance model of a photo collection, a refiner, a codebook of Gaussian attributes). The reference has no counterpart. Tensors are
 float32, bfloat16 or float16 on the GPU; outputs and gradients are written into the tensors given,
 on the current stream, without synchronisation. temp is scratch of the size its function's
-*_temp() gives: with None a call allocates its own.
+*_temp() gives: with None a call allocates its own. cross_attention, group_norm and embedding are the
+same operators as functions that torch can differentiate.
 """
 from __future__ import annotations
 
@@ -328,3 +329,84 @@ def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None,
                                     tokens.data_ptr(), size, n, -1 if padding is None else padding, scale, t, ts, vocab,
                                     dim, *_temp(temp, dtable)))
     return dtable
+
+
+# ------------------------------------------------------------------------------------
+# As differentiable functions
+# ------------------------------------------------------------------------------------
+
+def _rows_contiguous(t):
+    """t, or a copy where its last dimension is not contiguous (a gradient may come as any view)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, kv_lengths, kv_mask):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+        cross_attention_(out, q, k, v, scale=scale, kv_lengths=kv_lengths, kv_mask=kv_mask, lse=lse)
+        ctx.save_for_backward(q, k, v, out, lse, kv_lengths, kv_mask)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse, kv_lengths, kv_mask = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        cross_attention_grad_(dq, dk, dv, dout.contiguous(), out, lse, q, k, v, scale=ctx.scale, kv_lengths=kv_lengths,
+                              kv_mask=kv_mask)
+        return dq, dk, dv, None, None, None
+
+
+def cross_attention(q, k, v, *, scale=None, kv_lengths=None, kv_mask=None):
+    """cross_attention_ as a differentiable function of q, k and v."""
+    return _CrossAttention.apply(_rows_contiguous(q), _rows_contiguous(k), _rows_contiguous(v), scale, kv_lengths,
+                                 kv_mask)
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, activation):
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
+        group_norm_(out, x, groups, weight, bias, eps=eps, activation=activation, stats=stats)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.activation = groups, activation
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        x, weight, bias, stats = ctx.saved_tensors
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dweight, dbias = (None if p is None else torch.empty_like(p) for p in (weight, bias))
+        group_norm_grad_(dx, dweight, dbias, dout.contiguous(), x, stats, ctx.groups, weight, bias,
+                         activation=ctx.activation)
+        return dx, dweight, dbias, None, None, None
+
+
+def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation="silu"):
+    """group_norm_ as a differentiable function of x, weight and bias."""
+    return _GroupNorm.apply(_rows_contiguous(x), weight, bias, groups, eps, activation)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, tokens, scale, padding):
+        out = torch.empty((*tokens.shape, table.shape[1]), dtype=table.dtype, device=table.device)
+        embedding_lookup_(out if out.dim() > 1 else out[None], table, tokens, scale=scale)
+        ctx.save_for_backward(tokens)
+        ctx.shape, ctx.scale, ctx.padding = table.shape, scale, padding
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        tokens, = ctx.saved_tensors
+        dtable = torch.empty(ctx.shape, dtype=dout.dtype, device=dout.device)
+        embedding_grad_(dtable, dout.reshape(-1, ctx.shape[1]).contiguous(), tokens, scale=ctx.scale, padding=ctx.padding)
+        return dtable, None, None, None
+
+
+def embedding(table, tokens, *, scale=1.0, padding=None):
+    """embedding_lookup_ as a differentiable function of the table; `padding` as in embedding_grad_."""
+    return _Embedding.apply(_rows_contiguous(table), tokens, scale, padding)
