@@ -692,32 +692,62 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     const int tiles = (a.rows + RT - 1) / RT, per = (tiles + a.splits - 1) / a.splits;
     const int t_end = blk * kAtWaves * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
     AtTile<T, DP, RT, kAtThreads, VEC> tq, td;
-    float st = 0.0f;
-    auto fetch = [&](int t) {
+    // Where chunk k's row stands, and how it goes RT rows on: a few additions, where at_row would divide. A row past the
+    // last stays on the last.
+    constexpr int PER = decltype(tq)::kPer;
+    int32_t row[PER], qi[PER], qh[PER];
+    int64_t at_q[PER], at_d[PER], at_s[PER];
+    float st[PER];
+    const int G = (int)a.by_g.d, step_i = RT / G, step_h = RT % G;
 #pragma unroll
-        for (int k = 0; k < tq.kPer; ++k) {
-            const AtRow at = at_row(a, kb, hk, min(t * RT + (tq.inside(k) ? tq.row(k) : 0), a.rows - 1));
-            tq.load_row(k, (const T*)a.q + at_offset(a.sq, at), a.d);
-            td.load_row(k, (const T*)a.dout + at_offset(a.sdo, at), a.d);
-        }
-        if (threadIdx.x < 2 * RT) {   // lse of the tile's rows, then delta
-            const int r = t * RT + (threadIdx.x & (RT - 1));
-            st = threadIdx.x < RT ? INFINITY : 0.0f;
-            if (r < a.rows) {
-                const int64_t at = at_stat(a, at_row(a, kb, hk, r));
-                st = threadIdx.x < RT ? at_lse2(a.lse[at]) : a.delta[at];
+    for (int k = 0; k < PER; ++k) {
+        row[k] = min(sp * per * RT + (tq.inside(k) ? tq.row(k) : 0), a.rows - 1);
+        if (a.rows <= 0) continue;
+        const AtRow at = at_row(a, kb, hk, row[k]);
+        qi[k] = at.i;
+        qh[k] = at.h - hk * G;
+        at_q[k] = at_offset(a.sq, at);
+        at_d[k] = at_offset(a.sdo, at);
+        at_s[k] = at_stat(a, at);
+    }
+    auto go = [&](int k, int di, int dh, int64_t ds) {   // di queries and dh heads on, ds statistics
+        qi[k] += di;
+        qh[k] += dh;
+        at_q[k] += di * a.sq.l + dh * a.sq.h;
+        at_d[k] += di * a.sdo.l + dh * a.sdo.h;
+        at_s[k] += ds;
+    };
+    auto fetch = [&]() {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            tq.load_row(k, (const T*)a.q + at_q[k], a.d);
+            td.load_row(k, (const T*)a.dout + at_d[k], a.d);
+            st[k] = (tq.col(k) == 0 ? a.lse : a.delta)[at_s[k]];   // the first chunk of a row brings lse, the others delta
+            if (row[k] + RT < a.rows) {
+                row[k] += RT;
+                go(k, step_i, step_h, step_i + (int64_t)step_h * a.q_len);
+                if (qh[k] >= G) go(k, 1, -G, 1 - (int64_t)G * a.q_len);
+                while (qi[k] >= a.q_len) {   // the next batch
+                    go(k, -a.q_len, 0, (int64_t)(a.heads - 1) * a.q_len);
+                    at_q[k] += a.sq.b;
+                    at_d[k] += a.sdo.b;
+                }
             }
         }
     };
-    if (sp * per < t_end) fetch(sp * per);
+    if (sp * per < t_end) fetch();
     for (int t = sp * per; t < t_end; ++t) {
         __syncthreads();
         tq.store(s_q, a.rows - t * RT, a.d);
         td.store(s_d, a.rows - t * RT, a.d);
-        if (threadIdx.x < RT) s_lse[threadIdx.x] = st;
-        else if (threadIdx.x < 2 * RT) s_delta[threadIdx.x - RT] = st;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const bool in = t * RT + tq.row(k) < a.rows;
+            if (tq.inside(k) && tq.col(k) == 0) s_lse[tq.row(k)] = in ? at_lse2(st[k]) : INFINITY;
+            if (tq.inside(k) && tq.col(k) == 8) s_delta[tq.row(k)] = in ? st[k] : 0.0f;
+        }
         __syncthreads();
-        if (t + 1 < t_end) fetch(t + 1);
+        if (t + 1 < t_end) fetch();
         if (!busy) continue;
         f32x16 s, dp;
 #pragma unroll
