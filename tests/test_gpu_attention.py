@@ -172,6 +172,18 @@ def test_peaked_rows(gpu, dtype):
     c.check(grad=False)
 
 
+@pytest.mark.parametrize("rise", [1.0, -1.0], ids=["rising", "falling"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_scores_that_rise_along_the_keys(gpu, dtype, rise):
+    """The largest score of a row comes late, and every tile's is far above (or below) the one before."""
+    c = Case(dtype, 1, 1, 70, 700, 2, 1, 64, seed=8)
+    along = torch.linspace(0, 1, 700, device="cuda")[None, :, None, None]
+    c.q.copy_(c.q.abs() + 0.5)
+    c.k.copy_(0.05 * c.k + rise * 8 * along)
+    c.run()
+    c.check()
+
+
 @pytest.mark.parametrize("lq,lk", [(0, 5), (5, 0), (0, 0)])
 def test_empty_lengths(gpu, lq, lk):
     c = Case(torch.bfloat16, 2, 2, lq, lk, 2, 1, 32)

@@ -345,54 +345,50 @@ __device__ __forceinline__ AtItem at_item(int i, int n, int kv_heads) {
     return {j % kv_heads, j / kv_heads * kXcds + i % kXcds};
 }
 
-// How far a score may exceed the reference m of its row, in powers of two, before O and l are brought to a new one:
-// p then reaches 2^8, which every type holds, and few tiles after the first rescale anything.
-constexpr float kAtSlack = 8.0f;
+// What a lane's p of a tile may add up to before its row's reference m is looked for again, and the scores, below
+// any score, that m starts from. p itself then stays below 2^10, which every type holds.
+constexpr float kAtLargest = 1024.0f, kAtLowest = -1e38f;
 
-// The forward kernel's workgroup: threads, row blocks per wavefront, and wavefronts per SIMD that its
-// registers leave room for.
+// The forward kernel's workgroup: threads, and wavefronts per SIMD that its registers leave room for. With 512
+// threads and four per SIMD a tile is staged once for 256 rows and the wavefronts cover each other's waits; two
+// blocks of rows per wavefront, or one wavefront per SIMD with twice the registers, were 3 to 70% slower
+// (32400 x 4096, 16 heads of 64: 726 to 1242 us against 725).
 template <class T, int DP>
 struct AtForward {
     static constexpr int kThreads = sizeof(T) == 2 && DP <= 64 ? 512 : 256;
-    static constexpr int kBlocks = 1;
     static constexpr int kPerSimd = sizeof(T) == 2 && DP <= 64 ? 4 : 2;
-    static constexpr int kRows = kThreads / kWave * kBlocks * 32;
+    static constexpr int kRows = kThreads / kWave * 32;
 };
 
-// Workgroup: wavefronts of QB * 32 rows each of one kv head, the keys of one split. Online softmax in
-// base 2: O and l are relative to m, the largest c s so far to within kAtSlack.
+// Workgroup: wavefronts of 32 rows each of one kv head, the keys of one split. Softmax in base 2: O and l are
+// relative to m, the largest c s of the first tile. It need not be the largest so far: only when a later tile's
+// p add up to more than kAtLargest are the scores taken again, m moved to their largest and O and l brought there, so
+// that almost every tile does without finding a maximum (5% of the kernel).
 template <class T, int DP, bool VEC, bool IDX, bool TWO>
 __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kPerSimd)) void k_attend(AtArgs a) {
-    constexpr int TH = AtForward<T, DP>::kThreads, QB = AtForward<T, DP>::kBlocks;
-    constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
+    constexpr int TH = AtForward<T, DP>::kThreads;
+    constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16, NK = KT / 32;
     __shared__ __attribute__((aligned(16))) T s_k[KT * P];
     __shared__ __attribute__((aligned(16))) T s_v[KT * P];
     const AtItem item = at_item(blockIdx.x, gridDim.x, a.kv_heads);
     const int blk = item.rest % a.blocks, sp = item.rest / a.blocks % a.splits, kb = item.rest / a.blocks / a.splits;
     const int hk = item.hk, kvh = kb * a.kv_heads + hk;
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
-    const int row0 = blk * AtForward<T, DP>::kRows + wave * (QB * 32) + (lane & 31);
+    const int r = blk * AtForward<T, DP>::kRows + wave * 32 + (lane & 31);
+    const bool in = r < a.rows;
 
-    typename Elem<T>::V8 qf[QB][NC];
-    f32x16 o[QB][NB];
-    float m[QB], l[QB];
+    typename Elem<T>::V8 qf[NC];
+    at_load_row<T, DP, VEC>(qf, in ? (const T*)a.q + at_offset(a.sq, at_row(a, kb, hk, r)) : nullptr, a.d);
+    f32x16 o[NB];
+    float m = kAtLowest, l = 0.0f;
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        const int r = row0 + qb * 32;
-        const T* p = nullptr;
-        if (r < a.rows) p = (const T*)a.q + at_offset(a.sq, at_row(a, kb, hk, r));
-        at_load_row<T, DP, VEC>(qf[qb], p, a.d);
-        m[qb] = -INFINITY;
-        l[qb] = 0.0f;
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
-        for (int db = 0; db < NB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[qb][db][i] = 0.0f;
-    }
-    const bool busy = blk * AtForward<T, DP>::kRows + wave * (QB * 32) < a.rows;   // (the others only bring keys)
+        for (int i = 0; i < 16; ++i) o[db][i] = 0.0f;
+    const bool busy = blk * AtForward<T, DP>::kRows + wave * 32 < a.rows;   // (the others only bring keys)
     const int len = at_length(a, kb);
     const int tiles = (len + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
-    const int t_end = min(tiles, (sp + 1) * per);
+    const int t0 = sp * per, t_end = min(tiles, t0 + per);
     const T* const kbase = (const T*)a.k + kb * a.sk.b + hk * a.sk.h;
     const T* const vbase = (const T*)a.v + kb * a.sv.b + hk * a.sv.h;
     AtTile<T, DP, KT, TH, VEC> tk, tv;
@@ -401,8 +397,51 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
         tk.template load<IDX>(kbase, a.sk.l, index, t * KT, len - t * KT, a.d);
         tv.template load<IDX>(vbase, a.sv.l, index, t * KT, len - t * KT, a.d);
     };
-    if (sp * per < t_end) fetch(sp * per);
-    for (int t = sp * per; t < t_end; ++t) {
+    f32x16 s[NK];
+    auto scores = [&](int left) {
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kk][i] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[kk] = mma(at_rows<T, DP>(s_k, kk * 32, c), qf[c], s[kk]);
+        }
+        if (left < KT) {
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[kk][i] = kk * 32 + (i >> 2) * 8 + (i & 3) < left - h * 4 ? s[kk][i] : -INFINITY;
+        }
+    };
+    auto move = [&]() {   // m to the largest score so far
+        float top = s[0][0];
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kk][i]);
+        top = fmaxf(max_halves(top) * a.c, m);
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        l *= f;
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] *= f;
+        m = top;
+    };
+    auto weights = [&]() {   // p in place of the scores; their sum
+        float sum = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kk][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk][i], a.c, -m));
+                sum += s[kk][i];
+            }
+        return sum;
+    };
+    if (t0 < t_end) fetch(t0);
+    for (int t = t0; t < t_end; ++t) {
         const int left = len - t * KT;
         __syncthreads();
         tk.store(s_k, left, a.d);
@@ -410,86 +449,33 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
         __syncthreads();
         if (t + 1 < t_end) fetch(t + 1);
         if (!busy) continue;
-        f32x16 s[QB][KT / 32];
-#pragma unroll
-        for (int kk = 0; kk < KT / 32; ++kk) {
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[qb][kk][i] = 0.0f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const auto f = at_rows<T, DP>(s_k, kk * 32, c);
-#pragma unroll
-                for (int qb = 0; qb < QB; ++qb) s[qb][kk] = mma(f, qf[qb][c], s[qb][kk]);
-            }
+        scores(left);
+        if (t == t0) move();
+        float sum = weights();
+        if (wave_any(!(sum <= kAtLargest))) {   // (NaN too, and then stays)
+            scores(left);
+            move();
+            sum = weights();
         }
-        if (left < KT) {
-#pragma unroll
-            for (int kk = 0; kk < KT / 32; ++kk)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const bool ok = kk * 32 + (i >> 2) * 8 + (i & 3) < left - h * 4;
-#pragma unroll
-                    for (int qb = 0; qb < QB; ++qb) s[qb][kk][i] = ok ? s[qb][kk][i] : -INFINITY;
-                }
-        }
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb) {
-            float top = s[qb][0][0];
-#pragma unroll
-            for (int kk = 0; kk < KT / 32; ++kk)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[qb][kk][i]);
-            top = max_halves(top) * a.c;
-            if (wave_any(top > m[qb] + kAtSlack)) {
-                top = fmaxf(top, m[qb]);
-                const float f = __builtin_amdgcn_exp2f(m[qb] - (top == -INFINITY ? 0.0f : top));
-                l[qb] *= f;
-#pragma unroll
-                for (int db = 0; db < NB; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[qb][db][i] *= f;
-                m[qb] = top;
-            }
-            const float base = m[qb] == -INFINITY ? 0.0f : m[qb];
-            float sum = 0.0f;
-#pragma unroll
-            for (int kk = 0; kk < KT / 32; ++kk)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[qb][kk][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][kk][i], a.c, -base));
-                    sum += s[qb][kk][i];
-                }
-            l[qb] += sum;
-        }
+        l += sum;
 #pragma unroll
         for (int ks = 0; ks < KT / 16; ++ks) {
+            const AtOperand<T, TWO> p(s[ks / 2], ks % 2);
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-                const AtOperand<T, TWO> p(s[qb][ks / 2], ks % 2);
-#pragma unroll
-                for (int db = 0; db < NB; ++db) o[qb][db] = p.product(at_cols<T, DP>(s_v, ks * 16, db), o[qb][db]);
-            }
+            for (int db = 0; db < NB; ++db) o[db] = p.product(at_cols<T, DP>(s_v, ks * 16, db), o[db]);
         }
     }
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-        const int r = row0 + qb * 32;
-        const bool in = r < a.rows;
-        const float sum = sum_halves(l[qb]);
-        if (a.splits == 1) {
-            const AtRow row = at_row(a, kb, hk, in ? r : 0);
-            at_store_row<T, DP>(in ? (T*)a.out + at_offset(a.so, row) : nullptr, o[qb], sum > 0.0f ? 1.0f / sum : 0.0f,
-                                a.d, a.vec_out);
-            if (in && a.lse && h == 0) a.lse[at_stat(a, row)] = (m[qb] + __builtin_amdgcn_logf(sum)) * kLn2;
-        } else if (in) {
-            const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
-            at_store_row<float, DP>(a.part + pr * DP, o[qb], 1.0f, DP, true);
-            if (h == 0) {
-                a.part_ml[2 * pr] = m[qb];
-                a.part_ml[2 * pr + 1] = sum;
-            }
+    l = sum_halves(l);
+    if (a.splits == 1) {
+        const AtRow row = at_row(a, kb, hk, in ? r : 0);
+        at_store_row<T, DP>(in ? (T*)a.out + at_offset(a.so, row) : nullptr, o, l > 0.0f ? 1.0f / l : 0.0f, a.d, a.vec_out);
+        if (in && a.lse && h == 0) a.lse[at_stat(a, row)] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+    } else if (in) {
+        const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
+        at_store_row<float, DP>(a.part + pr * DP, o, 1.0f, DP, true);
+        if (h == 0) {
+            a.part_ml[2 * pr] = m;
+            a.part_ml[2 * pr + 1] = l;
         }
     }
 }
@@ -504,21 +490,20 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, in
     const int per = kAtThreads / quads / SG, g = slot / per;   // rows per workgroup; this thread's share of the splits
     const int64_t pr0 = (int64_t)blockIdx.x * per + slot % per;
     const bool in = g < SG && pr0 < all_rows;
-    float top = -INFINITY, sum = 0.0f, base = 0.0f;
+    float top = kAtLowest, sum = 0.0f;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     if (in) {
         const float2* const ml = reinterpret_cast<const float2*>(a.part_ml) + pr0;
 #pragma unroll 8
         for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s * all_rows].x);
-        base = top == -INFINITY ? 0.0f : top;
         const f32x4* const part = reinterpret_cast<const f32x4*>(a.part + pr0 * dp) + q;
 #pragma unroll 4
         for (int s = g; s < a.splits; s += SG)
-            x += *(part + s * all_rows * quads) * __builtin_amdgcn_exp2f(ml[s * all_rows].x - base);
+            x += *(part + s * all_rows * quads) * __builtin_amdgcn_exp2f(ml[s * all_rows].x - top);
 #pragma unroll 8
         for (int s = 0; s < a.splits; ++s) {
             const float2 v = ml[s * all_rows];
-            sum = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x - base), v.y, sum);
+            sum = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x - top), v.y, sum);
         }
     }
     if constexpr (SG > 1) {
