@@ -153,6 +153,10 @@ SIZES = [
     (1, 1, 2, 5000, 4, 1, 64, "bhld", "keys"),
     (2, 2, 1, 3001, 8, 2, 128, "blhd", "lengths"),
     (1, 1, 1500, 3, 1, 1, 24, "blhd", "none"),
+    (2, 1, 150, 700, 4, 2, 64, "blhd", "both"),
+    (1, 1, 200, 600, 3, 3, 40, "sliced", "none"),
+    (2, 2, 90, 515, 2, 1, 33, "odd", "lengths"),
+    (3, 1, 7, 520, 6, 1, 16, "bhld", "keys"),
 ]
 
 

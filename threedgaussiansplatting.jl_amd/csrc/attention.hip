@@ -649,10 +649,13 @@ __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) v
 template <class T, int DP>
 constexpr int at_dkv_per_simd() { return sizeof(T) == 4 && DP > 96 ? 1 : 2; }
 
-// dK and dV. Workgroup: 4 wavefronts of 32 keys each, the rows of one split.
-template <class T, int DP, bool VEC, bool TWO>
-__global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(AtArgs a) {
-    constexpr int RT = 32, P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
+// dK and dV. Workgroup: TH / 64 wavefronts of 32 keys each, the rows of one split. Wide ones, of 256 keys, stage rows half as
+// often and 64 at a time: 343 -> 311 us for 64800 rows, 1024 keys and 8 heads of bfloat16; with 93 keys half
+// their wavefronts idle (30 -> 37).
+constexpr int kAtWide = 512;
+template <class T, int DP, int TH, bool VEC, bool TWO>
+__global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(AtArgs a) {
+    constexpr int RT = TH == kAtWide ? 64 : 32, P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
     __shared__ __attribute__((aligned(16))) T s_q[RT * P];
     __shared__ __attribute__((aligned(16))) T s_d[RT * P];
     __shared__ __attribute__((aligned(16))) float s_lse[RT];
@@ -661,9 +664,9 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
     const int sp = item % a.splits, blk = item / a.splits % a.blocks, kvh = item / a.splits / a.blocks;
     const int hk = kvh % a.kv_heads, kb = kvh / a.kv_heads;
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, h = lane >> 5;
-    const int j = (blk * kAtWaves + wave) * 32 + (lane & 31);
+    const int j = (blk * (TH / kWave) + wave) * 32 + (lane & 31);
     const int len = at_length(a, kb);
-    const bool ok = j < len, busy = (blk * kAtWaves + wave) * 32 < len;
+    const bool ok = j < len, busy = (blk * (TH / kWave) + wave) * 32 < len;
     const int64_t key = j < a.kv_len ? at_key(a, kb, j) : 0;
 
     typename Elem<T>::V8 kf[NC], vf[NC];
@@ -675,8 +678,8 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
 #pragma unroll
         for (int i = 0; i < 16; ++i) gk[db][i] = gv[db][i] = 0.0f;
     const int tiles = (a.rows + RT - 1) / RT, per = (tiles + a.splits - 1) / a.splits;
-    const int t_end = blk * kAtWaves * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
-    AtTile<T, DP, RT, kAtThreads, VEC> tq, td;
+    const int t_end = blk * (TH / kWave) * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
+    AtTile<T, DP, RT, TH, VEC> tq, td;
     // Where chunk k's row stands, and how it goes RT rows on: a few additions, where at_row would divide. A row past the
     // last stays on the last.
     constexpr int PER = decltype(tq)::kPer;
@@ -729,37 +732,45 @@ __global__ __launch_bounds__(kAtThreads, (at_dkv_per_simd<T, DP>())) void k_atte
         for (int k = 0; k < PER; ++k) {
             const bool in = t * RT + tq.row(k) < a.rows;
             if (tq.inside(k) && tq.col(k) == 0) s_lse[tq.row(k)] = in ? at_lse2(st[k]) : INFINITY;
-            if (tq.inside(k) && tq.col(k) == 8) s_delta[tq.row(k)] = in ? st[k] : 0.0f;
+            if (tq.inside(k) && tq.col(k) == 8) s_delta[tq.row(k)] = in ? -st[k] : 0.0f;
         }
         __syncthreads();
         if (t + 1 < t_end) fetch();
         if (!busy) continue;
-        f32x16 s, dp;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+        for (int rb = 0; rb < RT; rb += 32) {
+            f32x16 s, dp;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            s = mma(at_rows<T, DP>(s_q, 0, c), kf[c], s);
-            dp = mma(at_rows<T, DP>(s_d, 0, c), vf[c], dp);
-        }
+            for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const f32x4 ls = *reinterpret_cast<const f32x4*>(s_lse + k * 8 + h * 4);
-            const f32x4 de = *reinterpret_cast<const f32x4*>(s_delta + k * 8 + h * 4);
+            for (int k = 0; k < 4; ++k) {   // dP - delta: the product starts from -delta
+                const f32x4 de = *reinterpret_cast<const f32x4*>(s_delta + rb + k * 8 + h * 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k * 4 + i], a.c, -ls[i]));
-                s[k * 4 + i] = p;
-                dp[k * 4 + i] = p * (dp[k * 4 + i] - de[i]);
+                for (int i = 0; i < 4; ++i) dp[k * 4 + i] = de[i];
             }
-        }
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const AtOperand<T, TWO> p(s, ks), ds(dp, ks);
+            for (int c = 0; c < NC; ++c) {
+                s = mma(at_rows<T, DP>(s_q, rb, c), kf[c], s);
+                dp = mma(at_rows<T, DP>(s_d, rb, c), vf[c], dp);
+            }
 #pragma unroll
-            for (int db = 0; db < NB; ++db) {
-                gv[db] = p.product(at_cols<T, DP>(s_d, ks * 16, db), gv[db]);
-                gk[db] = ds.product(at_cols<T, DP>(s_q, ks * 16, db), gk[db]);
+            for (int k = 0; k < 4; ++k) {
+                const f32x4 ls = *reinterpret_cast<const f32x4*>(s_lse + rb + k * 8 + h * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k * 4 + i], a.c, -ls[i]));
+                    s[k * 4 + i] = p;
+                    dp[k * 4 + i] *= p;
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const AtOperand<T, TWO> p(s, ks), ds(dp, ks);
+#pragma unroll
+                for (int db = 0; db < NB; ++db) {
+                    gv[db] = p.product(at_cols<T, DP>(s_d, rb + ks * 16, db), gv[db]);
+                    gk[db] = ds.product(at_cols<T, DP>(s_q, rb + ks * 16, db), gk[db]);
+                }
             }
         }
     }
@@ -868,6 +879,7 @@ static int at_forward_rows(int32_t dtype, int dp) {
 struct AtPlan {
     int64_t kvh, rows;   // kv heads over all kv batches; rows of each
     int dp, rows_f, tile;
+    bool wide_k;
     int blocks_f, splits_f, blocks_q, splits_q, blocks_k, splits_k;
     size_t list_bytes, delta_bytes, forward_bytes, grad_bytes;   // (the first two within the last two)
 };
@@ -884,8 +896,9 @@ static AtPlan at_plan(const tdgs_attention* a, bool uneven) {
     p.splits_f = at_splits(p.blocks_f * p.kvh, key_tiles, uneven);
     p.blocks_q = (int)ceil_div(p.rows, kAtWaves * 32);
     p.splits_q = at_splits(p.blocks_q * p.kvh, key_tiles, uneven);
-    p.blocks_k = (int)ceil_div(a->kv_len, kAtWaves * 32);
-    p.splits_k = at_splits(p.blocks_k * p.kvh, row_tiles, uneven);
+    p.wide_k = a->dtype != TDGS_F32 && p.dp <= 64 && a->kv_len >= 512;   // (few idle wavefronts; registers to spare)
+    p.blocks_k = (int)ceil_div(a->kv_len, p.wide_k ? kAtWide / 2 : kAtWaves * 32);
+    p.splits_k = at_splits(p.blocks_k * p.kvh * (p.wide_k ? 2 : 1), p.wide_k ? ceil_div(p.rows, 64) : row_tiles, uneven);
     const size_t all_rows = (size_t)(p.kvh * p.rows), all_keys = (size_t)(p.kvh * a->kv_len);
     p.list_bytes = align_up((size_t)a->kv_batch * ((size_t)a->kv_len + 1) * sizeof(int32_t));
     p.delta_bytes = align_up(all_rows * sizeof(float));
@@ -1096,13 +1109,25 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
                 r.blocks = p.blocks_k;
                 r.splits = p.splits_k;
                 const unsigned grid = (unsigned)(p.kvh * p.splits_k * p.blocks_k);
-                auto launch = [&](auto two) {
+                const bool few = sizeof(T) == 2 && all_keys * a->head_dim <= kAtFewResults;
+                auto launch = [&](auto th, auto two) {
+                    constexpr int TH = decltype(th)::value;
                     constexpr bool TWO = decltype(two)::value;
-                    if (vec) k_attend_dkv<T, DP, true, TWO><<<grid, kAtThreads, 0, stream>>>(r);
-                    else k_attend_dkv<T, DP, false, TWO><<<grid, kAtThreads, 0, stream>>>(r);
+                    if (vec) k_attend_dkv<T, DP, TH, true, TWO><<<grid, TH, 0, stream>>>(r);
+                    else k_attend_dkv<T, DP, TH, false, TWO><<<grid, TH, 0, stream>>>(r);
                 };
-                if (sizeof(T) == 2 && all_keys * a->head_dim <= kAtFewResults) launch(std::integral_constant<bool, sizeof(T) == 2>{});
-                else launch(std::false_type{});
+                using Narrow = std::integral_constant<int, kAtThreads>;
+                using Two = std::integral_constant<bool, sizeof(T) == 2>;
+                if constexpr (sizeof(T) == 2 && DP <= 64) {
+                    using Wide = std::integral_constant<int, kAtWide>;
+                    if (p.wide_k && few) launch(Wide{}, Two{});
+                    else if (p.wide_k) launch(Wide{}, std::false_type{});
+                    else if (few) launch(Narrow{}, Two{});
+                    else launch(Narrow{}, std::false_type{});
+                } else {
+                    if (few) launch(Narrow{}, Two{});
+                    else launch(Narrow{}, std::false_type{});
+                }
                 TDGS_LAUNCHED();
                 if (p.splits_k > 1) {
                     k_attend_sum<T><<<(unsigned)ceil_div(2 * all_keys * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
