@@ -196,6 +196,21 @@ def test_empty_lengths(gpu, lq, lk):
     assert torch.isneginf(c.lse).all()
 
 
+@pytest.mark.parametrize("lq", [5, 3000])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_single_key(gpu, dtype, lq):
+    """The softmax of one key is constant: the output is its value, and no gradient reaches q or k."""
+    for kw in (dict(lk=1), dict(lk=700, mask="single")):
+        c = Case(dtype, 1, 1, lq, kw["lk"], 4, 2, 40, mask="none", seed=6)
+        if "mask" in kw:
+            c.keep[:] = False
+            c.keep[0, 77] = True
+            c.args = dict(kv_lengths=None, kv_mask=c.keep.cuda())
+        c.run()
+        c.check()
+        assert not c.dq.any() and not c.dk.any()
+
+
 def test_gradient_against_differences(gpu):
     """d/dt of sum(dout * out) along random directions, from central differences of the forward pass
     with step 2^-5 along unit directions: their error is the third derivative's, below 1e-3 of the

@@ -525,6 +525,9 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, in
 // The base-2 logarithm of a row's sum, from lse; +inf (all its p are 0) for a row without allowed keys.
 __device__ __forceinline__ float at_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
 
+// The factor of dQ and dK. The softmax of a single key is constant: its dP - delta is nothing but rounding.
+__device__ __forceinline__ float at_grad_scale(const AtArgs& a, int len) { return len > 1 ? a.scale : 0.0f; }
+
 // dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split.
 template <class T, int DP, bool VEC, bool IDX>
 __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) void k_attend_dq(AtArgs a) {
@@ -636,7 +639,7 @@ __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) v
         else a.part_ml[((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r] = sp == 0 ? delta + slip : slip;
     }
     if (a.splits == 1) {
-        at_store_row<T, DP>(r < a.rows ? (T*)a.dq + at_offset(a.sdq, row) : nullptr, o, a.scale, a.d, a.vec_out);
+        at_store_row<T, DP>(r < a.rows ? (T*)a.dq + at_offset(a.sdq, row) : nullptr, o, at_grad_scale(a, len), a.d, a.vec_out);
     } else if (r < a.rows) {
         const int64_t pr = ((int64_t)sp * gridDim.x / (a.blocks * a.splits) + kvh) * a.rows + r;
         at_store_row<float, DP>(a.part + pr * DP, o, 1.0f, DP, true);
@@ -782,7 +785,7 @@ __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(A
     }
     if (a.splits == 1) {
         const bool in = j < a.kv_len;
-        at_store_row<T, DP>(in ? (T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + key * a.sdk.l : nullptr, gk, a.scale, a.d, a.vec_out);
+        at_store_row<T, DP>(in ? (T*)a.dk + kb * a.sdk.b + hk * a.sdk.h + key * a.sdk.l : nullptr, gk, at_grad_scale(a, len), a.d, a.vec_out);
         at_store_row<T, DP>(in ? (T*)a.dv + kb * a.sdv.b + hk * a.sdv.h + key * a.sdv.l : nullptr, gv, 1.0f, a.d, a.vec_out);
     } else if (j < a.kv_len) {
         const int64_t all = (int64_t)(gridDim.x / (a.blocks * a.splits)) * a.kv_len;
@@ -807,7 +810,8 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
     if (what == 0) {
         const int kvh = (int)(pr / a.rows);
         const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr % a.rows));
-        at_store4<T>((T*)a.dq + at_offset(a.sdq, row) + e, x * a.scale, a.d - e, a.vec_out);
+        at_store4<T>((T*)a.dq + at_offset(a.sdq, row) + e, x * at_grad_scale(a, at_length(a, kvh / a.kv_heads)), a.d - e,
+                     a.vec_out);
         if (e == 0) {
             float delta = 0.0f;
             for (int s = 0; s < a.splits; ++s) delta += a.part_ml[s * n + pr];
@@ -820,7 +824,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
         const AtHeads& st = is_v ? a.sdv : a.sdk;
         T* const p = (T*)(is_v ? a.dv : a.dk) + kvh / a.kv_heads * st.b + kvh % a.kv_heads * st.h +
                      at_key(a, kvh / a.kv_heads, j) * st.l;
-        at_store4<T>(p + e, is_v ? x : x * a.scale, a.d - e, a.vec_out);
+        at_store4<T>(p + e, is_v ? x : x * at_grad_scale(a, at_length(a, kvh / a.kv_heads)), a.d - e, a.vec_out);
     }
 }
 
