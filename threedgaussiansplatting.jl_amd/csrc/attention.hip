@@ -482,10 +482,11 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
 
 // Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. A thread holds four
 // elements of a row; with SG > 1, for many splits of few rows, SG of them take every SG-th split and
-// are added up in LDS.
+// are joined likewise in LDS.
 template <class T, int SG>
 __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, int64_t all_rows) {
     __shared__ f32x4 s_x[SG > 1 ? kAtThreads : 1];
+    __shared__ float2 s_ml[SG > 1 ? kAtThreads : 1];
     const int quads = dp / 4, q = (int)threadIdx.x % quads, slot = (int)threadIdx.x / quads;
     const int per = kAtThreads / quads / SG, g = slot / per;   // rows per workgroup; this thread's share of the splits
     const int64_t pr0 = (int64_t)blockIdx.x * per + slot % per;
@@ -495,22 +496,32 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, in
     if (in) {
         const float2* const ml = reinterpret_cast<const float2*>(a.part_ml) + pr0;
 #pragma unroll 8
-        for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ml[s * all_rows].x);
+        for (int s = g; s < a.splits; s += SG) top = fmaxf(top, ml[s * all_rows].x);
         const f32x4* const part = reinterpret_cast<const f32x4*>(a.part + pr0 * dp) + q;
 #pragma unroll 4
-        for (int s = g; s < a.splits; s += SG)
-            x += *(part + s * all_rows * quads) * __builtin_amdgcn_exp2f(ml[s * all_rows].x - top);
-#pragma unroll 8
-        for (int s = 0; s < a.splits; ++s) {
+        for (int s = g; s < a.splits; s += SG) {
             const float2 v = ml[s * all_rows];
-            sum = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x - top), v.y, sum);
+            const float f = __builtin_amdgcn_exp2f(v.x - top);
+            x += *(part + s * all_rows * quads) * f;
+            sum = __builtin_fmaf(f, v.y, sum);
         }
     }
     if constexpr (SG > 1) {
         s_x[threadIdx.x] = x;
+        s_ml[threadIdx.x] = make_float2(top, sum);
         __syncthreads();
-        if (g == 0)
-            for (int i = 1; i < SG; ++i) x += s_x[threadIdx.x + i * per * quads];
+        if (g == 0) {
+            const int step = per * quads;
+            for (int i = 1; i < SG; ++i) top = fmaxf(top, s_ml[threadIdx.x + i * step].x);
+            x = {0.0f, 0.0f, 0.0f, 0.0f};
+            sum = 0.0f;
+            for (int i = 0; i < SG; ++i) {
+                const float2 v = s_ml[threadIdx.x + i * step];
+                const float f = __builtin_amdgcn_exp2f(v.x - top);
+                x += s_x[threadIdx.x + i * step] * f;
+                sum = __builtin_fmaf(f, v.y, sum);
+            }
+        }
     }
     if (!in || g > 0) return;
     const int kvh = (int)(pr0 / a.rows);
@@ -795,28 +806,46 @@ __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(A
     }
 }
 
-// Sums the splits' partial gradients, in order: dQ's rows (what 0), or dK's and dV's (what 1). One thread
-// per four elements.
-template <class T>
+// Sums the splits' partial gradients, always in the same order: dQ's rows (what 0), or dK's and dV's (what 1). One thread
+// per four elements; with SG > 1, for many splits, SG of them take every SG-th split and are added up in LDS.
+template <class T, int SG>
 __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int64_t all, int what) {
-    const int64_t id = (int64_t)blockIdx.x * kAtThreads + threadIdx.x;
+    __shared__ f32x4 s_x[SG > 1 ? kAtThreads : 1];
+    __shared__ float s_delta[SG > 1 ? kAtThreads : 1];
+    constexpr int per = kAtThreads / SG;
+    const int g = (int)threadIdx.x / per;
+    const int64_t id = (int64_t)blockIdx.x * per + (int)threadIdx.x % per;
     const int quads = dp / 4;
     const int64_t n = (what ? 2 : 1) * all;
     const int64_t pr = id / quads;
     const int e = (int)(id % quads) * 4;
-    if (pr >= n || e >= a.d) return;
+    const bool in = pr < n && e < a.d;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < a.splits; ++s) x += *reinterpret_cast<const f32x4*>(a.part + (s * n + pr) * dp + e);
+    float delta = 0.0f;
+    if (in) {
+#pragma unroll 8
+        for (int s = g; s < a.splits; s += SG) x += *reinterpret_cast<const f32x4*>(a.part + (s * n + pr) * dp + e);
+        if (what == 0 && e == 0)
+#pragma unroll 8
+            for (int s = g; s < a.splits; s += SG) delta += a.part_ml[s * n + pr];
+    }
+    if constexpr (SG > 1) {
+        s_x[threadIdx.x] = x;
+        s_delta[threadIdx.x] = delta;
+        __syncthreads();
+        if (g == 0)
+            for (int i = 1; i < SG; ++i) {
+                x += s_x[threadIdx.x + i * per];
+                delta += s_delta[threadIdx.x + i * per];
+            }
+    }
+    if (!in || g > 0) return;
     if (what == 0) {
         const int kvh = (int)(pr / a.rows);
         const AtRow row = at_row(a, kvh / a.kv_heads, kvh % a.kv_heads, (int)(pr % a.rows));
         at_store4<T>((T*)a.dq + at_offset(a.sdq, row) + e, x * at_grad_scale(a, at_length(a, kvh / a.kv_heads)), a.d - e,
                      a.vec_out);
-        if (e == 0) {
-            float delta = 0.0f;
-            for (int s = 0; s < a.splits; ++s) delta += a.part_ml[s * n + pr];
-            a.delta[at_stat(a, row)] = delta;
-        }
+        if (e == 0) a.delta[at_stat(a, row)] = delta;
     } else {
         const bool is_v = pr >= all;
         const int64_t rest = is_v ? pr - all : pr;
@@ -834,7 +863,7 @@ __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int
 // split into: as many as run together, since one more part for every workgroup would wait for a second round.
 // With lengths or a mask, workgroups end at different times, and twice as many parts even that out.
 constexpr int64_t kAtWorkgroups = 512;
-constexpr int kAtSplits = 64;
+constexpr int kAtSplits = 256;
 
 // Results (elements of out; of dK) up to which P, and dS for dK, keep their bits by a second product. Rounded to a 16-bit
 // type they leave an error as large as the results' own rounding, 1.4 times that together; over a large
@@ -946,6 +975,15 @@ static int at_check(const tdgs_attention* a) {
 }
 
 static AtHeads at_strides(const tdgs_heads& v) { return {v.stride_b, v.stride_l, v.stride_h}; }
+
+template <class T>
+static int at_sum(const AtArgs& r, int dp, int64_t all, int what, hipStream_t stream) {
+    const int64_t items = (what ? 2 : 1) * all * (dp / 4);
+    if (r.splits >= 16) k_attend_sum<T, 8><<<(unsigned)ceil_div(items, kAtThreads / 8), kAtThreads, 0, stream>>>(r, dp, all, what);
+    else k_attend_sum<T, 1><<<(unsigned)ceil_div(items, kAtThreads), kAtThreads, 0, stream>>>(r, dp, all, what);
+    TDGS_LAUNCHED();
+    return TDGS_OK;
+}
 
 // Whether rows of the view start on 16 bytes.
 static bool at_rows_aligned(const tdgs_heads& v, int64_t e) {
@@ -1104,9 +1142,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
                 else k_attend_dq<T, DP, false, true><<<grid, kAtThreads, 0, stream>>>(r);
                 TDGS_LAUNCHED();
                 if (p.splits_q > 1) {
-                    k_attend_sum<T><<<(unsigned)ceil_div(all_rows * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
-                        r, DP, all_rows, 0);
-                    TDGS_LAUNCHED();
+                    TDGS_TRY(at_sum<T>(r, DP, all_rows, 0, stream));
                 }
             }
             if (a->kv_len > 0) {
@@ -1134,9 +1170,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
                 }
                 TDGS_LAUNCHED();
                 if (p.splits_k > 1) {
-                    k_attend_sum<T><<<(unsigned)ceil_div(2 * all_keys * (DP / 4), kAtThreads), kAtThreads, 0, stream>>>(
-                        r, DP, all_keys, 1);
-                    TDGS_LAUNCHED();
+                    TDGS_TRY(at_sum<T>(r, DP, all_keys, 1, stream));
                 }
             }
             return TDGS_OK;
