@@ -16,6 +16,10 @@
 // and such keys, whatever they hold, are not read.
 // P and dS are rounded to the inputs' type for their products (the matrix cores take no wider
 // operand at that rate); maxima, sums, exponentials and every accumulator stay in 32 bits.
+//
+// What bounds the kernels: for 16-bit types the exponential of every score, at a quarter of the vector rate, next to
+// the products; for float the products themselves; for few rows over many keys the memory that
+// the keys are read from; for few rows and keys the latency of one or two tiles. Measured figures stand at each kernel.
 #include "internal.hpp"
 #include "elem.hpp"
 
@@ -351,8 +355,7 @@ constexpr float kAtLargest = 1024.0f, kAtLowest = -1e38f;
 
 // The forward kernel's workgroup: threads, and wavefronts per SIMD that its registers leave room for. With 512
 // threads and four per SIMD a tile is staged once for 256 rows and the wavefronts cover each other's waits; two
-// blocks of rows per wavefront, or one wavefront per SIMD with twice the registers, were 3 to 70% slower
-// (32400 x 4096, 16 heads of 64: 726 to 1242 us against 725).
+// blocks of rows per wavefront, or one wavefront per SIMD with twice the registers, were 0 to 70% slower.
 template <class T, int DP>
 struct AtForward {
     static constexpr int kThreads = sizeof(T) == 2 && DP <= 64 ? 512 : 256;
@@ -364,6 +367,10 @@ struct AtForward {
 // relative to m, the largest c s of the first tile. It need not be the largest so far: only when a later tile's
 // p add up to more than kAtLargest are the scores taken again, m moved to their largest and O and l brought there, so
 // that almost every tile does without finding a maximum (5% of the kernel).
+// bfloat16, heads of 64: 64800 rows x 1024 keys x 8 heads in 162 to 181 us (136 GFLOP: 750 to 840 TFLOP/s; a large
+// product reaches 1150), vector issue busy for 64% of it, the matrix cores for 38%; 32400 x 4096 x 16 in 594 us when
+// the card is cool, 720 when not (910 to 750 TFLOP/s at 2.1 to 1.75 GHz). float: matrix cores busy for half of the time.
+// One row of 16 heads over 8 caches of 10000 to 20011 keys: 40 us, 6 TB/s.
 template <class T, int DP, bool VEC, bool IDX, bool TWO>
 __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kPerSimd)) void k_attend(AtArgs a) {
     constexpr int TH = AtForward<T, DP>::kThreads;
@@ -482,7 +489,8 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
 
 // Joins the splits of a row: O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. A thread holds four
 // elements of a row; with SG > 1, for many splits of few rows, SG of them take every SG-th split and
-// are joined likewise in LDS.
+// are joined likewise in LDS. 128 rows of 32 splits: 4.6 us, nearly all latency; 60024 float rows of 64 elements
+// in two splits: 11 us, 4.1 TB/s.
 template <class T, int SG>
 __global__ __launch_bounds__(kAtThreads) void k_attend_join(AtArgs a, int dp, int64_t all_rows) {
     __shared__ f32x4 s_x[SG > 1 ? kAtThreads : 1];
@@ -539,7 +547,10 @@ __device__ __forceinline__ float at_lse2(float lse) { return lse == -INFINITY ? 
 // The factor of dQ and dK. The softmax of a single key is constant: its dP - delta is nothing but rounding.
 __device__ __forceinline__ float at_grad_scale(const AtArgs& a, int len) { return len > 1 ? a.scale : 0.0f; }
 
-// dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split.
+// dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split. 16-bit types up to 64 elements take three
+// per SIMD: 512 threads, two blocks of rows per wavefront, or tiles in two or three buffers were slower. Bound by vector
+// issue (72% busy, the matrix cores 44%): 64800 rows x 1024 keys x 8 heads of 64, bfloat16, in 296 to 320 us (204 GFLOP of
+// the formulas, 272 with the second product of dS: 850 to 920 TFLOP/s).
 template <class T, int DP, bool VEC, bool IDX>
 __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) void k_attend_dq(AtArgs a) {
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
@@ -665,7 +676,8 @@ constexpr int at_dkv_per_simd() { return sizeof(T) == 4 && DP > 96 ? 1 : 2; }
 
 // dK and dV. Workgroup: TH / 64 wavefronts of 32 keys each, the rows of one split. Wide ones, of 256 keys, stage rows half as
 // often and 64 at a time: 343 -> 311 us for 64800 rows, 1024 keys and 8 heads of bfloat16; with 93 keys half
-// their wavefronts idle (30 -> 37).
+// their wavefronts idle (30 -> 37). The matrix cores are busy for 44% of that, LDS for 48%, vector issue for 40%
+// (272 GFLOP: 890 to 980 TFLOP/s); for float the matrix cores for 51%.
 constexpr int kAtWide = 512;
 template <class T, int DP, int TH, bool VEC, bool TWO>
 __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(AtArgs a) {
@@ -807,7 +819,8 @@ __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(A
 }
 
 // Sums the splits' partial gradients, always in the same order: dQ's rows (what 0), or dK's and dV's (what 1). One thread
-// per four elements; with SG > 1, for many splits, SG of them take every SG-th split and are added up in LDS.
+// per four elements; with SG > 1, for many splits, SG of them take every SG-th split and are added up in LDS
+// (64 splits of few results: 17 to 21 us by one thread each, 4.4 by eight).
 template <class T, int SG>
 __global__ __launch_bounds__(kAtThreads) void k_attend_sum(AtArgs a, int dp, int64_t all, int what) {
     __shared__ f32x4 s_x[SG > 1 ? kAtThreads : 1];

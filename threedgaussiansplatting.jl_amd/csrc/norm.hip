@@ -12,7 +12,9 @@
 // a channel whose mean is large.
 //
 // Three launches (runs of pixels, their joining, the result), or one for images of few pixels, a
-// workgroup then taking all pixels of a few whole groups.
+// workgroup then taking all pixels of a few whole groups. 960x540x128 bfloat16 with SiLU: statistics 24 us (133 MB,
+// 5.6 TB/s), joining 6 (latency), result 49 (265 MB, 5.4 TB/s): a large copy reaches 5.1, and the image just fits
+// the last-level cache. Reading it once only would take a wait of all workgroups for each other in the middle.
 #include "internal.hpp"
 #include "elem.hpp"
 
@@ -360,7 +362,8 @@ __global__ __launch_bounds__(kGnThreads) void k_norm_apply(GnArgs a) {
     gn_apply<T, VW, ACT, kGnThreads>(a, (const T*)a.x + n * a.xn + c0, (T*)a.out + n * a.on + c0, ch, p0, p1, at);
 }
 
-// Workgroup (y, n): all pixels of channel block y, whole groups of a.vectors vectors, of image n.
+// Workgroup (y, n): all pixels of channel block y, whole groups of a.vectors vectors, of image n. 8x8x128 floats: 5.8 us,
+// the latency of one load, the joining and one store (three launches: 10.7).
 template <class T, int VW, int ACT>
 __global__ __launch_bounds__(kGnSmallThreads) void k_norm_small(GnArgs a) {
     __shared__ float s_mean[gn_lds<VW, kGnSmallThreads>()];
@@ -590,7 +593,8 @@ __device__ __forceinline__ float2 gn_group_means(const GnArgs& a, int g, Sum&& s
     return make_float2(gn_segment_sum(s1, kWave) / count, gn_segment_sum(s2, kWave) / count);
 }
 
-// The first workgroups also write dbias and dweight.
+// The first workgroups also write dbias and dweight. 3 x 33565 x 96 floats: 21 us (116 MB, 5.4 TB/s), the sums before it
+// 16 (77 MB, 4.9 TB/s).
 template <class T, int VW, int ACT>
 __global__ __launch_bounds__(kGnThreads) void k_norm_dx(GnArgs a) {
     __shared__ float2 s_means[kGnThreads * VW];
