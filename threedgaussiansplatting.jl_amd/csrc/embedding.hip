@@ -16,7 +16,8 @@ namespace tdgs {
 constexpr int kEmThreads = 256;
 constexpr int kEmBlock = 2048;   // the most sorted positions of a workgroup
 constexpr int kEmRun = 32;       // and of one of its runs
-constexpr int kEmFew = 4096;     // the most tokens that one launch is taken for
+constexpr int kEmFew = 4096;         // the most tokens that one launch is taken for, and
+constexpr int kEmFewThreads = 512;   // its workgroups' size
 
 struct EmArgs {
     const void *table, *dout, *tokens;
@@ -113,11 +114,11 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_keys(EmArgs a, uint32_t* _
 // the workgroup's lane groups takes `run` of them from g * run on. A token's sum goes to its row of the table;
 // that of the token `before` the block, and of one that goes on `after` it, to part (row 0 and row 1).
 // Every thread of the workgroup calls it. Returns whether a token starts here and goes on.
-template <class T, int VW>
-__device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key, const int32_t* s_row, int count, int run,
+template <class T, int VW, int TH, int U, class Row>
+__device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key, const Row* s_row, int count, int run,
                                          uint32_t before, uint32_t after, float* part, float* s_head, float* s_tail,
                                          uint32_t* s_flag) {
-    const int groups = kEmThreads / a.lanes, sub = (int)threadIdx.x / a.lanes, col = (int)threadIdx.x % a.lanes;
+    const int groups = TH / a.lanes, sub = (int)threadIdx.x / a.lanes, col = (int)threadIdx.x % a.lanes;
     const int vec = blockIdx.y * kWave + col, e = vec * VW;
     const bool on = sub < groups && vec < a.vectors;
     const uint32_t none = (uint32_t)a.vocab;
@@ -125,7 +126,7 @@ __device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key,
     constexpr uint32_t kHead = 1u, kThrough = 2u, kTail = 4u;
     auto keep = [&](float* s, const EmVec<T, VW>& v) {
 #pragma unroll
-        for (int i = 0; i < VW; ++i) s[i * kEmThreads + threadIdx.x] = v.f[i];
+        for (int i = 0; i < VW; ++i) s[i * TH + threadIdx.x] = v.f[i];
     };
     if (on && i0 < i1) {
         EmVec<T, VW> sum;
@@ -146,7 +147,6 @@ __device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key,
                 sum.store((T*)a.dtable + (int64_t)cur * a.dtable_stride + e, a.scale);
             }
         };
-        constexpr int U = VW == 1 ? 8 : 4;
         for (int i = i0; i < i1; i += U) {
             EmVec<T, VW> v[U];
             uint32_t key[U];
@@ -181,11 +181,11 @@ __device__ __forceinline__ bool em_block(const EmArgs& a, const uint32_t* s_key,
         auto chain = [&](const float* s, bool through, bool outside) {
             EmVec<T, VW> v;
 #pragma unroll
-            for (int i = 0; i < VW; ++i) v.f[i] = s[i * kEmThreads + threadIdx.x];
+            for (int i = 0; i < VW; ++i) v.f[i] = s[i * TH + threadIdx.x];
             int g = sub + 1;
             for (; through && g < groups && (s_flag[g] & kHead); ++g) {
 #pragma unroll
-                for (int i = 0; i < VW; ++i) v.f[i] += s_head[i * kEmThreads + g * a.lanes + col];
+                for (int i = 0; i < VW; ++i) v.f[i] += s_head[i * TH + g * a.lanes + col];
                 through = (s_flag[g] & kThrough) != 0;
             }
             const uint32_t key = s_key[i1 - 1];   // (of a tail; a head's that ends here is not stored to its row)
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_sums(EmArgs a) {
         s_row[i] = a.order[i0 + i];
     }
     __syncthreads();
-    const bool starts = em_block<T, VW>(a, s_key, s_row, (int)(i1 - i0), a.run, i0 > 0 ? a.keys[i0 - 1] : none,
+    const bool starts = em_block<T, VW, kEmThreads, (VW == 1 ? 8 : 4), int32_t>(a, s_key, s_row, (int)(i1 - i0), a.run, i0 > 0 ? a.keys[i0 - 1] : none,
                                         i1 < a.n ? a.keys[i1] : none, a.part + 2 * blockIdx.x * ((int64_t)a.vectors * VW),
                                         s_head, s_tail, s_flag);
     if (starts && blockIdx.y == 0 && threadIdx.x % a.lanes == 0) a.list[atomicAdd(a.count, 1)] = (int32_t)blockIdx.x;
@@ -281,72 +281,110 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_join(EmArgs a) {
 }
 
 // One launch for a few tokens: workgroup x takes a.rows <= 4096 rows of the table, picks the tokens that name them,
-// sorts them (by token, then position), sums, and writes zeros where no token does. 96 tokens of 1000: 6 us where the
-// chain of launches takes 31.
+// sorts them (by token, then position) in LDS, sums, and writes zeros where no token does. Bound by latency: of the tokens,
+// two or four barriers a step of the sort, the rows. 96 tokens of 1000: 8 us where the chain of launches takes 31; 2476 of
+// 19635, rows of 48 floats: 14 (31); 2600 that are all one token: 23 (23).
 template <class T, int VW>
-__global__ __launch_bounds__(kEmThreads) void k_embed_few(EmArgs a) {
-    extern __shared__ uint32_t s_list[];   // keys, rows and positions of a.few tokens each
-    __shared__ float s_head[kEmThreads * VW];
-    __shared__ float s_tail[kEmThreads * VW];
-    __shared__ uint32_t s_flag[kEmThreads];
-    __shared__ int s_wave[kEmThreads / kWave], s_count;
-    uint32_t* const s_key = s_list;
-    int32_t* const s_row = (int32_t*)s_list + a.few;
-    uint16_t* const s_at = (uint16_t*)(s_list + 2 * a.few);
+__global__ __launch_bounds__(kEmFewThreads) void k_embed_few(EmArgs a) {
+    constexpr int TH = kEmFewThreads, W = TH / kWave, U = 4;
+    extern __shared__ uint32_t s_key[];   // keys and rows of a.few tokens each
+    __shared__ uint32_t s_other[2 * TH * VW > kEmFew ? 2 * TH * VW : kEmFew];   // the sort's second place, then the sums'
+    __shared__ uint32_t s_flag[TH];
+    __shared__ int s_wave[U * W], s_digit[64 * W];
+    uint16_t* const s_row = (uint16_t*)(s_key + a.few);
+    float *const s_head = (float*)s_other, *const s_tail = s_head + TH * VW;
     const int64_t v0 = (int64_t)blockIdx.x * a.rows, v1 = min(a.vocab, v0 + a.rows);
     const int lane = (int)__lane_id(), wave = threadIdx.x / kWave, n = (int)a.n;
-    if (threadIdx.x == 0) s_count = 0;
-    __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += kEmThreads) {
-        const int i = i0 + threadIdx.x;
-        int64_t tok = -1;
-        if (i < n) {
-            tok = em_token(a, i);
-            if ((tok < 0 || tok >= a.vocab) && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, kErrTokenRange);
-        }
-        const bool mine = i < n && tok >= v0 && tok < v1 && tok != a.padding;
-        const uint64_t votes = __ballot(mine);
-        if (lane == 0) s_wave[wave] = __popcll(votes);
-        __syncthreads();
-        int at = s_count;
-        for (int w = 0; w < wave; ++w) at += s_wave[w];
-        at += __popcll(votes & lanemask_lt());
-        if (mine) {
-            s_key[at] = (uint32_t)(tok - v0) << 12 | (uint32_t)at;   // (at < kEmFew = 2^12)
-            s_at[at] = (uint16_t)i;
+    int count = 0;
+    for (int i0 = 0; i0 < n; i0 += TH * U) {
+        int64_t tok[U];
+        uint64_t votes[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) tok[u] = em_token(a, min(i0 + u * TH + (int)threadIdx.x, n - 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = i0 + u * TH + (int)threadIdx.x < n;
+            if (in && (tok[u] < 0 || tok[u] >= a.vocab) && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, kErrTokenRange);
+            votes[u] = __ballot(in && tok[u] >= v0 && tok[u] < v1 && tok[u] != a.padding);
+            if (lane == 0) s_wave[u * W + wave] = __popcll(votes[u]);
         }
         __syncthreads();
-        if (threadIdx.x == kEmThreads - 1) s_count = at + (mine ? 1 : 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (w == wave) at[u] = count;
+                count += s_wave[u * W + w];
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (votes[u] >> lane & 1) {
+                const int p = at[u] + __popcll(votes[u] & lanemask_lt());
+                s_key[p] = (uint32_t)(tok[u] - v0) << 12 | (uint32_t)(i0 + u * TH + threadIdx.x);   // (n <= kEmFew = 2^12)
+            }
         __syncthreads();
     }
-    const int count = s_count;
-    // sort by halves that rise and fall, padded to a power of two (at most a.few, which is one)
-    int size = 1;
-    while (size < count) size *= 2;
-    for (int i = count + threadIdx.x; i < size; i += kEmThreads) s_key[i] = 0xffffffffu;
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < size / 2; t += kEmThreads) {
-                const int lo = (t & (j - 1)) | (t & ~(j - 1)) << 1, hi = lo | j;
-                const uint32_t x = s_key[lo], y = s_key[hi];
-                if ((x > y) == ((lo & k) == 0)) {
-                    s_key[lo] = y;
-                    s_key[hi] = x;
+    // sort by token, six bits at a time, each wavefront a piece; positions stay in order
+    uint32_t *from = s_key, *to = s_other;
+    const int piece = (count + W * kWave - 1) / (W * kWave) * kWave, p0 = wave * piece, p1 = min(count, p0 + piece);
+    for (int shift = 12; count > 1 && (a.rows - 1) >> (shift - 12) > 0; shift += 6) {
+        auto each = [&](auto&& f) {   // f(key, its digit, the lanes of that digit)
+            for (int i = p0; i < p1; i += kWave) {
+                const bool in = i + lane < p1;
+                const uint32_t key = from[in ? i + lane : i];
+                const int digit = (int)(key >> shift & 63u);
+                uint64_t same = __ballot(in);
+#pragma unroll
+                for (int b = 0; b < 6; ++b) {
+                    const uint64_t ones = __ballot(digit >> b & 1);
+                    same &= digit >> b & 1 ? ones : ~ones;
                 }
+                if (in) f(key, digit, same);
             }
+        };
+        int* const mine = s_digit + wave * 64;
+        s_digit[threadIdx.x] = 0;
+        __syncthreads();
+        each([&](uint32_t, int digit, uint64_t same) {
+            if ((same & lanemask_lt()) == 0) mine[digit] += __popcll(same);
+        });
+        __syncthreads();
+        // where each digit of each piece goes, digit by digit
+        int* const slot = s_digit + (int)threadIdx.x % W * 64 + (int)threadIdx.x / W;
+        const int number = *slot;
+        int upto = number;
+#pragma unroll
+        for (int w = 1; w < kWave; w *= 2) {
+            const int x = __shfl_up(upto, w, kWave);
+            if (lane >= w) upto += x;
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < count; i += kEmThreads) {
-        const uint32_t key = s_key[i];
-        s_row[i] = s_at[key & 0xfffu];
+        if (lane == kWave - 1) s_wave[wave] = upto;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) upto += s_wave[w];
+        *slot = upto - number;
+        __syncthreads();
+        each([&](uint32_t key, int digit, uint64_t same) {
+            const int at = mine[digit];
+            to[at + __popcll(same & lanemask_lt())] = key;
+            if ((same & lanemask_lt()) == 0) mine[digit] = at + __popcll(same);
+        });
+        __syncthreads();
+        uint32_t* const next = from;
+        from = to;
+        to = next;
+    }
+    for (int i = threadIdx.x; i < count; i += TH) {
+        const uint32_t key = from[i];
+        s_row[i] = (uint16_t)(key & 0xfffu);
         s_key[i] = (uint32_t)v0 + (key >> 12);
     }
     __syncthreads();
-    const int groups = kEmThreads / a.lanes, sub = (int)threadIdx.x / a.lanes;
+    const int groups = TH / a.lanes, sub = (int)threadIdx.x / a.lanes;
     const int vec = blockIdx.y * kWave + (int)threadIdx.x % a.lanes;
     const uint32_t none = (uint32_t)a.vocab;
-    em_block<T, VW>(a, s_key, s_row, count, (count + groups - 1) / groups, none, none, nullptr, s_head, s_tail, s_flag);
+    em_block<T, VW, TH, (VW == 8 ? 8 : 16), uint16_t>(a, s_key, s_row, count, (count + groups - 1) / groups, none, none, nullptr,
+                                                      s_head, s_tail, s_flag);
     if (sub >= groups || vec >= a.vectors) return;
     EmVec<T, VW> z;
     z.zero();
@@ -381,7 +419,8 @@ static int em_run(int64_t n, int groups) {
 static int em_lanes(int vectors) { return vectors < kWave ? vectors : kWave; }
 
 // Whether one launch takes n tokens: a thousand, or more where a workgroup has so many lane groups that even if they
-// are all one token, a group has 64 rows to add.
+// are all one token, a group has 64 rows to add (where that then takes as long as the chain of launches, to 1.5 times that;
+// tokens of any spread half of it).
 static bool em_few(int64_t n, int groups) {
     const int64_t most = 64 * groups < kEmFew ? 64 * groups : kEmFew;
     return n <= (most > 1024 ? most : 1024);
@@ -398,9 +437,9 @@ static EmPlan em_plan(int64_t n, int64_t vocab, int32_t dim, int vw) {
     EmPlan p = {};
     p.vectors = dim / vw;
     p.lanes = em_lanes(p.vectors);
-    const int groups = kEmThreads / p.lanes;
-    p.few = em_few(n, groups);
+    p.few = em_few(n, kEmFewThreads / p.lanes);
     if (p.few) return p;
+    const int groups = kEmThreads / p.lanes;
     p.run = em_run(n, groups);
     p.blocks = ceil_div(n, (int64_t)groups * p.run);
     p.sort_bytes = radix_temp_bytes(n);
@@ -534,20 +573,19 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     a.lanes = p.lanes;
     a.run = p.run;
     a.blocks = p.blocks;
-    const int groups = kEmThreads / a.lanes;
     const unsigned column_blocks = (unsigned)ceil_div(a.vectors, kWave);
     if (p.few) {
-        // a group of lanes takes a row at a time; four workgroups per CU where the table has the rows, but
+        // a group of lanes takes a row at a time; two workgroups per CU where the table has the rows, but
         // no more than 2^12 of them in one
-        int64_t rows = ceil_div(vocab, 1024);
-        if (rows < groups) rows = groups;
+        int64_t rows = ceil_div(vocab, 512);
+        if (rows < kEmFewThreads / a.lanes) rows = kEmFewThreads / a.lanes;
         if (rows > kEmFew) rows = kEmFew;
         a.rows = (int32_t)rows;
         a.few = 1;
         while (a.few < n) a.few *= 2;
         return em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
-            k_embed_few<decltype(t), decltype(w)::value><<<dim3((unsigned)ceil_div(vocab, rows), column_blocks), kEmThreads,
-                                                           (size_t)a.few * (2 * sizeof(uint32_t) + sizeof(uint16_t)), stream>>>(a);
+            k_embed_few<decltype(t), decltype(w)::value><<<dim3((unsigned)ceil_div(vocab, rows), column_blocks), kEmFewThreads,
+                                                           (size_t)a.few * (sizeof(uint32_t) + sizeof(uint16_t)), stream>>>(a);
             TDGS_LAUNCHED();
             return TDGS_OK;
         });
