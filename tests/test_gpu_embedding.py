@@ -44,6 +44,11 @@ SIZES = [
     (4096, 100000, 16, "any"),
     (3000, 5000000, 1, "any"),     # more rows than 2^12 for each of 1024 workgroups
     (100000, 3, 5, "skewed"),
+    (2688, 20000, 48, "skewed"),   # the most that one launch takes of rows of 12 vectors, and one more
+    (2689, 20000, 48, "skewed"),
+    (4096, 300000, 8, "one"),      # one workgroup has all tokens, and rows of two sorting steps
+    (4095, 300000, 8, "ends"),
+    (513, 700000, 24, "any"),
 ]
 
 
