@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_join(EmArgs a) {
 
 // One launch for a few tokens: workgroup x takes a.rows <= 4096 rows of the table, picks the tokens that name them,
 // sorts them (by token, then position) in LDS, sums, and writes zeros where no token does. Bound by latency: of the tokens,
-// two or four barriers a step of the sort, the rows. 96 tokens of 1000: 8 us where the chain of launches takes 31; 2476 of
+// five barriers for six bits of the sort, the rows. 96 tokens of 1000: 8 us where the chain of launches takes 31; 2476 of
 // 19635, rows of 48 floats: 14 (31); 2600 that are all one token: 23 (23).
 template <class T, int VW>
 __global__ __launch_bounds__(kEmFewThreads) void k_embed_few(EmArgs a) {
