@@ -243,7 +243,7 @@ template <int VW, int THREADS>
 constexpr int gn_lds() { return VW * THREADS * 3 / 2; }
 
 // Workgroup (b, y, n): statistics of run b of image n's pixels, channel block y; per group where a
-// workgroup holds all channels.
+// workgroup holds all channels (which a.parts does not tell: it is groups and channels in one for groups of one channel).
 template <class T, int VW>
 __global__ __launch_bounds__(kGnThreads) void k_norm_stats(GnArgs a) {
     __shared__ float s_mean[gn_lds<VW, kGnThreads>()];
@@ -253,7 +253,7 @@ __global__ __launch_bounds__(kGnThreads) void k_norm_stats(GnArgs a) {
     const int64_t p0 = b * a.per, p1 = min(a.pixels, p0 + a.per);
     gn_stats<T, VW, kGnThreads>((const T*)a.x + n * a.xn + c0, a.xp, p0, p1, vectors, s_mean, s_m2);
     float2* const out = (float2*)a.part + ((int64_t)n * a.blocks + b) * a.parts;
-    if (a.parts == a.groups) {
+    if (a.vectors <= kGnThreads) {
         gn_groups(s_mean, s_m2, a.groups, a.group_size, (float)(p1 - p0), kGnThreads,
                   [&](int g, float m, float s2) { out[g] = make_float2(m, s2); });
     } else {
