@@ -15,6 +15,7 @@ import ctypes as C
 import struct
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import abi
 from .core import _handle, check, dptr, lib
@@ -332,7 +333,7 @@ def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None,
 
 
 # ------------------------------------------------------------------------------------
-# As differentiable functions
+# As differentiable functions: once, their gradients have no kernels of their own
 # ------------------------------------------------------------------------------------
 
 def _rows_contiguous(t):
@@ -351,6 +352,7 @@ class _CrossAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, kv_mask = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -376,6 +378,7 @@ class _GroupNorm(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         x, weight, bias, stats = ctx.saved_tensors
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -400,6 +403,7 @@ class _Embedding(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         tokens, = ctx.saved_tensors
         dtable = torch.empty(ctx.shape, dtype=dout.dtype, device=dout.device)
