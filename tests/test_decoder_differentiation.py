@@ -82,6 +82,9 @@ def test_second_derivative_raises(stand_ins, name):
     """The gradients are no function of their operands for torch: a gradient of them has to be refused, not to lack a part
     in silence where the loss has another path to the leaf."""
     f, leaf = _calls()[name]
-    g, = torch.autograd.grad(f().sum() + (leaf ** 3).sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
-        torch.autograd.grad((g ** 2).sum(), leaf)
+    for loss in (lambda: f().sum(), lambda: (f() ** 2).sum()):   # the operator's dout: constant, and not
+        g, = torch.autograd.grad(loss() + (leaf ** 3).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad((g ** 2).sum(), leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            (g ** 2).sum().backward()

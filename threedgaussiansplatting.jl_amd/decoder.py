@@ -12,10 +12,10 @@ same operators as functions that torch can differentiate.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import abi
 from .core import _handle, check, dptr, lib
@@ -341,6 +341,36 @@ def _rows_contiguous(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+class _Refused(torch.autograd.Function):
+    """The first n tensors as they are, as a function of the others that cannot be differentiated."""
+
+    @staticmethod
+    def forward(ctx, n, *tensors):
+        return tensors[:n]
+
+    @staticmethod
+    def backward(ctx, *douts):
+        raise RuntimeError("the gradients of the decoder operators cannot be differentiated again")
+
+
+def _once(backward):
+    """backward, whose gradients come from kernels, for a function that can be differentiated once: where torch builds
+    a graph of the gradients, they hang on everything that they were made from, so that a second derivative
+    raises. (once_differentiable refuses only what comes through dout, and takes them for constants otherwise.)"""
+    @functools.wraps(backward)
+    def wrapped(ctx, dout):
+        with torch.no_grad():
+            grads = backward(ctx, dout)
+        made_from = [t for t in (dout, *ctx.saved_tensors) if t is not None and t.requires_grad] \
+            if torch.is_grad_enabled() else ()
+        if made_from:
+            given = [g for g in grads if g is not None]
+            refused = iter(_Refused.apply(len(given), *given, *made_from))
+            grads = tuple(None if g is None else next(refused) for g in grads)
+        return grads
+    return wrapped
+
+
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, kv_lengths, kv_mask):
@@ -352,7 +382,7 @@ class _CrossAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, kv_mask = ctx.saved_tensors
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -378,7 +408,7 @@ class _GroupNorm(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         x, weight, bias, stats = ctx.saved_tensors
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -403,7 +433,7 @@ class _Embedding(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         tokens, = ctx.saved_tensors
         dtable = torch.empty(ctx.shape, dtype=dout.dtype, device=dout.device)
