@@ -113,3 +113,17 @@ def test_zero_and_infinite_rows(gpu):
     assert not torch.isfinite(c.dq[0, 17]).any()
     c.dq[0, 17] = want[0, 17]
     assert torch.equal(c.dq, want)
+
+
+@pytest.mark.parametrize("lq,h", [(20, 2), (16384, 8)])   # P by two operands; by one, every workgroup taking all keys
+def test_one_key_far_above_the_others(gpu, lq, h):
+    """A key that takes nearly all of every query's weight and has no value: the output is the others' small weights, which
+    are alike, so that what half loses of one it loses of all."""
+    c = Case(torch.float16, 1, 1, lq, 128, h, h, 32, seed=9)
+    c.q.copy_(0.1 * c.q + 1)
+    c.k.zero_()
+    c.k[:, 0] = 2.0
+    c.v.copy_(0.1 * c.v + 1)
+    c.v[:, 0] = 0
+    c.run(grad=False)
+    c.check(grad=False)

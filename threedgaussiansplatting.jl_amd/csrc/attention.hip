@@ -385,9 +385,14 @@ __device__ __forceinline__ AtItem at_item(int i, int n, int kv_heads) {
     return {j % kv_heads, j / kv_heads * kXcds + i % kXcds};
 }
 
-// What a lane's p of a tile may add up to before its row's reference m is looked for again, and the scores, below
-// any score, that m starts from. p itself then stays below 2^10, which every type holds.
-constexpr float kAtLargest = 1024.0f, kAtLowest = -1e38f;
+// How far below the largest c s of a tile its row's reference m is put, and what a lane's p of a tile may add up to before
+// m is looked for again: 2^10 times that of the largest. In half both are up by 2^5, and p stays below 2^15: weights down to
+// 2^-19 of the largest so keep all of half's bits, which matters where the key that has the largest has no value of its own.
+template <class T>
+constexpr float at_below() { return std::is_same<T, f16>::value ? 5.0f : 0.0f; }
+template <class T>
+constexpr float at_largest() { return std::is_same<T, f16>::value ? 0x1p15f : 0x1p10f; }
+constexpr float kAtLowest = -1e38f;   // below any score: what m starts from
 
 // The forward kernel's workgroup: threads, and wavefronts per SIMD that its registers leave room for. With 512
 // threads and four per SIMD a tile is staged once for 256 rows and the wavefronts cover each other's waits; two
@@ -401,7 +406,7 @@ struct AtForward {
 
 // Workgroup: wavefronts of 32 rows each of one kv head, the keys of one split. Softmax in base 2: O and l are
 // relative to m, the largest c s of the first tile. It need not be the largest so far: only when a later tile's
-// p add up to more than kAtLargest are the scores taken again, m moved to their largest and O and l brought there, so
+// p add up to more than at_largest are the scores taken again, m moved to their largest and O and l brought there, so
 // that almost every tile does without finding a maximum (5% of the kernel).
 // bfloat16, heads of 64: 64800 rows x 1024 keys x 8 heads in 162 to 181 us (136 GFLOP: 750 to 840 TFLOP/s; a large
 // product reaches 1150), vector issue busy for 64% of it, the matrix cores for 38%; 32400 x 4096 x 16 in 594 us when
@@ -463,7 +468,7 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
         for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kk][i]);
-        top = fmaxf(max_halves(top) * a.c, m);
+        top = fmaxf(max_halves(top) * a.c - at_below<T>(), m);
         const float f = __builtin_amdgcn_exp2f(m - top);
         l *= f;
 #pragma unroll
@@ -495,7 +500,7 @@ __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kP
         scores(left);
         if (t == t0) move();
         float sum = weights();
-        if (wave_any(!(sum <= kAtLargest))) {   // (NaN too, and then stays)
+        if (wave_any(!(sum <= at_largest<T>()))) {   // (NaN too, and then stays)
             scores(left);
             move();
             sum = weights();
