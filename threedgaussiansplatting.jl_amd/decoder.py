@@ -73,7 +73,7 @@ def _heads(t, name, shape, like):
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     b, l, h, d = t.stride()
-    if d != 1 and shape[3] > 1:
+    if d != 1 and shape[3] > 1 and t.numel():
         raise ValueError(f"the last dimension of {name} must be contiguous")
     return t.data_ptr(), b, l, h
 
@@ -168,6 +168,8 @@ def _pixels(t, name, like):
     if t.shape != like.shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(like.shape)}")
     s, n = t.stride(), t.shape
+    if not t.numel():   # (of any strides)
+        return t.data_ptr(), 0, 0
     if s[-1] != 1 and n[-1] > 1:
         raise ValueError(f"the channels of {name} must be contiguous")
     if len(n) == 3:
@@ -295,7 +297,7 @@ def _rows(t, name, rows, dim, like):
             raise ValueError(f"{name} must be contiguous, or two-dimensional")
         return t.data_ptr(), dim
     row, element = t.stride()
-    if element != 1 and dim > 1:
+    if element != 1 and dim > 1 and rows:
         raise ValueError(f"the rows of {name} must be contiguous")
     return t.data_ptr(), row if rows > 1 else dim
 
