@@ -1,0 +1,23 @@
+"""Attention: forms of a call that the formulas' tests leave out."""
+import pytest
+import torch
+
+from tdgs_amd import decoder
+from test_gpu_attention import Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("mask", ["none", "lengths", "keys"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16], ids=["f32", "f16"])
+def test_no_queries_of_shared_states(gpu, dtype, mask):
+    """Sums over no batches: the states' gradients are zeros."""
+    c = Case(dtype, 0, 1, 7, 600, 4, 2, 40, mask=mask)
+    c.run()
+    assert not c.dk.any() and not c.dv.any()
+    k = torch.randn((1, 600, 2, 40), device="cuda", requires_grad=True)
+    out = decoder.cross_attention(torch.randn((0, 7, 4, 40), device="cuda", requires_grad=True), k, k)
+    assert out.shape == (0, 7, 4, 40)
+    torch.full((4096, 600), 7.0, device="cuda")   # (left where new tensors are taken from)
+    out.sum().backward()
+    assert not k.grad.any()

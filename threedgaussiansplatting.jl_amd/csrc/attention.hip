@@ -1107,7 +1107,7 @@ using namespace tdgs;
 extern "C" {
 
 size_t tdgs_cross_attention_temp_bytes(const tdgs_attention* a, int32_t grad) {
-    if (at_check(a) != TDGS_OK || a->batch == 0) return 0;
+    if (at_check(a) != TDGS_OK || a->kv_batch == 0) return 0;
     size_t bytes = 0;
     for (int uneven = 0; uneven < 2; ++uneven) {
         const AtPlan p = at_plan(a, uneven != 0);
@@ -1172,8 +1172,10 @@ int tdgs_cross_attention(void* stream_, const tdgs_attention* a) {
 int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs_attention_grads* g) {
     TDGS_TRY(at_check(a));
     TDGS_REQUIRE(g != nullptr, "attention: null gradients");
-    if (a->batch == 0 || (a->q_len == 0 && a->kv_len == 0)) return TDGS_OK;
-    if (a->q_len > 0) {
+    // without queries dk and dv are zero, and written (a batch of none may share states)
+    const bool queries = a->batch > 0 && a->q_len > 0;
+    if (!queries && (a->kv_batch == 0 || a->kv_len == 0)) return TDGS_OK;
+    if (queries) {
         TDGS_TRY(at_check_view(&a->q, "q", a, false, false));
         TDGS_TRY(at_check_view(&a->out, "out", a, false, false));
         TDGS_TRY(at_check_view(&g->dout, "dout", a, false, false));
@@ -1188,7 +1190,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
     }
     const bool uneven = a->kv_lengths || a->kv_mask;
     const AtPlan p = at_plan(a, uneven);
-    TDGS_REQUIRE(a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16),
+    TDGS_REQUIRE(p.grad_bytes == 0 || (a->temp && a->temp_bytes >= p.grad_bytes && aligned_to(a->temp, 16)),
                  "attention: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0,
                  p.grad_bytes);
     hipStream_t stream = (hipStream_t)stream_;
@@ -1213,7 +1215,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
         using T = decltype(t);
         return with_padded(p.dp, [&](auto dp) -> int {
             constexpr int DP = decltype(dp)::value;
-            if (a->q_len > 0) {
+            if (queries) {
                 r.blocks = p.blocks_q;
                 r.splits = p.splits_q;
                 r.part_ml = r.part + p.splits_q * all_rows * DP;
