@@ -261,7 +261,9 @@ int tdgs_host_free(void* ptr);
  * context detected after that call returned (for example radix-sort counts that disagree
  * with the keys, which leaves sorted lists incomplete): TDGS_ERR_DEVICE with a message, and
  * the condition is cleared. Every call of the library that synchronises (tdgs_render,
- * tdgs_project, tdgs_fill_fgidx_to_gidx, tdgs_scan_counts, tdgs_adc_plan) checks it too. */
+ * tdgs_project, tdgs_fill_fgidx_to_gidx, tdgs_scan_counts, tdgs_adc_plan) checks it too. This
+ * call alone also reports, and clears, that an embedding call was given a token outside its
+ * table: such a token is no error of the renders that share the context. */
 int tdgs_ctx_check(tdgs_ctx* ctx, void* stream);
 
 /* Stage profiler (calling host thread): while enabled, library calls record a pair of HIP
@@ -638,7 +640,7 @@ int tdgs_group_norm_grad(void* stream, const tdgs_norm* a, const tdgs_norm_grads
 
 /* Embedding: out_i = scale table[tokens_i] for n tokens of index_bytes (4 or 8) bytes each; rows of
  * dim elements, table_stride and out_stride elements apart. A token outside [0, vocab) gives a row of zeros
- * and raises an error on ctx (tdgs_ctx_check). */
+ * and an error at the next tdgs_ctx_check of ctx (other calls on ctx do not report it). */
 int tdgs_embedding_lookup(tdgs_ctx* ctx, void* stream, int32_t dtype, const void* table, int64_t table_stride,
                           int64_t vocab, int32_t dim, const void* tokens, int32_t index_bytes, int64_t n,
                           float scale, void* out, int64_t out_stride);

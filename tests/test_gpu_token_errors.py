@@ -1,0 +1,40 @@
+"""A token outside an embedding's table is an error of the embedding call, and of no other on its context."""
+import ctypes as C
+
+import pytest
+import torch
+
+from tdgs_amd import core, decoder, host, synthetic
+
+pytestmark = pytest.mark.gpu
+
+
+def _bad_lookup(ctx=None):
+    table = torch.randn((20, 8), device="cuda")
+    decoder.embedding_lookup_(torch.empty((2, 8), device="cuda"), table, torch.tensor([3, 20], device="cuda"), ctx=ctx)
+
+
+@pytest.mark.parametrize("grad", [False, True], ids=["lookup", "grad"])
+def test_renders_and_scans_go_on(gpu, grad):
+    ctx = core.Context(0)
+    if grad:
+        n = 100000   # the tokens are sorted
+        tokens = torch.full((n,), -5, device="cuda")
+        decoder.embedding_grad_(torch.empty((20, 8), device="cuda"), torch.ones((n, 8), device="cuda"), tokens, ctx=ctx)
+    else:
+        _bad_lookup(ctx)
+    w = synthetic.config(0, n=500)
+    cam = w.cameras[0]
+    t = host.Tiling.for_camera(cam, 16, 16)
+    g = gpu.TrainableGaussiansVector.from_host(w.gaussians, 0)
+    options = host.RenderOptions.for_camera(cam, w.gaussians.sh_degree)
+    for device_counts in (False, True):
+        out = gpu.RenderOutputs.for_camera(cam, 0)
+        gpu.render_(out, g, cam, t, options, gpu.RenderBuffers(len(g), t, 0, 100_000), device_counts=device_counts, ctx=ctx)
+    torch.cuda.synchronize()
+    monitor = C.POINTER(C.c_int64)()
+    core.check(core.lib().tdgs_ctx_frame_monitor(ctx.handle, C.byref(monitor)))
+    assert (monitor[0], monitor[4]) == (1, 0)   # no error of the frame with its counts on the device
+    with pytest.raises(core.TdgsError, match="outside its table"):
+        core.ctx_check(0, ctx)
+    core.ctx_check(0, ctx)

@@ -34,9 +34,6 @@ int read_counters(tdgs_ctx* ctx, hipStream_t stream) {
         if (flags & kErrSortCounts)
             set_error("a radix sort on this context found counts that disagree with its keys; the sorted "
                       "lists of that call are incomplete (device flags 0x%x)", flags);
-        else if (flags & kErrTokenRange)
-            set_error("an embedding call on this context was given a token outside its table; it took it for a "
-                      "row of zeros (device flags 0x%x)", flags);
         else
             set_error("device error flags 0x%x raised on this context", flags);
         return TDGS_ERR_DEVICE;
@@ -274,7 +271,15 @@ int tdgs_host_free(void* ptr) {
 
 int tdgs_ctx_check(tdgs_ctx* ctx, void* stream) {
     TDGS_REQUIRE(ctx, "null ctx");
-    return read_counters(ctx, (hipStream_t)stream);
+    hipStream_t s = (hipStream_t)stream;
+    TDGS_TRY(read_counters(ctx, s));
+    if (ctx->h_counters[kTokenSlot] != 0) {
+        TDGS_HIP(hipMemsetAsync(ctx->d_counters + kTokenSlot, 0, sizeof(int64_t), s));
+        TDGS_HIP(hipStreamSynchronize(s));
+        set_error("an embedding call on this context was given a token outside its table; it took it for a row of zeros");
+        return TDGS_ERR_DEVICE;
+    }
+    return TDGS_OK;
 }
 
 int tdgs_ctx_frame_monitor(tdgs_ctx* ctx, const int64_t** monitor_out) {

@@ -27,7 +27,7 @@ struct EmArgs {
     const int32_t* order;    // their positions
     float* part;             // 2 rows per block: of the token it begins within, of the token it ends within
     int32_t *list, *count;   // blocks that a token starts in and goes on past; their number
-    uint32_t* err;
+    uint32_t* bad_token;
     float scale;
     int32_t dim, vectors, lanes;   // elements, vectors and lanes per row
     int32_t run, rows, few;        // positions per run; of one launch: table rows per workgroup, tokens (2^k)
@@ -80,7 +80,7 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_lookup(EmArgs a, FastDiv b
         EmVec<T, VW> v;
         v.zero();
         if (tok >= 0 && tok < a.vocab) v.load((const T*)a.table + tok * a.table_stride + e);
-        else atomicOr(a.err, kErrTokenRange);
+        else atomicOr(a.bad_token, 1u);
         v.store((T*)a.out + row * a.out_stride + e, a.scale);
     }
 }
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kEmThreads) void k_embed_keys(EmArgs a, uint32_t* _
     for (int64_t i = id; i < a.n; i += step) {
         const int64_t tok = em_token(a, i);
         const bool in = tok >= 0 && tok < a.vocab;
-        if (!in) atomicOr(a.err, kErrTokenRange);
+        if (!in) atomicOr(a.bad_token, 1u);
         keys[i] = in && tok != a.padding ? (uint32_t)tok : (uint32_t)a.vocab;
         values[i] = (int32_t)i;
     }
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(kEmFewThreads) void k_embed_few(EmArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool in = i0 + u * TH + (int)threadIdx.x < n;
-            if (in && (tok[u] < 0 || tok[u] >= a.vocab) && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, kErrTokenRange);
+            if (in && (tok[u] < 0 || tok[u] >= a.vocab) && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(a.bad_token, 1u);
             votes[u] = __ballot(in && tok[u] >= v0 && tok[u] < v1 && tok[u] != a.padding);
             if (lane == 0) s_wave[u * W + wave] = __popcll(votes[u]);
         }
@@ -517,7 +517,7 @@ int tdgs_embedding_lookup(tdgs_ctx* ctx, void* stream_, int32_t dtype, const voi
     a.vocab = vocab;
     a.scale = scale;
     a.dim = dim;
-    a.err = ctx_error_word(ctx);
+    a.bad_token = ctx_token_word(ctx);
     const int vw = em_vw(dtype, dim, table, table_stride, out, out_stride);
     a.vectors = dim / vw;
     int64_t blocks = ceil_div(n * a.vectors, kEmThreads);
@@ -568,7 +568,7 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     a.padding = padding;
     a.scale = scale;
     a.dim = dim;
-    a.err = ctx_error_word(ctx);
+    a.bad_token = ctx_token_word(ctx);
     a.vectors = p.vectors;
     a.lanes = p.lanes;
     a.run = p.run;
@@ -614,7 +614,7 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     }));
     TDGS_TRY(radix_sort_pairs_grouped<uint32_t>(k[0], k[1], v[0], v[1], k[2], v[2], n, 0, em_bits(vocab), sort_temp,
                                                 p.sort_bytes, p.group_words > 0 ? clear : nullptr, p.group_words,
-                                                stream, a.err));
+                                                stream, ctx_error_word(ctx)));
     return em_dispatch(dtype, vw, [&](auto t, auto w) -> int {
         using T = decltype(t);
         constexpr int VW = decltype(w)::value;

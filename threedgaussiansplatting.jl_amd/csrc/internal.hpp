@@ -25,9 +25,12 @@ constexpr int kMonitor = 5;
 // kErr* bits into it; every host synchronisation through read_counters reports and clears it.
 constexpr int kErrSlot = 7;
 constexpr uint32_t kErrSortCounts = 1u;   // radix-sort counts disagreed with the keys
-constexpr uint32_t kErrTokenRange = 2u;   // an embedding token outside the table
+// Slot for what is wrong with a caller's data, not with the calls that share the context, and is therefore reported (and
+// cleared) by tdgs_ctx_check only: non-zero after an embedding token outside its table.
+constexpr int kTokenSlot = 10;
 
 inline uint32_t* ctx_error_word(tdgs_ctx* ctx) { return reinterpret_cast<uint32_t*>(ctx->d_counters + kErrSlot); }
+inline uint32_t* ctx_token_word(tdgs_ctx* ctx) { return reinterpret_cast<uint32_t*>(ctx->d_counters + kTokenSlot); }
 
 // Other slots of ctx->d_counters: 0 filtered count N_f, 1 key count M, 2 ADC count, 4 count of
 // non-empty Gaussians, 8 entries of the coarse blocks' lists; in a render with
