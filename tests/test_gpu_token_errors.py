@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tdgs_amd import core, decoder, host, synthetic
+from tdgs_amd import appearance, core, decoder, host, synthetic
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,13 @@ def test_renders_and_scans_go_on(gpu, grad):
     with pytest.raises(core.TdgsError, match="outside its table"):
         core.ctx_check(0, ctx)
     core.ctx_check(0, ctx)
+
+
+@pytest.mark.parametrize("image", [-1, 3])
+def test_photographs_outside_the_collection(gpu, image):
+    """Refused on the host, before any token is looked up."""
+    dec = appearance.AppearanceDecoder(3, channels=32, groups=4)
+    with pytest.raises(ValueError, match="of a collection of 3"):
+        dec(torch.rand((8, 8, 3), device="cuda"), image)
+    dec(torch.rand((8, 8, 3), device="cuda"), 2)
+    core.ctx_check(0)
