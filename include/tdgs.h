@@ -645,7 +645,8 @@ int tdgs_embedding_lookup(tdgs_ctx* ctx, void* stream, int32_t dtype, const void
                           int64_t vocab, int32_t dim, const void* tokens, int32_t index_bytes, int64_t n,
                           float scale, void* out, int64_t out_stride);
 /* The gradient of sum(dout * out) for the table: dtable_v = scale * the sum, in 32 bits, of the dout_i
- * with tokens_i = v; every row of dtable is written. The token `padding` (-1: none) gives no gradient.
+ * with tokens_i = v; every row of dtable is written. The token `padding`, a row of the
+ * table or -1 (none), gives no gradient.
  * The tokens are sorted and added up in order, so that the result is the same every time. */
 size_t tdgs_embedding_grad_temp_bytes(int64_t n, int64_t vocab, int32_t dim);
 int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream, int32_t dtype, const void* dout, int64_t dout_stride,

@@ -548,6 +548,8 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream_, int32_t dtype, const void*
     TDGS_REQUIRE(ctx != nullptr, "embedding: null context");
     TDGS_TRY(em_check(dtype, index_bytes, vocab, dim, n));
     if (vocab == 0) return TDGS_OK;
+    TDGS_REQUIRE(padding >= -1 && padding < vocab, "embedding: padding %lld is no row of a table of %lld", (long long)padding,
+                 (long long)vocab);
     TDGS_REQUIRE(n == 0 || (tokens && aligned_to(tokens, (size_t)index_bytes)), "embedding: tokens are null or misaligned");
     TDGS_TRY(em_check_rows(dout, "dout", dtype, dout_stride, dim, n, false));
     TDGS_TRY(em_check_rows(dtable, "dtable", dtype, dtable_stride, dim, vocab, true));

@@ -302,6 +302,12 @@ def _rows(t, name, rows, dim, like):
     return t.data_ptr(), row if rows > 1 else dim
 
 
+def _check_padding(padding, vocab):
+    # (counted from the end elsewhere: neither that nor "none" can be told from -1)
+    if padding is not None and not 0 <= padding < vocab:
+        raise ValueError(f"padding {padding} is no row of a table of {vocab}")
+
+
 def embedding_lookup_(out, table, tokens, *, scale=1.0, ctx=None):
     """out[i] = scale table[tokens[i]] (tdgs_embedding_lookup). table is (vocab, dim), tokens int32 or int64
     of any shape, out their shape with dim behind. A token outside the table gives a row of zeros and an
@@ -322,8 +328,10 @@ def embedding_temp(table, tokens):
 
 def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None, ctx=None):
     """dtable[v] = scale times the sum of the dout rows whose token is v, in 32 bits and in the tokens'
-    order (tdgs_embedding_grad); every row is written. The token `padding` gives no gradient."""
+    order (tdgs_embedding_grad); every row is written. The token `padding`, a row of the table, gives no
+    gradient (None: every token does)."""
     vocab, dim, t, ts = _table(dtable, "dtable")
+    _check_padding(padding, vocab)
     size, n = _tokens(tokens, dtable), tokens.numel()
     d, ds = _rows(dout, "dout", n, dim, dtable)
     if temp is None:
@@ -445,4 +453,5 @@ class _Embedding(torch.autograd.Function):
 
 def embedding(table, tokens, *, scale=1.0, padding=None):
     """embedding_lookup_ as a differentiable function of the table; `padding` as in embedding_grad_."""
+    _check_padding(padding, table.shape[0])
     return _Embedding.apply(_rows_contiguous(table), tokens, scale, padding)
