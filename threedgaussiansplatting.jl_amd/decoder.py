@@ -37,6 +37,16 @@ assert (_ATTENTION.size, _ATTENTION_GRADS.size, _NORM.size, _NORM_GRADS.size) ==
     C.sizeof(t) for t in (abi.AttentionC, abi.AttentionGradsC, abi.NormC, abi.NormGradsC))
 
 
+def _call(f, t, *args):
+    """f(*args) on t's device (kernels are launched on the current one, whatever device a stream belongs to)."""
+    device = t.get_device()
+    if device == torch.cuda.current_device():
+        check(f(*args))
+    else:
+        with torch.cuda.device(device):
+            check(f(*args))
+
+
 def _stream(t):
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
@@ -137,7 +147,7 @@ def cross_attention_(out, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None,
     a = _attention(q, k, v, out, lse, scale, kv_lengths, kv_mask)
     if temp is None:
         temp = cross_attention_temp(q, k)
-    check(lib().tdgs_cross_attention(_stream(q), _ATTENTION.pack(*a, *_temp(temp, q))))
+    _call(lib().tdgs_cross_attention, q, _stream(q), _ATTENTION.pack(*a, *_temp(temp, q)))
     return out
 
 
@@ -152,7 +162,7 @@ def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv
          *_heads(dv, "dv", k.shape, q))
     if temp is None:
         temp = cross_attention_temp(q, k, grad=True)
-    check(lib().tdgs_cross_attention_grad(_stream(q), _ATTENTION.pack(*a, *_temp(temp, q)), _ATTENTION_GRADS.pack(*g)))
+    _call(lib().tdgs_cross_attention_grad, q, _stream(q), _ATTENTION.pack(*a, *_temp(temp, q)), _ATTENTION_GRADS.pack(*g))
     return dq, dk, dv
 
 
@@ -241,7 +251,7 @@ def group_norm_(out, x, groups, weight=None, bias=None, *, eps=1e-5, activation=
     a = _norm(x, out, groups, weight, bias, eps, activation, stats)
     if temp is None:
         temp = group_norm_temp(x, groups)
-    check(lib().tdgs_group_norm(_stream(x), _NORM.pack(*a, *_temp(temp, x))))
+    _call(lib().tdgs_group_norm, x, _stream(x), _NORM.pack(*a, *_temp(temp, x)))
     return out
 
 
@@ -259,7 +269,7 @@ def group_norm_grad_(dx, dweight, dbias, dout, x, stats, groups, weight=None, bi
     g = (*_pixels(dout, "dout", x), *_pixels(dx, "dx", x), dptr(dweight) or 0, dptr(dbias) or 0)
     if temp is None:
         temp = group_norm_temp(x, groups, grad=True)
-    check(lib().tdgs_group_norm_grad(_stream(x), _NORM.pack(*a, *_temp(temp, x)), _NORM_GRADS.pack(*g)))
+    _call(lib().tdgs_group_norm_grad, x, _stream(x), _NORM.pack(*a, *_temp(temp, x)), _NORM_GRADS.pack(*g))
     return dx, dweight, dbias
 
 
@@ -315,8 +325,8 @@ def embedding_lookup_(out, table, tokens, *, scale=1.0, ctx=None):
     vocab, dim, t, ts = _table(table, "table")
     size, n = _tokens(tokens, table), tokens.numel()
     o, os = _rows(out, "out", n, dim, table)
-    check(lib().tdgs_embedding_lookup(_handle(ctx, table.get_device()), _stream(table), DTYPES[table.dtype], t, ts, vocab,
-                                      dim, tokens.data_ptr(), size, n, scale, o, os))
+    _call(lib().tdgs_embedding_lookup, table, _handle(ctx, table.get_device()), _stream(table), DTYPES[table.dtype], t, ts,
+          vocab, dim, tokens.data_ptr(), size, n, scale, o, os)
     return out
 
 
@@ -336,9 +346,8 @@ def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None,
     d, ds = _rows(dout, "dout", n, dim, dtable)
     if temp is None:
         temp = embedding_temp(dtable, tokens)
-    check(lib().tdgs_embedding_grad(_handle(ctx, dtable.get_device()), _stream(dtable), DTYPES[dtable.dtype], d, ds,
-                                    tokens.data_ptr(), size, n, -1 if padding is None else padding, scale, t, ts, vocab,
-                                    dim, *_temp(temp, dtable)))
+    _call(lib().tdgs_embedding_grad, dtable, _handle(ctx, dtable.get_device()), _stream(dtable), DTYPES[dtable.dtype], d, ds,
+          tokens.data_ptr(), size, n, -1 if padding is None else padding, scale, t, ts, vocab, dim, *_temp(temp, dtable))
     return dtable
 
 
