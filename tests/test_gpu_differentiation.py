@@ -31,3 +31,31 @@ def test_empty_gradients(gpu):
         f().sum().backward()
     for t in (q, k, x, w, table):
         assert t.grad.shape == t.shape and not t.grad.any()
+
+
+def test_views_of_any_strides(gpu):
+    """The functions take what torch's own take: crops, transposed tensors and every other token, as if they had been copied."""
+    gen = torch.Generator().manual_seed(3)
+
+    def leaf(*shape):
+        return torch.randn(shape, generator=gen).cuda().requires_grad_(True)
+
+    wide, params, table = leaf(2, 12, 11, 16), leaf(16, 2), leaf(30, 24)
+    q, k = leaf(2, 6, 4, 8), leaf(2, 9, 2, 8)
+    tokens = torch.randint(0, 30, (7, 10), generator=gen).cuda()
+    mask = (torch.rand((9, 2), generator=gen) < 0.7).cuda()
+    lengths = torch.tensor([[9, 0], [5, 0]], dtype=torch.int32, device="cuda")
+    calls = {
+        "crop": (lambda c: decoder.group_norm(c(wide[:, 1:9, 2:9]), 4, c(params[:, 0]), c(params[:, 1])), (wide, params)),
+        "every other row": (lambda c: decoder.group_norm(c(wide[:, ::2]), 4), (wide,)),
+        "images apart": (lambda c: decoder.group_norm(c(wide.transpose(0, 1)), 4), (wide,)),
+        "channels apart": (lambda c: decoder.group_norm(c(wide.permute(0, 3, 1, 2)[..., :8]), 4), (wide,)),
+        "tokens": (lambda c: decoder.embedding(c(table[:, ::2]), c(tokens.t()[::3])), (table,)),
+        "mask": (lambda c: decoder.cross_attention(c(q), c(k), c(k), kv_mask=c(mask.t()), kv_lengths=c(lengths[:, 0])), (q, k)),
+    }
+    for name, (f, leaves) in calls.items():
+        out, want = f(lambda t: t), f(lambda t: t.contiguous())
+        assert torch.equal(out, want), name
+        coef = torch.randn(out.shape, generator=gen).cuda()
+        for a, b in zip(torch.autograd.grad((out * coef).sum(), leaves), torch.autograd.grad((want * coef).sum(), leaves)):
+            assert torch.equal(a, b), name

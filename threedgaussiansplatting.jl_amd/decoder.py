@@ -170,6 +170,22 @@ def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv
 # Group norm with an activation
 # ------------------------------------------------------------------------------------
 
+def _pixel_step(t):
+    """The stride between the pixels of a (n, .., channels) tensor, None where they are not evenly strided."""
+    s, n = t.stride(), t.shape
+    if len(n) == 3:
+        return s[1]
+    step, count = n[-1], 1
+    for i in range(len(n) - 2, 0, -1):
+        if n[i] > 1:
+            if count == 1:
+                step = s[i]
+            elif s[i] != step * count:
+                return None
+            count *= n[i]
+    return step
+
+
 def _pixels(t, name, like):
     """The fields of the tdgs_pixels of a (n, .., channels) tensor whose middle dimensions are evenly strided."""
     _check_tensor(t, name, like)
@@ -177,22 +193,14 @@ def _pixels(t, name, like):
         raise ValueError(f"{name} is {t.dtype}, not {like.dtype}")
     if t.shape != like.shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(like.shape)}")
-    s, n = t.stride(), t.shape
     if not t.numel():   # (of any strides)
         return t.data_ptr(), 0, 0
-    if s[-1] != 1 and n[-1] > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"the channels of {name} must be contiguous")
-    if len(n) == 3:
-        return t.data_ptr(), s[0], s[1]
-    step, count = n[-1], 1
-    for i in range(len(n) - 2, 0, -1):
-        if n[i] > 1:
-            if count == 1:
-                step = s[i]
-            elif s[i] != step * count:
-                raise ValueError(f"the pixels of {name} must be evenly strided")
-            count *= n[i]
-    return t.data_ptr(), s[0], step
+    step = _pixel_step(t)
+    if step is None:
+        raise ValueError(f"the pixels of {name} must be evenly strided")
+    return t.data_ptr(), t.stride(0), step
 
 
 _NO_PIXELS = (0, 0, 0)
@@ -356,8 +364,12 @@ def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None,
 # ------------------------------------------------------------------------------------
 
 def _rows_contiguous(t):
-    """t, or a copy where its last dimension is not contiguous (a gradient may come as any view)."""
+    """t, or a copy where its last dimension is not contiguous."""
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _contiguous(t):
+    return None if t is None else t.contiguous()
 
 
 class _Refused(torch.autograd.Function):
@@ -411,9 +423,9 @@ class _CrossAttention(torch.autograd.Function):
 
 
 def cross_attention(q, k, v, *, scale=None, kv_lengths=None, kv_mask=None):
-    """cross_attention_ as a differentiable function of q, k and v."""
-    return _CrossAttention.apply(_rows_contiguous(q), _rows_contiguous(k), _rows_contiguous(v), scale, kv_lengths,
-                                 kv_mask)
+    """cross_attention_ as a differentiable function of q, k and v, all tensors of any strides."""
+    return _CrossAttention.apply(_rows_contiguous(q), _rows_contiguous(k), _rows_contiguous(v), scale,
+                                 _contiguous(kv_lengths), None if kv_mask is None else _rows_contiguous(kv_mask))
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -438,8 +450,10 @@ class _GroupNorm(torch.autograd.Function):
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation="silu"):
-    """group_norm_ as a differentiable function of x, weight and bias."""
-    return _GroupNorm.apply(_rows_contiguous(x), weight, bias, groups, eps, activation)
+    """group_norm_ as a differentiable function of x, weight and bias, all of any strides."""
+    x = _rows_contiguous(x)
+    return _GroupNorm.apply(x if _pixel_step(x) is not None else x.contiguous(), _contiguous(weight), _contiguous(bias),
+                            groups, eps, activation)
 
 
 class _Embedding(torch.autograd.Function):
@@ -461,6 +475,7 @@ class _Embedding(torch.autograd.Function):
 
 
 def embedding(table, tokens, *, scale=1.0, padding=None):
-    """embedding_lookup_ as a differentiable function of the table; `padding` as in embedding_grad_."""
+    """embedding_lookup_ as a differentiable function of the table, it and the tokens of any strides; `padding` as in
+    embedding_grad_."""
     _check_padding(padding, table.shape[0])
-    return _Embedding.apply(_rows_contiguous(table), tokens, scale, padding)
+    return _Embedding.apply(_rows_contiguous(table), tokens.contiguous(), scale, padding)
