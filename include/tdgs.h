@@ -585,7 +585,7 @@ typedef struct tdgs_attention {
 } tdgs_attention;
 
 /* The gradients' tensors: dout as q's shape; dq, dk, dv as q's, k's and v's (dk and dv summed over the
- * query heads and, where kv_batch is 1, over the batches that share a key). */
+ * query heads and, where kv_batch is 1, over the batches that share a key; both null: not wanted). */
 typedef struct tdgs_attention_grads {
     tdgs_heads dout, dq, dk, dv;
 } tdgs_attention_grads;

@@ -88,3 +88,31 @@ def test_second_derivative_raises(stand_ins, name):
             torch.autograd.grad((g ** 2).sum(), leaf, retain_graph=True)
         with pytest.raises(RuntimeError, match="differentiated again"):
             (g ** 2).sum().backward()
+
+
+def test_gradients_that_nothing_needs(stand_ins, monkeypatch):
+    """Frozen states and parameters: their gradients are not asked for, the others are the same."""
+    asked = {}
+
+    def record(name, n):
+        f = getattr(decoder, name)
+        monkeypatch.setattr(decoder, name, lambda *a, **kw: (asked.update({name: [t is not None for t in a[:n]]}), f(*a, **kw))[1])
+
+    record("cross_attention_grad_", 3)
+    record("group_norm_grad_", 3)
+    gen = torch.Generator().manual_seed(4)
+    q, k, v, x = (torch.randn(s, generator=gen, dtype=torch.float64) for s in ((1, 5, 2, 4), (1, 3, 2, 4), (1, 3, 2, 4), (1, 6, 4)))
+    w, b = torch.ones(4, dtype=torch.float64), torch.zeros(4, dtype=torch.float64)
+
+    def grads(f, *leaves):
+        for t in (q, k, v, x, w, b):
+            t.requires_grad_(any(t is u for u in leaves))
+        return torch.autograd.grad((f() ** 2).sum(), leaves)
+
+    attention, norm = lambda: decoder.cross_attention(q, k, v), lambda: decoder.group_norm(x, 2, w, b)   # noqa: E731
+    every = grads(attention, q, k, v) + grads(norm, x, w, b)
+    assert asked == {"cross_attention_grad_": [True, True, True], "group_norm_grad_": [True, True, True]}
+    some = grads(attention, q) + grads(norm, x, b)
+    assert asked == {"cross_attention_grad_": [True, False, False], "group_norm_grad_": [True, False, True]}
+    for a, g in zip(some, (every[0], every[3], every[5])):
+        assert torch.equal(a, g)

@@ -9,7 +9,10 @@ def test_no_batches_of_shared_states(lib):  # noqa: F811
     """There are gradients of the states to write (zeros), so the call is checked as any other."""
     a = _attention(batch=0, kv_batch=1)
     assert lib.tdgs_cross_attention(None, C.byref(a)) == abi.TDGS_OK
-    assert lib.tdgs_cross_attention_grad(None, C.byref(a), C.byref(abi.AttentionGradsC())) == abi.TDGS_ERR_INVALID
+    g = abi.AttentionGradsC()
+    assert lib.tdgs_cross_attention_grad(None, C.byref(a), C.byref(g)) == abi.TDGS_OK   # (not wanted)
+    g.dk.data = g.dv.data = 64
+    assert lib.tdgs_cross_attention_grad(None, C.byref(a), C.byref(g)) == abi.TDGS_ERR_INVALID
     assert b"k is null" in lib.tdgs_last_error()
     a.kv_lengths = 64
     assert lib.tdgs_cross_attention_temp_bytes(C.byref(a), 1) >= 4 * (9 + 1)   # the list of keys

@@ -21,3 +21,18 @@ def test_no_queries_of_shared_states(gpu, dtype, mask):
     torch.full((4096, 600), 7.0, device="cuda")   # (left where new tensors are taken from)
     out.sum().backward()
     assert not k.grad.any()
+
+
+@pytest.mark.parametrize("mask", ["none", "both"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_queries_gradient_alone(gpu, dtype, mask):
+    """Without dk and dv the call writes the same dq, and no other."""
+    c = Case(dtype, 2, 1, 70, 600, 4, 2, 40, mask=mask)
+    c.run()
+    want = c.dq.clone()
+    c.dq.zero_()
+    decoder.cross_attention_grad_(c.dq, None, None, c.dout, c.out, c.lse, c.q, c.k, c.v, **c.args)
+    assert torch.equal(c.dq, want)
+    for dk, dv in ((c.dk, None), (None, c.dv)):
+        with pytest.raises(ValueError):
+            decoder.cross_attention_grad_(c.dq, dk, dv, c.dout, c.out, c.lse, c.q, c.k, c.v, **c.args)

@@ -1174,7 +1174,8 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
     TDGS_REQUIRE(g != nullptr, "attention: null gradients");
     // without queries dk and dv are zero, and written (a batch of none may share states)
     const bool queries = a->batch > 0 && a->q_len > 0;
-    if (!queries && (a->kv_batch == 0 || a->kv_len == 0)) return TDGS_OK;
+    const bool keys = a->kv_batch > 0 && a->kv_len > 0, key_grads = keys && (g->dk.data || g->dv.data);
+    if (!queries && !key_grads) return TDGS_OK;
     if (queries) {
         TDGS_TRY(at_check_view(&a->q, "q", a, false, false));
         TDGS_TRY(at_check_view(&a->out, "out", a, false, false));
@@ -1182,9 +1183,11 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
         TDGS_TRY(at_check_view(&g->dq, "dq", a, false, true));
         TDGS_REQUIRE(a->lse != nullptr, "attention: the gradient needs the forward call's lse");
     }
-    if (a->kv_len > 0) {
+    if (keys) {
         TDGS_TRY(at_check_view(&a->k, "k", a, true, false));
         TDGS_TRY(at_check_view(&a->v, "v", a, true, false));
+    }
+    if (key_grads) {
         TDGS_TRY(at_check_view(&g->dk, "dk", a, true, true));
         TDGS_TRY(at_check_view(&g->dv, "dv", a, true, true));
     }
@@ -1228,7 +1231,7 @@ int tdgs_cross_attention_grad(void* stream_, const tdgs_attention* a, const tdgs
                     TDGS_TRY(at_sum<T>(r, DP, all_rows, 0, stream));
                 }
             }
-            if (a->kv_len > 0) {
+            if (key_grads) {
                 r.blocks = p.blocks_k;
                 r.splits = p.splits_k;
                 const unsigned grid = (unsigned)(p.kvh * p.splits_k * p.blocks_k);

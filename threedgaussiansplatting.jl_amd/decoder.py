@@ -154,12 +154,12 @@ def cross_attention_(out, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None,
 def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None,
                           temp=None):
     """The gradients of sum(dout * out) for cross_attention_'s operands (tdgs_cross_attention_grad), from
-    its out and lse. dk and dv are summed over the heads, and batches, that share a key."""
+    its out and lse. dk and dv are summed over the heads, and batches, that share a key; both may be None."""
     if lse is None:
         raise ValueError("the gradient needs the forward call's lse")
     a = _attention(q, k, v, out, lse, scale, kv_lengths, kv_mask)
-    g = (*_heads(dout, "dout", q.shape, q), *_heads(dq, "dq", q.shape, q), *_heads(dk, "dk", k.shape, q),
-         *_heads(dv, "dv", k.shape, q))
+    keys = _NO_HEADS * 2 if dk is None and dv is None else (*_heads(dk, "dk", k.shape, q), *_heads(dv, "dv", k.shape, q))
+    g = (*_heads(dout, "dout", q.shape, q), *_heads(dq, "dq", q.shape, q), *keys)
     if temp is None:
         temp = cross_attention_temp(q, k, grad=True)
     _call(lib().tdgs_cross_attention_grad, q, _stream(q), _ATTENTION.pack(*a, *_temp(temp, q)), _ATTENTION_GRADS.pack(*g))
@@ -416,7 +416,10 @@ class _CrossAttention(torch.autograd.Function):
     @_once
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths, kv_mask = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        # (dq also leaves what dk and dv are computed from)
+        wanted = (True, any(ctx.needs_input_grad[1:3]), any(ctx.needs_input_grad[1:3]))
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if w else None
+                      for t, w in zip((q, k, v), wanted))
         cross_attention_grad_(dq, dk, dv, dout.contiguous(), out, lse, q, k, v, scale=ctx.scale, kv_lengths=kv_lengths,
                               kv_mask=kv_mask)
         return dq, dk, dv, None, None, None
@@ -443,7 +446,7 @@ class _GroupNorm(torch.autograd.Function):
     def backward(ctx, dout):
         x, weight, bias, stats = ctx.saved_tensors
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dweight, dbias = (None if p is None else torch.empty_like(p) for p in (weight, bias))
+        dweight, dbias = (torch.empty_like(p) if w else None for p, w in zip((weight, bias), ctx.needs_input_grad[1:3]))
         group_norm_grad_(dx, dweight, dbias, dout.contiguous(), x, stats, ctx.groups, weight, bias,
                          activation=ctx.activation)
         return dx, dweight, dbias, None, None, None
