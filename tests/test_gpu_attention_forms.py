@@ -36,3 +36,16 @@ def test_queries_gradient_alone(gpu, dtype, mask):
     for dk, dv in ((c.dk, None), (None, c.dv)):
         with pytest.raises(ValueError):
             decoder.cross_attention_grad_(c.dq, dk, dv, c.dout, c.out, c.lse, c.q, c.k, c.v, **c.args)
+
+
+@pytest.mark.parametrize("size", [
+    # b, lq, lk, h, hk, d: rows go on by whole batches, by queries and heads with and without carries
+    (150, 1, 40, 2, 2, 16), (150, 1, 600, 3, 1, 40), (67, 3, 520, 6, 2, 16), (40, 7, 90, 5, 1, 33), (9, 32, 70, 2, 2, 64),
+    (9, 33, 530, 4, 2, 64), (3, 40, 70, 40, 1, 8), (5, 64, 20, 1, 1, 32), (2, 100, 33, 70, 1, 8),
+], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["f32", "bf16", "f16"])
+def test_shared_states_of_batches_of_few_queries(gpu, dtype, size):
+    b, lq, lk, h, hk, d = size
+    c = Case(dtype, b, 1, lq, lk, h, hk, d, "bhld", seed=b)
+    c.run()
+    c.check()

@@ -761,13 +761,18 @@ __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(A
     const int tiles = (a.rows + RT - 1) / RT, per = (tiles + a.splits - 1) / a.splits;
     const int t_end = blk * (TH / kWave) * 32 < len ? min(tiles, (sp + 1) * per) : 0;   // no allowed key: no rows
     AtTile<T, DP, RT, TH, VEC> tq, td;
-    // Where chunk k's row stands, and how it goes RT rows on: a few additions, where at_row would divide. A row past the
-    // last stays on the last.
+    // Where chunk k's row stands, and how it goes RT rows on: a few additions, where at_row would divide. RT is so many batches,
+    // queries and heads, each with one carry at most, however few queries a batch has. A row past the last stays on the last.
     constexpr int PER = decltype(tq)::kPer;
     int32_t row[PER], qi[PER], qh[PER];
     int64_t at_q[PER], at_d[PER], at_s[PER];
     float st[PER];
-    const int G = (int)a.by_g.d, step_i = RT / G, step_h = RT % G;
+    const int G = (int)a.by_g.d, per_batch = (int)a.by_lg.d;
+    const int step_b = RT / per_batch, step_i = RT % per_batch / G, step_h = RT % per_batch % G;
+    const int64_t batch_s = (int64_t)a.heads * a.q_len;
+    const int64_t step_q = step_b * a.sq.b + step_i * a.sq.l + step_h * a.sq.h;
+    const int64_t step_d = step_b * a.sdo.b + step_i * a.sdo.l + step_h * a.sdo.h;
+    const int64_t step_s = step_b * batch_s + step_i + (int64_t)step_h * a.q_len;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
         row[k] = min(sp * per * RT + (tq.inside(k) ? tq.row(k) : 0), a.rows - 1);
@@ -779,13 +784,6 @@ __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(A
         at_d[k] = at_offset(a.sdo, at);
         at_s[k] = at_stat(a, at);
     }
-    auto go = [&](int k, int di, int dh, int64_t ds) {   // di queries and dh heads on, ds statistics
-        qi[k] += di;
-        qh[k] += dh;
-        at_q[k] += di * a.sq.l + dh * a.sq.h;
-        at_d[k] += di * a.sdo.l + dh * a.sdo.h;
-        at_s[k] += ds;
-    };
     auto fetch = [&]() {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -794,12 +792,23 @@ __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(A
             st[k] = (tq.col(k) == 0 ? a.lse : a.delta)[at_s[k]];   // the first chunk of a row brings lse, the others delta
             if (row[k] + RT < a.rows) {
                 row[k] += RT;
-                go(k, step_i, step_h, step_i + (int64_t)step_h * a.q_len);
-                if (qh[k] >= G) go(k, 1, -G, 1 - (int64_t)G * a.q_len);
-                while (qi[k] >= a.q_len) {   // the next batch
-                    go(k, -a.q_len, 0, (int64_t)(a.heads - 1) * a.q_len);
-                    at_q[k] += a.sq.b;
-                    at_d[k] += a.sdo.b;
+                qi[k] += step_i;
+                qh[k] += step_h;
+                at_q[k] += step_q;
+                at_d[k] += step_d;
+                at_s[k] += step_s;
+                if (qh[k] >= G) {   // the next query
+                    qh[k] -= G;
+                    qi[k] += 1;
+                    at_q[k] += a.sq.l - G * a.sq.h;
+                    at_d[k] += a.sdo.l - G * a.sdo.h;
+                    at_s[k] += 1 - (int64_t)G * a.q_len;
+                }
+                if (qi[k] >= a.q_len) {   // the next batch
+                    qi[k] -= a.q_len;
+                    at_q[k] += a.sq.b - a.q_len * a.sq.l;
+                    at_d[k] += a.sdo.b - a.q_len * a.sdo.l;
+                    at_s[k] += batch_s - a.q_len;
                 }
             }
         }
