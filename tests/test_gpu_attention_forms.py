@@ -49,3 +49,13 @@ def test_shared_states_of_batches_of_few_queries(gpu, dtype, size):
     c = Case(dtype, b, 1, lq, lk, h, hk, d, "bhld", seed=b)
     c.run()
     c.check()
+
+
+def test_no_batches_of_many_queries(gpu):
+    """Queries times shared heads do not fit 32 bits, but there are no batches of them."""
+    q = torch.empty((0, 1 << 30, 4, 8), device="cuda")
+    k = torch.randn((1, 5, 1, 8), device="cuda")
+    dk, dv = torch.full_like(k, 7.0), torch.full_like(k, 7.0)
+    decoder.cross_attention_(q, q, k, k)
+    decoder.cross_attention_grad_(q, dk, dv, q, q, torch.empty((0, 4, 1 << 30), device="cuda"), q, k, k)
+    assert not dk.any() and not dv.any()

@@ -1104,7 +1104,7 @@ static AtArgs at_args(const tdgs_attention* a, const AtPlan& p) {
     r.c = a->scale * kLog2e;
     const uint32_t g = (uint32_t)(a->heads / a->kv_heads);
     r.by_g = FastDiv(g);
-    r.by_lg = FastDiv(g * (uint32_t)(a->q_len > 0 ? a->q_len : 1));
+    r.by_lg = FastDiv(p.rows > 0 ? g * (uint32_t)a->q_len : 1);   // (no rows: never divided by)
     r.vec_out = a->head_dim % 8 == 0 && at_rows_aligned(a->out, e);
     return r;
 }
