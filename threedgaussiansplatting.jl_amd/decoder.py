@@ -143,7 +143,11 @@ def cross_attention_(out, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None,
     up to 128, scale head_dim ** -0.5 by default. kv_lengths (kv_batch int32) allows each batch's first
     keys, kv_mask (kv_batch, kv_len; bool or uint8) single ones; k and v may hold anything where a key is not
     allowed. A query without allowed keys gets zeros. lse (batch, heads, q_len; float32), where given,
-    receives the logarithm of each softmax's sum, which the gradient needs."""
+    receives the logarithm of each softmax's sum, which the gradient needs.
+
+    With 16-bit types the weights are rounded to the type before their product with v where out has more than
+    65536 elements, and keep twice its bits otherwise, so that a query's result may differ by 1.4 of its own
+    rounding between a small call and a large one (tdgs_attention says it for the gradients)."""
     a = _attention(q, k, v, out, lse, scale, kv_lengths, kv_mask)
     if temp is None:
         temp = cross_attention_temp(q, k)
