@@ -1,6 +1,7 @@
 """A token outside an embedding's table is an error of the embedding call, and of no other on its context."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -40,7 +41,7 @@ def test_renders_and_scans_go_on(gpu, grad):
     core.ctx_check(0, ctx)
 
 
-@pytest.mark.parametrize("image", [-1, 3])
+@pytest.mark.parametrize("image", [-1, 3, np.int64(5)])
 def test_photographs_outside_the_collection(gpu, image):
     """Refused on the host, before any token is looked up."""
     dec = appearance.AppearanceDecoder(3, channels=32, groups=4)

@@ -54,7 +54,7 @@ class AppearanceDecoder:
     def __call__(self, rgb, image, states=None):
         """The corrected (w, h, 3) float32 image of the rendered one, as photograph `image` of the collection
         shows it; states (length, states_dim) are an encoder's. Differentiable for rgb and the parameters."""
-        if isinstance(image, int) and not 0 <= image < self.nb_images:
+        if not isinstance(image, torch.Tensor) and not 0 <= image < self.nb_images:
             raise ValueError(f"photograph {image} of a collection of {self.nb_images}")
         p, s, c = self.parameters, self.patch, self.channels
         w, h, _ = rgb.shape
