@@ -32,7 +32,7 @@ def test_launched_on_the_tensors_device(monkeypatch, name, current):
         def __getattr__(self, entry):
             return lambda *args: 64 if entry.endswith("temp_bytes") else seen.append((entry, now[0])) or 0
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
     monkeypatch.setattr(torch.cuda, "device", device)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
     monkeypatch.setattr(decoder, "lib", Library)

@@ -37,18 +37,16 @@ assert (_ATTENTION.size, _ATTENTION_GRADS.size, _NORM.size, _NORM_GRADS.size) ==
     C.sizeof(t) for t in (abi.AttentionC, abi.AttentionGradsC, abi.NormC, abi.NormGradsC))
 
 
-def _call(f, t, *args):
-    """f(*args) on t's device (kernels are launched on the current one, whatever device a stream belongs to)."""
+def _call(f, t, args, ctx=()):
+    """f(*ctx, stream, *args) on t's device and its current stream: kernels are launched on the current device, whatever
+    device a stream belongs to."""
     device = t.get_device()
-    if device == torch.cuda.current_device():
-        check(f(*args))
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch._C._cuda_getDevice():
+        check(f(*ctx, stream, *args))
     else:
         with torch.cuda.device(device):
-            check(f(*args))
-
-
-def _stream(t):
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+            check(f(*ctx, stream, *args))
 
 
 def _check_tensor(t, name, like):
@@ -151,7 +149,7 @@ def cross_attention_(out, q, k, v, *, scale=None, kv_lengths=None, kv_mask=None,
     a = _attention(q, k, v, out, lse, scale, kv_lengths, kv_mask)
     if temp is None:
         temp = cross_attention_temp(q, k)
-    _call(lib().tdgs_cross_attention, q, _stream(q), _ATTENTION.pack(*a, *_temp(temp, q)))
+    _call(lib().tdgs_cross_attention, q, (_ATTENTION.pack(*a, *_temp(temp, q)),))
     return out
 
 
@@ -166,7 +164,7 @@ def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv
     g = (*_heads(dout, "dout", q.shape, q), *_heads(dq, "dq", q.shape, q), *keys)
     if temp is None:
         temp = cross_attention_temp(q, k, grad=True)
-    _call(lib().tdgs_cross_attention_grad, q, _stream(q), _ATTENTION.pack(*a, *_temp(temp, q)), _ATTENTION_GRADS.pack(*g))
+    _call(lib().tdgs_cross_attention_grad, q, (_ATTENTION.pack(*a, *_temp(temp, q)), _ATTENTION_GRADS.pack(*g)))
     return dq, dk, dv
 
 
@@ -174,11 +172,9 @@ def cross_attention_grad_(dq, dk, dv, dout, out, lse, q, k, v, *, scale=None, kv
 # Group norm with an activation
 # ------------------------------------------------------------------------------------
 
-def _pixel_step(t):
-    """The stride between the pixels of a (n, .., channels) tensor, None where they are not evenly strided."""
-    s, n = t.stride(), t.shape
-    if len(n) == 3:
-        return s[1]
+def _pixel_step(s, n):
+    """The stride between the pixels of a (n, .., channels) tensor of strides s and shape n, None where they are not evenly
+    strided."""
     step, count = n[-1], 1
     for i in range(len(n) - 2, 0, -1):
         if n[i] > 1:
@@ -195,16 +191,17 @@ def _pixels(t, name, like):
     _check_tensor(t, name, like)
     if t.dtype is not like.dtype:
         raise ValueError(f"{name} is {t.dtype}, not {like.dtype}")
-    if t.shape != like.shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(like.shape)}")
-    if not t.numel():   # (of any strides)
-        return t.data_ptr(), 0, 0
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    s, n = t.stride(), t.shape
+    if n != like.shape:
+        raise ValueError(f"{name} has shape {tuple(n)}, not {tuple(like.shape)}")
+    if s[-1] != 1 and n[-1] > 1 and t.numel():
         raise ValueError(f"the channels of {name} must be contiguous")
-    step = _pixel_step(t)
+    step = s[1] if len(n) == 3 else _pixel_step(s, n)
     if step is None:
-        raise ValueError(f"the pixels of {name} must be evenly strided")
-    return t.data_ptr(), t.stride(0), step
+        if t.numel():
+            raise ValueError(f"the pixels of {name} must be evenly strided")
+        step = n[-1]
+    return t.data_ptr(), s[0], step
 
 
 _NO_PIXELS = (0, 0, 0)
@@ -263,7 +260,7 @@ def group_norm_(out, x, groups, weight=None, bias=None, *, eps=1e-5, activation=
     a = _norm(x, out, groups, weight, bias, eps, activation, stats)
     if temp is None:
         temp = group_norm_temp(x, groups)
-    _call(lib().tdgs_group_norm, x, _stream(x), _NORM.pack(*a, *_temp(temp, x)))
+    _call(lib().tdgs_group_norm, x, (_NORM.pack(*a, *_temp(temp, x)),))
     return out
 
 
@@ -281,7 +278,7 @@ def group_norm_grad_(dx, dweight, dbias, dout, x, stats, groups, weight=None, bi
     g = (*_pixels(dout, "dout", x), *_pixels(dx, "dx", x), dptr(dweight) or 0, dptr(dbias) or 0)
     if temp is None:
         temp = group_norm_temp(x, groups, grad=True)
-    _call(lib().tdgs_group_norm_grad, x, _stream(x), _NORM.pack(*a, *_temp(temp, x)), _NORM_GRADS.pack(*g))
+    _call(lib().tdgs_group_norm_grad, x, (_NORM.pack(*a, *_temp(temp, x)), _NORM_GRADS.pack(*g)))
     return dx, dweight, dbias
 
 
@@ -337,8 +334,9 @@ def embedding_lookup_(out, table, tokens, *, scale=1.0, ctx=None):
     vocab, dim, t, ts = _table(table, "table")
     size, n = _tokens(tokens, table), tokens.numel()
     o, os = _rows(out, "out", n, dim, table)
-    _call(lib().tdgs_embedding_lookup, table, _handle(ctx, table.get_device()), _stream(table), DTYPES[table.dtype], t, ts,
-          vocab, dim, tokens.data_ptr(), size, n, scale, o, os)
+    _call(lib().tdgs_embedding_lookup, table,
+          (DTYPES[table.dtype], t, ts, vocab, dim, tokens.data_ptr(), size, n, scale, o, os),
+          (_handle(ctx, table.get_device()),))
     return out
 
 
@@ -358,8 +356,9 @@ def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None,
     d, ds = _rows(dout, "dout", n, dim, dtable)
     if temp is None:
         temp = embedding_temp(dtable, tokens)
-    _call(lib().tdgs_embedding_grad, dtable, _handle(ctx, dtable.get_device()), _stream(dtable), DTYPES[dtable.dtype], d, ds,
-          tokens.data_ptr(), size, n, -1 if padding is None else padding, scale, t, ts, vocab, dim, *_temp(temp, dtable))
+    _call(lib().tdgs_embedding_grad, dtable,
+          (DTYPES[dtable.dtype], d, ds, tokens.data_ptr(), size, n, -1 if padding is None else padding, scale, t, ts, vocab,
+           dim, *_temp(temp, dtable)), (_handle(ctx, dtable.get_device()),))
     return dtable
 
 
@@ -459,8 +458,9 @@ class _GroupNorm(torch.autograd.Function):
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation="silu"):
     """group_norm_ as a differentiable function of x, weight and bias, all of any strides."""
     x = _rows_contiguous(x)
-    return _GroupNorm.apply(x if _pixel_step(x) is not None else x.contiguous(), _contiguous(weight), _contiguous(bias),
-                            groups, eps, activation)
+    if _pixel_step(x.stride(), x.shape) is None:
+        x = x.contiguous()
+    return _GroupNorm.apply(x, _contiguous(weight), _contiguous(bias), groups, eps, activation)
 
 
 class _Embedding(torch.autograd.Function):
