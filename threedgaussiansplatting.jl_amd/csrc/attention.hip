@@ -15,7 +15,8 @@
 // gradients stored, so that the kernels see a shorter sequence: they do no work for single keys that are not allowed,
 // and such keys, whatever they hold, are not read.
 // P and dS are rounded to the inputs' type for their products (the matrix cores take no wider
-// operand at that rate), in half after a power of two that brings them into its range; maxima, sums, exponentials and every accumulator stay in 32 bits.
+// operand at that rate), in half after a power of two that brings them into its range; maxima, sums,
+// exponentials and every accumulator stay in 32 bits.
 //
 // What bounds the kernels: for 16-bit types the exponential of every score, at a quarter of the vector rate, next to
 // the products; for float the products themselves; for few rows over many keys the memory that
@@ -408,9 +409,9 @@ struct AtForward {
 // relative to m, the largest c s of the first tile. It need not be the largest so far: only when a later tile's
 // p add up to more than at_largest are the scores taken again, m moved to their largest and O and l brought there, so
 // that almost every tile does without finding a maximum (5% of the kernel).
-// bfloat16, heads of 64: 64800 rows x 1024 keys x 8 heads in 162 to 181 us (136 GFLOP: 750 to 840 TFLOP/s; a large
+// bfloat16, heads of 64: 64800 rows x 1024 keys x 8 heads in 162 to 184 us (136 GFLOP: 740 to 840 TFLOP/s; a large
 // product reaches 1150), vector issue busy for 64% of it, the matrix cores for 38%; 32400 x 4096 x 16 in 594 us when
-// the card is cool, 720 when not (910 to 750 TFLOP/s at 2.1 to 1.75 GHz). float: matrix cores busy for half of the time.
+// the card is cool, 760 when not (910 to 710 TFLOP/s at 2.1 to 1.7 GHz). float: matrix cores busy for half of the time.
 // One row of 16 heads over 8 caches of 10000 to 20011 keys: 40 us, 6 TB/s.
 template <class T, int DP, bool VEC, bool IDX, bool TWO>
 __global__ __launch_bounds__((AtForward<T, DP>::kThreads), (AtForward<T, DP>::kPerSimd)) void k_attend(AtArgs a) {
@@ -590,8 +591,8 @@ __device__ __forceinline__ float at_grad_scale(const AtArgs& a, int len) { retur
 
 // dQ and delta. Workgroup: 4 wavefronts of 32 rows each, the keys of one split. 16-bit types up to 64 elements take three
 // per SIMD: 512 threads, two blocks of rows per wavefront, or tiles in two or three buffers were slower. Bound by vector
-// issue (72% busy, the matrix cores 44%): 64800 rows x 1024 keys x 8 heads of 64, bfloat16, in 296 to 320 us (204 GFLOP of
-// the formulas, 272 with the second product of dS: 850 to 920 TFLOP/s).
+// issue (72% busy, the matrix cores 44%): 64800 rows x 1024 keys x 8 heads of 64, bfloat16, in 296 to 329 us (204 GFLOP of
+// the formulas, 272 with the second product of dS: 830 to 920 TFLOP/s).
 template <class T, int DP, bool VEC, bool IDX>
 __global__ __launch_bounds__(kAtThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 2)) void k_attend_dq(AtArgs a) {
     constexpr int KT = at_tile<T>(), P = at_pitch<T, DP>(), NB = DP / 32, NC = DP / 16;
@@ -731,7 +732,7 @@ constexpr int at_dkv_per_simd() { return sizeof(T) == 4 && DP > 96 ? 1 : 2; }
 // dK and dV. Workgroup: TH / 64 wavefronts of 32 keys each, the rows of one split. Wide ones, of 256 keys, stage rows half as
 // often and 64 at a time: 343 -> 311 us for 64800 rows, 1024 keys and 8 heads of bfloat16; with 93 keys half
 // their wavefronts idle (30 -> 37). The matrix cores are busy for 44% of that, LDS for 48%, vector issue for 40%
-// (272 GFLOP: 890 to 980 TFLOP/s); for float the matrix cores for 51%.
+// (272 GFLOP: 860 to 980 TFLOP/s), and wavefronts wait for 36%: no unit bounds it; for float the matrix cores for 51%.
 constexpr int kAtWide = 512;
 template <class T, int DP, int TH, bool VEC, bool TWO>
 __global__ __launch_bounds__(TH, (at_dkv_per_simd<T, DP>())) void k_attend_dkv(AtArgs a) {
