@@ -257,13 +257,13 @@ struct AtOperand {
     }
 };
 
-// Brings dS into the range of its operand. A lane's registers hold dS of one row (dQ) or one key (dK), whose result no other
-// lane but its partner in the other half of the wavefront adds to, so each takes its own power of two out of it. bfloat16 and float
-// hold any dS; half would make infinities of those above 65504, which a scaled loss reaches, and lose bits of those below 6e-5,
-// which a mean over many pixels does. g, by which dS is multiplied, starts above all that half's q, k, v and dout can make
-// (|dP| is at least 2^-48 or 0, and 2^40 at most) and is lowered, with what was added up before, where dS would pass 2^15; the
-// largest dS is then brought to 2^8, so that it may grow 2^7 times before that happens again.
-// Forward and backward of 64800 rows x 1024 keys x 8 heads of 64 take 833 us with it, 804 without.
+// Brings dS into the range of its operand. A lane's registers hold dS of one row (dQ) or one key (dK), whose result no
+// other lane but its partner in the other half of the wavefront adds to, so each takes its own power of two out of it.
+// bfloat16 and float hold any dS; half would make infinities of those above 65504, which a scaled loss reaches, and lose
+// bits of those below 6e-5, which a mean over many pixels gives. g, by which dS is multiplied, starts above all that half's
+// q, k, v and dout can make (|dP| is at least 2^-48 or 0, and 2^40 at most) and is lowered, with what was added up before,
+// where dS would pass 2^15; the largest dS is then brought to 2^8, so that it may grow 2^7 times before that happens
+// again. Forward and backward of 64800 rows x 1024 keys x 8 heads of 64 take 833 us with it, 804 without.
 template <class T>
 struct AtRange {
     static constexpr bool kOn = std::is_same<T, f16>::value;
@@ -386,9 +386,9 @@ __device__ __forceinline__ AtItem at_item(int i, int n, int kv_heads) {
     return {j % kv_heads, j / kv_heads * kXcds + i % kXcds};
 }
 
-// How far below the largest c s of a tile its row's reference m is put, and what a lane's p of a tile may add up to before
-// m is looked for again: 2^10 times that of the largest. In half both are up by 2^5, and p stays below 2^15: weights down to
-// 2^-19 of the largest so keep all of half's bits, which matters where the key that has the largest has no value of its own.
+// How far below the largest c s of a tile its row's reference m is put, and what a lane's p of a tile may add up to
+// before m is looked for again: 2^10 times that of the largest. In half both are up by 2^5, and p stays below 2^15: weights
+// down to 2^-19 of the largest so keep all of half's bits, which matters where the key that has it has no value.
 template <class T>
 constexpr float at_below() { return std::is_same<T, f16>::value ? 5.0f : 0.0f; }
 template <class T>
