@@ -86,7 +86,7 @@ static __global__ __launch_bounds__(kAtListThreads) void k_attend_list(const uin
     const int kb = blockIdx.x, lane = (int)__lane_id(), wave = threadIdx.x / kWave, len = at_length(a, kb);
     const uint8_t* const row = mask + kb * stride;
     int32_t* const list = index + (int64_t)kb * a.kv_len;
-    int done = 0;   // allowed keys before this round's
+    int done = 0;   // allowed keys before these
     for (int r0 = 0; r0 < a.kv_len; r0 += kAtListThreads * PER) {
         // a wavefront takes PER * 64 neighbouring keys
         const int j0 = r0 + wave * (kWave * PER) + lane;
