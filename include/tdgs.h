@@ -662,6 +662,119 @@ int tdgs_embedding_grad(tdgs_ctx* ctx, void* stream, int32_t dtype, const void* 
                         void* dtable, int64_t dtable_stride, int64_t vocab, int32_t dim, void* temp,
                         size_t temp_bytes);
 
+/* A matrix: its rows `stride` elements apart, the elements of a row contiguous. */
+typedef struct tdgs_rows {
+    void* data;
+    int64_t stride;
+} tdgs_rows;
+
+/* How a (in_features, out_features) weight matrix lies in memory: rows of out_features elements, or its
+ * transpose's rows of in_features elements. */
+enum { TDGS_WEIGHT_IN_OUT = 0, TDGS_WEIGHT_OUT_IN = 1 };
+
+/* Linear layer: with z = x W + bias, out = residual + act(z); x is rows x in_features, the others rows x
+ * out_features, act as in tdgs_norm. Sums are held in 32 bits and z, act(z) and the sum with the residual are
+ * rounded once, on their way to pre and out. */
+typedef struct tdgs_linear {
+    int32_t dtype;              /* of every tensor */
+    int32_t activation;
+    int64_t rows;
+    int32_t in_features, out_features;
+    int32_t weight_layout;
+    int32_t reserved;
+    tdgs_rows x, weight, out;   /* out is not read by the gradient */
+    tdgs_rows residual;         /* data null: 0; may be out; not read by the gradient */
+    tdgs_rows pre;              /* z: written by the forward call (where data is not null), read by the gradient
+                                   where the activation is not the identity */
+    const void* bias;           /* out_features; null: 0; not read by the gradient */
+    void* temp;                 /* scratch of tdgs_linear_temp_bytes() bytes */
+    size_t temp_bytes;
+} tdgs_linear;
+
+/* dout as out; dx as x, dweight as the weight (in a layout of its own) and dbias as the bias; data null: not wanted. The
+ * residual's gradient is dout. */
+typedef struct tdgs_linear_grads {
+    tdgs_rows dout, dx, dweight;
+    void* dbias;
+    int32_t dweight_layout;
+    int32_t reserved;
+} tdgs_linear_grads;
+
+/* Scratch of tdgs_linear (grad 0) or of that and tdgs_linear_grad (grad 1). */
+size_t tdgs_linear_temp_bytes(const tdgs_linear* a, int32_t grad);
+int tdgs_linear_forward(void* stream, const tdgs_linear* a);
+/* The gradients of sum(dout * out): with dz = dout act'(z), dx = dz W^T, dweight = x^T dz, dbias the sum of dz's rows. dz
+ * is rounded to the type (the operand of two matrix products) after a power of two that brings its largest
+ * value into float16's range; dbias is summed from what is not rounded. z is rounded to the type in pre, which
+ * leaves act'(z) as exact as that. */
+int tdgs_linear_grad(void* stream, const tdgs_linear* a, const tdgs_linear_grads* g);
+
+enum { TDGS_PAIRS_HALVES = 0, TDGS_PAIRS_INTERLEAVED = 1 };
+enum { TDGS_POSITION_I32 = 0, TDGS_POSITION_I64 = 1, TDGS_POSITION_F32 = 2 };
+
+/* Norm of each head of queries and keys, and its rotation by position, in one pass:
+ * y_i = x_i weight_i / sqrt(mean x^2 + eps) over the head's elements (norm 0: y = x), then with t = position * frequency the
+ * pair (y_a, y_b) becomes (y_a cos t - y_b sin t, y_a sin t + y_b cos t). Pair p < pairs is elements (p, p + pairs)
+ * (TDGS_PAIRS_HALVES) or (2 p, 2 p + 1) (TDGS_PAIRS_INTERLEAVED); elements from 2 pairs on are not rotated. Its axis is
+ * the one in whose section of sections[0], sections[1], .. neighbouring pairs it lies. Angles are made in 64 bits. Queries
+ * and keys are of the same positions; a call may be for one of them (heads or kv_heads 0). */
+typedef struct tdgs_head_norm {
+    int32_t dtype;              /* of q, k, their results and gradients */
+    int32_t param_dtype;        /* of the weights and their gradients: TDGS_F32 or dtype */
+    int32_t batch, length;
+    int32_t heads, kv_heads;
+    int32_t head_dim;           /* 1 to 256 */
+    int32_t norm;               /* 0: rotation only */
+    float eps;
+    int32_t pairs;              /* rotated pairs; 0: norm only */
+    int32_t pair_layout;
+    int32_t axes;               /* 1 to 4 where pairs is not 0 */
+    int32_t sections[4];        /* pairs of each axis, positive; their sum is `pairs` */
+    int32_t inverse;            /* rotate the other way (the gradient of a rotation) */
+    int32_t position_type;
+    const double* turns;        /* pairs entries: frequency / (2 pi), turns for a step of one */
+    const void* positions;      /* element position_batch_stride b + axes l + axis */
+    int64_t position_batch_stride;   /* 0: the same for every batch */
+    tdgs_heads q, k, q_out, k_out;   /* q_out may be q and k_out k; the gradient does not read them */
+    const void* q_weight;       /* head_dim; null: 1 */
+    const void* k_weight;
+    void* temp;                 /* scratch of the gradient, tdgs_head_norm_temp_bytes() bytes */
+    size_t temp_bytes;
+} tdgs_head_norm;
+
+/* The results' gradients; dq and dk (dq may be dq_out, dk dk_out), and those of the weights, of their type (null: not
+ * wanted). */
+typedef struct tdgs_head_norm_grads {
+    tdgs_heads dq_out, dk_out, dq, dk;
+    void* dq_weight;
+    void* dk_weight;
+} tdgs_head_norm_grads;
+
+int tdgs_head_norm_forward(void* stream, const tdgs_head_norm* a);
+size_t tdgs_head_norm_temp_bytes(const tdgs_head_norm* a);
+/* The gradients of sum(dq_out * q_out) + sum(dk_out * k_out) with norm (without it, the gradient of a rotation is the
+ * forward call with `inverse`). */
+int tdgs_head_norm_grad(void* stream, const tdgs_head_norm* a, const tdgs_head_norm_grads* g);
+
+/* Dropout: out = residual + (kept ? x / (1 - p) : 0) for rows x cols elements. Element i = row * cols + col is kept where
+ * word i % 4 of Philox4x32-10 (Salmon, Moraes, Dror & Shaw 2011) of key `seed` and counter
+ * (low and high word of i / 4, low and high word of call) is at least floor(p 2^32), p in [0, 1]; what x holds where it is
+ * dropped does not matter. call_dev, where not null, is one int64 on the device that is read instead of `call` (a
+ * captured call so takes another mask at each replay). The gradient for x is the same call on dout without a
+ * residual: the mask is made again and never stored. out may be x or residual. */
+typedef struct tdgs_dropout {
+    int32_t dtype;
+    int32_t reserved;
+    int64_t rows, cols;
+    double p;
+    uint64_t seed, call;
+    const uint64_t* call_dev;
+    tdgs_rows x, out;
+    tdgs_rows residual;         /* data null: 0 */
+} tdgs_dropout;
+
+int tdgs_dropout_apply(void* stream, const tdgs_dropout* a);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,13 @@ TDGS_ACT_IDENTITY = 0
 TDGS_ACT_SILU = 1
 TDGS_ACT_GELU = 2
 TDGS_ACT_RELU = 3
+TDGS_WEIGHT_IN_OUT = 0
+TDGS_WEIGHT_OUT_IN = 1
+TDGS_PAIRS_HALVES = 0
+TDGS_PAIRS_INTERLEAVED = 1
+TDGS_POSITION_I32 = 0
+TDGS_POSITION_I64 = 1
+TDGS_POSITION_F32 = 2
 
 fp = C.POINTER(C.c_float)
 i32p = C.POINTER(C.c_int32)
@@ -132,6 +139,43 @@ class NormC(C.Structure):
 
 class NormGradsC(C.Structure):
     _fields_ = [("dout", PixelsC), ("dx", PixelsC), ("dweight", C.c_void_p), ("dbias", C.c_void_p)]
+
+
+class RowsC(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64)]
+
+
+class LinearC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("rows", C.c_int64), ("in_features", C.c_int32),
+                ("out_features", C.c_int32), ("weight_layout", C.c_int32), ("reserved", C.c_int32), ("x", RowsC),
+                ("weight", RowsC), ("out", RowsC), ("residual", RowsC), ("pre", RowsC), ("bias", C.c_void_p),
+                ("temp", C.c_void_p), ("temp_bytes", C.c_size_t)]
+
+
+class LinearGradsC(C.Structure):
+    _fields_ = [("dout", RowsC), ("dx", RowsC), ("dweight", RowsC), ("dbias", C.c_void_p),
+                ("dweight_layout", C.c_int32), ("reserved", C.c_int32)]
+
+
+class HeadNormC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("param_dtype", C.c_int32), ("batch", C.c_int32), ("length", C.c_int32),
+                ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("norm", C.c_int32),
+                ("eps", C.c_float), ("pairs", C.c_int32), ("pair_layout", C.c_int32), ("axes", C.c_int32),
+                ("sections", C.c_int32 * 4), ("inverse", C.c_int32), ("position_type", C.c_int32),
+                ("turns", C.c_void_p), ("positions", C.c_void_p), ("position_batch_stride", C.c_int64),
+                ("q", HeadsC), ("k", HeadsC), ("q_out", HeadsC), ("k_out", HeadsC), ("q_weight", C.c_void_p),
+                ("k_weight", C.c_void_p), ("temp", C.c_void_p), ("temp_bytes", C.c_size_t)]
+
+
+class HeadNormGradsC(C.Structure):
+    _fields_ = [("dq_out", HeadsC), ("dk_out", HeadsC), ("dq", HeadsC), ("dk", HeadsC), ("dq_weight", C.c_void_p),
+                ("dk_weight", C.c_void_p)]
+
+
+class DropoutC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("reserved", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("p", C.c_double), ("seed", C.c_uint64), ("call", C.c_uint64), ("call_dev", C.c_void_p), ("x", RowsC),
+                ("out", RowsC), ("residual", RowsC)]
 
 
 def sh_coeffs_per_channel(degree: int) -> int:

@@ -16,7 +16,7 @@ INCLUDE = os.path.join(HERE, "..", "include")
 LIB = os.path.join(HERE, "libtdgs.so")
 OBJDIR = os.path.join(HERE, "_build")
 SOURCES = ["context.hip", "forward.hip", "backward.hip", "train.hip", "loss.hip", "image.hip",
-           "attention.hip", "norm.hip", "embedding.hip"]
+           "attention.hip", "norm.hip", "embedding.hip", "linear.hip", "heads.hip", "dropout.hip"]
 ARCH = os.environ.get("TDGS_OFFLOAD_ARCH", "gfx950")
 
 

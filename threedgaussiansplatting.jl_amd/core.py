@@ -48,7 +48,7 @@ def lib():
         L.tdgs_last_error.restype = C.c_char_p
         for name in ("tdgs_scan_temp_bytes", "tdgs_sort_pairs_temp_bytes", "tdgs_render_temp_bytes",
                      "tdgs_loss_temp_bytes", "tdgs_cross_attention_temp_bytes", "tdgs_group_norm_temp_bytes",
-                     "tdgs_embedding_grad_temp_bytes"):
+                     "tdgs_embedding_grad_temp_bytes", "tdgs_linear_temp_bytes", "tdgs_head_norm_temp_bytes"):
             getattr(L, name).restype = C.c_size_t
         L.tdgs_loss_temp_bytes.argtypes = [C.c_int32, C.c_int32]
         L.tdgs_scan_temp_bytes.argtypes = [C.c_int64]
@@ -77,6 +77,13 @@ def lib():
         L.tdgs_embedding_grad.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
                                           C.c_int32, C.c_int64, C.c_int64, C.c_float, C.c_void_p, C.c_int64,
                                           C.c_int64, C.c_int32, C.c_void_p, C.c_size_t]
+        L.tdgs_linear_temp_bytes.argtypes = [C.c_void_p, C.c_int32]
+        L.tdgs_linear_forward.argtypes = [C.c_void_p, C.c_void_p]
+        L.tdgs_linear_grad.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.tdgs_head_norm_temp_bytes.argtypes = [C.c_void_p]
+        L.tdgs_head_norm_forward.argtypes = [C.c_void_p, C.c_void_p]
+        L.tdgs_head_norm_grad.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.tdgs_dropout_apply.argtypes = [C.c_void_p, C.c_void_p]
         _LIB = L
     return _LIB
 

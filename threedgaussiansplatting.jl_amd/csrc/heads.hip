@@ -1,0 +1,565 @@
+// heads.hip — norms of queries and keys for each head with their rotation by position on several axes in the
+// same pass, and its gradient.
+//
+// A head's row of d elements is split into units of V pairs, one per lane: V elements of each half (pairs p,
+// p + pairs), or 2 V neighbours (pairs 2 p, 2 p + 1, and what is not rotated), so that both elements of a pair
+// are in one lane and the norm's sum takes a few exchanges among the row's G lanes. A workgroup takes a
+// few tokens at a time: it makes their cosines and sines once, in LDS, and uses them for all heads of queries and keys.
+//
+// The angle of a far position has few bits left in 32: position * frequency / (2 pi) is taken in 64 bits, as turns,
+// whose whole part is dropped; the rest is exact to 2^-26 in 32 bits, from which sinpi and cospi go on.
+//
+// With r = 1 / sqrt(mean x^2 + eps), xhat = r x, u the output's gradient rotated back and e = u w:
+// dw = sum u xhat, dx = r (e - xhat mean(e xhat)); r is computed again from x, which is read anyway. All of it is
+// bound by memory: each row is read once and written once.
+#include "internal.hpp"
+#include "elem.hpp"
+
+namespace tdgs {
+
+constexpr int kHnThreads = 256;
+constexpr int kHnAngles = 4096;     // of a workgroup's tokens, in LDS: 32 KB
+constexpr int kHnBlocks = 1024;     // workgroups of the gradient, which leave one partial sum of dw each
+constexpr int kHnMaxDim = 256;
+
+struct HnTensor {
+    const void *x, *dout;
+    void* out;                       // y, or dx
+    int64_t xb, xl, xh, db, dl, dh, ob, ol, oh;
+    const void* weight;
+};
+
+struct HnArgs {
+    HnTensor t[2];                   // queries, keys
+    const double* turns;
+    const void* positions;
+    int64_t position_batch, tokens;  // tokens: batch * length
+    float* part;
+    int32_t length, heads, all_heads, d, pairs, axes;
+    int32_t ends[4];                 // pairs of the axes up to and with this one
+    int32_t position_type, per;      // per: tokens at a time
+    int32_t lanes, units, rotated_units;   // lanes of a row (a power of two), of which units hold something
+    int32_t row_shift;               // log2(lanes)
+    float eps, inv_d, sign;
+    bool norm, interleaved, param_f32;
+    FastDiv by_heads, by_length;
+};
+
+__device__ __forceinline__ double hn_position(const HnArgs& a, int64_t i) {
+    switch (a.position_type) {
+        case TDGS_POSITION_I32: return (double)((const int32_t*)a.positions)[i];
+        case TDGS_POSITION_I64: return (double)((const int64_t*)a.positions)[i];
+        default: return (double)((const float*)a.positions)[i];
+    }
+}
+
+// Cosine and sine of the pairs of `count` tokens from `first` on.
+__device__ __forceinline__ void hn_angles(const HnArgs& a, int64_t first, int count, float2* s) {
+    for (int i = threadIdx.x; i < count * a.pairs; i += kHnThreads) {
+        const int token = i / a.pairs, p = i - token * a.pairs;
+        const uint32_t row = (uint32_t)(first + token), b = a.by_length.div(row), l = row - b * a.by_length.d;
+        int axis = 0;
+        while (p >= a.ends[axis]) ++axis;
+        const double t = hn_position(a, b * a.position_batch + (int64_t)l * a.axes + axis) * a.turns[p];
+        const float half = 2.0f * (float)(t - rint(t));
+        s[i] = make_float2(cospif(half), a.sign * sinpif(half));
+    }
+}
+
+// The two sets of V elements of unit j of a row: where they start, how far elements of a set are apart and whether they
+// are rotated.
+template <int V>
+struct HnUnit {
+    int first, second, step, pair;
+    bool on, rotated;
+    __device__ __forceinline__ HnUnit(const HnArgs& a, int j) {
+        on = j < a.units;
+        rotated = j < a.rotated_units;
+        pair = j * V;
+        if (rotated && !a.interleaved) {
+            first = j * V;
+            second = a.pairs + j * V;
+            step = 1;
+        } else {
+            first = rotated ? 2 * j * V : 2 * a.pairs + 2 * (j - a.rotated_units) * V;
+            second = first + 1;
+            step = 2;
+        }
+    }
+};
+
+// A unit's 2 V elements at p, as V first and V second ones of its pairs.
+template <class T, int V>
+__device__ __forceinline__ void hn_load(const T* __restrict__ p, const HnUnit<V>& u, int d, float (&a)[V], float (&b)[V]) {
+    if constexpr (V == 1) {
+        a[0] = u.on ? (float)p[u.first] : 0.0f;
+        b[0] = u.on && u.second < d ? (float)p[u.second] : 0.0f;
+    } else {
+        typedef T W __attribute__((ext_vector_type(V)));
+        typedef T Wa __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+        W x, y;
+        const int at = u.on ? u.first : 0;
+        x = *reinterpret_cast<const Wa*>(p + at);
+        y = *reinterpret_cast<const Wa*>(p + (u.step == 1 ? u.second : at + V));
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            // neighbours: element 2 i and 2 i + 1 of the 2 V
+            const T even = 2 * i < V ? x[2 * i % V] : y[2 * i % V], odd = 2 * i < V ? x[(2 * i + 1) % V] : y[(2 * i + 1) % V];
+            a[i] = u.on ? (float)(u.step == 1 ? x[i] : even) : 0.0f;
+            b[i] = u.on ? (float)(u.step == 1 ? y[i] : odd) : 0.0f;
+        }
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void hn_store(T* __restrict__ p, const HnUnit<V>& u, int d, const float (&a)[V], const float (&b)[V]) {
+    if (!u.on) return;
+    if constexpr (V == 1) {
+        p[u.first] = (T)a[0];
+        if (u.second < d) p[u.second] = (T)b[0];
+    } else {
+        typedef T W __attribute__((ext_vector_type(V)));
+        typedef T Wa __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+        W x, y;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float lo = i % 2 ? b[i / 2] : a[i / 2], hi = i % 2 ? b[(V + i) / 2] : a[(V + i) / 2];
+            x[i] = (T)(u.step == 1 ? a[i] : lo);
+            y[i] = (T)(u.step == 1 ? b[i] : hi);
+        }
+        *reinterpret_cast<Wa*>(p + u.first) = x;
+        *reinterpret_cast<Wa*>(p + (u.step == 1 ? u.second : u.first + V)) = y;
+    }
+}
+
+template <class T, int V>
+__device__ __forceinline__ void hn_weights(const HnArgs& a, const void* w, const HnUnit<V>& u, float (&x)[V], float (&y)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        x[i] = y[i] = 1.0f;
+        if (!w || !u.on) continue;
+        const int f = u.first + i * u.step, s = u.second + i * u.step;
+        x[i] = a.param_f32 ? ((const float*)w)[f] : (float)((const T*)w)[f];
+        if (s < a.d) y[i] = a.param_f32 ? ((const float*)w)[s] : (float)((const T*)w)[s];
+    }
+}
+
+__device__ __forceinline__ float hn_row_sum(float x, int lanes) {
+    for (int w = lanes >> 1; w > 0; w >>= 1) x += __shfl_xor(x, w, kWave);
+    return x;
+}
+
+// (a, b) turned by the angles of s; by the opposite ones with BACK.
+template <int V, bool BACK>
+__device__ __forceinline__ void hn_turn(const float2* s, float (&a)[V], float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float2 cs = s[i];
+        const float sn = BACK ? -cs.y : cs.y, x = a[i], y = b[i];
+        a[i] = __builtin_fmaf(x, cs.x, -(y * sn));
+        b[i] = __builtin_fmaf(x, sn, y * cs.x);
+    }
+}
+
+// A row of the workgroup's tokens: its token, head and tensor.
+struct HnRow {
+    int token, head, k;
+    int64_t b, l;
+    __device__ __forceinline__ HnRow(const HnArgs& a, int64_t first, int r) {
+        token = (int)a.by_heads.div((uint32_t)r);
+        head = r - token * a.all_heads;
+        k = head >= a.heads;
+        if (k) head -= a.heads;
+        const uint32_t row = (uint32_t)(first + token);
+        b = a.by_length.div(row);
+        l = row - b * a.by_length.d;
+    }
+};
+
+// N units per lane (two where a head of more than 128 elements goes by single pairs).
+template <class T, int V, int N>
+__global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
+    extern __shared__ float2 s_angles[];
+    const int lane = (int)threadIdx.x & (a.lanes - 1), sub = (int)threadIdx.x >> a.row_shift, rows_at = kHnThreads >> a.row_shift;
+    for (int64_t first = (int64_t)blockIdx.x * a.per; first < a.tokens; first += (int64_t)gridDim.x * a.per) {
+        const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per), rows = count * a.all_heads;
+        if (a.pairs) {
+            __syncthreads();   // (the tokens before)
+            hn_angles(a, first, count, s_angles);
+            __syncthreads();
+        }
+        // every lane of a row's stays for its sum
+        for (int r0 = 0; r0 < rows; r0 += rows_at) {
+            const bool valid = r0 + sub < rows;
+            const HnRow row(a, first, valid ? r0 + sub : rows - 1);
+            const HnTensor& t = a.t[row.k];
+            const T* const x = (const T*)t.x + row.b * t.xb + row.l * t.xl + row.head * t.xh;
+            float ya[N][V], yb[N][V], sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) hn_load<T, V>(x, HnUnit<V>(a, lane + n * a.lanes), a.d, ya[n], yb[n]);
+            if (a.norm) {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum = __builtin_fmaf(ya[n][i], ya[n][i], __builtin_fmaf(yb[n][i], yb[n][i], sum));
+                sum = rsqrtf(__builtin_fmaf(hn_row_sum(sum, a.lanes), a.inv_d, a.eps));
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const HnUnit<V> u(a, lane + n * a.lanes);
+                if (a.norm) {
+                    float wa[V], wb[V];
+                    hn_weights<T, V>(a, t.weight, u, wa, wb);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        ya[n][i] *= sum * wa[i];
+                        yb[n][i] *= sum * wb[i];
+                    }
+                }
+                if (u.on && u.rotated) hn_turn<V, false>(s_angles + row.token * a.pairs + u.pair, ya[n], yb[n]);
+                if (valid) hn_store<T, V>((T*)t.out + row.b * t.ob + row.l * t.ol + row.head * t.oh, u, a.d, ya[n], yb[n]);
+            }
+        }
+    }
+}
+
+// dx, and this workgroup's sums for dw: part[block][queries, keys][d].
+template <class T, int V, int N>
+__global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
+    extern __shared__ float2 s_angles[];
+    __shared__ float s_sums[kHnThreads / kWave][kHnMaxDim];
+    const int lane = (int)threadIdx.x & (a.lanes - 1), sub = (int)threadIdx.x >> a.row_shift, rows_at = kHnThreads >> a.row_shift;
+    float da[2][N][V], db[2][N][V];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < V; ++i) da[k][n][i] = db[k][n][i] = 0.0f;
+    for (int64_t first = (int64_t)blockIdx.x * a.per; first < a.tokens; first += (int64_t)gridDim.x * a.per) {
+        const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per), rows = count * a.all_heads;
+        if (a.pairs) {
+            __syncthreads();
+            hn_angles(a, first, count, s_angles);
+            __syncthreads();
+        }
+        for (int r0 = 0; r0 < rows; r0 += rows_at) {
+            const bool valid = r0 + sub < rows;
+            const HnRow row(a, first, valid ? r0 + sub : rows - 1);
+            const HnTensor& t = a.t[row.k];
+            const T* const x = (const T*)t.x + row.b * t.xb + row.l * t.xl + row.head * t.xh;
+            const T* const dout = (const T*)t.dout + row.b * t.db + row.l * t.dl + row.head * t.dh;
+            float xa[N][V], xb[N][V], ea[N][V], eb[N][V], sum = 0.0f, mean = 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const HnUnit<V> u(a, lane + n * a.lanes);
+                hn_load<T, V>(x, u, a.d, xa[n], xb[n]);
+                hn_load<T, V>(dout, u, a.d, ea[n], eb[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum = __builtin_fmaf(xa[n][i], xa[n][i], __builtin_fmaf(xb[n][i], xb[n][i], sum));
+            const float r = rsqrtf(__builtin_fmaf(hn_row_sum(sum, a.lanes), a.inv_d, a.eps));
+            const float mine = valid ? 1.0f : 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const HnUnit<V> u(a, lane + n * a.lanes);
+                if (u.on && u.rotated) hn_turn<V, true>(s_angles + row.token * a.pairs + u.pair, ea[n], eb[n]);
+                float wa[V], wb[V];
+                hn_weights<T, V>(a, t.weight, u, wa, wb);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    xa[n][i] *= r;
+                    xb[n][i] *= r;
+                    const float pa = ea[n][i] * xa[n][i], pb = eb[n][i] * xb[n][i];
+                    if (valid) {
+                        da[0][n][i] += row.k ? 0.0f : pa;
+                        db[0][n][i] += row.k ? 0.0f : pb;
+                        da[1][n][i] += row.k ? pa : 0.0f;
+                        db[1][n][i] += row.k ? pb : 0.0f;
+                    }
+                    mean = __builtin_fmaf(pa, wa[i], __builtin_fmaf(pb, wb[i], mean));
+                    ea[n][i] *= wa[i];
+                    eb[n][i] *= wb[i];
+                }
+            }
+            mean = hn_row_sum(mean, a.lanes) * a.inv_d;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    xa[n][i] = r * __builtin_fmaf(-mean, xa[n][i], ea[n][i]);
+                    xb[n][i] = r * __builtin_fmaf(-mean, xb[n][i], eb[n][i]);
+                }
+                if (valid)
+                    hn_store<T, V>((T*)t.out + row.b * t.ob + row.l * t.ol + row.head * t.oh,
+                                   HnUnit<V>(a, lane + n * a.lanes), a.d, xa[n], xb[n]);
+            }
+        }
+    }
+    if (!a.part) return;
+    // over the wavefront's rows, then over its wavefronts
+    const int wave = (int)threadIdx.x / kWave;
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const HnUnit<V> u(a, lane + n * a.lanes);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float x = k ? da[1][n][i] : da[0][n][i], y = k ? db[1][n][i] : db[0][n][i];
+                for (int w = kWave / 2; w >= a.lanes; w >>= 1) {
+                    x += __shfl_xor(x, w, kWave);
+                    y += __shfl_xor(y, w, kWave);
+                }
+                if ((int)__lane_id() < a.lanes && u.on) {
+                    s_sums[wave][u.first + i * u.step] = x;
+                    if (u.second + i * u.step < a.d) s_sums[wave][u.second + i * u.step] = y;
+                }
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.d; c += kHnThreads) {
+            float x = 0.0f;
+            for (int w = 0; w < kHnThreads / kWave; ++w) x += s_sums[w][c];
+            a.part[((int64_t)blockIdx.x * 2 + k) * a.d + c] = x;
+        }
+        __syncthreads();
+    }
+}
+
+// Column c of part's 2 d, its blocks shared out over 32 lanes.
+constexpr int kHnJoinCols = 8;
+template <class T>
+__global__ __launch_bounds__(kHnThreads) void k_head_norm_join(const float* __restrict__ part, int blocks, int d, void* dq, void* dk,
+                                                               bool f32) {
+    __shared__ float s[kHnThreads / kHnJoinCols][kHnJoinCols + 1];
+    const int c = blockIdx.x * kHnJoinCols + (int)threadIdx.x % kHnJoinCols, y = (int)threadIdx.x / kHnJoinCols;
+    float x = 0.0f;
+    if (c < 2 * d)
+        for (int b = y; b < blocks; b += kHnThreads / kHnJoinCols) x += part[(int64_t)b * 2 * d + c];
+    s[y][threadIdx.x % kHnJoinCols] = x;
+    __syncthreads();
+    if (y != 0 || c >= 2 * d) return;
+    for (int i = 1; i < kHnThreads / kHnJoinCols; ++i) x += s[i][threadIdx.x];
+    void* const p = c < d ? dq : dk;
+    if (!p) return;
+    const int e = c < d ? c : c - d;
+    if (f32) ((float*)p)[e] = x;
+    else ((T*)p)[e] = (T)x;
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+static int hn_check(const tdgs_head_norm* a) {
+    TDGS_REQUIRE(a != nullptr, "head norm: null arguments");
+    TDGS_REQUIRE(known_dtype(a->dtype), "head norm: unknown element type %d", a->dtype);
+    TDGS_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == TDGS_F32,
+                 "head norm: weights must be float32 or of the input's type");
+    TDGS_REQUIRE(a->batch >= 0 && a->length >= 0 && a->heads >= 0 && a->kv_heads >= 0, "head norm: negative size");
+    TDGS_REQUIRE(a->heads <= 65536 && a->kv_heads <= 65536, "head norm: %d and %d heads", a->heads, a->kv_heads);
+    TDGS_REQUIRE((int64_t)a->batch * a->length <= INT32_MAX - 65536, "head norm: too many tokens");
+    TDGS_REQUIRE(a->head_dim >= 1 && a->head_dim <= kHnMaxDim, "head norm: head dimension %d is not in 1 to %d", a->head_dim,
+                 kHnMaxDim);
+    TDGS_REQUIRE(a->eps >= 0.0f && a->eps < INFINITY, "head norm: eps must be finite and not negative");
+    TDGS_REQUIRE(a->pairs >= 0 && 2 * (int64_t)a->pairs <= a->head_dim, "head norm: %d rotated pairs in a head of %d", a->pairs,
+                 a->head_dim);
+    if (a->pairs > 0) {
+        TDGS_REQUIRE(a->axes >= 1 && a->axes <= 4, "head norm: %d axes", a->axes);
+        int64_t sum = 0;
+        for (int i = 0; i < a->axes; ++i) {
+            TDGS_REQUIRE(a->sections[i] > 0, "head norm: axis %d has %d pairs", i, a->sections[i]);
+            sum += a->sections[i];
+        }
+        TDGS_REQUIRE(sum == a->pairs, "head norm: the axes have %lld pairs, not %d", (long long)sum, a->pairs);
+        TDGS_REQUIRE(a->pair_layout == TDGS_PAIRS_HALVES || a->pair_layout == TDGS_PAIRS_INTERLEAVED,
+                     "head norm: unknown layout of pairs %d", a->pair_layout);
+        TDGS_REQUIRE(a->position_type >= TDGS_POSITION_I32 && a->position_type <= TDGS_POSITION_F32,
+                     "head norm: unknown type of positions %d", a->position_type);
+        TDGS_REQUIRE(a->turns && aligned_to(a->turns, 8), "head norm: the frequencies are null or not aligned");
+        TDGS_REQUIRE(a->positions && aligned_to(a->positions, a->position_type == TDGS_POSITION_I64 ? 8 : 4),
+                     "head norm: the positions are null or not aligned");
+        TDGS_REQUIRE(a->position_batch_stride >= 0, "head norm: positions have a negative stride");
+    }
+    return TDGS_OK;
+}
+
+static int hn_check_view(const tdgs_heads* v, const char* name, const tdgs_head_norm* a, int heads, bool written) {
+    TDGS_REQUIRE(v->data != nullptr, "head norm: %s is null", name);
+    TDGS_REQUIRE(aligned_to(v->data, (size_t)dtype_size(a->dtype)), "head norm: %s is not aligned to its element type", name);
+    TDGS_REQUIRE(v->stride_b >= 0 && v->stride_l >= 0 && v->stride_h >= 0, "head norm: %s has a negative stride", name);
+    if (written)
+        TDGS_REQUIRE((a->batch <= 1 || v->stride_b >= a->head_dim) && (a->length <= 1 || v->stride_l >= a->head_dim) &&
+                         (heads <= 1 || v->stride_h >= a->head_dim),
+                     "head norm: rows of %s overlap", name);
+    return TDGS_OK;
+}
+
+struct HnPlan {
+    int v, blocks;
+    size_t lds;
+};
+
+// Elements a lane takes of each half: eight of a 16-bit type (16 bytes) or four, where the pairs and what is not rotated
+// divide into them, or single ones.
+static HnPlan hn_plan(const tdgs_head_norm* a, HnArgs* r, bool grad) {
+    HnPlan p;
+    const int rest = a->head_dim - 2 * a->pairs;
+    auto fits = [&](int v) { return a->pairs % v == 0 && rest % (2 * v) == 0; };
+    p.v = a->dtype != TDGS_F32 && fits(8) ? 8 : fits(4) ? 4 : 1;
+    r->rotated_units = a->pairs / p.v;
+    r->units = r->rotated_units + (rest + 2 * p.v - 1) / (2 * p.v);
+    r->lanes = 1;
+    r->row_shift = 0;
+    while (r->lanes < r->units && r->lanes < kWave) {
+        r->lanes *= 2;
+        ++r->row_shift;
+    }
+    // tokens at a time: rows for every thread's lanes four times over, fewer where that would leave
+    // compute units idle, and what LDS holds
+    const int64_t tokens = (int64_t)a->batch * a->length, heads = (int64_t)a->heads + a->kv_heads;
+    int64_t per = 4 * (kHnThreads / r->lanes) / (heads > 0 ? heads : 1);
+    if (per > tokens / kHnBlocks) per = tokens / kHnBlocks;
+    if (a->pairs && per > kHnAngles / a->pairs) per = kHnAngles / a->pairs;
+    if (per < 1) per = 1;
+    r->per = (int32_t)per;
+    const int64_t blocks = ceil_div(tokens, per);
+    p.blocks = (int)(grad && blocks > kHnBlocks ? kHnBlocks : blocks);
+    p.lds = (size_t)(per * a->pairs * (int64_t)sizeof(float2));
+    return p;
+}
+
+static HnArgs hn_args(const tdgs_head_norm* a) {
+    HnArgs r = {};
+    const tdgs_heads* const x[2] = {&a->q, &a->k};
+    for (int i = 0; i < 2; ++i) {
+        r.t[i].x = x[i]->data;
+        r.t[i].xb = x[i]->stride_b;
+        r.t[i].xl = x[i]->stride_l;
+        r.t[i].xh = x[i]->stride_h;
+        r.t[i].weight = i ? a->k_weight : a->q_weight;
+    }
+    r.turns = a->turns;
+    r.positions = a->positions;
+    r.position_batch = a->position_batch_stride;
+    r.tokens = (int64_t)a->batch * a->length;
+    r.length = a->length;
+    r.heads = a->heads;
+    r.all_heads = a->heads + a->kv_heads;
+    r.d = a->head_dim;
+    r.pairs = a->pairs;
+    r.axes = a->axes;
+    for (int i = 0, sum = 0; i < 4; ++i) {
+        if (i < a->axes && a->pairs) sum += a->sections[i];
+        r.ends[i] = sum;
+    }
+    r.position_type = a->position_type;
+    r.eps = a->eps;
+    r.inv_d = 1.0f / (float)a->head_dim;
+    r.sign = a->inverse ? -1.0f : 1.0f;
+    r.norm = a->norm != 0;
+    r.interleaved = a->pair_layout == TDGS_PAIRS_INTERLEAVED;
+    r.param_f32 = a->param_dtype == TDGS_F32;
+    r.by_heads = FastDiv((uint32_t)(r.all_heads > 0 ? r.all_heads : 1));
+    r.by_length = FastDiv((uint32_t)(a->length > 0 ? a->length : 1));
+    return r;
+}
+
+static void hn_out(HnTensor* t, const tdgs_heads& v) {
+    t->out = v.data;
+    t->ob = v.stride_b;
+    t->ol = v.stride_l;
+    t->oh = v.stride_h;
+}
+
+// f(T{}, elements of a half per lane, units per lane)
+template <class F>
+static int hn_dispatch(const tdgs_head_norm* a, const HnPlan& p, F&& f) {
+    return with_dtype(a->dtype, [&](auto t) -> int {
+        using One = std::integral_constant<int, 1>;
+        if (p.v == 1) return a->head_dim > 128 ? f(t, One{}, std::integral_constant<int, 2>{}) : f(t, One{}, One{});
+        if constexpr (sizeof(t) == 2)
+            if (p.v == 8) return f(t, std::integral_constant<int, 8>{}, One{});
+        return f(t, std::integral_constant<int, 4>{}, One{});
+    });
+}
+
+}  // namespace tdgs
+
+using namespace tdgs;
+
+extern "C" {
+
+int tdgs_head_norm_forward(void* stream_, const tdgs_head_norm* a) {
+    TDGS_TRY(hn_check(a));
+    if (a->batch == 0 || a->length == 0 || a->heads + a->kv_heads == 0) return TDGS_OK;
+    HnArgs r = hn_args(a);
+    if (a->heads > 0) {
+        TDGS_TRY(hn_check_view(&a->q, "q", a, a->heads, false));
+        TDGS_TRY(hn_check_view(&a->q_out, "q_out", a, a->heads, true));
+        hn_out(&r.t[0], a->q_out);
+    }
+    if (a->kv_heads > 0) {
+        TDGS_TRY(hn_check_view(&a->k, "k", a, a->kv_heads, false));
+        TDGS_TRY(hn_check_view(&a->k_out, "k_out", a, a->kv_heads, true));
+        hn_out(&r.t[1], a->k_out);
+    }
+    const HnPlan p = hn_plan(a, &r, false);
+    hipStream_t stream = (hipStream_t)stream_;
+    return hn_dispatch(a, p, [&](auto t, auto v, auto n) -> int {
+        k_head_norm<decltype(t), decltype(v)::value, decltype(n)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
+        TDGS_LAUNCHED();
+        return TDGS_OK;
+    });
+}
+
+size_t tdgs_head_norm_temp_bytes(const tdgs_head_norm* a) {
+    if (hn_check(a) != TDGS_OK) return 0;
+    const int64_t tokens = (int64_t)a->batch * a->length;   // (however the call's positions cut them)
+    return align_up((size_t)(tokens < kHnBlocks ? tokens : kHnBlocks) * 2 * a->head_dim * sizeof(float));
+}
+
+int tdgs_head_norm_grad(void* stream_, const tdgs_head_norm* a, const tdgs_head_norm_grads* g) {
+    TDGS_TRY(hn_check(a));
+    TDGS_REQUIRE(g != nullptr, "head norm: null gradients");
+    TDGS_REQUIRE(a->norm, "head norm: the gradient of a rotation alone is the inverse rotation");
+    HnArgs r = hn_args(a);
+    const bool empty = a->batch == 0 || a->length == 0 || a->heads + a->kv_heads == 0;
+    auto view = [&](int i, const tdgs_heads& x, const tdgs_heads& d, const tdgs_heads& dx, int heads, const char* const* names) -> int {
+        TDGS_TRY(hn_check_view(&x, names[0], a, heads, false));
+        TDGS_TRY(hn_check_view(&d, names[1], a, heads, false));
+        TDGS_TRY(hn_check_view(&dx, names[2], a, heads, true));
+        r.t[i].dout = d.data;
+        r.t[i].db = d.stride_b;
+        r.t[i].dl = d.stride_l;
+        r.t[i].dh = d.stride_h;
+        hn_out(&r.t[i], dx);
+        return TDGS_OK;
+    };
+    static const char* const kNames[2][3] = {{"q", "dq_out", "dq"}, {"k", "dk_out", "dk"}};
+    if (!empty && a->heads > 0) TDGS_TRY(view(0, a->q, g->dq_out, g->dq, a->heads, kNames[0]));
+    if (!empty && a->kv_heads > 0) TDGS_TRY(view(1, a->k, g->dk_out, g->dk, a->kv_heads, kNames[1]));
+    HnPlan p = hn_plan(a, &r, true);
+    const bool weights = g->dq_weight || g->dk_weight;
+    const size_t bytes = (size_t)p.blocks * 2 * a->head_dim * sizeof(float);
+    TDGS_REQUIRE(!weights || empty || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
+                 "head norm: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0, bytes);
+    hipStream_t stream = (hipStream_t)stream_;
+    r.part = weights ? (float*)a->temp : nullptr;
+    if (empty) p.blocks = 0;   // (the weights' gradients are zero)
+    return hn_dispatch(a, p, [&](auto t, auto v, auto n) -> int {
+        using T = decltype(t);
+        if (!empty) {
+            k_head_norm_grad<T, decltype(v)::value, decltype(n)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
+            TDGS_LAUNCHED();
+        }
+        if (weights) {
+            k_head_norm_join<T><<<(unsigned)ceil_div(2 * a->head_dim, kHnJoinCols), kHnThreads, 0, stream>>>(
+                r.part, p.blocks, a->head_dim, g->dq_weight, g->dk_weight, r.param_f32);
+            TDGS_LAUNCHED();
+        }
+        return TDGS_OK;
+    });
+}
+
+}  // extern "C"

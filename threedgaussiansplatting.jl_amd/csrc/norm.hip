@@ -18,6 +18,7 @@
 // all workgroups for each other in the middle.
 #include "internal.hpp"
 #include "elem.hpp"
+#include "activation.hpp"
 
 namespace tdgs {
 
@@ -75,38 +76,6 @@ struct GnVec {
         }
     }
 };
-
-// act(z), and its derivative in *slope where wanted. SiLU: z s, s + y (1 - s) with s = 1 / (1 + e^-z).
-// GELU: z cdf(z), cdf + z e^(-z^2 / 2) / sqrt(2 pi); the normal distribution's tail is
-// erfc(x) = (a1 t + .. + a5 t^5) e^(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most (Abramowitz & Stegun
-// 7.1.26), which takes the exponential that the derivative needs anyway: 0.8e-7 in cdf, one rounding.
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ float gn_act(float z, float* slope) {
-    if constexpr (ACT == TDGS_ACT_IDENTITY) {
-        if (SLOPE) *slope = 1.0f;
-        return z;
-    } else if constexpr (ACT == TDGS_ACT_RELU) {
-        if (SLOPE) *slope = z > 0.0f ? 1.0f : 0.0f;
-        return z < 0.0f ? 0.0f : z;   // (NaN stays)
-    } else if constexpr (ACT == TDGS_ACT_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
-        const float y = z * s;
-        if (SLOPE) *slope = __builtin_fmaf(y, 1.0f - s, s);
-        return y;
-    } else {
-        const float ax = fabsf(z) * 0.70710678118654752f;
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, ax, 1.0f));
-        const float e = __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
-        float a = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-        a = __builtin_fmaf(a, t, 1.421413741f);
-        a = __builtin_fmaf(a, t, -0.284496736f);
-        a = __builtin_fmaf(a, t, 0.254829592f);
-        const float tail = 0.5f * a * t * e;
-        const float cdf = z < 0.0f ? tail : 1.0f - tail;
-        if (SLOPE) *slope = __builtin_fmaf(z * 0.39894228040143268f, e, cdf);
-        return z * cdf;
-    }
-}
 
 // Where a thread of a workgroup of THREADS stands among `vectors` channel vectors.
 template <int THREADS>
@@ -330,7 +299,7 @@ __device__ __forceinline__ void gn_apply(const GnArgs& a, const T* __restrict__ 
         float none;
 #pragma unroll
         for (int i = 0; i < VW; ++i)
-            v.f[i] = gn_act<ACT, false>(__builtin_fmaf(v.f[i] - ch.mean[i], rw[i], ch.b[i]), &none);
+            v.f[i] = act_value<ACT, false>(__builtin_fmaf(v.f[i] - ch.mean[i], rw[i], ch.b[i]), &none);
     };
     constexpr int U = 4;
     int64_t p = p0 + at.pl;
@@ -403,7 +372,7 @@ __device__ __forceinline__ void gn_slope(const GnChannels<T, VW>& ch, const GnVe
     for (int i = 0; i < VW; ++i) {
         float slope;
         xhat[i] = (x.f[i] - ch.mean[i]) * ch.r[i];
-        gn_act<ACT, true>(__builtin_fmaf(xhat[i], ch.w[i], ch.b[i]), &slope);
+        act_value<ACT, true>(__builtin_fmaf(xhat[i], ch.w[i], ch.b[i]), &slope);
         e[i] = d.f[i] * slope;
     }
 }

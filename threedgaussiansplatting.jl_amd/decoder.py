@@ -1,24 +1,26 @@
 """Operators of a learned decoder of rendered images over libtdgs.so: cross attention to an
-encoder's states, group norm with an activation (channels last) and embedding lookup, each with
-its gradients.
+encoder's states, group norm with an activation (channels last), embedding lookup, linear layers with
+bias, activation and residual, norms of queries and keys for each head with their rotation by position, and
+dropout, each with its gradients.
 
-What a network that turns rendered features into images needs besides matrix products (an
-appearance model of a photo collection, a refiner, a codebook of Gaussian attributes). The reference has no counterpart. Tensors are
+What a network that turns rendered features into images needs (an appearance model of a photo collection, a
+refiner, a codebook of Gaussian attributes). The reference has no counterpart. Tensors are
 float32, bfloat16 or float16 on the GPU; outputs and gradients are written into the tensors given,
 on the current stream, without synchronisation. temp is scratch of the size its function's
-*_temp() gives: with None a call allocates its own. cross_attention, group_norm and embedding are the
-same operators as functions that torch can differentiate.
+*_temp() gives: with None a call allocates its own. cross_attention, group_norm, embedding, linear, head_norm, rotate
+and dropout are the same operators as functions that torch can differentiate.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 import struct
 
 import torch
 
 from . import abi
-from .core import _handle, check, dptr, lib
+from .core import _dev, _handle, check, dptr, lib
 
 DTYPES = {torch.float32: abi.TDGS_F32, torch.bfloat16: abi.TDGS_BF16, torch.float16: abi.TDGS_F16}
 
@@ -33,8 +35,15 @@ _ATTENTION = struct.Struct("@8ifi" + 4 * "Pqqq" + "PPqPPN")
 _ATTENTION_GRADS = struct.Struct("@" + 4 * "Pqqq")
 _NORM = struct.Struct("@6ifiq" + 2 * "Pqq" + "PPPPN")
 _NORM_GRADS = struct.Struct("@" + 2 * "Pqq" + "PP")
-assert (_ATTENTION.size, _ATTENTION_GRADS.size, _NORM.size, _NORM_GRADS.size) == tuple(
-    C.sizeof(t) for t in (abi.AttentionC, abi.AttentionGradsC, abi.NormC, abi.NormGradsC))
+_LINEAR = struct.Struct("@2iq4i" + 5 * "Pq" + "PPN")
+_LINEAR_GRADS = struct.Struct("@" + 3 * "Pq" + "P2i")
+_HEAD_NORM = struct.Struct("@8if3i4i2iPPq" + 4 * "Pqqq" + "PPPN")
+_HEAD_NORM_GRADS = struct.Struct("@" + 4 * "Pqqq" + "PP")
+_DROPOUT = struct.Struct("@2i2qd2QP" + 3 * "Pq")
+assert (_ATTENTION.size, _ATTENTION_GRADS.size, _NORM.size, _NORM_GRADS.size, _LINEAR.size, _LINEAR_GRADS.size,
+        _HEAD_NORM.size, _HEAD_NORM_GRADS.size, _DROPOUT.size) == tuple(
+    C.sizeof(t) for t in (abi.AttentionC, abi.AttentionGradsC, abi.NormC, abi.NormGradsC, abi.LinearC, abi.LinearGradsC,
+                          abi.HeadNormC, abi.HeadNormGradsC, abi.DropoutC))
 
 
 def _call(f, t, args, ctx=()):
@@ -363,6 +372,318 @@ def embedding_grad_(dtable, dout, tokens, *, scale=1.0, padding=None, temp=None,
 
 
 # ------------------------------------------------------------------------------------
+# Linear layers with bias, activation and residual
+# ------------------------------------------------------------------------------------
+
+def _even_rows(t):
+    """The stride between the rows of a (.., n) tensor, None where they are not evenly strided."""
+    n, s = t.shape, t.stride()
+    if len(n) == 2:
+        return s[0]
+    step, count = n[-1], 1
+    for i in range(len(n) - 2, -1, -1):
+        if n[i] > 1:
+            if count == 1:
+                step = s[i]
+            elif s[i] != step * count:
+                return None
+            count *= n[i]
+    return step
+
+
+def _matrix(t, name, lead, cols, like):
+    """(pointer, row stride) of a tensor of shape (*lead, cols) with evenly strided rows of contiguous elements."""
+    _check_tensor(t, name, like)
+    if t.dtype is not like.dtype:
+        raise ValueError(f"{name} is {t.dtype}, not {like.dtype}")
+    n = t.shape
+    if n[:-1] != lead or n[-1] != cols:
+        raise ValueError(f"{name} has shape {tuple(n)}, not {(*lead, cols)}")
+    if cols > 1 and t.stride(-1) != 1 and t.numel():
+        raise ValueError(f"the rows of {name} must be contiguous")
+    step = _even_rows(t)
+    if step is None:
+        if t.numel():
+            raise ValueError(f"the rows of {name} must be evenly strided")
+        step = cols
+    return t.data_ptr(), step
+
+
+_NO_ROWS = (0, 0)
+
+
+def _weight(w, name, like, shape=None):
+    """(layout, pointer, row stride) of an (in, out) matrix that lies either way round."""
+    _check_tensor(w, name, like)
+    if w.dtype is not like.dtype:
+        raise ValueError(f"{name} is {w.dtype}, not {like.dtype}")
+    if w.dim() != 2 or (shape is not None and w.shape != shape):
+        raise ValueError(f"{name} has shape {tuple(w.shape)}, not {'(in, out)' if shape is None else tuple(shape)}")
+    (rows, cols), (row, element) = w.shape, w.stride()
+    if element == 1 or cols == 1:
+        # (one column of a transposed matrix: rows of one element, or one row of them, whichever is contiguous)
+        if cols > 1 or row != 1:
+            return abi.TDGS_WEIGHT_IN_OUT, w.data_ptr(), row
+    if row == 1 or rows == 1:
+        return abi.TDGS_WEIGHT_OUT_IN, w.data_ptr(), element
+    raise ValueError(f"the rows or the columns of {name} must be contiguous")
+
+
+def _linear(x, weight, bias, activation, pre):
+    """The fields of the tdgs_linear of these tensors up to out, and those from pre to bias."""
+    _check_tensor(x, "x", x)
+    dtype = DTYPES.get(x.dtype)
+    if dtype is None:
+        raise ValueError(f"x is {x.dtype}: float32, bfloat16 and float16 are supported")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
+    if x.dim() < 1:
+        raise ValueError("x must be (.., in)")
+    layout, w, ws = _weight(weight, "weight", x)
+    features, outputs = weight.shape
+    lead = x.shape[:-1]
+    xp, xs = _matrix(x, "x", lead, features, x)
+    b = 0
+    if bias is not None:
+        _check_vector(bias, "bias", outputs, x)
+        b = bias.data_ptr()
+    rows = x.numel() // features if features else 0
+    return ((dtype, act, rows, features, outputs, layout, 0, xp, xs, w, ws),
+            (*(_NO_ROWS if pre is None else _matrix(pre, "pre", lead, outputs, x)), b))
+
+
+def _check_vector(p, name, n, like):
+    _check_tensor(p, name, like)
+    if p.dtype is not like.dtype or p.shape != (n,) or not p.is_contiguous():
+        raise ValueError(f"{name} must be {n} contiguous values of {like.dtype}")
+
+
+def linear_temp(x, weight, grad=False):
+    """Scratch for linear_ (with grad also linear_grad_, whatever its activation) on tensors of these sizes."""
+    a, b = _linear(x, weight, None, "silu", None)
+    return _new_temp(lib().tdgs_linear_temp_bytes, _LINEAR.pack(*a, *_NO_ROWS, *_NO_ROWS, *b, 0, 0), grad, x)
+
+
+def linear_(out, x, weight, bias=None, *, residual=None, activation="identity", pre=None, temp=None):
+    """out = residual + act(x weight + bias) (tdgs_linear_forward).
+
+    x is (.., in), weight (in, out), the others (.., out), all of one type, their rows contiguous and evenly strided; of the
+    weight the rows or the columns are (the transpose of an (out, in) matrix is taken as it is). activation is identity,
+    silu, gelu or relu. pre, where given, receives x weight + bias, which the gradient needs unless the activation is the
+    identity. residual may be out; out and pre overlap nothing else."""
+    a, b = _linear(x, weight, bias, activation, pre)
+    lead, outputs = x.shape[:-1], weight.shape[1]
+    o = _matrix(out, "out", lead, outputs, x)
+    r = _NO_ROWS if residual is None else _matrix(residual, "residual", lead, outputs, x)
+    if temp is None:
+        temp = _new_temp(lib().tdgs_linear_temp_bytes, _LINEAR.pack(*a, *o, *r, *b, 0, 0), False, x)
+    _call(lib().tdgs_linear_forward, x, (_LINEAR.pack(*a, *o, *r, *b, *_temp(temp, x)),))
+    return out
+
+
+def linear_grad_(dx, dweight, dbias, dout, x, weight, *, activation="identity", pre=None, temp=None):
+    """The gradients of sum(dout * out) for linear_'s x, weight and bias (tdgs_linear_grad), from its pre; any of them may
+    be None. dweight lies either way round, whatever weight does. The residual's gradient is dout.
+
+    dout act'(pre) is an operand of two matrix products and rounded to the type for them; dbias is summed before."""
+    if pre is None and activation != "identity":
+        raise ValueError("the gradient needs the forward call's pre")
+    a, b = _linear(x, weight, None, activation, pre)
+    lead, outputs = x.shape[:-1], weight.shape[1]
+    d = _matrix(dout, "dout", lead, outputs, x)
+    g = _NO_ROWS if dx is None else _matrix(dx, "dx", lead, weight.shape[0], x)
+    layout, w, ws = (0, 0, 0) if dweight is None else _weight(dweight, "dweight", x, weight.shape)
+    db = 0
+    if dbias is not None:
+        _check_vector(dbias, "dbias", outputs, x)
+        db = dbias.data_ptr()
+    if temp is None:
+        temp = _new_temp(lib().tdgs_linear_temp_bytes, _LINEAR.pack(*a, *_NO_ROWS, *_NO_ROWS, *b, 0, 0), True, x)
+    _call(lib().tdgs_linear_grad, x, (_LINEAR.pack(*a, *_NO_ROWS, *_NO_ROWS, *b, *_temp(temp, x)),
+                                      _LINEAR_GRADS.pack(*d, *g, w, ws, db, layout, 0)))
+    return dx, dweight, dbias
+
+
+# ------------------------------------------------------------------------------------
+# Norms of queries and keys for each head, and their rotation by position
+# ------------------------------------------------------------------------------------
+
+_PAIRS = {"halves": abi.TDGS_PAIRS_HALVES, "interleaved": abi.TDGS_PAIRS_INTERLEAVED}
+_POSITIONS = {torch.int32: abi.TDGS_POSITION_I32, torch.int64: abi.TDGS_POSITION_I64,
+              torch.float32: abi.TDGS_POSITION_F32}
+
+
+class Rotary:
+    """The rotation of pairs of a head's elements by position on several axes (time, row, column, ..).
+
+    sections holds the pairs of each axis, in order: pair j of an axis of n pairs turns by position * base ** (-j / n)
+    radians, or by position * frequencies[pair] where these are given (one per pair of all sections). pairs
+    says which elements are a pair: "halves", p and p + sum(sections), or "interleaved", 2 p and 2 p + 1. Elements of a head
+    behind the pairs are not rotated."""
+
+    def __init__(self, sections, *, base=10000.0, pairs="halves", frequencies=None, device=0):
+        self.sections = tuple(int(s) for s in sections)
+        if not 1 <= len(self.sections) <= 4 or min(self.sections) < 1:
+            raise ValueError(f"sections {sections} are not one to four axes of one pair or more")
+        if pairs not in _PAIRS:
+            raise ValueError(f"pairs {pairs!r} are none of {', '.join(_PAIRS)}")
+        if not base > 0:
+            raise ValueError("the base must be positive")
+        self.pairs, self.layout, self.axes = sum(self.sections), pairs, len(self.sections)
+        if frequencies is None:
+            frequencies = [base ** (-j / n) for n in self.sections for j in range(n)]
+        f = torch.as_tensor(frequencies, dtype=torch.float64)
+        if f.shape != (self.pairs,):
+            raise ValueError(f"{tuple(f.shape)} frequencies of {self.pairs} pairs")
+        self.turns = (f / (2 * math.pi)).to(_dev(device))
+        self._fields = (self.pairs, _PAIRS[pairs], self.axes, *self.sections, *(0,) * (4 - self.axes))
+
+
+def _head_norm(q, k, q_weight, k_weight, norm, eps, rotary, positions, inverse):
+    """The fields of the tdgs_head_norm of these tensors up to q, and those of the weights."""
+    _check_tensor(q, "q", q)
+    dtype = DTYPES.get(q.dtype)
+    if dtype is None:
+        raise ValueError(f"q is {q.dtype}: float32, bfloat16 and float16 are supported")
+    if q.dim() != 4:
+        raise ValueError("q must be (batch, length, heads, head_dim)")
+    b, l, h, d = q.shape
+    hk = 0
+    if k is not None:
+        if k.dim() != 4 or k.shape[:2] != (b, l) or k.shape[3] != d:
+            raise ValueError(f"k has shape {tuple(k.shape)}, not ({b}, {l}, heads, {d})")
+        hk = k.shape[2]
+    first = q_weight if q_weight is not None else k_weight
+    param = abi.TDGS_F32
+    if first is not None:
+        param = DTYPES.get(first.dtype)
+        if first.dtype is not torch.float32 and first.dtype is not q.dtype:
+            raise ValueError(f"q_weight and k_weight must be of one type, float32 or {q.dtype}")
+        for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            if w is not None:
+                _check_vector(w, name, d, first)
+                _check_tensor(w, name, q)
+    if rotary is None:
+        if positions is not None:
+            raise ValueError("positions without a rotary")
+        rotation, place = (0,) * 7, (0, 0, 0, 0)
+    else:
+        _check_tensor(rotary.turns, "the rotary", q)
+        _check_tensor(positions, "positions", q)
+        kind = _POSITIONS.get(positions.dtype)
+        if kind is None:
+            raise ValueError(f"positions are {positions.dtype}: int32, int64 and float32 are supported")
+        n = positions.shape
+        if (n != (l, rotary.axes) and n != (b, l, rotary.axes)) or not positions.is_contiguous():
+            raise ValueError(f"positions must be contiguous, ({l}, {rotary.axes}) or ({b}, {l}, {rotary.axes})")
+        rotation = rotary._fields
+        place = (kind, rotary.turns.data_ptr(), positions.data_ptr(), l * rotary.axes if len(n) == 3 else 0)
+    return ((dtype, param, b, l, h, hk, d, int(norm), eps, *rotation, int(inverse), *place),
+            (dptr(q_weight) or 0, dptr(k_weight) or 0))
+
+
+def _head_views(names, tensors, like):
+    """The tdgs_heads fields of tensors like (q, k): k's may be missing."""
+    q, k = like
+    out = _heads(tensors[0], names[0], q.shape, q)
+    if k is None:
+        if tensors[1] is not None:
+            raise ValueError(f"{names[1]} without k")
+        return (*out, *_NO_HEADS)
+    return (*out, *_heads(tensors[1], names[1], k.shape, q))
+
+
+def head_norm_(q_out, k_out, q, k=None, q_weight=None, k_weight=None, *, eps=1e-6, rotary=None, positions=None):
+    """Each head of q and k divided by the root of its mean square plus eps and multiplied by its weight; with a
+    Rotary, rotated by position in the same pass (tdgs_head_norm_forward).
+
+    q and k are (batch, length, heads, head_dim), of any strides with the last dimension contiguous, head_dim up to 256; k (and
+    k_out) may be None. weights are head_dim values, float32 or of q's type; None: ones. positions are (length, axes) or
+    (batch, length, axes), int32, int64 or float32; their angles are made in 64 bits. q_out may be q and k_out k."""
+    a, w = _head_norm(q, k, q_weight, k_weight, True, eps, rotary, positions, False)
+    x = _head_views(("q", "k"), (q, k), (q, k))
+    o = _head_views(("q_out", "k_out"), (q_out, k_out), (q, k))
+    _call(lib().tdgs_head_norm_forward, q, (_HEAD_NORM.pack(*a, *x, *o, *w, 0, 0),))
+    return q_out, k_out
+
+
+def head_norm_temp(q, k=None):
+    """Scratch for head_norm_grad_ on tensors of these sizes."""
+    a, w = _head_norm(q, k, None, None, True, 0.0, None, None, False)
+    n = lib().tdgs_head_norm_temp_bytes(_HEAD_NORM.pack(*a, *_NO_HEADS * 4, *w, 0, 0))
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=q.device)
+
+
+def head_norm_grad_(dq, dk, dq_weight, dk_weight, dq_out, dk_out, q, k=None, q_weight=None, k_weight=None, *, eps=1e-6,
+                    rotary=None, positions=None, temp=None):
+    """The gradients of sum(dq_out * q_out) + sum(dk_out * k_out) for head_norm_'s operands (tdgs_head_norm_grad).
+    dq_weight and dk_weight (of the weights' type, float32 without them) may be None; dq may be dq_out and dk dk_out."""
+    a, w = _head_norm(q, k, q_weight, k_weight, True, eps, rotary, positions, False)
+    x = _head_views(("q", "k"), (q, k), (q, k))
+    first = q_weight if q_weight is not None else k_weight
+    for p, name in ((dq_weight, "dq_weight"), (dk_weight, "dk_weight")):
+        if p is not None:
+            _check_tensor(p, name, q)
+            dtype = torch.float32 if first is None else first.dtype
+            if p.dtype is not dtype or p.shape != (q.shape[3],) or not p.is_contiguous():
+                raise ValueError(f"{name} must be {q.shape[3]} contiguous values of {dtype}")
+    g = (*_head_views(("dq_out", "dk_out"), (dq_out, dk_out), (q, k)), *_head_views(("dq", "dk"), (dq, dk), (q, k)))
+    if temp is None:
+        temp = head_norm_temp(q, k)
+    _call(lib().tdgs_head_norm_grad, q, (_HEAD_NORM.pack(*a, *x, *_NO_HEADS * 2, *w, *_temp(temp, q)),
+                                         _HEAD_NORM_GRADS.pack(*g, dptr(dq_weight) or 0, dptr(dk_weight) or 0)))
+    return dq, dk, dq_weight, dk_weight
+
+
+def rotate_(q_out, k_out, q, k, rotary, positions, *, inverse=False):
+    """head_norm_'s rotation alone; the other way round with inverse, which is its gradient."""
+    if rotary is None:
+        raise ValueError("a rotation needs a Rotary")
+    a, w = _head_norm(q, k, None, None, False, 0.0, rotary, positions, inverse)
+    x = _head_views(("q", "k"), (q, k), (q, k))
+    o = _head_views(("q_out", "k_out"), (q_out, k_out), (q, k))
+    _call(lib().tdgs_head_norm_forward, q, (_HEAD_NORM.pack(*a, *x, *o, *w, 0, 0),))
+    return q_out, k_out
+
+
+# ------------------------------------------------------------------------------------
+# Dropout
+# ------------------------------------------------------------------------------------
+
+def dropout_(out, x, p, seed, *, call=0, residual=None):
+    """out = residual + x / (1 - p) where an element is kept, with probability 1 - p, and residual where it is dropped
+    (tdgs_dropout_apply).
+
+    Tensors are (.., n), their rows contiguous and evenly strided. Which elements are kept is a function of seed (64 bits), call and an
+    element's place among x's, not of strides or type: the same call on dout, without a residual, is the gradient for x.
+    call, a count that a program advances with every use, is a whole number, or an int64 tensor of one value on the GPU that
+    the kernel reads (a captured call then takes another mask at each replay). out may be x or residual."""
+    _check_tensor(x, "x", x)
+    dtype = DTYPES.get(x.dtype)
+    if dtype is None:
+        raise ValueError(f"x is {x.dtype}: float32, bfloat16 and float16 are supported")
+    if not 0 <= p <= 1:
+        raise ValueError(f"dropout of {p}, which is no probability")
+    if x.dim() == 0:
+        raise ValueError("x must have a dimension")
+    lead, cols = x.shape[:-1], x.shape[-1]
+    number = device_call = 0
+    if isinstance(call, torch.Tensor):
+        _check_tensor(call, "call", x)
+        if call.dtype is not torch.int64 or call.numel() != 1:
+            raise ValueError("call must be a whole number or one int64 value")
+        device_call = call.data_ptr()
+    else:
+        number = int(call) & (2 ** 64 - 1)
+    r = _NO_ROWS if residual is None else _matrix(residual, "residual", lead, cols, x)
+    fields = (dtype, 0, x.numel() // cols if cols else 0, cols, p, int(seed) & (2 ** 64 - 1), number, device_call,
+              *_matrix(x, "x", lead, cols, x), *_matrix(out, "out", lead, cols, x), *r)
+    _call(lib().tdgs_dropout_apply, x, (_DROPOUT.pack(*fields),))
+    return out
+
+
+# ------------------------------------------------------------------------------------
 # As differentiable functions: once, their gradients have no kernels of their own
 # ------------------------------------------------------------------------------------
 
@@ -392,10 +713,10 @@ def _once(backward):
     a graph of the gradients, they hang on everything that they were made from, so that a second derivative
     raises. (once_differentiable refuses only what comes through dout, and takes them for constants otherwise.)"""
     @functools.wraps(backward)
-    def wrapped(ctx, dout):
+    def wrapped(ctx, *douts):
         with torch.no_grad():
-            grads = backward(ctx, dout)
-        made_from = [t for t in (dout, *ctx.saved_tensors) if t is not None and t.requires_grad] \
+            grads = backward(ctx, *douts)
+        made_from = [t for t in (*douts, *ctx.saved_tensors) if t is not None and t.requires_grad] \
             if torch.is_grad_enabled() else ()
         if made_from:
             given = [g for g in grads if g is not None]
@@ -486,3 +807,129 @@ def embedding(table, tokens, *, scale=1.0, padding=None):
     embedding_grad_."""
     _check_padding(padding, table.shape[0])
     return _Embedding.apply(_rows_contiguous(table), tokens.contiguous(), scale, padding)
+
+
+def _rows_even(t):
+    """t, or a copy where its rows are not contiguous and evenly strided."""
+    if t is None:
+        return None
+    t = _rows_contiguous(t)
+    return t if _even_rows(t) is not None else t.contiguous()
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        out = torch.empty((*x.shape[:-1], weight.shape[1]), dtype=x.dtype, device=x.device)
+        pre = torch.empty_like(out) if activation != "identity" and any(ctx.needs_input_grad[:3]) else None
+        linear_(out, x, weight, bias, residual=residual, activation=activation, pre=pre)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @_once
+    def backward(ctx, dout):
+        x, weight, pre = ctx.saved_tensors
+        wants = ctx.needs_input_grad
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if wants[0] else None
+        # (laid out as the weight is)
+        dweight = torch.empty_strided(weight.shape, _dense(weight), dtype=x.dtype, device=x.device) if wants[1] else None
+        dbias = torch.empty(weight.shape[1:], dtype=x.dtype, device=x.device) if wants[2] else None
+        if any(wants[:3]):
+            linear_grad_(dx, dweight, dbias, _rows_even(dout), x, weight, activation=ctx.activation, pre=pre)
+        return dx, dweight, dbias, dout if wants[3] else None, None
+
+
+def _dense(weight):
+    """The strides of a dense matrix that lies as weight does."""
+    rows, cols = weight.shape
+    return (cols, 1) if weight.stride(1) == 1 else (1, rows)
+
+
+def linear(x, weight, bias=None, *, residual=None, activation="identity"):
+    """linear_ as a differentiable function of x, weight, bias and residual, all of any strides."""
+    if weight.dim() == 2 and weight.stride(0) != 1:
+        weight = _rows_contiguous(weight)
+    return _Linear.apply(_rows_even(x), weight, _contiguous(bias), _rows_even(residual), activation)
+
+
+class _HeadNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, eps, rotary, positions):
+        outs = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
+        head_norm_(*outs, q, k, q_weight, k_weight, eps=eps, rotary=rotary, positions=positions)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions)
+        ctx.eps, ctx.rotary = eps, rotary
+        ctx.set_materialize_grads(True)
+        return outs[0] if k is None else tuple(outs)
+
+    @staticmethod
+    @_once
+    def backward(ctx, *douts):
+        q, k, q_weight, k_weight, positions = ctx.saved_tensors
+        dq, dk = (None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+        weights = [torch.empty_like(w) if want else None for w, want in zip((q_weight, k_weight), ctx.needs_input_grad[2:4])]
+        douts = [_rows_contiguous(d) for d in douts] + [None] * (k is None)
+        head_norm_grad_(dq, dk, *weights, *douts, q, k, q_weight, k_weight, eps=ctx.eps, rotary=ctx.rotary,
+                        positions=positions)
+        return dq, dk, *weights, None, None, None
+
+
+def head_norm(q, k=None, q_weight=None, k_weight=None, *, eps=1e-6, rotary=None, positions=None):
+    """head_norm_ as a differentiable function of q, k and their weights, all of any strides; returns q's result, or q's
+    and k's."""
+    return _HeadNorm.apply(_rows_contiguous(q), None if k is None else _rows_contiguous(k), _contiguous(q_weight),
+                           _contiguous(k_weight), eps, rotary, _contiguous(positions))
+
+
+class _Rotate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, rotary, positions, inverse):
+        outs = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
+        rotate_(*outs, q, k, rotary, positions, inverse=inverse)
+        ctx.save_for_backward(positions)
+        ctx.rotary, ctx.inverse = rotary, inverse
+        ctx.set_materialize_grads(True)
+        return outs[0] if k is None else tuple(outs)
+
+    @staticmethod
+    @_once
+    def backward(ctx, *douts):
+        positions, = ctx.saved_tensors
+        douts = [_rows_contiguous(d) for d in douts]
+        grads = [torch.empty(d.shape, dtype=d.dtype, device=d.device) for d in douts]
+        rotate_(grads[0], grads[1] if len(grads) > 1 else None, douts[0], douts[1] if len(douts) > 1 else None, ctx.rotary,
+                positions, inverse=not ctx.inverse)
+        return grads[0], grads[1] if len(grads) > 1 else None, None, None, None
+
+
+def rotate(q, k, rotary, positions, *, inverse=False):
+    """rotate_ as a differentiable function of q and k (k may be None), all of any strides."""
+    return _Rotate.apply(_rows_contiguous(q), None if k is None else _rows_contiguous(k), rotary, _contiguous(positions),
+                         inverse)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, call):
+        # (a call number on the device may move on before the gradient is asked for)
+        call = call.clone() if isinstance(call, torch.Tensor) else call
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dropout_(out, x, p, seed, call=call, residual=residual)
+        ctx.p, ctx.seed, ctx.call = p, seed, call
+        return out
+
+    @staticmethod
+    @_once
+    def backward(ctx, dout):
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty(dout.shape, dtype=dout.dtype, device=dout.device)
+            dropout_(dx, _rows_even(dout), ctx.p, ctx.seed, call=ctx.call)
+        return dx, dout if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x, p, seed, *, call=0, residual=None):
+    """dropout_ as a differentiable function of x and residual, of any strides."""
+    return _Dropout.apply(_rows_even(x), _rows_even(residual), p, seed, call)
