@@ -3,8 +3,10 @@
 //
 // A head's row of d elements is split into units of V pairs, one per lane: V elements of each half (pairs p,
 // p + pairs), or 2 V neighbours (pairs 2 p, 2 p + 1, and what is not rotated), so that both elements of a pair
-// are in one lane and the norm's sum takes a few exchanges among the row's G lanes. A workgroup takes a
-// few tokens at a time: it makes their cosines and sines once, in LDS, and uses them for all heads of queries and keys.
+// are in one lane and the norm's sum takes a few exchanges among the row's lanes; a wavefront takes as many whole rows as it
+// has lanes for. A workgroup takes a few tokens at a time: it makes their cosines and sines, and the places of their
+// rows, once, in LDS, and uses them for all heads, of the queries first and then of the keys, whose weights
+// stay in registers.
 //
 // The angle of a far position has few bits left in 32: position * frequency / (2 pi) is taken in 64 bits, as turns,
 // whose whole part is dropped; the rest is exact to 2^-26 in 32 bits, from which sinpi and cospi go on.
@@ -21,6 +23,7 @@ constexpr int kHnThreads = 256;
 constexpr int kHnAngles = 4096;     // of a workgroup's tokens, in LDS: 32 KB
 constexpr int kHnBlocks = 1024;     // workgroups of the gradient, which leave one partial sum of dw each
 constexpr int kHnMaxDim = 256;
+constexpr int kHnTokens = 64;       // of a workgroup at a time, at most
 
 struct HnTensor {
     const void *x, *dout;
@@ -35,14 +38,13 @@ struct HnArgs {
     const void* positions;
     int64_t position_batch, tokens;  // tokens: batch * length
     float* part;
-    int32_t length, heads, all_heads, d, pairs, axes;
+    int32_t length, heads[2], d, pairs, axes;
     int32_t ends[4];                 // pairs of the axes up to and with this one
     int32_t position_type, per;      // per: tokens at a time
-    int32_t lanes, units, rotated_units;   // lanes of a row (a power of two), of which units hold something
-    int32_t row_shift;               // log2(lanes)
+    int32_t lanes, units, rotated_units;   // lanes of a row, with one unit each or (N = 2) two
     float eps, inv_d, sign;
     bool norm, interleaved, param_f32;
-    FastDiv by_heads, by_length;
+    FastDiv by_heads[2], by_length, by_pairs;
 };
 
 __device__ __forceinline__ double hn_position(const HnArgs& a, int64_t i) {
@@ -53,16 +55,31 @@ __device__ __forceinline__ double hn_position(const HnArgs& a, int64_t i) {
     }
 }
 
-// Cosine and sine of the pairs of `count` tokens from `first` on.
-__device__ __forceinline__ void hn_angles(const HnArgs& a, int64_t first, int count, float2* s) {
+// Where the rows of the tokens at hand start: x, output, output's gradient; of queries and keys.
+struct HnPlaces {
+    int64_t x[2][kHnTokens], out[2][kHnTokens], dout[2][kHnTokens];
+};
+
+// The places of `count` tokens from `first` on, and cosine and sine of their pairs.
+template <bool GRAD>
+__device__ __forceinline__ void hn_tokens(const HnArgs& a, int64_t first, int count, HnPlaces& at, float2* s) {
+    for (int i = threadIdx.x; i < 2 * count; i += kHnThreads) {
+        const int token = i >> 1, k = i & 1;
+        const HnTensor& t = a.t[k];
+        const uint32_t row = (uint32_t)(first + token), b = a.by_length.div(row), l = row - b * a.by_length.d;
+        at.x[k][token] = b * t.xb + l * t.xl;
+        at.out[k][token] = b * t.ob + l * t.ol;
+        if (GRAD) at.dout[k][token] = b * t.db + l * t.dl;
+    }
     for (int i = threadIdx.x; i < count * a.pairs; i += kHnThreads) {
-        const int token = i / a.pairs, p = i - token * a.pairs;
+        const int token = (int)a.by_pairs.div((uint32_t)i), p = i - token * a.pairs;
         const uint32_t row = (uint32_t)(first + token), b = a.by_length.div(row), l = row - b * a.by_length.d;
         int axis = 0;
         while (p >= a.ends[axis]) ++axis;
         const double t = hn_position(a, b * a.position_batch + (int64_t)l * a.axes + axis) * a.turns[p];
-        const float half = 2.0f * (float)(t - rint(t));
-        s[i] = make_float2(cospif(half), a.sign * sinpif(half));
+        float sn, cs;
+        sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
+        s[i] = make_float2(cs, a.sign * sn);
     }
 }
 
@@ -132,21 +149,41 @@ __device__ __forceinline__ void hn_store(T* __restrict__ p, const HnUnit<V>& u, 
     }
 }
 
-template <class T, int V>
-__device__ __forceinline__ void hn_weights(const HnArgs& a, const void* w, const HnUnit<V>& u, float (&x)[V], float (&y)[V]) {
+// A lane's weights, of queries and of keys: they stay in registers.
+template <class T, int V, int N>
+struct HnWeights {
+    float x[2][N][V], y[2][N][V];
+    __device__ __forceinline__ HnWeights(const HnArgs& a, int lane) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        x[i] = y[i] = 1.0f;
-        if (!w || !u.on) continue;
-        const int f = u.first + i * u.step, s = u.second + i * u.step;
-        x[i] = a.param_f32 ? ((const float*)w)[f] : (float)((const T*)w)[f];
-        if (s < a.d) y[i] = a.param_f32 ? ((const float*)w)[s] : (float)((const T*)w)[s];
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const HnUnit<V> u(a, lane + n * a.lanes);
+                const void* const w = a.t[k].weight;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    x[k][n][i] = y[k][n][i] = 1.0f;
+                    if (!w || !u.on) continue;
+                    const int f = u.first + i * u.step, s = u.second + i * u.step;
+                    x[k][n][i] = a.param_f32 ? ((const float*)w)[f] : (float)((const T*)w)[f];
+                    if (s < a.d) y[k][n][i] = a.param_f32 ? ((const float*)w)[s] : (float)((const T*)w)[s];
+                }
+            }
     }
-}
+};
 
-__device__ __forceinline__ float hn_row_sum(float x, int lanes) {
-    for (int w = lanes >> 1; w > 0; w >>= 1) x += __shfl_xor(x, w, kWave);
-    return x;
+// The sum of a row's lanes, of which this is lane j of `lanes` neighbours, in all of them.
+__device__ __forceinline__ float hn_row_sum(float x, int j, int lanes) {
+    if ((lanes & (lanes - 1)) == 0) {
+        for (int w = lanes >> 1; w > 0; w >>= 1) x += __shfl_xor(x, w, kWave);
+        return x;
+    }
+    const int me = (int)__lane_id();
+    for (int w = 1; w < lanes; w <<= 1) {   // lane j then holds those from j up to j + 2 w
+        const float y = __shfl(x, me + w, kWave);
+        x += j + w < lanes ? y : 0.0f;
+    }
+    return __shfl(x, me - j, kWave);
 }
 
 // (a, b) turned by the angles of s; by the opposite ones with BACK.
@@ -161,18 +198,16 @@ __device__ __forceinline__ void hn_turn(const float2* s, float (&a)[V], float (&
     }
 }
 
-// A row of the workgroup's tokens: its token, head and tensor.
-struct HnRow {
-    int token, head, k;
-    int64_t b, l;
-    __device__ __forceinline__ HnRow(const HnArgs& a, int64_t first, int r) {
-        token = (int)a.by_heads.div((uint32_t)r);
-        head = r - token * a.all_heads;
-        k = head >= a.heads;
-        if (k) head -= a.heads;
-        const uint32_t row = (uint32_t)(first + token);
-        b = a.by_length.div(row);
-        l = row - b * a.by_length.d;
+// A thread's place: unit j of the sub-th of the rows that a workgroup takes at once.
+struct HnLane {
+    int j, sub, rows;
+    bool on;
+    __device__ __forceinline__ HnLane(const HnArgs& a) {
+        const int lane = (int)__lane_id(), per = kWave / a.lanes, row = lane / a.lanes;
+        j = lane - row * a.lanes;
+        on = row < per;
+        sub = (int)threadIdx.x / kWave * per + (on ? row : 0);
+        rows = kHnThreads / kWave * per;
     }
 };
 
@@ -180,44 +215,50 @@ struct HnRow {
 template <class T, int V, int N>
 __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
     extern __shared__ float2 s_angles[];
-    const int lane = (int)threadIdx.x & (a.lanes - 1), sub = (int)threadIdx.x >> a.row_shift, rows_at = kHnThreads >> a.row_shift;
+    __shared__ HnPlaces s_at;
+    const HnLane lane(a);
+    const HnWeights<T, V, N> w(a, lane.j);
     for (int64_t first = (int64_t)blockIdx.x * a.per; first < a.tokens; first += (int64_t)gridDim.x * a.per) {
-        const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per), rows = count * a.all_heads;
-        if (a.pairs) {
-            __syncthreads();   // (the tokens before)
-            hn_angles(a, first, count, s_angles);
-            __syncthreads();
-        }
-        // every lane of a row's stays for its sum
-        for (int r0 = 0; r0 < rows; r0 += rows_at) {
-            const bool valid = r0 + sub < rows;
-            const HnRow row(a, first, valid ? r0 + sub : rows - 1);
-            const HnTensor& t = a.t[row.k];
-            const T* const x = (const T*)t.x + row.b * t.xb + row.l * t.xl + row.head * t.xh;
-            float ya[N][V], yb[N][V], sum = 0.0f;
+        const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per);
+        __syncthreads();   // (the tokens before)
+        hn_tokens<false>(a, first, count, s_at, s_angles);
+        __syncthreads();
 #pragma unroll
-            for (int n = 0; n < N; ++n) hn_load<T, V>(x, HnUnit<V>(a, lane + n * a.lanes), a.d, ya[n], yb[n]);
-            if (a.norm) {
+        for (int k = 0; k < 2; ++k) {
+            const HnTensor& t = a.t[k];
+            const int rows = count * a.heads[k];
+            // (every lane stays for the sums)
+            for (int r0 = 0; r0 < rows; r0 += lane.rows) {
+                const bool valid = lane.on && r0 + lane.sub < rows;
+                const int r = r0 + lane.sub < rows ? r0 + lane.sub : rows - 1;
+                const int token = (int)a.by_heads[k].div((uint32_t)r), head = r - token * a.heads[k];
+                const T* const x = (const T*)t.x + s_at.x[k][token] + head * t.xh;
+                float ya[N][V], yb[N][V];
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) sum = __builtin_fmaf(ya[n][i], ya[n][i], __builtin_fmaf(yb[n][i], yb[n][i], sum));
-                sum = rsqrtf(__builtin_fmaf(hn_row_sum(sum, a.lanes), a.inv_d, a.eps));
-            }
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const HnUnit<V> u(a, lane + n * a.lanes);
+                for (int n = 0; n < N; ++n) hn_load<T, V>(x, HnUnit<V>(a, lane.j + n * a.lanes), a.d, ya[n], yb[n]);
                 if (a.norm) {
-                    float wa[V], wb[V];
-                    hn_weights<T, V>(a, t.weight, u, wa, wb);
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        ya[n][i] *= sum * wa[i];
-                        yb[n][i] *= sum * wb[i];
-                    }
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            sum = __builtin_fmaf(ya[n][i], ya[n][i], __builtin_fmaf(yb[n][i], yb[n][i], sum));
+                    sum = rsqrtf(__builtin_fmaf(hn_row_sum(sum, lane.j, a.lanes), a.inv_d, a.eps));
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            ya[n][i] *= sum * w.x[k][n][i];
+                            yb[n][i] *= sum * w.y[k][n][i];
+                        }
                 }
-                if (u.on && u.rotated) hn_turn<V, false>(s_angles + row.token * a.pairs + u.pair, ya[n], yb[n]);
-                if (valid) hn_store<T, V>((T*)t.out + row.b * t.ob + row.l * t.ol + row.head * t.oh, u, a.d, ya[n], yb[n]);
+                T* const out = (T*)t.out + s_at.out[k][token] + head * t.oh;
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const HnUnit<V> u(a, lane.j + n * a.lanes);
+                    if (u.on && u.rotated) hn_turn<V, false>(s_angles + token * a.pairs + u.pair, ya[n], yb[n]);
+                    if (valid) hn_store<T, V>(out, u, a.d, ya[n], yb[n]);
+                }
             }
         }
     }
@@ -227,8 +268,9 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
 template <class T, int V, int N>
 __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
     extern __shared__ float2 s_angles[];
-    __shared__ float s_sums[kHnThreads / kWave][kHnMaxDim];
-    const int lane = (int)threadIdx.x & (a.lanes - 1), sub = (int)threadIdx.x >> a.row_shift, rows_at = kHnThreads >> a.row_shift;
+    __shared__ HnPlaces s_at;
+    const HnLane lane(a);
+    const HnWeights<T, V, N> w(a, lane.j);
     float da[2][N][V], db[2][N][V];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -237,94 +279,82 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) da[k][n][i] = db[k][n][i] = 0.0f;
     for (int64_t first = (int64_t)blockIdx.x * a.per; first < a.tokens; first += (int64_t)gridDim.x * a.per) {
-        const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per), rows = count * a.all_heads;
-        if (a.pairs) {
-            __syncthreads();
-            hn_angles(a, first, count, s_angles);
-            __syncthreads();
-        }
-        for (int r0 = 0; r0 < rows; r0 += rows_at) {
-            const bool valid = r0 + sub < rows;
-            const HnRow row(a, first, valid ? r0 + sub : rows - 1);
-            const HnTensor& t = a.t[row.k];
-            const T* const x = (const T*)t.x + row.b * t.xb + row.l * t.xl + row.head * t.xh;
-            const T* const dout = (const T*)t.dout + row.b * t.db + row.l * t.dl + row.head * t.dh;
-            float xa[N][V], xb[N][V], ea[N][V], eb[N][V], sum = 0.0f, mean = 0.0f;
+        const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per);
+        __syncthreads();
+        hn_tokens<true>(a, first, count, s_at, s_angles);
+        __syncthreads();
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const HnUnit<V> u(a, lane + n * a.lanes);
-                hn_load<T, V>(x, u, a.d, xa[n], xb[n]);
-                hn_load<T, V>(dout, u, a.d, ea[n], eb[n]);
-            }
+        for (int k = 0; k < 2; ++k) {
+            const HnTensor& t = a.t[k];
+            const int rows = count * a.heads[k];
+            for (int r0 = 0; r0 < rows; r0 += lane.rows) {
+                const bool valid = lane.on && r0 + lane.sub < rows;
+                const int row = r0 + lane.sub < rows ? r0 + lane.sub : rows - 1;
+                const int token = (int)a.by_heads[k].div((uint32_t)row), head = row - token * a.heads[k];
+                const T* const x = (const T*)t.x + s_at.x[k][token] + head * t.xh;
+                const T* const dout = (const T*)t.dout + s_at.dout[k][token] + head * t.dh;
+                float xa[N][V], xb[N][V], ea[N][V], eb[N][V], sum = 0.0f, mean = 0.0f;
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+                for (int n = 0; n < N; ++n) {
+                    const HnUnit<V> u(a, lane.j + n * a.lanes);
+                    hn_load<T, V>(x, u, a.d, xa[n], xb[n]);
+                    hn_load<T, V>(dout, u, a.d, ea[n], eb[n]);
+                }
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum = __builtin_fmaf(xa[n][i], xa[n][i], __builtin_fmaf(xb[n][i], xb[n][i], sum));
-            const float r = rsqrtf(__builtin_fmaf(hn_row_sum(sum, a.lanes), a.inv_d, a.eps));
-            const float mine = valid ? 1.0f : 0.0f;
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const HnUnit<V> u(a, lane + n * a.lanes);
-                if (u.on && u.rotated) hn_turn<V, true>(s_angles + row.token * a.pairs + u.pair, ea[n], eb[n]);
-                float wa[V], wb[V];
-                hn_weights<T, V>(a, t.weight, u, wa, wb);
+                    for (int i = 0; i < V; ++i) sum = __builtin_fmaf(xa[n][i], xa[n][i], __builtin_fmaf(xb[n][i], xb[n][i], sum));
+                const float r = rsqrtf(__builtin_fmaf(hn_row_sum(sum, lane.j, a.lanes), a.inv_d, a.eps));
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    xa[n][i] *= r;
-                    xb[n][i] *= r;
-                    const float pa = ea[n][i] * xa[n][i], pb = eb[n][i] * xb[n][i];
-                    if (valid) {
-                        da[0][n][i] += row.k ? 0.0f : pa;
-                        db[0][n][i] += row.k ? 0.0f : pb;
-                        da[1][n][i] += row.k ? pa : 0.0f;
-                        db[1][n][i] += row.k ? pb : 0.0f;
+                for (int n = 0; n < N; ++n) {
+                    const HnUnit<V> u(a, lane.j + n * a.lanes);
+                    if (u.on && u.rotated) hn_turn<V, true>(s_angles + token * a.pairs + u.pair, ea[n], eb[n]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        xa[n][i] *= r;
+                        xb[n][i] *= r;
+                        const float pa = ea[n][i] * xa[n][i], pb = eb[n][i] * xb[n][i];
+                        da[k][n][i] += valid ? pa : 0.0f;
+                        db[k][n][i] += valid ? pb : 0.0f;
+                        mean = __builtin_fmaf(pa, w.x[k][n][i], __builtin_fmaf(pb, w.y[k][n][i], mean));
                     }
-                    mean = __builtin_fmaf(pa, wa[i], __builtin_fmaf(pb, wb[i], mean));
-                    ea[n][i] *= wa[i];
-                    eb[n][i] *= wb[i];
                 }
-            }
-            mean = hn_row_sum(mean, a.lanes) * a.inv_d;
+                mean = hn_row_sum(mean, lane.j, a.lanes) * a.inv_d;
+                T* const out = (T*)t.out + s_at.out[k][token] + head * t.oh;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
+                for (int n = 0; n < N; ++n) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    xa[n][i] = r * __builtin_fmaf(-mean, xa[n][i], ea[n][i]);
-                    xb[n][i] = r * __builtin_fmaf(-mean, xb[n][i], eb[n][i]);
+                    for (int i = 0; i < V; ++i) {
+                        xa[n][i] = r * __builtin_fmaf(-mean, xa[n][i], ea[n][i] * w.x[k][n][i]);
+                        xb[n][i] = r * __builtin_fmaf(-mean, xb[n][i], eb[n][i] * w.y[k][n][i]);
+                    }
+                    if (valid) hn_store<T, V>(out, HnUnit<V>(a, lane.j + n * a.lanes), a.d, xa[n], xb[n]);
                 }
-                if (valid)
-                    hn_store<T, V>((T*)t.out + row.b * t.ob + row.l * t.ol + row.head * t.oh,
-                                   HnUnit<V>(a, lane + n * a.lanes), a.d, xa[n], xb[n]);
             }
         }
     }
     if (!a.part) return;
-    // over the wavefront's rows, then over its wavefronts
-    const int wave = (int)threadIdx.x / kWave;
+    // over the rows that were taken at once: every thread's 2 N V elements
+    __shared__ float s_sums[kHnThreads * 2 * V * N];
+#pragma unroll
     for (int k = 0; k < 2; ++k) {
+        __syncthreads();
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const HnUnit<V> u(a, lane + n * a.lanes);
+            const HnUnit<V> u(a, lane.j + n * a.lanes);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float x = k ? da[1][n][i] : da[0][n][i], y = k ? db[1][n][i] : db[0][n][i];
-                for (int w = kWave / 2; w >= a.lanes; w >>= 1) {
-                    x += __shfl_xor(x, w, kWave);
-                    y += __shfl_xor(y, w, kWave);
-                }
-                if ((int)__lane_id() < a.lanes && u.on) {
-                    s_sums[wave][u.first + i * u.step] = x;
-                    if (u.second + i * u.step < a.d) s_sums[wave][u.second + i * u.step] = y;
-                }
+                if (!lane.on || !u.on) continue;
+                s_sums[lane.sub * a.d + u.first + i * u.step] = da[k][n][i];
+                if (u.second + i * u.step < a.d) s_sums[lane.sub * a.d + u.second + i * u.step] = db[k][n][i];
             }
         }
         __syncthreads();
         for (int c = threadIdx.x; c < a.d; c += kHnThreads) {
             float x = 0.0f;
-            for (int w = 0; w < kHnThreads / kWave; ++w) x += s_sums[w][c];
+            for (int r = 0; r < lane.rows; ++r) x += s_sums[r * a.d + c];
             a.part[((int64_t)blockIdx.x * 2 + k) * a.d + c] = x;
         }
-        __syncthreads();
     }
 }
 
@@ -336,8 +366,10 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_join(const float* __re
     __shared__ float s[kHnThreads / kHnJoinCols][kHnJoinCols + 1];
     const int c = blockIdx.x * kHnJoinCols + (int)threadIdx.x % kHnJoinCols, y = (int)threadIdx.x / kHnJoinCols;
     float x = 0.0f;
-    if (c < 2 * d)
+    if (c < 2 * d) {
+#pragma unroll 8
         for (int b = y; b < blocks; b += kHnThreads / kHnJoinCols) x += part[(int64_t)b * 2 * d + c];
+    }
     s[y][threadIdx.x % kHnJoinCols] = x;
     __syncthreads();
     if (y != 0 || c >= 2 * d) return;
@@ -409,18 +441,15 @@ static HnPlan hn_plan(const tdgs_head_norm* a, HnArgs* r, bool grad) {
     p.v = a->dtype != TDGS_F32 && fits(8) ? 8 : fits(4) ? 4 : 1;
     r->rotated_units = a->pairs / p.v;
     r->units = r->rotated_units + (rest + 2 * p.v - 1) / (2 * p.v);
-    r->lanes = 1;
-    r->row_shift = 0;
-    while (r->lanes < r->units && r->lanes < kWave) {
-        r->lanes *= 2;
-        ++r->row_shift;
-    }
-    // tokens at a time: rows for every thread's lanes four times over, fewer where that would leave
+    r->lanes = r->units < kWave ? r->units : kWave;
+    // tokens at a time: four rows per thread's lane of the fewer heads, fewer tokens where that would leave
     // compute units idle, and what LDS holds
-    const int64_t tokens = (int64_t)a->batch * a->length, heads = (int64_t)a->heads + a->kv_heads;
-    int64_t per = 4 * (kHnThreads / r->lanes) / (heads > 0 ? heads : 1);
+    const int64_t tokens = (int64_t)a->batch * a->length;
+    const int few = a->heads && (a->heads < a->kv_heads || !a->kv_heads) ? a->heads : a->kv_heads;
+    int64_t per = ceil_div(4 * (kHnThreads / kWave) * (kWave / r->lanes), few > 0 ? few : 1);
     if (per > tokens / kHnBlocks) per = tokens / kHnBlocks;
     if (a->pairs && per > kHnAngles / a->pairs) per = kHnAngles / a->pairs;
+    if (per > kHnTokens) per = kHnTokens;
     if (per < 1) per = 1;
     r->per = (int32_t)per;
     const int64_t blocks = ceil_div(tokens, per);
@@ -444,8 +473,8 @@ static HnArgs hn_args(const tdgs_head_norm* a) {
     r.position_batch = a->position_batch_stride;
     r.tokens = (int64_t)a->batch * a->length;
     r.length = a->length;
-    r.heads = a->heads;
-    r.all_heads = a->heads + a->kv_heads;
+    r.heads[0] = a->heads;
+    r.heads[1] = a->kv_heads;
     r.d = a->head_dim;
     r.pairs = a->pairs;
     r.axes = a->axes;
@@ -460,7 +489,8 @@ static HnArgs hn_args(const tdgs_head_norm* a) {
     r.norm = a->norm != 0;
     r.interleaved = a->pair_layout == TDGS_PAIRS_INTERLEAVED;
     r.param_f32 = a->param_dtype == TDGS_F32;
-    r.by_heads = FastDiv((uint32_t)(r.all_heads > 0 ? r.all_heads : 1));
+    for (int i = 0; i < 2; ++i) r.by_heads[i] = FastDiv((uint32_t)(r.heads[i] > 0 ? r.heads[i] : 1));
+    r.by_pairs = FastDiv((uint32_t)(a->pairs > 0 ? a->pairs : 1));
     r.by_length = FastDiv((uint32_t)(a->length > 0 ? a->length : 1));
     return r;
 }

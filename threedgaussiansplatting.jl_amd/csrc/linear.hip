@@ -33,7 +33,7 @@ struct LnArgs {
     int32_t act;
     LnMatrix out, residual, pre;
     const void* bias;
-    const float* scale;       // out = act(*scale C + ..); null: 1
+    const float* scale;       // null, or out = *scale C, without a bias
 };
 
 // Elements of 16 bytes.
@@ -45,46 +45,53 @@ constexpr int ln_chunk() { return 16 / (int)sizeof(T); }
 template <class T, bool DEPTH, int N>
 constexpr int ln_pitch() { return N + (DEPTH || sizeof(T) == 4 ? ln_chunk<T>() : 32); }
 
-// A tile of MAJ memory rows x MIN elements on its way to LDS, by TH threads.
+// A tile of MAJ memory rows x MIN elements on its way to LDS, by TH threads: a thread takes 16 bytes of every kStep-th
+// row, loaded from a uniform base and an offset of its own, so that a step of the depth moves the base alone.
 template <class T, int MAJ, int MIN, int TH, int PITCH>
 struct LnTile {
     static constexpr int C = ln_chunk<T>();
-    static constexpr int kChunks = MAJ * MIN / C;
-    static constexpr int kPer = (kChunks + TH - 1) / TH;
+    static constexpr int kStep = TH / (MIN / C);       // rows apart
+    static constexpr int kPer = MAJ / kStep;
+    static_assert(TH % (MIN / C) == 0 && MAJ % kStep == 0, "whole rows of threads");
     typedef uint32_t U4 __attribute__((ext_vector_type(4)));
     typedef T Ca __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
     U4 r[kPer];
-    __device__ __forceinline__ static int chunk(int k) { return (int)threadIdx.x + k * TH; }
-    __device__ __forceinline__ static bool inside(int k) { return kChunks % TH == 0 || chunk(k) < kChunks; }
-    __device__ __forceinline__ static int row(int k) { return inside(k) ? chunk(k) / (MIN / C) : 0; }
-    __device__ __forceinline__ static int col(int k) { return inside(k) ? chunk(k) % (MIN / C) * C : 0; }
-    // The tile at p, of whose rows `maj` > 0 and of whose elements `min` > 0 exist; the memory row holds C elements or more.
-    __device__ __forceinline__ void load(const T* p, int64_t stride, int maj, int min) {
+    uint32_t offset[kPer];   // bytes, from 16 bytes before the tile
+    __device__ __forceinline__ static int row(int k) { return (int)threadIdx.x / (MIN / C) + k * kStep; }
+    __device__ __forceinline__ static int col() { return (int)threadIdx.x % (MIN / C) * C; }
+    // Of the tile's rows `maj` > 0 and of their elements `min` > 0 exist; the memory row holds C elements or more, before the
+    // tile or in it. Chunks across its end, or behind it, are its last 16 bytes.
+    __device__ __forceinline__ void place(int64_t stride, int maj, int min) {
+        const int x = col() + C <= min ? col() : min - C;
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) {
-            const int y = row(k) < maj ? row(k) : maj - 1, x = col(k) + C <= min ? col(k) : min - C;
-            r[k] = __builtin_bit_cast(U4, *reinterpret_cast<const Ca*>(p + y * stride + x));
-        }
+        for (int k = 0; k < kPer; ++k)
+            offset[k] = (uint32_t)((row(k) < maj ? row(k) : maj - 1) * (int)(stride * sizeof(T)) + (x + C) * (int)sizeof(T));
+    }
+    __device__ __forceinline__ void load(const T* tile) {
+        const char* const base = (const char*)tile - 16;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) r[k] = __builtin_bit_cast(U4, *reinterpret_cast<const Ca*>(base + offset[k]));
     }
     // The same by single elements, for memory rows of fewer than C of them.
-    __device__ __forceinline__ void load_narrow(const T* p, int64_t stride, int maj, int min) {
+    __device__ __forceinline__ void load_narrow(const T* tile, int64_t stride, int maj, int min) {
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const int y = row(k) < maj ? row(k) : maj - 1;
             T e[C];
 #pragma unroll
-            for (int i = 0; i < C; ++i) e[i] = col(k) + i < min ? p[y * stride + col(k) + i] : (T)0.0f;
+            for (int i = 0; i < C; ++i) e[i] = col() + i < min ? tile[y * stride + col() + i] : (T)0.0f;
             r[k] = __builtin_bit_cast(U4, e);
         }
     }
     template <bool NARROW>
     __device__ __forceinline__ void store(T* lds, int maj, int min) {
         if (!NARROW && min < MIN) {   // chunks across the rows' end
-            const int rest = min % C;
+            if (col() >= min) {
 #pragma unroll
-            for (int k = 0; k < kPer; ++k) {
-                if (col(k) >= min) r[k] = (U4)0;
-                else if (col(k) + C > min) r[k] = shift_down(r[k], (C - rest) * (int)sizeof(T) * 8);
+                for (int k = 0; k < kPer; ++k) r[k] = (U4)0;
+            } else if (col() + C > min) {
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) r[k] = shift_down(r[k], (C - min % C) * (int)sizeof(T) * 8);
             }
         }
         if (maj < MAJ) {
@@ -93,8 +100,7 @@ struct LnTile {
                 if (row(k) >= maj) r[k] = (U4)0;
         }
 #pragma unroll
-        for (int k = 0; k < kPer; ++k)
-            if (inside(k)) *reinterpret_cast<U4*>(lds + row(k) * PITCH + col(k)) = r[k];
+        for (int k = 0; k < kPer; ++k) *reinterpret_cast<U4*>(lds + row(k) * PITCH + col()) = r[k];
     }
     // The 128 bits shifted down by `bits` of 1 to 127, zeros from above.
     __device__ __forceinline__ static U4 shift_down(U4 v, int bits) {
@@ -161,11 +167,39 @@ struct LnVec {   // up to eight neighbouring elements of a row
     }
 };
 
+// GELU as relu(z) - |z| cdf(-|z|), the tail by the formula of act_value: no selections, and twelve operations
+// next to the exponential and the reciprocal instead of fifteen.
+__device__ __forceinline__ float ln_gelu(float z) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    const float e = __builtin_amdgcn_exp2f(z * (-0.5f * kLog2e) * z);
+    float a = __builtin_fmaf(0.5f * 1.061405429f, t, -0.5f * 1.453152027f);
+    a = __builtin_fmaf(a, t, 0.5f * 1.421413741f);
+    a = __builtin_fmaf(a, t, -0.5f * 0.284496736f);
+    a = __builtin_fmaf(a, t, 0.5f * 0.254829592f);
+    // (infinity has a tail of 0, and 0 of it; NaN is the tail's)
+    return __builtin_fmaf(-fminf(fabsf(z), 1e30f), a * t * e, fmaxf(z, 0.0f));
+}
+
+// Its derivative: with s = |z| pdf(z) - cdf(-|z|), 1 + s for positive z and -s otherwise.
+__device__ __forceinline__ float ln_gelu_slope(float z) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    const float e = __builtin_amdgcn_exp2f(z * (-0.5f * kLog2e) * z);
+    float a = __builtin_fmaf(0.5f * 1.061405429f, t, -0.5f * 1.453152027f);
+    a = __builtin_fmaf(a, t, 0.5f * 1.421413741f);
+    a = __builtin_fmaf(a, t, -0.5f * 0.284496736f);
+    a = __builtin_fmaf(a, t, 0.5f * 0.254829592f);
+    const float s = e * __builtin_fmaf(fminf(fabsf(z), 1e30f), 0.39894228040143268f, -(a * t));
+    return z > 0.0f ? 1.0f + s : -s;
+}
+
 template <int ACT>
 __device__ __forceinline__ void ln_act8(float (&v)[8]) {
     float none;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_value<ACT, false>(v[i], &none);
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (ACT == TDGS_ACT_GELU) v[i] = ln_gelu(v[i]);
+        else v[i] = act_value<ACT, false>(v[i], &none);
+    }
 }
 __device__ __forceinline__ void ln_activate(int act, float (&v)[8]) {
     switch (act) {
@@ -176,19 +210,12 @@ __device__ __forceinline__ void ln_activate(int act, float (&v)[8]) {
     }
 }
 
-// The end of n (1 to 8) neighbouring results q.. of row p.
+// The end of n (1 to 8) neighbouring results q.. of row p: bias holds those of the bias, or zeros.
 template <class T>
-__device__ __forceinline__ void ln_finish(const LnArgs& a, float scale, int64_t p, int q, int n, float (&v)[8]) {
-    if (a.scale) {
+__device__ __forceinline__ void ln_finish(const LnArgs& a, float scale, const float (&bias)[8], int64_t p, int q, int n,
+                                          float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= scale;
-    }
-    if (a.bias) {
-        float b[8];
-        LnVec<T>::load((const T*)a.bias + q, n, b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += b[i];
-    }
+    for (int i = 0; i < 8; ++i) v[i] = a.scale ? v[i] * scale : v[i] + bias[i];   // (never both)
     if (a.pre.p) LnVec<T>::store((T*)a.pre.p + p * a.pre.stride + q, n, v);
     ln_activate(a.act, v);
     if (a.residual.p) {
@@ -198,6 +225,12 @@ __device__ __forceinline__ void ln_finish(const LnArgs& a, float scale, int64_t 
         for (int i = 0; i < 8; ++i) v[i] += r[i];
     }
     LnVec<T>::store((T*)a.out.p + p * a.out.stride + q, n, v);
+}
+template <class T>
+__device__ __forceinline__ void ln_bias(const LnArgs& a, int q, int n, float (&bias)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+    if (a.bias && n > 0) LnVec<T>::load((const T*)a.bias + q, n, bias);
 }
 
 // A kernel's tile: BP x BQ of C by WP x WQ wavefronts, BK deep. AD, BD: whether the operands' depth is contiguous in
@@ -218,6 +251,52 @@ struct LnShape {
     static constexpr size_t kEnd = (size_t)WP * WQ * 32 * kTurn * sizeof(float);
     static constexpr size_t kLds = kStages > kEnd ? kStages : kEnd;
 };
+
+// The end of a wavefront's blocks, which start at (p0, q0).
+template <class S>
+__device__ __forceinline__ void ln_end(const LnArgs& a, const f32x16 (&acc)[S::NP][S::NQ], float* mem, int p0, int q0, int split) {
+    using T = typename S::T;
+    const int lane = (int)__lane_id();
+    // 32 rows at a time through the wavefront's own part of LDS
+    float* const turn = mem + (int)threadIdx.x / kWave * 32 * S::kTurn;
+    const float scale = a.scale ? *a.scale : 1.0f;
+    constexpr int kPerRow = S::NQ * 4;          // lanes of a row, with eight results each
+    constexpr int kRows = kWave / kPerRow;
+    const int x = lane % kPerRow * 8, q = q0 + x, n = min(8, a.Q - q);
+    float bias[8];
+    ln_bias<T>(a, q, n, bias);
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i) {
+#pragma unroll
+        for (int j = 0; j < S::NQ; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
+                *reinterpret_cast<f32x4*>(turn + (lane & 31) * S::kTurn + j * 32 + g * 8 + (lane >> 5) * 4) = v;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += kRows) {
+            const int y = r0 + lane / kPerRow, p = p0 + i * 32 + y;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(turn + y * S::kTurn + x);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(turn + y * S::kTurn + x + 4);
+            if (p >= a.P || n <= 0) continue;
+            if (a.part) {
+                f32x4* const o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.P + p) * a.part_q + q);
+                o[0] = lo;
+                o[1] = hi;
+            } else {
+                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                ln_finish<T>(a, scale, bias, p, q, n, v);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
 
 template <class S>
 __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
@@ -243,17 +322,26 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     LnTile<T, S::AMAJ, S::AMIN, S::TH, S::APITCH> ta;
     LnTile<T, S::BMAJ, S::BMIN, S::TH, S::BPITCH> tb;
     const int np = min(S::BP, a.P - p0), nq = min(S::BQ, a.Q - q0);
+    const int64_t step_a = S::AD ? S::BK : S::BK * a.a.stride, step_b = S::BD ? S::BK : S::BK * a.b.stride;
+    const T* pa = (const T*)a.a.p + (S::AD ? p0 * a.a.stride + r_begin : r_begin * a.a.stride + p0);
+    const T* pb = (const T*)a.b.p + (S::BD ? q0 * a.b.stride + r_begin : r_begin * a.b.stride + q0);
+    auto place = [&](int nr) {
+        ta.place(a.a.stride, S::AD ? np : nr, S::AD ? nr : np);
+        tb.place(a.b.stride, S::BD ? nq : nr, S::BD ? nr : nq);
+    };
+    // (in the order of the steps)
     auto load = [&](int step) {
-        const int r0 = r_begin + step * S::BK, nr = r_end - r0;
-        const T* const pa = (const T*)a.a.p + (S::AD ? p0 * a.a.stride + r0 : r0 * a.a.stride + p0);
-        const T* const pb = (const T*)a.b.p + (S::BD ? q0 * a.b.stride + r0 : r0 * a.b.stride + q0);
+        const int nr = r_end - r_begin - step * S::BK;
         if constexpr (S::NARROW) {
             ta.load_narrow(pa, a.a.stride, S::AD ? np : nr, S::AD ? nr : np);
             tb.load_narrow(pb, a.b.stride, S::BD ? nq : nr, S::BD ? nr : nq);
         } else {
-            ta.load(pa, a.a.stride, S::AD ? np : nr, S::AD ? nr : np);
-            tb.load(pb, a.b.stride, S::BD ? nq : nr, S::BD ? nr : nq);
+            if (nr < S::BK) place(nr);
+            ta.load(pa);
+            tb.load(pb);
         }
+        pa += step_a;
+        pb += step_b;
     };
     auto store = [&](int step) {
         const int nr = r_end - r_begin - step * S::BK;
@@ -261,6 +349,7 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
         ta.template store<S::NARROW>(at, S::AD ? np : nr, S::AD ? nr : np);
         tb.template store<S::NARROW>(at + S::kA, S::BD ? nq : nr, S::BD ? nr : nq);
     };
+    if constexpr (!S::NARROW) place(S::BK);
     if (steps > 0) {
         load(0);
         store(0);
@@ -287,65 +376,231 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     }
     __syncthreads();
 
-    // 32 rows at a time through the wavefront's own part of LDS
-    float* const turn = reinterpret_cast<float*>(s_mem) + wave * 32 * S::kTurn;
-    const float scale = a.scale ? *a.scale : 1.0f;
-    constexpr int kPerRow = S::NQ * 4;          // lanes of a row, with eight results each
-    constexpr int kRows = kWave / kPerRow;
+    ln_end<S>(a, acc, reinterpret_cast<float*>(s_mem), p0 + wp, q0 + wq, split);
+}
+
+// ---- the same with tiles that go from memory to LDS directly ------------------------------------
+
+// Rows of LDS are not padded then (a wavefront's 16 byte pieces arrive side by side); instead the pieces of a row change
+// places by an exclusive or with bits of the row, so that a read covers the banks once: 16 neighbouring rows where
+// the depth is contiguous, four rows x 64 bytes where the items are.
+template <bool DEPTH, int MIN>
+__device__ __forceinline__ int lf_key(int row) {
+    if constexpr (!DEPTH) return MIN == 64 ? (row & 2) << 1 : (row & 3) << 2;
+    else if constexpr (MIN == 32) return (row >> 2) & 3;
+    else return (row >> 1) & 7;
+}
+
+template <class T, bool DEPTH, int MAJ, int MIN, int TH>
+struct LfTile {
+    static constexpr int CR = MIN / 8;             // pieces of a row
+    static constexpr int kStep = TH / CR, kPer = MAJ / kStep;
+    static_assert(sizeof(T) == 2 && TH % CR == 0 && MAJ % kStep == 0, "whole rows of threads");
+    uint32_t offset[kPer];
+    __device__ __forceinline__ static int row(int k) { return (int)threadIdx.x / CR + k * kStep; }
+    __device__ __forceinline__ static int col(int k) { return (((int)threadIdx.x % CR) ^ lf_key<DEPTH, MIN>(row(k))) * 8; }
+    __device__ __forceinline__ void place(int64_t stride, int maj, int min) {
 #pragma unroll
-    for (int i = 0; i < S::NP; ++i) {
+        for (int k = 0; k < kPer; ++k)
+            offset[k] = (uint32_t)((row(k) < maj ? row(k) : maj - 1) * (int)(stride * 2) + (col(k) < min ? col(k) : min - 8) * 2);
+    }
+    // All of the tile to LDS, in flight.
+    __device__ __forceinline__ void start(const T* tile, uint32_t lds) const {
+        const uint32_t at = __builtin_amdgcn_readfirstlane(lds + (uint32_t)threadIdx.x / kWave * 1024);
 #pragma unroll
-        for (int j = 0; j < S::NQ; ++j)
+        for (int k = 0; k < kPer; ++k)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :: "s"(at + k * TH * 16), "v"(offset[k]), "s"(tile) : "memory", "m0");
+    }
+    // A tile whose depth ends in it, through registers.
+    __device__ __forceinline__ void tail(const T* tile, int64_t stride, T* lds, int maj, int min) const {
+        typedef T V8u __attribute__((ext_vector_type(8), aligned(16)));
+        typename Elem<T>::V8 r[kPer];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f32x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * g + e];
-                *reinterpret_cast<f32x4*>(turn + (lane & 31) * S::kTurn + j * 32 + g * 8 + (lane >> 5) * 4) = v;
-            }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += kRows) {
-            const int y = r0 + lane / kPerRow, x = lane % kPerRow * 8, p = p0 + wp + i * 32 + y, q = q0 + wq + x;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(turn + y * S::kTurn + x);
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(turn + y * S::kTurn + x + 4);
-            if (p >= a.P || q >= a.Q) continue;
-            if (a.part) {
-                f32x4* const o = reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.P + p) * a.part_q + q);
-                o[0] = lo;
-                o[1] = hi;
+        for (int k = 0; k < kPer; ++k) {
+            const int y = row(k) < maj ? row(k) : maj - 1;
+            const T* const p = tile + y * stride + col(k);
+            if (col(k) + 8 <= min || !DEPTH) {
+                r[k] = *reinterpret_cast<const V8u*>(tile + y * stride + (DEPTH || col(k) < min ? col(k) : min - 8));
             } else {
-                float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                ln_finish<T>(a, scale, p, q, min(8, a.Q - q), v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[k][i] = col(k) + i < min ? p[i] : (T)0.0f;
             }
         }
-        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            if (!DEPTH && row(k) >= maj) r[k] = zero8<T>();
+            *reinterpret_cast<typename Elem<T>::V8a*>(lds + (threadIdx.x + k * TH) * 8) = r[k];
+        }
+    }
+};
+
+// ln_operand of such a tile.
+template <class T, bool DEPTH, int MIN>
+__device__ __forceinline__ typename Elem<T>::V8 lf_operand(const T* lds, int base, int c) {
+    const int l = (int)__lane_id();
+    if constexpr (DEPTH) {
+        const int row = base + (l & 31);
+        return *reinterpret_cast<const typename Elem<T>::V8a*>(lds + row * MIN + ((c * 2 + (l >> 5)) ^ lf_key<true, MIN>(l & 31)) * 8);
+    } else {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        const int row = c * 16 + (l >> 5) * 8 + ((l & 15) >> 2), piece = base / 8 + ((l >> 4) & 1) * 2 + ((l & 3) >> 1);
+        const T* p = lds + row * MIN + (piece ^ lf_key<false, MIN>((l >> 2) & 3)) * 8 + (l & 1) * 4;
+        typedef __attribute__((address_space(3))) s4* lp;
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * MIN));
+        return __builtin_bit_cast(typename Elem<T>::V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 }
 
-// Joins the splits' sums, eight neighbouring results per thread.
-constexpr int kLnThreads = 256;
-template <class T>
-__global__ __launch_bounds__(kLnThreads) void k_linear_join(LnArgs a) {
-    const int chunks = a.part_q / 8;
-    const int64_t i = (int64_t)blockIdx.x * kLnThreads + threadIdx.x;
-    if (i >= (int64_t)a.P * chunks) return;
-    const int64_t p = i / chunks;
-    const int q = (int)(i - p * chunks) * 8;
-    const float scale = a.scale ? *a.scale : 1.0f;
-    float v[8] = {};
-    for (int s = 0; s < a.splits; ++s) {
-        const f32x4* const o = reinterpret_cast<const f32x4*>(a.part + ((int64_t)s * a.P + p) * a.part_q + q);
-        const f32x4 lo = o[0], hi = o[1];
+template <class T_, int BP_, int BQ_, int WP_, int WQ_, int BK_, int STAGES_, int PER_CU_, bool AD_, bool BD_>
+struct LfShape {
+    typedef T_ T;
+    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, BK = BK_, STAGES = STAGES_, PER_CU = PER_CU_;
+    static constexpr bool AD = AD_, BD = BD_;
+    static constexpr int TH = WP * WQ * kWave;
+    static constexpr int NP = BP / WP / 32, NQ = BQ / WQ / 32;
+    static constexpr int AMAJ = AD ? BP : BK, AMIN = AD ? BK : BP;
+    static constexpr int BMAJ = BD ? BQ : BK, BMIN = BD ? BK : BQ;
+    static constexpr int kA = BP * BK, kB = BQ * BK;
+    static constexpr int kTurn = BQ / WQ + 4;
+    static constexpr size_t kStages = STAGES * (size_t)(kA + kB) * sizeof(T);
+    static constexpr size_t kEnd = (size_t)WP * WQ * 32 * kTurn * sizeof(float);
+    static constexpr size_t kLds = kStages > kEnd ? kStages : kEnd;
+};
+
+template <int N>
+__device__ __forceinline__ void lf_wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+// All wavefronts have read what they read from LDS, and all loads waited for before are there.
+__device__ __forceinline__ void lf_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class S>
+__global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direct(LnArgs a) {
+    using T = typename S::T;
+    __shared__ __attribute__((aligned(1024))) char s_mem[S::kLds];
+    T* const s = reinterpret_cast<T*>(s_mem);
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem;
+    const int wave = (int)threadIdx.x / kWave;
+    const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
+    const int item = xcd_band_item(blockIdx.x, gridDim.x);
+    const int tiles = a.tiles_p * a.tiles_q, split = item / tiles, tile = item - split * tiles;
+    const int p0 = tile / a.tiles_q * S::BP, q0 = tile % a.tiles_q * S::BQ;
+    const int r_begin = split * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
+    const int steps = (r_end - r_begin) / S::BK, rest = (r_end - r_begin) % S::BK;
+
+    f32x16 acc[S::NP][S::NQ];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] += lo[e];
-            v[e + 4] += hi[e];
+    for (int i = 0; i < S::NP; ++i)
+#pragma unroll
+        for (int j = 0; j < S::NQ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    LfTile<T, S::AD, S::AMAJ, S::AMIN, S::TH> ta;
+    LfTile<T, S::BD, S::BMAJ, S::BMIN, S::TH> tb;
+    const int np = min(S::BP, a.P - p0), nq = min(S::BQ, a.Q - q0);
+    const int64_t step_a = S::AD ? S::BK : S::BK * a.a.stride, step_b = S::BD ? S::BK : S::BK * a.b.stride;
+    const T* pa = (const T*)a.a.p + (S::AD ? p0 * a.a.stride + r_begin : r_begin * a.a.stride + p0);
+    const T* pb = (const T*)a.b.p + (S::BD ? q0 * a.b.stride + r_begin : r_begin * a.b.stride + q0);
+    ta.place(a.a.stride, S::AD ? np : S::BK, S::AD ? S::BK : np);
+    tb.place(a.b.stride, S::BD ? nq : S::BK, S::BD ? S::BK : nq);
+    constexpr int kStage = S::kA + S::kB, kLoads = decltype(ta)::kPer + decltype(tb)::kPer;
+    auto start = [&](int stage) {
+        const uint32_t at = lds + stage * kStage * (int)sizeof(T);
+        ta.start(pa, at);
+        tb.start(pb, at + S::kA * (int)sizeof(T));
+        pa += step_a;
+        pb += step_b;
+    };
+    auto multiply = [&](int stage) {
+        const T* const la = s + stage * kStage;
+        const T* const lb = la + S::kA;
+        constexpr int NC = S::BK / 16;
+        typename Elem<T>::V8 fa[2][S::NP], fb[2][S::NQ];
+        auto fetch = [&](int c) {
+#pragma unroll
+            for (int i = 0; i < S::NP; ++i) fa[c & 1][i] = lf_operand<T, S::AD, S::AMIN>(la, wp + i * 32, c);
+#pragma unroll
+            for (int j = 0; j < S::NQ; ++j) fb[c & 1][j] = lf_operand<T, S::BD, S::BMIN>(lb, wq + j * 32, c);
+        };
+        fetch(0);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (c + 1 < NC) fetch(c + 1);
+#pragma unroll
+            for (int i = 0; i < S::NP; ++i)
+#pragma unroll
+                for (int j = 0; j < S::NQ; ++j) acc[i][j] = mma(fb[c & 1][j], fa[c & 1][i], acc[i][j]);
         }
+        constexpr int kReads = S::NP * (S::AD ? 1 : 2) + S::NQ * (S::BD ? 1 : 2), kProducts = S::NP * S::NQ;
+#ifndef LN_NOSCHED
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+#pragma unroll
+        for (int c = 0; c + 1 < NC; ++c) {
+#pragma unroll
+            for (int m = 0; m < kProducts; ++m) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if ((m + 1) * kReads / kProducts > m * kReads / kProducts)
+                    __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kProducts - 1) / kProducts, 0);
+            }
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+#endif
+    };
+#pragma unroll
+    for (int n = 0; n < S::STAGES - 1; ++n)
+        if (n < steps) start(n);
+    int stage = 0, next = S::STAGES - 1;
+    const int all = steps + (rest > 0);
+    for (int step = 0; step < all; ++step) {
+        if (step + S::STAGES - 2 < steps) lf_wait_loads<(S::STAGES - 2) * kLoads>();
+        else lf_wait_loads<0>();
+        lf_barrier();
+        if (step + S::STAGES - 1 < steps) start(next);
+        if (step == steps) {   // the depth's end
+            ta.tail(pa, a.a.stride, s + stage * kStage, S::AD ? np : rest, S::AD ? rest : np);
+            tb.tail(pb, a.b.stride, s + stage * kStage + S::kA, S::BD ? nq : rest, S::BD ? rest : nq);
+            lf_barrier();
+        }
+        multiply(stage);
+        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        next = next + 1 == S::STAGES ? 0 : next + 1;
     }
-    ln_finish<T>(a, scale, p, q, min(8, a.Q - q), v);
+    lf_barrier();
+    ln_end<S>(a, acc, reinterpret_cast<float*>(s_mem), p0 + wp, q0 + wq, split);
+}
+
+// Joins the splits' sums, eight neighbouring results by G threads, each of which takes every G-th split.
+constexpr int kLnThreads = 256;
+template <class T, int G>
+__global__ __launch_bounds__(kLnThreads) void k_linear_join(LnArgs a) {
+    constexpr int N = kLnThreads / G;
+    __shared__ f32x8 s[G > 1 ? G : 1][G > 1 ? N : 1];
+    const int chunks = a.part_q / 8, x = (int)threadIdx.x % N, y = (int)threadIdx.x / N;
+    const int64_t i = (int64_t)blockIdx.x * N + x, all = (int64_t)a.P * chunks;
+    const int64_t p = (i < all ? i : all - 1) / chunks;
+    const int q = (int)((i < all ? i : all - 1) - p * chunks) * 8;
+    f32x8 sum = {};
+    for (int k = y; k < a.splits; k += G) sum += *reinterpret_cast<const f32x8*>(a.part + ((int64_t)k * a.P + p) * a.part_q + q);
+    if constexpr (G > 1) {
+        s[y][x] = sum;
+        __syncthreads();
+        if (y != 0) return;
+#pragma unroll 4
+        for (int g = 1; g < G; ++g) sum += s[g][x];
+    }
+    if (i >= all) return;
+    float v[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = sum[e];
+    const int n = min(8, a.Q - q);
+    ln_bias<T>(a, q, n, bias);
+    ln_finish<T>(a, a.scale ? *a.scale : 1.0f, bias, p, q, n, v);
 }
 
 // ---- the gradient's elementwise part: dz = dout act'(z), and its columns' sums ------------------
@@ -353,8 +608,7 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_join(LnArgs a) {
 struct LnGradArgs {
     LnMatrix dout, pre, dz;     // dz null: not wanted
     int64_t rows;
-    int32_t n, act, blocks;
-    int64_t per;                // rows per workgroup
+    int32_t n, act, blocks, shift;
     float* sums;                // blocks x n; null: not wanted
     const float* top;           // float16: partial maxima of |dout|; null: dz is not scaled
     int32_t tops;
@@ -393,56 +647,70 @@ __device__ __forceinline__ float ln_range(float m) {
     return __builtin_bit_cast(float, (uint32_t)(14 - e + 127) << 23);
 }
 
-// Workgroup (x, y): 64 chunks of eight columns by four rows at a time, of the y-th run of rows.
+// Workgroup (x, y): 2^shift chunks of eight columns by 256 >> shift rows at a time, the workgroups' rows in turn: all of
+// them together go through memory from front to back (64800 x 2048 bfloat16 with GELU, 796 MB: 155 us, 5.1 TB/s; with a run of
+// rows for each 203). With the sums of the columns, if wanted, before dz is rounded.
 template <class T, int ACT>
 __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
-    __shared__ float s[kLnThreads / kWave][kWave * 8];
-    const int lane = (int)__lane_id(), wave = (int)threadIdx.x / kWave, q = ((int)blockIdx.x * kWave + lane) * 8;
+    __shared__ float s[kLnThreads * 8];
+    const int t = (int)threadIdx.x, across = 1 << a.shift, down = kLnThreads >> a.shift;
+    const int q = ((int)blockIdx.x * across + (t & (across - 1))) * 8, y = t >> a.shift;
     float up = 1.0f;
     if (a.top) {
-        float m = a.top[threadIdx.x % a.tops];
+        float m = a.top[t % a.tops];
         for (int w = kWave / 2; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, kWave));
-        if (lane == 0) s[wave][0] = m;
+        s[t] = m;
         __syncthreads();
-        for (int w = 0; w < kLnThreads / kWave; ++w) m = fmaxf(m, s[w][0]);
+        for (int w = 0; w < kLnThreads; w += kWave) m = fmaxf(m, s[w]);
         __syncthreads();
         up = ln_range(m);
-        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.scale = 1.0f / up;
+        if (blockIdx.x == 0 && blockIdx.y == 0 && t == 0) *a.scale = 1.0f / up;
     }
     const int n = a.n - q;
     float sum[8] = {};
     if (n > 0) {
-        const int64_t end = min(a.rows, (blockIdx.y + (int64_t)1) * a.per);
-        for (int64_t r = blockIdx.y * a.per + wave; r < end; r += kLnThreads / kWave) {
-            float d[8];
-            LnVec<T>::load((const T*)a.dout.p + r * a.dout.stride + q, n, d);
-            if constexpr (ACT != TDGS_ACT_IDENTITY) {
-                float z[8], slope;
-                LnVec<T>::load((const T*)a.pre.p + r * a.pre.stride + q, n, z);
+        auto rows = [&](int64_t r, auto count) {   // this row and, `down` rows apart, those after it
+            constexpr int U = decltype(count)::value;
+            float d[U][8], z[U][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    act_value<ACT, true>(z[i], &slope);
-                    d[i] *= slope;
-                }
+            for (int u = 0; u < U; ++u) {
+                LnVec<T>::load((const T*)a.dout.p + (r + u * down) * a.dout.stride + q, n, d[u]);
+                if constexpr (ACT != TDGS_ACT_IDENTITY) LnVec<T>::load((const T*)a.pre.p + (r + u * down) * a.pre.stride + q, n, z[u]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += d[i];
-            if (a.dz.p) {
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] *= up;
-                LnVec<T>::store((T*)a.dz.p + r * a.dz.stride + q, n, d);
+                for (int i = 0; i < 8; ++i) {
+                    float slope = 1.0f;
+                    if constexpr (ACT == TDGS_ACT_GELU) slope = ln_gelu_slope(z[u][i]);
+                    else if constexpr (ACT != TDGS_ACT_IDENTITY) act_value<ACT, true>(z[u][i], &slope);
+                    d[u][i] *= slope;
+                    sum[i] += d[u][i];
+                    if constexpr (std::is_same<T, f16>::value) d[u][i] *= up;
+                }
+                if (a.dz.p) LnVec<T>::store((T*)a.dz.p + (r + u * down) * a.dz.stride + q, n, d[u]);
+            }
+        };
+        constexpr int U = 2;
+        const int64_t step = (int64_t)gridDim.y * U * down;
+        for (int64_t r = (int64_t)blockIdx.y * U * down + y; r < a.rows; r += step) {
+            if (r + (U - 1) * down < a.rows) {
+                rows(r, std::integral_constant<int, U>{});
+            } else {
+                for (int u = 0; u < U; ++u)
+                    if (r + u * down < a.rows) rows(r + u * down, std::integral_constant<int, 1>{});
             }
         }
     }
     if (!a.sums) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[wave][lane * 8 + i] = sum[i];
+    for (int i = 0; i < 8; ++i) s[t * 8 + i] = sum[i];
     __syncthreads();
-    for (int c = threadIdx.x; c < kWave * 8; c += kLnThreads) {
-        const int col = (int)blockIdx.x * kWave * 8 + c;
+    for (int c = t; c < across * 8; c += kLnThreads) {
+        const int col = (int)blockIdx.x * across * 8 + c;
         if (col >= a.n) break;
         float x = 0.0f;
-        for (int w = 0; w < kLnThreads / kWave; ++w) x += s[w][c];
+        for (int w = 0; w < down; ++w) x += s[w * across * 8 + c];
         a.sums[(int64_t)blockIdx.y * a.n + col] = x;
     }
 }
@@ -454,8 +722,10 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dbias(const float* __rest
     __shared__ float s[kLnThreads / kLnBiasCols][kLnBiasCols + 1];
     const int x = (int)threadIdx.x % kLnBiasCols, y = (int)threadIdx.x / kLnBiasCols, c = blockIdx.x * kLnBiasCols + x;
     float v = 0.0f;
-    if (c < n)
+    if (c < n) {
+#pragma unroll 8
         for (int b = y; b < blocks; b += kLnThreads / kLnBiasCols) v += sums[(int64_t)b * n + c];
+    }
     s[y][x] = v;
     __syncthreads();
     if (y != 0 || c >= n) return;
@@ -472,41 +742,83 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_zero(T* p, int64_t rows, 
 
 // ---- host ----------------------------------------------------------------------------------
 
-// Workgroups that fill the card, and the least depth (in steps) of a split.
-constexpr int64_t kLnWorkgroups = 512;
-constexpr int kLnLeastSteps = 8;
-
+// The forms of a product: tile, depth of a step, workgroups per CU, and what they take by measurement, in us: a
+// workgroup's start and end, a step of one alone on its CU, and a step's share where the CU is full. (256x256: 1.93 us a
+// step is 1110 TFLOP/s.)
+struct LnForm {
+    int bp, bq, bk, per_cu;
+    float ends, alone, full;
+};
+enum { kLnStaged64, kLnStaged128, kLnDirect64, kLnDirect128x64, kLnDirect128, kLnDirect256, kLnForms };
 template <class T>
 constexpr int ln_depth() { return sizeof(T) == 4 ? 16 : 32; }
+constexpr LnForm kLnF32[2] = {{64, 64, ln_depth<float>(), 8, 3.0f, 0.5f, 0.3f}, {128, 128, ln_depth<float>(), 3, 5.0f, 1.3f, 1.2f}};
+constexpr LnForm kLn16[kLnForms] = {{64, 64, ln_depth<bf16>(), 6, 3.0f, 0.5f, 0.25f}, {128, 128, ln_depth<bf16>(), 3, 5.0f, 0.8f, 0.42f},
+                                    {64, 64, 64, 4, 3.0f, 0.46f, 0.206f},  {128, 64, 64, 3, 4.0f, 0.6f, 0.34f},
+                                    {128, 128, 64, 2, 5.0f, 0.85f, 0.59f}, {256, 256, 64, 1, 8.0f, 1.93f, 1.93f}};
+constexpr int kLnCus = 256;
+constexpr int kLnLeastSteps = 4;   // of a split
 
 // How a product is cut.
 struct LnPlan {
-    bool large;        // 128 x 128 tiles, 64 x 64 otherwise
-    int tiles_p, tiles_q, splits, steps, part_q;
+    int form, tiles_p, tiles_q, splits, steps, part_q;
     size_t bytes;
 };
 
-static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R) {
-    LnPlan p;
-    const int depth = dtype == TDGS_F32 ? ln_depth<float>() : ln_depth<bf16>();
-    p.large = ceil_div(P, 128) * ceil_div(Q, 128) >= 256 || (P > 64 && Q > 64 && R >= 4096);
-    const int side = p.large ? 128 : 64;
-    p.tiles_p = (int)ceil_div(P, side);
-    p.tiles_q = (int)ceil_div(Q, side);
-    const int64_t tiles = (int64_t)p.tiles_p * p.tiles_q, steps = ceil_div(R, depth);
-    int64_t splits = tiles > 0 ? kLnWorkgroups / tiles : 1;
-    if (splits > steps / kLnLeastSteps) splits = steps / kLnLeastSteps;
-    if (splits < 1) splits = 1;
-    p.steps = (int)ceil_div(steps, splits);
-    p.splits = (int)(p.steps > 0 ? ceil_div(steps, p.steps) : 1);
-    p.part_q = (int)(ceil_div(Q, 8) * 8);
-    p.bytes = p.splits > 1 ? align_up((size_t)p.splits * P * p.part_q * sizeof(float)) : 0;
-    return p;
+// The form and the splits that take the least time: rounds of the workgroups of the fullest CU, and the join, which
+// reads at 6 TB/s what the splits have left in the last-level cache.
+static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direct) {
+    if (P < 1 || Q < 1 || R < 1) return {};
+    const bool f32 = dtype == TDGS_F32;
+    const int chunk = f32 ? 4 : 8;
+    const bool narrow = P < chunk || Q < chunk || R < chunk;
+    const bool pieces = direct && !f32 && !narrow;
+    const int first = pieces ? kLnDirect64 : kLnStaged64;
+    const int last = narrow ? kLnStaged64 : pieces ? kLnDirect256 : kLnStaged128;
+    LnPlan best = {};
+    float least = INFINITY;
+    for (int form = first; form <= last; ++form) {
+        const LnForm& f = f32 ? kLnF32[form] : kLn16[form];
+        const int64_t tiles = ceil_div(P, f.bp) * ceil_div(Q, f.bq), steps = ceil_div(R, f.bk);
+        for (int fill = 0; fill <= f.per_cu; ++fill) {   // one split, or as many as put `fill` workgroups on each CU
+            int64_t splits = fill ? (int64_t)fill * kLnCus / tiles : 1;
+            if (splits > steps / kLnLeastSteps) splits = steps / kLnLeastSteps;
+            if (splits < 1 || (fill && splits == 1)) {
+                if (fill) continue;
+                splits = 1;
+            }
+            const int64_t per = ceil_div(steps, splits);
+            splits = ceil_div(steps, per);
+            const int64_t on = ceil_div(tiles * splits, kLnCus), together = on < f.per_cu ? on : f.per_cu;
+            const float step = f.full * together > f.alone ? f.full * together : f.alone;
+            float time = (float)ceil_div(on, f.per_cu) * (f.ends + per * step);
+            if (splits > 1) time += 3.0f + (float)splits * P * Q * 4.0f / 6e6f;
+            if (time < least) {
+                least = time;
+                best.form = form;
+                best.tiles_p = (int)ceil_div(P, f.bp);
+                best.tiles_q = (int)ceil_div(Q, f.bq);
+                best.splits = (int)splits;
+                best.steps = (int)per;
+            }
+        }
+    }
+    best.part_q = (int)(ceil_div(Q, 8) * 8);
+    best.bytes = best.splits > 1 ? align_up((size_t)best.splits * P * best.part_q * sizeof(float)) : 0;
+    return best;
+}
+
+// Whether an operand's tiles can go to LDS directly: 16 byte pieces on their boundaries, whole where the items are contiguous.
+static bool ln_aligned(const LnMatrix& m, bool depth, int64_t items) {
+    return aligned_to(m.p, 16) && m.stride % 8 == 0 && m.stride < (1 << 21) && (depth || items % 8 == 0);
 }
 
 // C = A B, with what follows it in `r`.
 template <class T, bool AD, bool BD>
-static int ln_product(LnArgs r, const LnPlan& p, void* temp, hipStream_t stream) {
+static int ln_product(LnArgs r, void* temp, hipStream_t stream) {
+    const int32_t dtype = sizeof(T) == 4 ? TDGS_F32 : std::is_same<T, bf16>::value ? TDGS_BF16 : TDGS_F16;
+    const bool aligned = sizeof(T) == 2 && ln_aligned(r.a, AD, r.P) && ln_aligned(r.b, BD, r.Q);
+    const LnPlan p = ln_plan(dtype, r.P, r.Q, r.R, aligned);
     r.tiles_p = p.tiles_p;
     r.tiles_q = p.tiles_q;
     r.splits = p.splits;
@@ -516,18 +828,33 @@ static int ln_product(LnArgs r, const LnPlan& p, void* temp, hipStream_t stream)
     const int64_t grid = (int64_t)p.tiles_p * p.tiles_q * p.splits;
     TDGS_REQUIRE(grid <= INT32_MAX, "linear: too many tiles");
     constexpr int C = ln_chunk<T>(), D = ln_depth<T>();
-    const bool narrow = (AD ? r.R : r.P) < C || (BD ? r.R : r.Q) < C;
-    auto launch = [&](auto shape) {
+    auto staged = [&](auto shape) {
         using S = decltype(shape);
         k_linear<S><<<(unsigned)grid, S::TH, 0, stream>>>(r);
     };
-    if (p.large && !narrow) launch(LnShape<T, 128, 128, 2, 2, D, AD, BD, false>{});
-    else if (p.large) launch(LnShape<T, 128, 128, 2, 2, D, AD, BD, true>{});
-    else if (!narrow) launch(LnShape<T, 64, 64, 2, 2, D, AD, BD, false>{});
-    else launch(LnShape<T, 64, 64, 2, 2, D, AD, BD, true>{});
+    auto direct = [&](auto shape) {
+        using S = decltype(shape);
+        k_linear_direct<S><<<(unsigned)grid, S::TH, 0, stream>>>(r);
+    };
+    if ((AD ? r.R : r.P) < C || (BD ? r.R : r.Q) < C) staged(LnShape<T, 64, 64, 2, 2, D, AD, BD, true>{});
+    else if (p.form == kLnStaged64) staged(LnShape<T, 64, 64, 2, 2, D, AD, BD, false>{});
+    else if (p.form == kLnStaged128) staged(LnShape<T, 128, 128, 2, 2, D, AD, BD, false>{});
+    if constexpr (sizeof(T) == 2) {
+        if (p.form == kLnDirect64) direct(LfShape<T, 64, 64, 2, 2, 64, 2, 4, AD, BD>{});
+        else if (p.form == kLnDirect128x64) direct(LfShape<T, 128, 64, 2, 2, 64, 2, 3, AD, BD>{});
+        else if (p.form == kLnDirect128) direct(LfShape<T, 128, 128, 2, 2, 64, 2, 2, AD, BD>{});
+        else if (p.form == kLnDirect256) direct(LfShape<T, 256, 256, 2, 4, 64, 2, 1, AD, BD>{});
+    }
     TDGS_LAUNCHED();
     if (p.splits > 1) {
-        k_linear_join<T><<<(unsigned)ceil_div((int64_t)r.P * (p.part_q / 8), kLnThreads), kLnThreads, 0, stream>>>(r);
+        const int64_t chunks = (int64_t)r.P * (p.part_q / 8);
+        auto join = [&](auto g) {
+            constexpr int G = decltype(g)::value;
+            k_linear_join<T, G><<<(unsigned)ceil_div(chunks, kLnThreads / G), kLnThreads, 0, stream>>>(r);
+        };
+        if (p.splits < 8) join(std::integral_constant<int, 1>{});
+        else if (p.splits < 64) join(std::integral_constant<int, 4>{});
+        else join(std::integral_constant<int, 32>{});
         TDGS_LAUNCHED();
     }
     return TDGS_OK;
@@ -565,30 +892,36 @@ static LnMatrix ln_matrix(const tdgs_rows& v) { return {v.data, v.stride}; }
 
 // The gradient's scratch: dz, its power of two, maxima and columns' sums, then a product's partial sums.
 struct LnGradPlan {
-    LnPlan dx, dw;
-    int64_t dz_stride, per;
-    int blocks;
+    int64_t dz_stride;
+    int blocks, shift;
     size_t dz, small, sums, part, bytes;
 };
+
+// Scratch of a product, whatever its operands' alignment.
+static size_t ln_part_bytes(int32_t dtype, int64_t P, int64_t Q, int64_t R) {
+    const size_t a = ln_plan(dtype, P, Q, R, false).bytes, b = ln_plan(dtype, P, Q, R, true).bytes;
+    return a > b ? a : b;
+}
 
 static LnGradPlan ln_grad_plan(const tdgs_linear* a) {
     LnGradPlan g;
     const bool slope = a->activation != TDGS_ACT_IDENTITY;
-    g.dx = ln_plan(a->dtype, a->rows, a->in_features, a->out_features);
-    // (the weight's gradient or its transpose, whichever is asked for: the larger of both is kept room for)
-    g.dw = ln_plan(a->dtype, a->in_features, a->out_features, a->rows);
-    const LnPlan t = ln_plan(a->dtype, a->out_features, a->in_features, a->rows);
     g.dz_stride = ceil_div(a->out_features, 8) * 8;
     g.dz = slope ? align_up((size_t)a->rows * g.dz_stride * dtype_size(a->dtype)) : 0;
     g.small = align_up((kLnTops + 1) * sizeof(float));
-    const int64_t across = ceil_div(a->out_features, kWave * 8);
-    int64_t blocks = ceil_div(2048, across);
-    if (blocks > ceil_div(a->rows, 16)) blocks = ceil_div(a->rows, 16);
-    g.per = ceil_div(a->rows, blocks > 0 ? blocks : 1);
-    g.blocks = (int)(g.per > 0 ? ceil_div(a->rows, g.per) : 0);
+    g.shift = 0;
+    while (g.shift < 6 && (8 << g.shift) < a->out_features) ++g.shift;
+    const int64_t down = kLnThreads >> g.shift;
+    int64_t blocks = ceil_div(1024, ceil_div(a->out_features, 8 << g.shift));
+    if (blocks > ceil_div(a->rows, 2 * down)) blocks = ceil_div(a->rows, 2 * down);
+    g.blocks = (int)blocks;
     g.sums = align_up((size_t)g.blocks * a->out_features * sizeof(float));
-    g.part = g.dx.bytes > g.dw.bytes ? g.dx.bytes : g.dw.bytes;
-    if (t.bytes > g.part) g.part = t.bytes;
+    // (the weight's gradient or its transpose, whichever is asked for)
+    g.part = ln_part_bytes(a->dtype, a->rows, a->in_features, a->out_features);
+    const size_t dw = ln_part_bytes(a->dtype, a->in_features, a->out_features, a->rows);
+    const size_t t = ln_part_bytes(a->dtype, a->out_features, a->in_features, a->rows);
+    if (dw > g.part) g.part = dw;
+    if (t > g.part) g.part = t;
     g.bytes = g.dz + g.small + g.sums + g.part;
     return g;
 }
@@ -601,7 +934,7 @@ extern "C" {
 
 size_t tdgs_linear_temp_bytes(const tdgs_linear* a, int32_t grad) {
     if (ln_check(a) != TDGS_OK) return 0;
-    size_t bytes = ln_plan(a->dtype, a->rows, a->out_features, a->in_features).bytes;
+    size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features);
     if (grad) {
         const size_t g = ln_grad_plan(a).bytes;
         if (g > bytes) bytes = g;
@@ -618,9 +951,9 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     if (a->residual.data) TDGS_TRY(ln_check_rows(a->residual, "residual", a->dtype, a->rows, a->out_features, false));
     if (a->pre.data) TDGS_TRY(ln_check_rows(a->pre, "pre", a->dtype, a->rows, a->out_features, true));
     TDGS_REQUIRE(aligned_to(a->bias, (size_t)dtype_size(a->dtype)), "linear: bias is not aligned to its element type");
-    const LnPlan p = ln_plan(a->dtype, a->rows, a->out_features, a->in_features);
-    TDGS_REQUIRE(p.bytes == 0 || (a->temp && a->temp_bytes >= p.bytes && aligned_to(a->temp, 16)),
-                 "linear: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, p.bytes);
+    const size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features);
+    TDGS_REQUIRE(bytes == 0 || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
+                 "linear: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, bytes);
     LnArgs r = {};
     r.a = ln_matrix(a->x);
     r.b = ln_matrix(a->weight);
@@ -635,8 +968,8 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     hipStream_t stream = (hipStream_t)stream_;
     return with_dtype(a->dtype, [&](auto t) -> int {
         using T = decltype(t);
-        return a->weight_layout == TDGS_WEIGHT_IN_OUT ? ln_product<T, true, false>(r, p, a->temp, stream)
-                                                      : ln_product<T, true, true>(r, p, a->temp, stream);
+        return a->weight_layout == TDGS_WEIGHT_IN_OUT ? ln_product<T, true, false>(r, a->temp, stream)
+                                                      : ln_product<T, true, true>(r, a->temp, stream);
     });
 }
 
@@ -696,7 +1029,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     e.n = a->out_features;
     e.act = a->activation;
     e.blocks = p.blocks;
-    e.per = p.per;
+    e.shift = p.shift;
     // float16 and a slope: the products of both may pass the type's range, or leave it with few bits
     const bool ranged = slope && a->activation != TDGS_ACT_RELU && a->dtype == TDGS_F16;
     LnArgs r = {};
@@ -714,7 +1047,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             TDGS_LAUNCHED();
         }
         if (slope || want_db) {
-            const dim3 grid((unsigned)ceil_div(a->out_features, kWave * 8), (unsigned)p.blocks);
+            const dim3 grid((unsigned)ceil_div(a->out_features, 8 << p.shift), (unsigned)p.blocks);
             switch (a->activation) {
                 case TDGS_ACT_IDENTITY: k_linear_dz<T, TDGS_ACT_IDENTITY><<<grid, kLnThreads, 0, stream>>>(e); break;
                 case TDGS_ACT_SILU: k_linear_dz<T, TDGS_ACT_SILU><<<grid, kLnThreads, 0, stream>>>(e); break;
@@ -735,8 +1068,8 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             x.Q = a->in_features;
             x.R = a->out_features;
             x.out = ln_matrix(g->dx);
-            if (a->weight_layout == TDGS_WEIGHT_IN_OUT) TDGS_TRY((ln_product<T, true, true>(x, p.dx, part, stream)));
-            else TDGS_TRY((ln_product<T, true, false>(x, p.dx, part, stream)));
+            if (a->weight_layout == TDGS_WEIGHT_IN_OUT) TDGS_TRY((ln_product<T, true, true>(x, part, stream)));
+            else TDGS_TRY((ln_product<T, true, false>(x, part, stream)));
         }
         if (want_dw) {
             LnArgs w = r;   // dW = x^T dz, or its transpose dz^T x
@@ -746,8 +1079,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             w.Q = dw_in_out ? a->out_features : a->in_features;
             w.b = dw_in_out ? r.a : ln_matrix(a->x);
             w.a = dw_in_out ? ln_matrix(a->x) : r.a;
-            const LnPlan dw = ln_plan(a->dtype, w.P, w.Q, w.R);
-            TDGS_TRY((ln_product<T, false, false>(w, dw, part, stream)));
+            TDGS_TRY((ln_product<T, false, false>(w, part, stream)));
         }
         return TDGS_OK;
     });
