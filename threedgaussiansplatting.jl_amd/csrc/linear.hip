@@ -603,6 +603,134 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_join(LnArgs a) {
     ln_finish<T>(a, a.scale ? *a.scale : 1.0f, bias, p, q, n, v);
 }
 
+// ---- few rows: the weight is read once, by vectors, in one launch ----------------------------
+
+// Up to eight rows (four of 16-bit types) fill a fraction of a tile of the matrix cores, and what counts is how soon and how fast the weight comes
+// from memory: every thread loads 16 bytes of it at a time, several in flight, and multiplies them by the rows' elements in
+// 32 bits. The depth is shared out over a workgroup's threads and joined by exchanges and in LDS.
+constexpr int kLsThreads = 512, kLsRows = 8;
+
+template <class T>
+struct LsChunk {   // 16 bytes
+    static constexpr int C = ln_chunk<T>();
+    typedef T Va __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    float f[C];
+    __device__ __forceinline__ void load(const T* p, int n) {   // n of them exist
+        if (n >= C) {
+            const Va v = *reinterpret_cast<const Va*>(p);
+#pragma unroll
+            for (int i = 0; i < C; ++i) f[i] = (float)v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) f[i] = i < n ? (float)p[i] : 0.0f;
+        }
+    }
+};
+
+// Items contiguous: a workgroup takes four chunks of columns, whose lanes are neighbours, and a thread every 128th depth.
+template <class T, int ROWS>
+__global__ __launch_bounds__(kLsThreads) void k_linear_few_items(LnArgs a) {
+    constexpr int C = ln_chunk<T>(), W = kLsThreads / kWave, U = 4;
+    __shared__ float s[W][4][ROWS * C];
+    const int t = (int)threadIdx.x, chunk = t & 3, q = ((int)blockIdx.x * 4 + chunk) * C, n = a.Q - q;
+    float sum[ROWS][C] = {};
+    if (n > 0) {
+        const T* const b = (const T*)a.b.p + q;
+        const T* const x = (const T*)a.a.p;
+        for (int r0 = t >> 2; r0 < a.R; r0 += U * (kLsThreads / 4)) {
+            LsChunk<T> w[U];
+            float e[U][ROWS];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * (kLsThreads / 4), at = r < a.R ? r : a.R - 1;
+                w[u].load(b + at * a.b.stride, n);
+#pragma unroll
+                for (int p = 0; p < ROWS; ++p) e[u][p] = (float)x[(p < a.P ? p : 0) * a.a.stride + at];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r0 + u * (kLsThreads / 4) >= a.R) break;
+#pragma unroll
+                for (int p = 0; p < ROWS; ++p)
+#pragma unroll
+                    for (int i = 0; i < C; ++i) sum[p][i] = __builtin_fmaf(e[u][p], w[u].f[i], sum[p][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < ROWS; ++p)
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            float v = sum[p][i];
+            for (int m = kWave / 2; m >= 4; m >>= 1) v += __shfl_xor(v, m, kWave);
+            if (__lane_id() < 4) s[t / kWave][chunk][p * C + i] = v;
+        }
+    __syncthreads();
+    // eight results to a thread
+    constexpr int N = 4 * C / 8;
+    for (int i = t; i < N * ROWS; i += kLsThreads) {
+        const int p = i / N, c = i % N * 8, col = (int)blockIdx.x * 4 * C + c;
+        if (p >= a.P || col >= a.Q) continue;
+        float v[8], bias[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = 0.0f;
+            for (int w = 0; w < W; ++w) v[k] += s[w][(c + k) / C][p * C + (c + k) % C];
+        }
+        const int left = min(8, a.Q - col);
+        ln_bias<T>(a, col, left, bias);
+        ln_finish<T>(a, a.scale ? *a.scale : 1.0f, bias, p, col, left, v);
+    }
+}
+
+// Depth contiguous: a wavefront takes two columns, and a lane every 64th chunk of them.
+template <class T, int ROWS>
+__global__ __launch_bounds__(kLsThreads) void k_linear_few_depth(LnArgs a) {
+    constexpr int C = ln_chunk<T>(), W = kLsThreads / kWave, COLS = 2, U = 2;
+    __shared__ float s[W * COLS][ROWS];
+    const int t = (int)threadIdx.x, lane = (int)__lane_id(), q0 = ((int)blockIdx.x * W + t / kWave) * COLS;
+    float sum[COLS][ROWS] = {};
+    for (int r0 = lane * C; r0 < a.R; r0 += U * kWave * C) {
+        LsChunk<T> w[U][COLS], x[U][ROWS];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = r0 + u * kWave * C, left = a.R - r, at = left > 0 ? r : 0;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) w[u][c].load((const T*)a.b.p + (q0 + c < a.Q ? q0 + c : a.Q - 1) * a.b.stride + at, left);
+#pragma unroll
+            for (int p = 0; p < ROWS; ++p) x[u][p].load((const T*)a.a.p + (p < a.P ? p : 0) * a.a.stride + at, left);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int p = 0; p < ROWS; ++p)
+#pragma unroll
+                    for (int i = 0; i < C; ++i) sum[c][p] = __builtin_fmaf(x[u][p].f[i], w[u][c].f[i], sum[c][p]);
+    }
+#pragma unroll
+    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int p = 0; p < ROWS; ++p) {
+            float v = sum[c][p];
+            for (int m = kWave / 2; m > 0; m >>= 1) v += __shfl_xor(v, m, kWave);
+            if (lane == 0) s[t / kWave * COLS + c][p] = v;
+        }
+    __syncthreads();
+    constexpr int N = W * COLS / 8;
+    for (int i = t; i < N * ROWS; i += kLsThreads) {
+        const int p = i / N, c = i % N * 8, col = (int)blockIdx.x * W * COLS + c;
+        if (p >= a.P || col >= a.Q) continue;
+        float v[8], bias[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = s[c + k][p];
+        const int left = min(8, a.Q - col);
+        ln_bias<T>(a, col, left, bias);
+        ln_finish<T>(a, a.scale ? *a.scale : 1.0f, bias, p, col, left, v);
+    }
+}
+
 // ---- the gradient's elementwise part: dz = dout act'(z), and its columns' sums ------------------
 
 struct LnGradArgs {
@@ -813,10 +941,30 @@ static bool ln_aligned(const LnMatrix& m, bool depth, int64_t items) {
     return aligned_to(m.p, 16) && m.stride % 8 == 0 && m.stride < (1 << 21) && (depth || items % 8 == 0);
 }
 
+// Whether a product of few rows goes by vectors. float: 1 to 8 rows x 4096 x 4096 take 22 to 28 us so, 30 by tiles; 512 x 2048
+// 10 and 13 (9.5 of them the call). 16-bit types have tiles that are read faster than this: 1 and 4 rows x 2048 x 512 11
+// and 13 us, 15 and 13 by tiles; but 8 rows 18 and 14, one row x 4096 x 4096 20 and 14.
+static bool ln_few(int64_t size, int64_t P, int64_t Q, int64_t R) {
+    return size == 4 ? P <= kLsRows : P <= 4 && Q * R <= (1 << 21);
+}
+
 // C = A B, with what follows it in `r`.
 template <class T, bool AD, bool BD>
 static int ln_product(LnArgs r, void* temp, hipStream_t stream) {
     const int32_t dtype = sizeof(T) == 4 ? TDGS_F32 : std::is_same<T, bf16>::value ? TDGS_BF16 : TDGS_F16;
+    if (AD && ln_few(sizeof(T), r.P, r.Q, r.R)) {
+        auto few = [&](auto rows) {
+            constexpr int ROWS = decltype(rows)::value;
+            const int64_t cols = BD ? kLsThreads / kWave * 2 : 4 * ln_chunk<T>();
+            if constexpr (BD) k_linear_few_depth<T, ROWS><<<(unsigned)ceil_div(r.Q, cols), kLsThreads, 0, stream>>>(r);
+            else k_linear_few_items<T, ROWS><<<(unsigned)ceil_div(r.Q, cols), kLsThreads, 0, stream>>>(r);
+        };
+        if (r.P == 1) few(std::integral_constant<int, 1>{});
+        else if (r.P <= 4) few(std::integral_constant<int, 4>{});
+        else if constexpr (sizeof(T) == 4) few(std::integral_constant<int, kLsRows>{});
+        TDGS_LAUNCHED();
+        return TDGS_OK;
+    }
     const bool aligned = sizeof(T) == 2 && ln_aligned(r.a, AD, r.P) && ln_aligned(r.b, BD, r.Q);
     const LnPlan p = ln_plan(dtype, r.P, r.Q, r.R, aligned);
     r.tiles_p = p.tiles_p;

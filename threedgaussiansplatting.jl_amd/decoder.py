@@ -391,14 +391,21 @@ def _even_rows(t):
     return step
 
 
-def _matrix(t, name, lead, cols, like):
-    """(pointer, row stride) of a tensor of shape (*lead, cols) with evenly strided rows of contiguous elements."""
+def _matrix(t, name, shape, like, device):
+    """(pointer, row stride) of a tensor of this shape, like's type and device, with evenly strided rows of contiguous
+    elements."""
+    # what is usual is looked at once: most of what a call on a few rows costs is this
+    if isinstance(t, torch.Tensor) and len(shape) == 2 and t.shape == shape and t.dtype is like.dtype \
+            and t.get_device() == device:
+        row, element = t.stride()
+        if element == 1 or shape[1] <= 1 or not t.numel():
+            return t.data_ptr(), row
     _check_tensor(t, name, like)
     if t.dtype is not like.dtype:
         raise ValueError(f"{name} is {t.dtype}, not {like.dtype}")
-    n = t.shape
-    if n[:-1] != lead or n[-1] != cols:
-        raise ValueError(f"{name} has shape {tuple(n)}, not {(*lead, cols)}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    cols = shape[-1]
     if cols > 1 and t.stride(-1) != 1 and t.numel():
         raise ValueError(f"the rows of {name} must be contiguous")
     step = _even_rows(t)
@@ -414,7 +421,8 @@ _NO_ROWS = (0, 0)
 
 def _weight(w, name, like, shape=None):
     """(layout, pointer, row stride) of an (in, out) matrix that lies either way round."""
-    _check_tensor(w, name, like)
+    if not isinstance(w, torch.Tensor) or w.get_device() != like.get_device():
+        _check_tensor(w, name, like)
     if w.dtype is not like.dtype:
         raise ValueError(f"{name} is {w.dtype}, not {like.dtype}")
     if w.dim() != 2 or (shape is not None and w.shape != shape):
@@ -430,27 +438,33 @@ def _weight(w, name, like, shape=None):
 
 
 def _linear(x, weight, bias, activation, pre):
-    """The fields of the tdgs_linear of these tensors up to out, and those from pre to bias."""
-    _check_tensor(x, "x", x)
+    """The fields of the tdgs_linear of these tensors up to out, those from pre to bias, the outputs' shape and the device."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        _check_tensor(x, "x", x)
     dtype = DTYPES.get(x.dtype)
     if dtype is None:
         raise ValueError(f"x is {x.dtype}: float32, bfloat16 and float16 are supported")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
-    if x.dim() < 1:
+    shape = x.shape
+    if len(shape) < 1:
         raise ValueError("x must be (.., in)")
+    device = x.get_device()
     layout, w, ws = _weight(weight, "weight", x)
     features, outputs = weight.shape
-    lead = x.shape[:-1]
-    xp, xs = _matrix(x, "x", lead, features, x)
+    if shape[-1] != features:
+        raise ValueError(f"x has {shape[-1]} features, the weight {features}")
+    xp, xs = _matrix(x, "x", shape, x, device)
+    shape = (*shape[:-1], outputs)
     b = 0
     if bias is not None:
-        _check_vector(bias, "bias", outputs, x)
+        if bias.dtype is not x.dtype or bias.shape != (outputs,) or bias.get_device() != device or not bias.is_contiguous():
+            _check_vector(bias, "bias", outputs, x)
         b = bias.data_ptr()
     rows = x.numel() // features if features else 0
     return ((dtype, act, rows, features, outputs, layout, 0, xp, xs, w, ws),
-            (*(_NO_ROWS if pre is None else _matrix(pre, "pre", lead, outputs, x)), b))
+            (*(_NO_ROWS if pre is None else _matrix(pre, "pre", shape, x, device)), b), shape, device)
 
 
 def _check_vector(p, name, n, like):
@@ -461,7 +475,7 @@ def _check_vector(p, name, n, like):
 
 def linear_temp(x, weight, grad=False):
     """Scratch for linear_ (with grad also linear_grad_, whatever its activation) on tensors of these sizes."""
-    a, b = _linear(x, weight, None, "silu", None)
+    a, b, _, _ = _linear(x, weight, None, "silu", None)
     return _new_temp(lib().tdgs_linear_temp_bytes, _LINEAR.pack(*a, *_NO_ROWS, *_NO_ROWS, *b, 0, 0), grad, x)
 
 
@@ -472,10 +486,9 @@ def linear_(out, x, weight, bias=None, *, residual=None, activation="identity", 
     weight the rows or the columns are (the transpose of an (out, in) matrix is taken as it is). activation is identity,
     silu, gelu or relu. pre, where given, receives x weight + bias, which the gradient needs unless the activation is the
     identity. residual may be out; out and pre overlap nothing else."""
-    a, b = _linear(x, weight, bias, activation, pre)
-    lead, outputs = x.shape[:-1], weight.shape[1]
-    o = _matrix(out, "out", lead, outputs, x)
-    r = _NO_ROWS if residual is None else _matrix(residual, "residual", lead, outputs, x)
+    a, b, shape, device = _linear(x, weight, bias, activation, pre)
+    o = _matrix(out, "out", shape, x, device)
+    r = _NO_ROWS if residual is None else _matrix(residual, "residual", shape, x, device)
     if temp is None:
         temp = _new_temp(lib().tdgs_linear_temp_bytes, _LINEAR.pack(*a, *o, *r, *b, 0, 0), False, x)
     _call(lib().tdgs_linear_forward, x, (_LINEAR.pack(*a, *o, *r, *b, *_temp(temp, x)),))
@@ -489,10 +502,10 @@ def linear_grad_(dx, dweight, dbias, dout, x, weight, *, activation="identity", 
     dout act'(pre) is an operand of two matrix products and rounded to the type for them; dbias is summed before."""
     if pre is None and activation != "identity":
         raise ValueError("the gradient needs the forward call's pre")
-    a, b = _linear(x, weight, None, activation, pre)
-    lead, outputs = x.shape[:-1], weight.shape[1]
-    d = _matrix(dout, "dout", lead, outputs, x)
-    g = _NO_ROWS if dx is None else _matrix(dx, "dx", lead, weight.shape[0], x)
+    a, b, shape, device = _linear(x, weight, None, activation, pre)
+    outputs = shape[-1]
+    d = _matrix(dout, "dout", shape, x, device)
+    g = _NO_ROWS if dx is None else _matrix(dx, "dx", x.shape, x, device)
     layout, w, ws = (0, 0, 0) if dweight is None else _weight(dweight, "dweight", x, weight.shape)
     db = 0
     if dbias is not None:
@@ -537,6 +550,7 @@ class Rotary:
         if f.shape != (self.pairs,):
             raise ValueError(f"{tuple(f.shape)} frequencies of {self.pairs} pairs")
         self.turns = (f / (2 * math.pi)).to(_dev(device))
+        self.device, self.pointer = self.turns.get_device(), self.turns.data_ptr()
         self._fields = (self.pairs, _PAIRS[pairs], self.axes, *self.sections, *(0,) * (4 - self.axes))
 
 
@@ -561,16 +575,18 @@ def _head_norm(q, k, q_weight, k_weight, norm, eps, rotary, positions, inverse):
         if first.dtype is not torch.float32 and first.dtype is not q.dtype:
             raise ValueError(f"q_weight and k_weight must be of one type, float32 or {q.dtype}")
         for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-            if w is not None:
-                _check_vector(w, name, d, first)
+            if w is not None and (w.dtype is not first.dtype or w.shape != (d,) or w.get_device() != q.get_device()
+                                  or not w.is_contiguous()):
                 _check_tensor(w, name, q)
+                raise ValueError(f"{name} must be {d} contiguous values of {first.dtype}")
     if rotary is None:
         if positions is not None:
             raise ValueError("positions without a rotary")
         rotation, place = (0,) * 7, (0, 0, 0, 0)
     else:
-        _check_tensor(rotary.turns, "the rotary", q)
-        _check_tensor(positions, "positions", q)
+        if not isinstance(positions, torch.Tensor) or not q.get_device() == positions.get_device() == rotary.device:
+            _check_tensor(rotary.turns, "the rotary", q)
+            _check_tensor(positions, "positions", q)
         kind = _POSITIONS.get(positions.dtype)
         if kind is None:
             raise ValueError(f"positions are {positions.dtype}: int32, int64 and float32 are supported")
@@ -578,20 +594,30 @@ def _head_norm(q, k, q_weight, k_weight, norm, eps, rotary, positions, inverse):
         if (n != (l, rotary.axes) and n != (b, l, rotary.axes)) or not positions.is_contiguous():
             raise ValueError(f"positions must be contiguous, ({l}, {rotary.axes}) or ({b}, {l}, {rotary.axes})")
         rotation = rotary._fields
-        place = (kind, rotary.turns.data_ptr(), positions.data_ptr(), l * rotary.axes if len(n) == 3 else 0)
+        place = (kind, rotary.pointer, positions.data_ptr(), l * rotary.axes if len(n) == 3 else 0)
     return ((dtype, param, b, l, h, hk, d, int(norm), eps, *rotation, int(inverse), *place),
             (dptr(q_weight) or 0, dptr(k_weight) or 0))
+
+
+def _head_view(t, name, shape, like, device):
+    """_heads, for which what is usual is looked at once."""
+    if isinstance(t, torch.Tensor) and t.dtype is like.dtype and t.shape == shape and t.get_device() == device:
+        b, l, h, d = t.stride()
+        if d == 1:
+            return t.data_ptr(), b, l, h
+    return _heads(t, name, shape, like)
 
 
 def _head_views(names, tensors, like):
     """The tdgs_heads fields of tensors like (q, k): k's may be missing."""
     q, k = like
-    out = _heads(tensors[0], names[0], q.shape, q)
+    device = q.get_device()
+    out = _head_view(tensors[0], names[0], q.shape, q, device)
     if k is None:
         if tensors[1] is not None:
             raise ValueError(f"{names[1]} without k")
         return (*out, *_NO_HEADS)
-    return (*out, *_heads(tensors[1], names[1], k.shape, q))
+    return (*out, *_head_view(tensors[1], names[1], k.shape, q, device))
 
 
 def head_norm_(q_out, k_out, q, k=None, q_weight=None, k_weight=None, *, eps=1e-6, rotary=None, positions=None):
@@ -667,7 +693,8 @@ def dropout_(out, x, p, seed, *, call=0, residual=None):
         raise ValueError(f"dropout of {p}, which is no probability")
     if x.dim() == 0:
         raise ValueError("x must have a dimension")
-    lead, cols = x.shape[:-1], x.shape[-1]
+    shape, device = x.shape, x.get_device()
+    cols = shape[-1]
     number = device_call = 0
     if isinstance(call, torch.Tensor):
         _check_tensor(call, "call", x)
@@ -676,9 +703,9 @@ def dropout_(out, x, p, seed, *, call=0, residual=None):
         device_call = call.data_ptr()
     else:
         number = int(call) & (2 ** 64 - 1)
-    r = _NO_ROWS if residual is None else _matrix(residual, "residual", lead, cols, x)
+    r = _NO_ROWS if residual is None else _matrix(residual, "residual", shape, x, device)
     fields = (dtype, 0, x.numel() // cols if cols else 0, cols, p, int(seed) & (2 ** 64 - 1), number, device_call,
-              *_matrix(x, "x", lead, cols, x), *_matrix(out, "out", lead, cols, x), *r)
+              *_matrix(x, "x", shape, x, device), *_matrix(out, "out", shape, x, device), *r)
     _call(lib().tdgs_dropout_apply, x, (_DROPOUT.pack(*fields),))
     return out
 
