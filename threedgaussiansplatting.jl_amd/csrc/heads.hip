@@ -83,17 +83,21 @@ __device__ __forceinline__ void hn_tokens(const HnArgs& a, int64_t first, int co
     }
 }
 
+// What the units of a call are: elements of both halves all, neighbours all (interleaved pairs, or none rotated), or
+// halves with a rest that is not rotated.
+enum { kHnHalves, kHnNeighbours, kHnMixed };
+
 // The two sets of V elements of unit j of a row: where they start, how far elements of a set are apart and whether they
-// are rotated.
-template <int V>
+// are rotated. ALL: there is a unit for every lane.
+template <int V, int KIND, bool ALL>
 struct HnUnit {
     int first, second, step, pair;
     bool on, rotated;
     __device__ __forceinline__ HnUnit(const HnArgs& a, int j) {
-        on = j < a.units;
-        rotated = j < a.rotated_units;
+        on = ALL || j < a.units;
+        rotated = KIND == kHnHalves || j < a.rotated_units;
         pair = j * V;
-        if (rotated && !a.interleaved) {
+        if (KIND == kHnHalves || (KIND == kHnMixed && rotated)) {
             first = j * V;
             second = a.pairs + j * V;
             step = 1;
@@ -106,30 +110,30 @@ struct HnUnit {
 };
 
 // A unit's 2 V elements at p, as V first and V second ones of its pairs.
-template <class T, int V>
-__device__ __forceinline__ void hn_load(const T* __restrict__ p, const HnUnit<V>& u, int d, float (&a)[V], float (&b)[V]) {
+template <class T, int V, int KIND, bool ALL>
+__device__ __forceinline__ void hn_load(const T* __restrict__ p, const HnUnit<V, KIND, ALL>& u, int d, float (&a)[V], float (&b)[V]) {
     if constexpr (V == 1) {
         a[0] = u.on ? (float)p[u.first] : 0.0f;
         b[0] = u.on && u.second < d ? (float)p[u.second] : 0.0f;
     } else {
         typedef T W __attribute__((ext_vector_type(V)));
         typedef T Wa __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-        W x, y;
-        const int at = u.on ? u.first : 0;
-        x = *reinterpret_cast<const Wa*>(p + at);
-        y = *reinterpret_cast<const Wa*>(p + (u.step == 1 ? u.second : at + V));
+        const bool halves = KIND == kHnHalves || (KIND == kHnMixed && u.step == 1);
+        const W x = *reinterpret_cast<const Wa*>(p + u.first);
+        const W y = *reinterpret_cast<const Wa*>(p + (halves ? u.second : u.first + V));
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             // neighbours: element 2 i and 2 i + 1 of the 2 V
             const T even = 2 * i < V ? x[2 * i % V] : y[2 * i % V], odd = 2 * i < V ? x[(2 * i + 1) % V] : y[(2 * i + 1) % V];
-            a[i] = u.on ? (float)(u.step == 1 ? x[i] : even) : 0.0f;
-            b[i] = u.on ? (float)(u.step == 1 ? y[i] : odd) : 0.0f;
+            a[i] = (float)(halves ? x[i] : even);
+            b[i] = (float)(halves ? y[i] : odd);
         }
     }
 }
 
-template <class T, int V>
-__device__ __forceinline__ void hn_store(T* __restrict__ p, const HnUnit<V>& u, int d, const float (&a)[V], const float (&b)[V]) {
+template <class T, int V, int KIND, bool ALL>
+__device__ __forceinline__ void hn_store(T* __restrict__ p, const HnUnit<V, KIND, ALL>& u, int d, const float (&a)[V],
+                                         const float (&b)[V]) {
     if (!u.on) return;
     if constexpr (V == 1) {
         p[u.first] = (T)a[0];
@@ -137,20 +141,21 @@ __device__ __forceinline__ void hn_store(T* __restrict__ p, const HnUnit<V>& u, 
     } else {
         typedef T W __attribute__((ext_vector_type(V)));
         typedef T Wa __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+        const bool halves = KIND == kHnHalves || (KIND == kHnMixed && u.step == 1);
         W x, y;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const float lo = i % 2 ? b[i / 2] : a[i / 2], hi = i % 2 ? b[(V + i) / 2] : a[(V + i) / 2];
-            x[i] = (T)(u.step == 1 ? a[i] : lo);
-            y[i] = (T)(u.step == 1 ? b[i] : hi);
+            x[i] = (T)(halves ? a[i] : lo);
+            y[i] = (T)(halves ? b[i] : hi);
         }
         *reinterpret_cast<Wa*>(p + u.first) = x;
-        *reinterpret_cast<Wa*>(p + (u.step == 1 ? u.second : u.first + V)) = y;
+        *reinterpret_cast<Wa*>(p + (halves ? u.second : u.first + V)) = y;
     }
 }
 
 // A lane's weights, of queries and of keys: they stay in registers.
-template <class T, int V, int N>
+template <class T, int V, int N, int KIND>
 struct HnWeights {
     float x[2][N][V], y[2][N][V];
     __device__ __forceinline__ HnWeights(const HnArgs& a, int lane) {
@@ -158,7 +163,7 @@ struct HnWeights {
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const HnUnit<V> u(a, lane + n * a.lanes);
+                const HnUnit<V, KIND, N == 1> u(a, lane + n * a.lanes);
                 const void* const w = a.t[k].weight;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -212,12 +217,12 @@ struct HnLane {
 };
 
 // N units per lane (two where a head of more than 128 elements goes by single pairs).
-template <class T, int V, int N>
+template <class T, int V, int N, int KIND>
 __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
     extern __shared__ float2 s_angles[];
     __shared__ HnPlaces s_at;
     const HnLane lane(a);
-    const HnWeights<T, V, N> w(a, lane.j);
+    const HnWeights<T, V, N, KIND> w(a, lane.j);
     for (int64_t first = (int64_t)blockIdx.x * a.per; first < a.tokens; first += (int64_t)gridDim.x * a.per) {
         const int count = (int)(a.tokens - first < a.per ? a.tokens - first : a.per);
         __syncthreads();   // (the tokens before)
@@ -235,7 +240,7 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
                 const T* const x = (const T*)t.x + s_at.x[k][token] + head * t.xh;
                 float ya[N][V], yb[N][V];
 #pragma unroll
-                for (int n = 0; n < N; ++n) hn_load<T, V>(x, HnUnit<V>(a, lane.j + n * a.lanes), a.d, ya[n], yb[n]);
+                for (int n = 0; n < N; ++n) hn_load<T>(x, HnUnit<V, KIND, N == 1>(a, lane.j + n * a.lanes), a.d, ya[n], yb[n]);
                 if (a.norm) {
                     float sum = 0.0f;
 #pragma unroll
@@ -255,9 +260,9 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
                 T* const out = (T*)t.out + s_at.out[k][token] + head * t.oh;
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    const HnUnit<V> u(a, lane.j + n * a.lanes);
+                    const HnUnit<V, KIND, N == 1> u(a, lane.j + n * a.lanes);
                     if (u.on && u.rotated) hn_turn<V, false>(s_angles + token * a.pairs + u.pair, ya[n], yb[n]);
-                    if (valid) hn_store<T, V>(out, u, a.d, ya[n], yb[n]);
+                    if (valid) hn_store<T>(out, u, a.d, ya[n], yb[n]);
                 }
             }
         }
@@ -265,12 +270,12 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
 }
 
 // dx, and this workgroup's sums for dw: part[block][queries, keys][d].
-template <class T, int V, int N>
+template <class T, int V, int N, int KIND>
 __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
     extern __shared__ float2 s_angles[];
     __shared__ HnPlaces s_at;
     const HnLane lane(a);
-    const HnWeights<T, V, N> w(a, lane.j);
+    const HnWeights<T, V, N, KIND> w(a, lane.j);
     float da[2][N][V], db[2][N][V];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -296,9 +301,9 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
                 float xa[N][V], xb[N][V], ea[N][V], eb[N][V], sum = 0.0f, mean = 0.0f;
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    const HnUnit<V> u(a, lane.j + n * a.lanes);
-                    hn_load<T, V>(x, u, a.d, xa[n], xb[n]);
-                    hn_load<T, V>(dout, u, a.d, ea[n], eb[n]);
+                    const HnUnit<V, KIND, N == 1> u(a, lane.j + n * a.lanes);
+                    hn_load<T>(x, u, a.d, xa[n], xb[n]);
+                    hn_load<T>(dout, u, a.d, ea[n], eb[n]);
                 }
 #pragma unroll
                 for (int n = 0; n < N; ++n)
@@ -307,7 +312,7 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
                 const float r = rsqrtf(__builtin_fmaf(hn_row_sum(sum, lane.j, a.lanes), a.inv_d, a.eps));
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    const HnUnit<V> u(a, lane.j + n * a.lanes);
+                    const HnUnit<V, KIND, N == 1> u(a, lane.j + n * a.lanes);
                     if (u.on && u.rotated) hn_turn<V, true>(s_angles + token * a.pairs + u.pair, ea[n], eb[n]);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
@@ -328,7 +333,7 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
                         xa[n][i] = r * __builtin_fmaf(-mean, xa[n][i], ea[n][i] * w.x[k][n][i]);
                         xb[n][i] = r * __builtin_fmaf(-mean, xb[n][i], eb[n][i] * w.y[k][n][i]);
                     }
-                    if (valid) hn_store<T, V>(out, HnUnit<V>(a, lane.j + n * a.lanes), a.d, xa[n], xb[n]);
+                    if (valid) hn_store<T>(out, HnUnit<V, KIND, N == 1>(a, lane.j + n * a.lanes), a.d, xa[n], xb[n]);
                 }
             }
         }
@@ -341,7 +346,7 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const HnUnit<V> u(a, lane.j + n * a.lanes);
+            const HnUnit<V, KIND, N == 1> u(a, lane.j + n * a.lanes);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if (!lane.on || !u.on) continue;
@@ -502,15 +507,28 @@ static void hn_out(HnTensor* t, const tdgs_heads& v) {
     t->oh = v.stride_h;
 }
 
-// f(T{}, elements of a half per lane, units per lane)
+// f(T{}, elements of a half per lane, units per lane, their kind)
 template <class F>
 static int hn_dispatch(const tdgs_head_norm* a, const HnPlan& p, F&& f) {
+    using One = std::integral_constant<int, 1>;
+    using Neighbours = std::integral_constant<int, kHnNeighbours>;
+    const bool neighbours = a->pairs == 0 || a->pair_layout == TDGS_PAIRS_INTERLEAVED;
     return with_dtype(a->dtype, [&](auto t) -> int {
-        using One = std::integral_constant<int, 1>;
-        if (p.v == 1) return a->head_dim > 128 ? f(t, One{}, std::integral_constant<int, 2>{}) : f(t, One{}, One{});
+        // (single pairs: every kind is as quick as any)
+        if (p.v == 1) {
+            using Mixed = std::integral_constant<int, kHnMixed>;
+            if (a->head_dim > 128) return neighbours ? f(t, One{}, std::integral_constant<int, 2>{}, Neighbours{})
+                                                     : f(t, One{}, std::integral_constant<int, 2>{}, Mixed{});
+            return neighbours ? f(t, One{}, One{}, Neighbours{}) : f(t, One{}, One{}, Mixed{});
+        }
+        auto kinds = [&](auto v) -> int {
+            if (neighbours) return f(t, v, One{}, Neighbours{});
+            if (2 * a->pairs == a->head_dim) return f(t, v, One{}, std::integral_constant<int, kHnHalves>{});
+            return f(t, v, One{}, std::integral_constant<int, kHnMixed>{});
+        };
         if constexpr (sizeof(t) == 2)
-            if (p.v == 8) return f(t, std::integral_constant<int, 8>{}, One{});
-        return f(t, std::integral_constant<int, 4>{}, One{});
+            if (p.v == 8) return kinds(std::integral_constant<int, 8>{});
+        return kinds(std::integral_constant<int, 4>{});
     });
 }
 
@@ -536,8 +554,8 @@ int tdgs_head_norm_forward(void* stream_, const tdgs_head_norm* a) {
     }
     const HnPlan p = hn_plan(a, &r, false);
     hipStream_t stream = (hipStream_t)stream_;
-    return hn_dispatch(a, p, [&](auto t, auto v, auto n) -> int {
-        k_head_norm<decltype(t), decltype(v)::value, decltype(n)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
+    return hn_dispatch(a, p, [&](auto t, auto v, auto n, auto kind) -> int {
+        k_head_norm<decltype(t), decltype(v)::value, decltype(n)::value, decltype(kind)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
         TDGS_LAUNCHED();
         return TDGS_OK;
     });
@@ -577,10 +595,10 @@ int tdgs_head_norm_grad(void* stream_, const tdgs_head_norm* a, const tdgs_head_
     hipStream_t stream = (hipStream_t)stream_;
     r.part = weights ? (float*)a->temp : nullptr;
     if (empty) p.blocks = 0;   // (the weights' gradients are zero)
-    return hn_dispatch(a, p, [&](auto t, auto v, auto n) -> int {
+    return hn_dispatch(a, p, [&](auto t, auto v, auto n, auto kind) -> int {
         using T = decltype(t);
         if (!empty) {
-            k_head_norm_grad<T, decltype(v)::value, decltype(n)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
+            k_head_norm_grad<T, decltype(v)::value, decltype(n)::value, decltype(kind)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
             TDGS_LAUNCHED();
         }
         if (weights) {
