@@ -219,6 +219,7 @@ struct HnLane {
 // N units per lane (two where a head of more than 128 elements goes by single pairs).
 template <class T, int V, int N, int KIND>
 __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
+    constexpr int U = 4;
     extern __shared__ float2 s_angles[];
     __shared__ HnPlaces s_at;
     const HnLane lane(a);
@@ -232,37 +233,47 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm(HnArgs a) {
         for (int k = 0; k < 2; ++k) {
             const HnTensor& t = a.t[k];
             const int rows = count * a.heads[k];
-            // (every lane stays for the sums)
-            for (int r0 = 0; r0 < rows; r0 += lane.rows) {
-                const bool valid = lane.on && r0 + lane.sub < rows;
-                const int r = r0 + lane.sub < rows ? r0 + lane.sub : rows - 1;
-                const int token = (int)a.by_heads[k].div((uint32_t)r), head = r - token * a.heads[k];
-                const T* const x = (const T*)t.x + s_at.x[k][token] + head * t.xh;
-                float ya[N][V], yb[N][V];
+            // U rows at once, for their loads (every lane stays for the sums)
+            for (int r0 = 0; r0 < rows; r0 += U * lane.rows) {
+                float ya[U][N][V], yb[U][N][V];
+                int token[U], head[U];
 #pragma unroll
-                for (int n = 0; n < N; ++n) hn_load<T>(x, HnUnit<V, KIND, N == 1>(a, lane.j + n * a.lanes), a.d, ya[n], yb[n]);
-                if (a.norm) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int n = 0; n < N; ++n)
-#pragma unroll
-                        for (int i = 0; i < V; ++i)
-                            sum = __builtin_fmaf(ya[n][i], ya[n][i], __builtin_fmaf(yb[n][i], yb[n][i], sum));
-                    sum = rsqrtf(__builtin_fmaf(hn_row_sum(sum, lane.j, a.lanes), a.inv_d, a.eps));
+                for (int m = 0; m < U; ++m) {
+                    const int at = r0 + m * lane.rows + lane.sub, r = at < rows ? at : rows - 1;
+                    token[m] = (int)a.by_heads[k].div((uint32_t)r);
+                    head[m] = r - token[m] * a.heads[k];
+                    const T* const x = (const T*)t.x + s_at.x[k][token[m]] + head[m] * t.xh;
 #pragma unroll
                     for (int n = 0; n < N; ++n)
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            ya[n][i] *= sum * w.x[k][n][i];
-                            yb[n][i] *= sum * w.y[k][n][i];
-                        }
+                        hn_load<T>(x, HnUnit<V, KIND, N == 1>(a, lane.j + n * a.lanes), a.d, ya[m][n], yb[m][n]);
                 }
-                T* const out = (T*)t.out + s_at.out[k][token] + head * t.oh;
 #pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const HnUnit<V, KIND, N == 1> u(a, lane.j + n * a.lanes);
-                    if (u.on && u.rotated) hn_turn<V, false>(s_angles + token * a.pairs + u.pair, ya[n], yb[n]);
-                    if (valid) hn_store<T>(out, u, a.d, ya[n], yb[n]);
+                for (int m = 0; m < U; ++m) {
+                    if (m > 0 && r0 + m * lane.rows >= rows) break;
+                    if (a.norm) {
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < N; ++n)
+#pragma unroll
+                            for (int i = 0; i < V; ++i)
+                                sum = __builtin_fmaf(ya[m][n][i], ya[m][n][i], __builtin_fmaf(yb[m][n][i], yb[m][n][i], sum));
+                        sum = rsqrtf(__builtin_fmaf(hn_row_sum(sum, lane.j, a.lanes), a.inv_d, a.eps));
+#pragma unroll
+                        for (int n = 0; n < N; ++n)
+#pragma unroll
+                            for (int i = 0; i < V; ++i) {
+                                ya[m][n][i] *= sum * w.x[k][n][i];
+                                yb[m][n][i] *= sum * w.y[k][n][i];
+                            }
+                    }
+                    T* const out = (T*)t.out + s_at.out[k][token[m]] + head[m] * t.oh;
+                    const bool valid = lane.on && r0 + m * lane.rows + lane.sub < rows;
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const HnUnit<V, KIND, N == 1> u(a, lane.j + n * a.lanes);
+                        if (u.on && u.rotated) hn_turn<V, false>(s_angles + token[m] * a.pairs + u.pair, ya[m][n], yb[m][n]);
+                        if (valid) hn_store<T>(out, u, a.d, ya[m][n], yb[m][n]);
+                    }
                 }
             }
         }
@@ -437,13 +448,14 @@ struct HnPlan {
     size_t lds;
 };
 
-// Elements a lane takes of each half: eight of a 16-bit type (16 bytes) or four, where the pairs and what is not rotated
-// divide into them, or single ones.
+// Elements a lane takes of each half: eight of a 16-bit type (16 bytes; in the gradient, whose sums for dw would then leave
+// room for three wavefronts a SIMD, four: 32 heads of 64 bfloat16 146 us instead of 157) or four, where the pairs and
+// what is not rotated divide into them, or single ones.
 static HnPlan hn_plan(const tdgs_head_norm* a, HnArgs* r, bool grad) {
     HnPlan p;
     const int rest = a->head_dim - 2 * a->pairs;
     auto fits = [&](int v) { return a->pairs % v == 0 && rest % (2 * v) == 0; };
-    p.v = a->dtype != TDGS_F32 && fits(8) ? 8 : fits(4) ? 4 : 1;
+    p.v = a->dtype != TDGS_F32 && !grad && fits(8) ? 8 : fits(4) ? 4 : 1;
     r->rotated_units = a->pairs / p.v;
     r->units = r->rotated_units + (rest + 2 * p.v - 1) / (2 * p.v);
     r->lanes = r->units < kWave ? r->units : kWave;
@@ -597,9 +609,12 @@ int tdgs_head_norm_grad(void* stream_, const tdgs_head_norm* a, const tdgs_head_
     if (empty) p.blocks = 0;   // (the weights' gradients are zero)
     return hn_dispatch(a, p, [&](auto t, auto v, auto n, auto kind) -> int {
         using T = decltype(t);
-        if (!empty) {
-            k_head_norm_grad<T, decltype(v)::value, decltype(n)::value, decltype(kind)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
-            TDGS_LAUNCHED();
+        constexpr int V = decltype(v)::value;
+        if constexpr (V <= 4) {
+            if (!empty) {
+                k_head_norm_grad<T, V, decltype(n)::value, decltype(kind)::value><<<(unsigned)p.blocks, kHnThreads, p.lds, stream>>>(r);
+                TDGS_LAUNCHED();
+            }
         }
         if (weights) {
             k_head_norm_join<T><<<(unsigned)ceil_div(2 * a->head_dim, kHnJoinCols), kHnThreads, 0, stream>>>(
