@@ -210,15 +210,19 @@ __device__ __forceinline__ void ln_activate(int act, float (&v)[8]) {
     }
 }
 
-// The end of n (1 to 8) neighbouring results q.. of row p: bias holds those of the bias, or zeros.
+// The end of n (1 to 8) neighbouring results q.. of row p: bias holds those of the bias, or zeros, and `residual`, where not
+// null, what has been loaded of the residual.
 template <class T>
 __device__ __forceinline__ void ln_finish(const LnArgs& a, float scale, const float (&bias)[8], int64_t p, int q, int n,
-                                          float (&v)[8]) {
+                                          float (&v)[8], const typename LnVec<T>::Va* residual = nullptr) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = a.scale ? v[i] * scale : v[i] + bias[i];   // (never both)
     if (a.pre.p) LnVec<T>::store((T*)a.pre.p + p * a.pre.stride + q, n, v);
     ln_activate(a.act, v);
-    if (a.residual.p) {
+    if (residual) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += (float)(*residual)[i];
+    } else if (a.residual.p) {
         float r[8];
         LnVec<T>::load((const T*)a.residual.p + p * a.residual.stride + q, n, r);
 #pragma unroll
@@ -265,8 +269,21 @@ __device__ __forceinline__ void ln_end(const LnArgs& a, const f32x16 (&acc)[S::N
     const int x = lane % kPerRow * 8, q = q0 + x, n = min(8, a.Q - q);
     float bias[8];
     ln_bias<T>(a, q, n, bias);
+    // The residual of 32 rows is on its way while the rows before are worked on.
+    constexpr int kAhead = 32 / kRows;
+    typename LnVec<T>::Va rest[2][kAhead];
+    const bool ahead = a.residual.p && !a.part && a.Q % 8 == 0;
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int r = 0; r < kAhead; ++r) {
+            const int p = min(p0 + i * 32 + r * kRows + lane / kPerRow, a.P - 1);
+            rest[i & 1][r] = *reinterpret_cast<const typename LnVec<T>::Va*>((const T*)a.residual.p + p * a.residual.stride + (n > 0 ? q : 0));
+        }
+    };
+    if (ahead) fetch(0);
 #pragma unroll
     for (int i = 0; i < S::NP; ++i) {
+        if (ahead && i + 1 < S::NP) fetch(i + 1);
 #pragma unroll
         for (int j = 0; j < S::NQ; ++j)
 #pragma unroll
@@ -291,7 +308,8 @@ __device__ __forceinline__ void ln_end(const LnArgs& a, const f32x16 (&acc)[S::N
                 o[1] = hi;
             } else {
                 float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                ln_finish<T>(a, scale, bias, p, q, n, v);
+                if (ahead) ln_finish<T>(a, scale, bias, p, q, n, v, &rest[i & 1][r0 / kRows]);
+                else ln_finish<T>(a, scale, bias, p, q, n, v);
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -871,19 +889,22 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_zero(T* p, int64_t rows, 
 // ---- host ----------------------------------------------------------------------------------
 
 // The forms of a product: tile, depth of a step, workgroups per CU, and what they take by measurement, in us: a
-// workgroup's start and end, a step of one alone on its CU, and a step's share where the CU is full. (256x256: 1.93 us a
-// step is 1110 TFLOP/s.)
+// workgroup's start and end, a step of one alone on its CU, and a step's share where the CU is full. 256x256 needs the fewest
+// bytes from LDS per product (1.93 us a step are 1110 TFLOP/s), but fills a CU alone, so that nothing is multiplied
+// while it ends; two workgroups of 128x256, with half the registers, end beside each other (64800 x 512 -> 2048 bfloat16 with
+// GELU: 223 us, 247 by 256x256; at a depth of 1024 they are even, at 8192 it is 1440 and 980). Small tiles leave fewer
+// CUs idle (34230 x 320 -> 320 float16 with a residual: 20 us by 128x64, 25 by 128x128, 43 by 256x256).
 struct LnForm {
     int bp, bq, bk, per_cu;
     float ends, alone, full;
 };
-enum { kLnStaged64, kLnStaged128, kLnDirect64, kLnDirect128x64, kLnDirect128, kLnDirect256, kLnForms };
+enum { kLnStaged64, kLnStaged128, kLnDirect64, kLnDirect128x64, kLnDirect128, kLnDirect128x256, kLnDirect256, kLnForms };
 template <class T>
 constexpr int ln_depth() { return sizeof(T) == 4 ? 16 : 32; }
 constexpr LnForm kLnF32[2] = {{64, 64, ln_depth<float>(), 8, 3.0f, 0.5f, 0.3f}, {128, 128, ln_depth<float>(), 3, 5.0f, 1.3f, 1.2f}};
 constexpr LnForm kLn16[kLnForms] = {{64, 64, ln_depth<bf16>(), 6, 3.0f, 0.5f, 0.25f}, {128, 128, ln_depth<bf16>(), 3, 5.0f, 0.8f, 0.42f},
                                     {64, 64, 64, 4, 3.0f, 0.46f, 0.206f},  {128, 64, 64, 3, 4.0f, 0.6f, 0.34f},
-                                    {128, 128, 64, 2, 5.0f, 0.85f, 0.59f}, {256, 256, 64, 1, 8.0f, 1.93f, 1.93f}};
+                                    {128, 128, 64, 2, 5.0f, 0.85f, 0.59f}, {128, 256, 32, 2, 3.0f, 0.8f, 0.62f}, {256, 256, 64, 1, 12.0f, 1.93f, 1.93f}};
 constexpr int kLnCus = 256;
 constexpr int kLnLeastSteps = 4;   // of a split
 
@@ -984,14 +1005,18 @@ static int ln_product(LnArgs r, void* temp, hipStream_t stream) {
         using S = decltype(shape);
         k_linear_direct<S><<<(unsigned)grid, S::TH, 0, stream>>>(r);
     };
-    if ((AD ? r.R : r.P) < C || (BD ? r.R : r.Q) < C) staged(LnShape<T, 64, 64, 2, 2, D, AD, BD, true>{});
-    else if (p.form == kLnStaged64) staged(LnShape<T, 64, 64, 2, 2, D, AD, BD, false>{});
-    else if (p.form == kLnStaged128) staged(LnShape<T, 128, 128, 2, 2, D, AD, BD, false>{});
-    if constexpr (sizeof(T) == 2) {
+    if ((AD ? r.R : r.P) < C || (BD ? r.R : r.Q) < C) {   // (the plan of such a product has the smallest tiles)
+        staged(LnShape<T, 64, 64, 2, 2, D, AD, BD, true>{});
+    } else if (p.form == kLnStaged64) {
+        staged(LnShape<T, 64, 64, 2, 2, D, AD, BD, false>{});
+    } else if (p.form == kLnStaged128) {
+        staged(LnShape<T, 128, 128, 2, 2, D, AD, BD, false>{});
+    } else if constexpr (sizeof(T) == 2) {
         if (p.form == kLnDirect64) direct(LfShape<T, 64, 64, 2, 2, 64, 2, 4, AD, BD>{});
         else if (p.form == kLnDirect128x64) direct(LfShape<T, 128, 64, 2, 2, 64, 2, 3, AD, BD>{});
         else if (p.form == kLnDirect128) direct(LfShape<T, 128, 128, 2, 2, 64, 2, 2, AD, BD>{});
-        else if (p.form == kLnDirect256) direct(LfShape<T, 256, 256, 2, 4, 64, 2, 1, AD, BD>{});
+        else if (p.form == kLnDirect128x256) direct(LfShape<T, 128, 256, 2, 4, 32, 3, 2, AD, BD>{});
+        else direct(LfShape<T, 256, 256, 2, 4, 64, 2, 1, AD, BD>{});
     }
     TDGS_LAUNCHED();
     if (p.splits > 1) {
