@@ -1047,11 +1047,17 @@ static int ln_check(const tdgs_linear* a) {
     return TDGS_OK;
 }
 
+// Tiles of up to 128 rows (256 of at most 2^22 bytes each where they go to LDS directly) are addressed by 32 bits.
+constexpr int64_t kLnRowBytes = 1 << 24;
+
 static int ln_check_rows(const tdgs_rows& v, const char* name, int32_t dtype, int64_t rows, int64_t cols, bool written) {
     TDGS_REQUIRE(v.data != nullptr, "linear: %s is null", name);
     TDGS_REQUIRE(aligned_to(v.data, (size_t)dtype_size(dtype)), "linear: %s is not aligned to its element type", name);
     TDGS_REQUIRE(v.stride >= 0, "linear: %s has a negative stride", name);
     if (written) TDGS_REQUIRE(rows <= 1 || v.stride >= cols, "linear: rows of %s overlap", name);
+    else TDGS_REQUIRE(rows <= 1 || v.stride * dtype_size(dtype) <= kLnRowBytes,
+                      "linear: rows of %s are too far apart: %lld bytes, %lld at most", name,
+                      (long long)(v.stride * dtype_size(dtype)), (long long)kLnRowBytes);
     return TDGS_OK;
 }
 
@@ -1062,6 +1068,13 @@ static int ln_check_weight(const tdgs_rows& v, const char* name, const tdgs_line
 }
 
 static LnMatrix ln_matrix(const tdgs_rows& v) { return {v.data, v.stride}; }
+// An operand: the stride of a single row means nothing, and must not be calculated with.
+static LnMatrix ln_operand_rows(const tdgs_rows& v, int64_t rows, int64_t cols) { return {v.data, rows > 1 ? v.stride : cols}; }
+
+static LnMatrix ln_weight(const tdgs_linear* a) {
+    return a->weight_layout == TDGS_WEIGHT_IN_OUT ? ln_operand_rows(a->weight, a->in_features, a->out_features)
+                                                  : ln_operand_rows(a->weight, a->out_features, a->in_features);
+}
 
 // The gradient's scratch: dz, its power of two, maxima and columns' sums, then a product's partial sums.
 struct LnGradPlan {
@@ -1128,8 +1141,8 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     TDGS_REQUIRE(bytes == 0 || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
                  "linear: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, bytes);
     LnArgs r = {};
-    r.a = ln_matrix(a->x);
-    r.b = ln_matrix(a->weight);
+    r.a = ln_operand_rows(a->x, a->rows, a->in_features);
+    r.b = ln_weight(a);
     r.P = (int32_t)a->rows;
     r.Q = a->out_features;
     r.R = a->in_features;
@@ -1206,7 +1219,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     // float16 and a slope: the products of both may pass the type's range, or leave it with few bits
     const bool ranged = slope && a->activation != TDGS_ACT_RELU && a->dtype == TDGS_F16;
     LnArgs r = {};
-    r.a = slope ? e.dz : ln_matrix(g->dout);
+    r.a = slope ? e.dz : ln_operand_rows(g->dout, a->rows, a->out_features);
     if (ranged) {
         e.top = top;
         e.tops = (int32_t)(a->rows < kLnTops ? a->rows : kLnTops);
@@ -1236,7 +1249,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
         }
         if (want_dx) {
             LnArgs x = r;   // dx = dz W^T
-            x.b = ln_matrix(a->weight);
+            x.b = ln_weight(a);
             x.P = (int32_t)a->rows;
             x.Q = a->in_features;
             x.R = a->out_features;
@@ -1250,8 +1263,9 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             w.out = ln_matrix(g->dweight);
             w.P = dw_in_out ? a->in_features : a->out_features;
             w.Q = dw_in_out ? a->out_features : a->in_features;
-            w.b = dw_in_out ? r.a : ln_matrix(a->x);
-            w.a = dw_in_out ? ln_matrix(a->x) : r.a;
+            const LnMatrix rows_x = ln_operand_rows(a->x, a->rows, a->in_features);
+            w.b = dw_in_out ? r.a : rows_x;
+            w.a = dw_in_out ? rows_x : r.a;
             TDGS_TRY((ln_product<T, false, false>(w, part, stream)));
         }
         return TDGS_OK;
