@@ -19,6 +19,8 @@
 
 namespace tdgs {
 
+constexpr int kLnCus = 256;
+
 struct LnMatrix {
     void* p;
     int64_t stride;
@@ -316,6 +318,22 @@ __device__ __forceinline__ void ln_end(const LnArgs& a, const f32x16 (&acc)[S::N
     }
 }
 
+// Which tile a workgroup takes. Items that follow each other run on one XCD (xcd_band_item) at the same time, and go down
+// kLnGroup tiles of rows before they go on to the next columns, so that fewer different pieces of A and B pass
+// through its L2 together (8192^3 bfloat16 by 256x256 876 us, 920 row by row; by 128x256 980 and 1268).
+constexpr int kLnGroup = 8;
+struct LnPlace {
+    int split, p, q;
+    __device__ __forceinline__ explicit LnPlace(const LnArgs& a) {
+        const int item = xcd_band_item(blockIdx.x, gridDim.x), tiles = a.tiles_p * a.tiles_q;
+        split = item / tiles;
+        const int tile = item - split * tiles, first = tile / (kLnGroup * a.tiles_q) * kLnGroup;
+        const int rows = min(kLnGroup, a.tiles_p - first), rest = tile - first * a.tiles_q;
+        q = rest / rows;
+        p = first + rest - q * rows;
+    }
+};
+
 template <class S>
 __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     using T = typename S::T;
@@ -323,9 +341,8 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     T* const s = reinterpret_cast<T*>(s_mem);
     const int wave = (int)threadIdx.x / kWave, lane = (int)__lane_id();
     const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
-    const int item = xcd_band_item(blockIdx.x, gridDim.x);
-    const int tiles = a.tiles_p * a.tiles_q, split = item / tiles, tile = item - split * tiles;
-    const int p0 = tile / a.tiles_q * S::BP, q0 = tile % a.tiles_q * S::BQ;
+    const LnPlace at(a);
+    const int split = at.split, p0 = at.p * S::BP, q0 = at.q * S::BQ;
     const int r_begin = split * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
     const int steps = (r_end - r_begin + S::BK - 1) / S::BK;
 
@@ -363,9 +380,9 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     };
     auto store = [&](int step) {
         const int nr = r_end - r_begin - step * S::BK;
-        T* const at = s + (step & 1) * (S::kA + S::kB);
-        ta.template store<S::NARROW>(at, S::AD ? np : nr, S::AD ? nr : np);
-        tb.template store<S::NARROW>(at + S::kA, S::BD ? nq : nr, S::BD ? nr : nq);
+        T* const lds = s + (step & 1) * (S::kA + S::kB);
+        ta.template store<S::NARROW>(lds, S::AD ? np : nr, S::AD ? nr : np);
+        tb.template store<S::NARROW>(lds + S::kA, S::BD ? nq : nr, S::BD ? nr : nq);
     };
     if constexpr (!S::NARROW) place(S::BK);
     if (steps > 0) {
@@ -505,9 +522,8 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)s_mem;
     const int wave = (int)threadIdx.x / kWave;
     const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
-    const int item = xcd_band_item(blockIdx.x, gridDim.x);
-    const int tiles = a.tiles_p * a.tiles_q, split = item / tiles, tile = item - split * tiles;
-    const int p0 = tile / a.tiles_q * S::BP, q0 = tile % a.tiles_q * S::BQ;
+    const LnPlace place(a);
+    const int split = place.split, p0 = place.p * S::BP, q0 = place.q * S::BQ;
     const int r_begin = split * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
     const int steps = (r_end - r_begin) / S::BK, rest = (r_end - r_begin) % S::BK;
 
@@ -761,19 +777,24 @@ struct LnGradArgs {
     float* scale;               // what undoes dz's power of two
 };
 
-// The largest |dout| of each workgroup's share (float16).
-constexpr int kLnTops = 256;
+// The largest |dout| of each workgroup's share (float16), which together go through memory from front to back.
+constexpr int kLnTops = 1024;
 template <class T>
 __global__ __launch_bounds__(kLnThreads) void k_linear_top(LnGradArgs a, float* top) {
     __shared__ float s[kLnThreads / kWave];
+    const int t = (int)threadIdx.x, across = 1 << a.shift, down = kLnThreads >> a.shift;
     float m = 0.0f;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* const p = (const T*)a.dout.p + r * a.dout.stride;
-        for (int q = (int)threadIdx.x * 8; q < a.n; q += kLnThreads * 8) {
-            float v[8];
-            LnVec<T>::load(p + q, min(8, a.n - q), v);
+    constexpr int U = 4;
+    for (int q = (t & (across - 1)) * 8; q < a.n; q += across * 8) {
+        for (int64_t r = (int64_t)blockIdx.x * U * down + (t >> a.shift); r < a.rows; r += (int64_t)gridDim.x * U * down) {
+            float v[U][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+            for (int u = 0; u < U; ++u)
+                LnVec<T>::load((const T*)a.dout.p + min(r + u * down, a.rows - 1) * a.dout.stride + q, min(8, a.n - q), v[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[u][i]));
         }
     }
     for (int w = kWave / 2; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, kWave));
@@ -803,7 +824,8 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
     const int q = ((int)blockIdx.x * across + (t & (across - 1))) * 8, y = t >> a.shift;
     float up = 1.0f;
     if (a.top) {
-        float m = a.top[t % a.tops];
+        float m = 0.0f;
+        for (int i = t; i < a.tops; i += kLnThreads) m = fmaxf(m, a.top[i]);
         for (int w = kWave / 2; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, kWave));
         s[t] = m;
         __syncthreads();
@@ -905,7 +927,6 @@ constexpr LnForm kLnF32[2] = {{64, 64, ln_depth<float>(), 8, 3.0f, 0.5f, 0.3f}, 
 constexpr LnForm kLn16[kLnForms] = {{64, 64, ln_depth<bf16>(), 6, 3.0f, 0.5f, 0.25f}, {128, 128, ln_depth<bf16>(), 3, 5.0f, 0.8f, 0.42f},
                                     {64, 64, 64, 4, 3.0f, 0.46f, 0.206f},  {128, 64, 64, 3, 4.0f, 0.6f, 0.34f},
                                     {128, 128, 64, 2, 5.0f, 0.85f, 0.59f}, {128, 256, 32, 2, 3.0f, 0.8f, 0.62f}, {256, 256, 64, 1, 12.0f, 1.93f, 1.93f}};
-constexpr int kLnCus = 256;
 constexpr int kLnLeastSteps = 4;   // of a split
 
 // How a product is cut.
@@ -915,7 +936,7 @@ struct LnPlan {
 };
 
 // The form and the splits that take the least time: rounds of the workgroups of the fullest CU, and the join, which
-// reads at 6 TB/s what the splits have left in the last-level cache.
+// reads at 6 TB/s what the splits have left in the last-level cache, one after the other.
 static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direct) {
     if (P < 1 || Q < 1 || R < 1) return {};
     const bool f32 = dtype == TDGS_F32;
@@ -941,7 +962,7 @@ static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direc
             const int64_t on = ceil_div(tiles * splits, kLnCus), together = on < f.per_cu ? on : f.per_cu;
             const float step = f.full * together > f.alone ? f.full * together : f.alone;
             float time = (float)ceil_div(on, f.per_cu) * (f.ends + per * step);
-            if (splits > 1) time += 3.0f + (float)splits * P * Q * 4.0f / 6e6f;
+            if (splits > 1) time += 3.0f + 0.012f * splits + (float)splits * P * Q * 4.0f / 6e6f;
             if (time < least) {
                 least = time;
                 best.form = form;
@@ -1038,7 +1059,7 @@ static int ln_check(const tdgs_linear* a) {
     TDGS_REQUIRE(known_dtype(a->dtype), "linear: unknown element type %d", a->dtype);
     TDGS_REQUIRE(a->activation >= TDGS_ACT_IDENTITY && a->activation <= TDGS_ACT_RELU, "linear: unknown activation %d",
                  a->activation);
-    TDGS_REQUIRE(a->rows >= 0 && a->rows <= INT32_MAX - 65536, "linear: %lld rows", (long long)a->rows);
+    TDGS_REQUIRE(a->rows >= 0 && a->rows <= INT32_MAX - (1 << 20), "linear: %lld rows", (long long)a->rows);
     TDGS_REQUIRE(a->in_features >= 1 && a->out_features >= 1 && a->in_features <= (1 << 20) && a->out_features <= (1 << 20) &&
                      (int64_t)a->in_features * a->out_features <= ((int64_t)1 << 36),
                  "linear: a weight matrix of %d x %d", a->in_features, a->out_features);
@@ -1222,7 +1243,8 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     r.a = slope ? e.dz : ln_operand_rows(g->dout, a->rows, a->out_features);
     if (ranged) {
         e.top = top;
-        e.tops = (int32_t)(a->rows < kLnTops ? a->rows : kLnTops);
+        const int64_t runs = ceil_div(a->rows, 4 * (kLnThreads >> p.shift));
+        e.tops = (int32_t)(runs < kLnTops ? runs : kLnTops);
         e.scale = top + kLnTops;
         r.scale = e.scale;
     }
