@@ -470,23 +470,52 @@ struct LfTile {
     }
 };
 
-// ln_operand of such a tile.
-template <class T, bool DEPTH, int MIN>
-__device__ __forceinline__ typename Elem<T>::V8 lf_operand(const T* lds, int base, int c) {
-    const int l = (int)__lane_id();
-    if constexpr (DEPTH) {
-        const int row = base + (l & 31);
-        return *reinterpret_cast<const typename Elem<T>::V8a*>(lds + row * MIN + ((c * 2 + (l >> 5)) ^ lf_key<true, MIN>(l & 31)) * 8);
-    } else {
-        typedef short s4 __attribute__((ext_vector_type(4)));
-        const int row = c * 16 + (l >> 5) * 8 + ((l & 15) >> 2), piece = base / 8 + ((l >> 4) & 1) * 2 + ((l & 3) >> 1);
-        const T* p = lds + row * MIN + (piece ^ lf_key<false, MIN>((l >> 2) & 3)) * 8 + (l & 1) * 4;
-        typedef __attribute__((address_space(3))) s4* lp;
-        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
-        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * MIN));
-        return __builtin_bit_cast(typename Elem<T>::V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+// The operands (ln_operand) of such a tile: N blocks of 32 items by NC chunks of the depth. Which piece a lane reads depends on
+// the chunk where the depth is contiguous and on the block where the items are; those places are made once, and all else
+// is a constant offset. (Left to itself, the compiler makes them again in every step: 25 vector operations next to 8
+// products.)
+template <class T, bool DEPTH, int MIN, int N, int NC>
+struct LfOperands {
+    static constexpr int K = DEPTH ? NC : N;
+    uint32_t at[K];
+    __device__ __forceinline__ LfOperands(uint32_t lds, int base) {
+        const int l = (int)__lane_id();
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            int e;
+            if constexpr (DEPTH) {
+                e = (base + (l & 31)) * MIN + ((k * 2 + (l >> 5)) ^ lf_key<true, MIN>(l & 31)) * 8;
+            } else {
+                const int row = (l >> 5) * 8 + ((l & 15) >> 2), piece = (base + k * 32) / 8 + ((l >> 4) & 1) * 2 + ((l & 3) >> 1);
+                e = row * MIN + (piece ^ lf_key<false, MIN>((l >> 2) & 3)) * 8 + (l & 1) * 4;
+            }
+            at[k] = lds + (uint32_t)e * (uint32_t)sizeof(T);
+            asm volatile("" : "+v"(at[k]));
+        }
     }
-}
+    // The places in the stage that starts `stage` bytes on.
+    __device__ __forceinline__ LfOperands(const LfOperands& first, uint32_t stage) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            at[k] = first.at[k] + stage;
+            asm volatile("" : "+v"(at[k]));
+        }
+    }
+    // Block i, chunk c.
+    __device__ __forceinline__ typename Elem<T>::V8 fetch(int i, int c) const {
+        if constexpr (DEPTH) {
+            typedef __attribute__((address_space(3))) const typename Elem<T>::V8a* lp;
+            return *(lp)(uintptr_t)(at[c] + (uint32_t)(i * 32 * MIN * (int)sizeof(T)));
+        } else {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s4* lp;
+            const uint32_t p = at[i] + (uint32_t)(c * 16 * MIN * (int)sizeof(T));
+            const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)p);
+            const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)(p + 4 * MIN * (int)sizeof(T)));
+            return __builtin_bit_cast(typename Elem<T>::V8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
 
 template <class T_, int BP_, int BQ_, int WP_, int WQ_, int BK_, int STAGES_, int PER_CU_, bool AD_, bool BD_>
 struct LfShape {
@@ -551,16 +580,18 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
         pa += step_a;
         pb += step_b;
     };
+    constexpr int NC = S::BK / 16;
+    const LfOperands<T, S::AD, S::AMIN, S::NP, NC> oa(lds, wp);
+    const LfOperands<T, S::BD, S::BMIN, S::NQ, NC> ob(lds + S::kA * (int)sizeof(T), wq);
     auto multiply = [&](int stage) {
-        const T* const la = s + stage * kStage;
-        const T* const lb = la + S::kA;
-        constexpr int NC = S::BK / 16;
+        const decltype(oa) la(oa, stage * kStage * (int)sizeof(T));
+        const decltype(ob) lb(ob, stage * kStage * (int)sizeof(T));
         typename Elem<T>::V8 fa[2][S::NP], fb[2][S::NQ];
         auto fetch = [&](int c) {
 #pragma unroll
-            for (int i = 0; i < S::NP; ++i) fa[c & 1][i] = lf_operand<T, S::AD, S::AMIN>(la, wp + i * 32, c);
+            for (int i = 0; i < S::NP; ++i) fa[c & 1][i] = la.fetch(i, c);
 #pragma unroll
-            for (int j = 0; j < S::NQ; ++j) fb[c & 1][j] = lf_operand<T, S::BD, S::BMIN>(lb, wq + j * 32, c);
+            for (int j = 0; j < S::NQ; ++j) fb[c & 1][j] = lb.fetch(j, c);
         };
         fetch(0);
 #pragma unroll
@@ -571,8 +602,8 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
 #pragma unroll
                 for (int j = 0; j < S::NQ; ++j) acc[i][j] = mma(fb[c & 1][j], fa[c & 1][i], acc[i][j]);
         }
+        // the reads of the next chunk go between the products of this one
         constexpr int kReads = S::NP * (S::AD ? 1 : 2) + S::NQ * (S::BD ? 1 : 2), kProducts = S::NP * S::NQ;
-#ifndef LN_NOSCHED
         __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
 #pragma unroll
         for (int c = 0; c + 1 < NC; ++c) {
@@ -584,7 +615,6 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
             }
         }
         __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
-#endif
     };
 #pragma unroll
     for (int n = 0; n < S::STAGES - 1; ++n)
