@@ -3,7 +3,8 @@
 //
 // Philox4x32-10 (Salmon, Moraes, Dror & Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011) encrypts
 // the counter (element / 4, call) with the seed as key into the four words of four neighbouring elements. All 32
-// bits decide, so that any p is met to 2^-32.
+// bits decide, so that any p is met to 2^-32. Ten rounds for four elements are as much as the memory is for: 64800 x 1024
+// bfloat16 with a residual take 69 us (398 MB, 5.8 TB/s, partly from the last-level cache) with vector issue busy for 92%.
 #include "internal.hpp"
 #include "elem.hpp"
 #include "philox.hpp"

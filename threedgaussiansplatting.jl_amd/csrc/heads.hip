@@ -13,7 +13,8 @@
 //
 // With r = 1 / sqrt(mean x^2 + eps), xhat = r x, u the output's gradient rotated back and e = u w:
 // dw = sum u xhat, dx = r (e - xhat mean(e xhat)); r is computed again from x, which is read anyway. All of it is
-// bound by memory: each row is read once and written once.
+// bound by memory: each row is read once and written once. 32400 tokens x 32 heads of 64 bfloat16: 60 us (265 MB, 4.4 TB/s),
+// the rotation alone 57, gradients 85; few tokens by the latency of their positions, rows and stores.
 #include "internal.hpp"
 #include "elem.hpp"
 
