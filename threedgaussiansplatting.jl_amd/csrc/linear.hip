@@ -9,7 +9,7 @@
 // whose items are contiguous are transposed by the reads from LDS. Where a row's end is no multiple of 16 bytes,
 // its last chunk is loaded from the row's last 16 bytes and shifted into place, so that nothing is
 // read past a row. The depth is split where there are few tiles, and partial sums of 32 bits joined by a
-// second kernel, in the order of the splits.
+// second kernel, which joins all that a call has left to join, in the order of the splits.
 //
 // The epilogue turns blocks through LDS, so that 16 bytes of a row are one lane's, and adds the bias, keeps z where
 // wanted, applies the activation and adds the residual, all in 32 bits; only what is stored is rounded.
@@ -652,24 +652,23 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
     ln_end<S>(a, acc, reinterpret_cast<float*>(s_mem), p0 + wp, q0 + wq, split);
 }
 
-// Joins the splits' sums, eight neighbouring results by G threads, each of which takes every G-th split.
+// Joins the splits' sums, eight neighbouring results by G threads, each of which takes every G-th split. Workgroup `block`.
 constexpr int kLnThreads = 256;
 template <class T, int G>
-__global__ __launch_bounds__(kLnThreads) void k_linear_join(LnArgs a) {
+__device__ __forceinline__ void ln_join(const LnArgs& a, int block, f32x8* s) {
     constexpr int N = kLnThreads / G;
-    __shared__ f32x8 s[G > 1 ? G : 1][G > 1 ? N : 1];
     const int chunks = a.part_q / 8, x = (int)threadIdx.x % N, y = (int)threadIdx.x / N;
-    const int64_t i = (int64_t)blockIdx.x * N + x, all = (int64_t)a.P * chunks;
+    const int64_t i = (int64_t)block * N + x, all = (int64_t)a.P * chunks;
     const int64_t p = (i < all ? i : all - 1) / chunks;
     const int q = (int)((i < all ? i : all - 1) - p * chunks) * 8;
     f32x8 sum = {};
     for (int k = y; k < a.splits; k += G) sum += *reinterpret_cast<const f32x8*>(a.part + ((int64_t)k * a.P + p) * a.part_q + q);
     if constexpr (G > 1) {
-        s[y][x] = sum;
+        s[threadIdx.x] = sum;
         __syncthreads();
         if (y != 0) return;
 #pragma unroll 4
-        for (int g = 1; g < G; ++g) sum += s[g][x];
+        for (int g = 1; g < G; ++g) sum += s[g * N + x];
     }
     if (i >= all) return;
     float v[8], bias[8];
@@ -678,6 +677,53 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_join(LnArgs a) {
     const int n = min(8, a.Q - q);
     ln_bias<T>(a, q, n, bias);
     ln_finish<T>(a, a.scale ? *a.scale : 1.0f, bias, p, q, n, v);
+}
+
+// dbias from the runs' sums: eight columns per workgroup.
+constexpr int kLnBiasCols = 8;
+template <class T>
+__device__ __forceinline__ void ln_dbias(const float* __restrict__ sums, int blocks, int n, T* dbias, int block, float* s) {
+    const int x = (int)threadIdx.x % kLnBiasCols, y = (int)threadIdx.x / kLnBiasCols, c = block * kLnBiasCols + x;
+    float v = 0.0f;
+    if (c < n) {
+#pragma unroll 8
+        for (int b = y; b < blocks; b += kLnThreads / kLnBiasCols) v += sums[(int64_t)b * n + c];
+    }
+    s[y * (kLnBiasCols + 1) + x] = v;
+    __syncthreads();
+    if (y != 0 || c >= n) return;
+    for (int i = 1; i < kLnThreads / kLnBiasCols; ++i) v += s[i * (kLnBiasCols + 1) + x];
+    dbias[c] = (T)v;
+}
+
+// What a call has to join, in one launch at its end: up to two products, and dbias.
+struct LnJoins {
+    LnArgs product[2];
+    int32_t together[2], blocks[2];   // ln_join's G; workgroups
+    int32_t products, sum_blocks, n, bias_blocks;
+    const float* sums;
+    void* dbias;
+    int64_t grid() const {
+        int64_t g = bias_blocks;
+        for (int i = 0; i < products; ++i) g += blocks[i];
+        return g;
+    }
+};
+template <class T>
+__global__ __launch_bounds__(kLnThreads) void k_linear_join(LnJoins j) {
+    __shared__ f32x8 s[kLnThreads];
+    int block = blockIdx.x;
+    for (int i = 0; i < j.products; ++i) {
+        if (block < j.blocks[i]) {
+            switch (j.together[i]) {
+                case 1: ln_join<T, 1>(j.product[i], block, s); return;
+                case 4: ln_join<T, 4>(j.product[i], block, s); return;
+                default: ln_join<T, 32>(j.product[i], block, s); return;
+            }
+        }
+        block -= j.blocks[i];
+    }
+    ln_dbias<T>(j.sums, j.sum_blocks, j.n, (T*)j.dbias, block, (float*)s);
 }
 
 // ---- few rows: the weight is read once, by vectors, in one launch ----------------------------
@@ -926,24 +972,6 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
     }
 }
 
-// dbias from the runs' sums: eight columns per workgroup.
-constexpr int kLnBiasCols = 8;
-template <class T>
-__global__ __launch_bounds__(kLnThreads) void k_linear_dbias(const float* __restrict__ sums, int blocks, int n, T* dbias) {
-    __shared__ float s[kLnThreads / kLnBiasCols][kLnBiasCols + 1];
-    const int x = (int)threadIdx.x % kLnBiasCols, y = (int)threadIdx.x / kLnBiasCols, c = blockIdx.x * kLnBiasCols + x;
-    float v = 0.0f;
-    if (c < n) {
-#pragma unroll 8
-        for (int b = y; b < blocks; b += kLnThreads / kLnBiasCols) v += sums[(int64_t)b * n + c];
-    }
-    s[y][x] = v;
-    __syncthreads();
-    if (y != 0 || c >= n) return;
-    for (int i = 1; i < kLnThreads / kLnBiasCols; ++i) v += s[i][x];
-    dbias[c] = (T)v;
-}
-
 // What is zero without rows (dweight and dbias).
 template <class T>
 __global__ __launch_bounds__(kLnThreads) void k_linear_zero(T* p, int64_t rows, int cols, int64_t stride) {
@@ -1033,9 +1061,19 @@ static bool ln_few(int64_t size, int64_t P, int64_t Q, int64_t R) {
     return size == 4 ? P <= kLsRows : P <= 4 && Q * R <= (1 << 21);
 }
 
-// C = A B, with what follows it in `r`.
+template <class T>
+static int ln_launch_joins(const LnJoins& j, hipStream_t stream) {
+    if (j.grid() == 0) return TDGS_OK;
+    TDGS_REQUIRE(j.grid() <= INT32_MAX, "linear: too many results to join");
+    k_linear_join<T><<<(unsigned)j.grid(), kLnThreads, 0, stream>>>(j);
+    TDGS_LAUNCHED();
+    return TDGS_OK;
+}
+
+// C = A B, with what follows it in `r`, but for the joining of splits, which is left to `joins`. Partial sums go to *temp, which is
+// moved on behind them.
 template <class T, bool AD, bool BD>
-static int ln_product(LnArgs r, void* temp, hipStream_t stream) {
+static int ln_product(LnArgs r, char** temp, LnJoins* joins, hipStream_t stream) {
     const int32_t dtype = sizeof(T) == 4 ? TDGS_F32 : std::is_same<T, bf16>::value ? TDGS_BF16 : TDGS_F16;
     if (AD && ln_few(sizeof(T), r.P, r.Q, r.R)) {
         auto few = [&](auto rows) {
@@ -1057,7 +1095,8 @@ static int ln_product(LnArgs r, void* temp, hipStream_t stream) {
     r.splits = p.splits;
     r.steps = p.steps;
     r.part_q = p.part_q;
-    r.part = p.splits > 1 ? (float*)temp : nullptr;
+    r.part = p.splits > 1 ? (float*)*temp : nullptr;
+    *temp += p.bytes;
     const int64_t grid = (int64_t)p.tiles_p * p.tiles_q * p.splits;
     TDGS_REQUIRE(grid <= INT32_MAX, "linear: too many tiles");
     constexpr int C = ln_chunk<T>(), D = ln_depth<T>();
@@ -1084,15 +1123,12 @@ static int ln_product(LnArgs r, void* temp, hipStream_t stream) {
     }
     TDGS_LAUNCHED();
     if (p.splits > 1) {
-        const int64_t chunks = (int64_t)r.P * (p.part_q / 8);
-        auto join = [&](auto g) {
-            constexpr int G = decltype(g)::value;
-            k_linear_join<T, G><<<(unsigned)ceil_div(chunks, kLnThreads / G), kLnThreads, 0, stream>>>(r);
-        };
-        if (p.splits < 8) join(std::integral_constant<int, 1>{});
-        else if (p.splits < 64) join(std::integral_constant<int, 4>{});
-        else join(std::integral_constant<int, 32>{});
-        TDGS_LAUNCHED();
+        const int i = joins->products++, g = p.splits < 8 ? 1 : p.splits < 64 ? 4 : 32;
+        joins->product[i] = r;
+        joins->together[i] = g;
+        const int64_t blocks = ceil_div((int64_t)r.P * (p.part_q / 8), kLnThreads / g);
+        TDGS_REQUIRE(blocks <= INT32_MAX, "linear: too many results to join");
+        joins->blocks[i] = (int32_t)blocks;
     }
     return TDGS_OK;
 }
@@ -1166,12 +1202,10 @@ static LnGradPlan ln_grad_plan(const tdgs_linear* a) {
     if (blocks > ceil_div(a->rows, 2 * down)) blocks = ceil_div(a->rows, 2 * down);
     g.blocks = (int)blocks;
     g.sums = align_up((size_t)g.blocks * a->out_features * sizeof(float));
-    // (the weight's gradient or its transpose, whichever is asked for)
-    g.part = ln_part_bytes(a->dtype, a->rows, a->in_features, a->out_features);
+    // dx and (the weight's gradient or its transpose, whichever is asked for)
     const size_t dw = ln_part_bytes(a->dtype, a->in_features, a->out_features, a->rows);
     const size_t t = ln_part_bytes(a->dtype, a->out_features, a->in_features, a->rows);
-    if (dw > g.part) g.part = dw;
-    if (t > g.part) g.part = t;
+    g.part = ln_part_bytes(a->dtype, a->rows, a->in_features, a->out_features) + (dw > t ? dw : t);
     g.bytes = g.dz + g.small + g.sums + g.part;
     return g;
 }
@@ -1218,8 +1252,11 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     hipStream_t stream = (hipStream_t)stream_;
     return with_dtype(a->dtype, [&](auto t) -> int {
         using T = decltype(t);
-        return a->weight_layout == TDGS_WEIGHT_IN_OUT ? ln_product<T, true, false>(r, a->temp, stream)
-                                                      : ln_product<T, true, true>(r, a->temp, stream);
+        LnJoins joins = {};
+        char* at = (char*)a->temp;
+        if (a->weight_layout == TDGS_WEIGHT_IN_OUT) TDGS_TRY((ln_product<T, true, false>(r, &at, &joins, stream)));
+        else TDGS_TRY((ln_product<T, true, true>(r, &at, &joins, stream)));
+        return ln_launch_joins<T>(joins, stream);
     });
 }
 
@@ -1274,7 +1311,6 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     at += p.small;
     e.sums = want_db ? (float*)at : nullptr;
     at += p.sums;
-    void* const part = at;
     e.rows = a->rows;
     e.n = a->out_features;
     e.act = a->activation;
@@ -1307,10 +1343,13 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             }
             TDGS_LAUNCHED();
         }
+        LnJoins joins = {};
         if (want_db) {
-            k_linear_dbias<T><<<(unsigned)ceil_div(a->out_features, kLnBiasCols), kLnThreads, 0, stream>>>(
-                e.sums, p.blocks, a->out_features, (T*)g->dbias);
-            TDGS_LAUNCHED();
+            joins.sums = e.sums;
+            joins.sum_blocks = p.blocks;
+            joins.n = a->out_features;
+            joins.dbias = g->dbias;
+            joins.bias_blocks = (int32_t)ceil_div(a->out_features, kLnBiasCols);
         }
         if (want_dx) {
             LnArgs x = r;   // dx = dz W^T
@@ -1319,8 +1358,8 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             x.Q = a->in_features;
             x.R = a->out_features;
             x.out = ln_matrix(g->dx);
-            if (a->weight_layout == TDGS_WEIGHT_IN_OUT) TDGS_TRY((ln_product<T, true, true>(x, part, stream)));
-            else TDGS_TRY((ln_product<T, true, false>(x, part, stream)));
+            if (a->weight_layout == TDGS_WEIGHT_IN_OUT) TDGS_TRY((ln_product<T, true, true>(x, &at, &joins, stream)));
+            else TDGS_TRY((ln_product<T, true, false>(x, &at, &joins, stream)));
         }
         if (want_dw) {
             LnArgs w = r;   // dW = x^T dz, or its transpose dz^T x
@@ -1331,9 +1370,9 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             const LnMatrix rows_x = ln_operand_rows(a->x, a->rows, a->in_features);
             w.b = dw_in_out ? r.a : rows_x;
             w.a = dw_in_out ? rows_x : r.a;
-            TDGS_TRY((ln_product<T, false, false>(w, part, stream)));
+            TDGS_TRY((ln_product<T, false, false>(w, &at, &joins, stream)));
         }
-        return TDGS_OK;
+        return ln_launch_joins<T>(joins, stream);
     });
 }
 
