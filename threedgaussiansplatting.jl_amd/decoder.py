@@ -556,47 +556,60 @@ class Rotary:
 
 def _head_norm(q, k, q_weight, k_weight, norm, eps, rotary, positions, inverse):
     """The fields of the tdgs_head_norm of these tensors up to q, and those of the weights."""
-    _check_tensor(q, "q", q)
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        _check_tensor(q, "q", q)
     dtype = DTYPES.get(q.dtype)
     if dtype is None:
         raise ValueError(f"q is {q.dtype}: float32, bfloat16 and float16 are supported")
     if q.dim() != 4:
         raise ValueError("q must be (batch, length, heads, head_dim)")
     b, l, h, d = q.shape
+    device = q.get_device()
     hk = 0
     if k is not None:
-        if k.dim() != 4 or k.shape[:2] != (b, l) or k.shape[3] != d:
+        if k.dim() != 4 or k.shape != (b, l, k.shape[2], d):
             raise ValueError(f"k has shape {tuple(k.shape)}, not ({b}, {l}, heads, {d})")
         hk = k.shape[2]
     first = q_weight if q_weight is not None else k_weight
-    param = abi.TDGS_F32
+    param, wq, wk = abi.TDGS_F32, 0, 0
     if first is not None:
-        param = DTYPES.get(first.dtype)
-        if first.dtype is not torch.float32 and first.dtype is not q.dtype:
+        kind = first.dtype
+        param = DTYPES.get(kind)
+        if kind is not torch.float32 and kind is not q.dtype:
             raise ValueError(f"q_weight and k_weight must be of one type, float32 or {q.dtype}")
-        for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-            if w is not None and (w.dtype is not first.dtype or w.shape != (d,) or w.get_device() != q.get_device()
-                                  or not w.is_contiguous()):
-                _check_tensor(w, name, q)
-                raise ValueError(f"{name} must be {d} contiguous values of {first.dtype}")
+        if q_weight is not None:
+            wq = _head_weight(q_weight, "q_weight", kind, d, q, device)
+        if k_weight is not None:
+            wk = _head_weight(k_weight, "k_weight", kind, d, q, device)
     if rotary is None:
         if positions is not None:
             raise ValueError("positions without a rotary")
-        rotation, place = (0,) * 7, (0, 0, 0, 0)
+        rotation, place = _NO_ROTATION, _NO_PLACE
     else:
-        if not isinstance(positions, torch.Tensor) or not q.get_device() == positions.get_device() == rotary.device:
+        if not isinstance(positions, torch.Tensor) or not device == positions.get_device() == rotary.device:
             _check_tensor(rotary.turns, "the rotary", q)
             _check_tensor(positions, "positions", q)
         kind = _POSITIONS.get(positions.dtype)
         if kind is None:
             raise ValueError(f"positions are {positions.dtype}: int32, int64 and float32 are supported")
-        n = positions.shape
-        if (n != (l, rotary.axes) and n != (b, l, rotary.axes)) or not positions.is_contiguous():
-            raise ValueError(f"positions must be contiguous, ({l}, {rotary.axes}) or ({b}, {l}, {rotary.axes})")
+        n, axes = positions.shape, rotary.axes
+        batched = len(n) == 3
+        if n != ((b, l, axes) if batched else (l, axes)) or not positions.is_contiguous():
+            raise ValueError(f"positions must be contiguous, ({l}, {axes}) or ({b}, {l}, {axes})")
         rotation = rotary._fields
-        place = (kind, rotary.pointer, positions.data_ptr(), l * rotary.axes if len(n) == 3 else 0)
-    return ((dtype, param, b, l, h, hk, d, int(norm), eps, *rotation, int(inverse), *place),
-            (dptr(q_weight) or 0, dptr(k_weight) or 0))
+        place = (kind, rotary.pointer, positions.data_ptr(), l * axes if batched else 0)
+    return ((dtype, param, b, l, h, hk, d, 1 if norm else 0, eps, *rotation, 1 if inverse else 0, *place), (wq, wk))
+
+
+_NO_ROTATION, _NO_PLACE = (0,) * 7, (0,) * 4
+
+
+def _head_weight(w, name, dtype, d, q, device):
+    """The pointer of d contiguous values of a type."""
+    if w.dtype is not dtype or w.shape != (d,) or w.get_device() != device or not w.is_contiguous():
+        _check_tensor(w, name, q)
+        raise ValueError(f"{name} must be {d} contiguous values of {dtype}")
+    return w.data_ptr()
 
 
 def _head_view(t, name, shape, like, device):
