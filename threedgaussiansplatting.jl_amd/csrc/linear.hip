@@ -42,6 +42,7 @@ struct LnArgs {
     LnMatrix out, residual, pre;
     const void* bias;
     const float* scale;       // null, or out = *scale C, without a bias
+    const void *a2, *b2;      // null, or C = A B + A2 B2 of matrices that lie as A and B do: the second half of the splits
 };
 
 // Elements of 16 bytes.
@@ -352,7 +353,8 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
     const LnPlace at(a);
     const int split = at.split, p0 = at.p * S::BP, q0 = at.q * S::BQ;
-    const int r_begin = split * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
+    const bool second = a.a2 && split >= a.splits / 2;
+    const int r_begin = (second ? split - a.splits / 2 : split) * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
     const int steps = (r_end - r_begin + S::BK - 1) / S::BK;
 
     f32x16 acc[S::NP][S::NQ];
@@ -367,8 +369,8 @@ __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     LnTile<T, S::BMAJ, S::BMIN, S::TH, S::BPITCH> tb;
     const int np = min(S::BP, a.P - p0), nq = min(S::BQ, a.Q - q0);
     const int64_t step_a = S::AD ? S::BK : S::BK * a.a.stride, step_b = S::BD ? S::BK : S::BK * a.b.stride;
-    const T* pa = (const T*)a.a.p + (S::AD ? p0 * a.a.stride + r_begin : r_begin * a.a.stride + p0);
-    const T* pb = (const T*)a.b.p + (S::BD ? q0 * a.b.stride + r_begin : r_begin * a.b.stride + q0);
+    const T* pa = (const T*)(second ? a.a2 : a.a.p) + (S::AD ? p0 * a.a.stride + r_begin : r_begin * a.a.stride + p0);
+    const T* pb = (const T*)(second ? a.b2 : a.b.p) + (S::BD ? q0 * a.b.stride + r_begin : r_begin * a.b.stride + q0);
     auto place = [&](int nr) {
         ta.place(a.a.stride, S::AD ? np : nr, S::AD ? nr : np);
         tb.place(a.b.stride, S::BD ? nq : nr, S::BD ? nr : nq);
@@ -566,7 +568,8 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
     const int wp = wave / S::WQ * (S::BP / S::WP), wq = wave % S::WQ * (S::BQ / S::WQ);
     const LnPlace place(a);
     const int split = place.split, p0 = place.p * S::BP, q0 = place.q * S::BQ;
-    const int r_begin = split * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
+    const bool second = a.a2 && split >= a.splits / 2;
+    const int r_begin = (second ? split - a.splits / 2 : split) * a.steps * S::BK, r_end = min(a.R, r_begin + a.steps * S::BK);
     const int steps = (r_end - r_begin) / S::BK, rest = (r_end - r_begin) % S::BK;
 
     f32x16 acc[S::NP][S::NQ];
@@ -581,8 +584,8 @@ __global__ __launch_bounds__(S::TH, S::PER_CU * S::TH / 256) void k_linear_direc
     LfTile<T, S::BD, S::BMAJ, S::BMIN, S::TH> tb;
     const int np = min(S::BP, a.P - p0), nq = min(S::BQ, a.Q - q0);
     const int64_t step_a = S::AD ? S::BK : S::BK * a.a.stride, step_b = S::BD ? S::BK : S::BK * a.b.stride;
-    const T* pa = (const T*)a.a.p + (S::AD ? p0 * a.a.stride + r_begin : r_begin * a.a.stride + p0);
-    const T* pb = (const T*)a.b.p + (S::BD ? q0 * a.b.stride + r_begin : r_begin * a.b.stride + q0);
+    const T* pa = (const T*)(second ? a.a2 : a.a.p) + (S::AD ? p0 * a.a.stride + r_begin : r_begin * a.a.stride + p0);
+    const T* pb = (const T*)(second ? a.b2 : a.b.p) + (S::BD ? q0 * a.b.stride + r_begin : r_begin * a.b.stride + q0);
     ta.place(a.a.stride, S::AD ? np : S::BK, S::AD ? S::BK : np);
     tb.place(a.b.stride, S::BD ? nq : S::BK, S::BD ? S::BK : nq);
     constexpr int kStage = S::kA + S::kB, kLoads = decltype(ta)::kPer + decltype(tb)::kPer;
@@ -768,7 +771,11 @@ __global__ __launch_bounds__(kLsThreads) void k_linear_few_items(LnArgs a) {
                 const int r = r0 + u * (kLsThreads / 4), at = r < a.R ? r : a.R - 1;
                 w[u].load(b + at * a.b.stride, n);
 #pragma unroll
-                for (int p = 0; p < ROWS; ++p) e[u][p] = (float)x[(p < a.P ? p : 0) * a.a.stride + at];
+                for (int p = 0; p < ROWS; ++p) {
+                    const int64_t i = (p < a.P ? p : 0) * a.a.stride + at;
+                    e[u][p] = (float)x[i];
+                    if (a.a2) e[u][p] += (float)((const T*)a.a2)[i];
+                }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -821,7 +828,16 @@ __global__ __launch_bounds__(kLsThreads) void k_linear_few_depth(LnArgs a) {
 #pragma unroll
             for (int c = 0; c < COLS; ++c) w[u][c].load((const T*)a.b.p + (q0 + c < a.Q ? q0 + c : a.Q - 1) * a.b.stride + at, left);
 #pragma unroll
-            for (int p = 0; p < ROWS; ++p) x[u][p].load((const T*)a.a.p + (p < a.P ? p : 0) * a.a.stride + at, left);
+            for (int p = 0; p < ROWS; ++p) {
+                const int64_t i = (p < a.P ? p : 0) * a.a.stride + at;
+                x[u][p].load((const T*)a.a.p + i, left);
+                if (a.a2) {
+                    LsChunk<T> rest;
+                    rest.load((const T*)a.a2 + i, left);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) x[u][p].f[c] += rest.f[c];
+                }
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -858,6 +874,7 @@ __global__ __launch_bounds__(kLsThreads) void k_linear_few_depth(LnArgs a) {
 
 struct LnGradArgs {
     LnMatrix dout, pre, dz;     // dz null: not wanted
+    void* rest;                 // null, or what its rounding leaves of dz, which lies as dz does
     int64_t rows;
     int32_t n, act, blocks, shift;
     float* sums;                // blocks x n; null: not wanted
@@ -946,6 +963,16 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
                     if constexpr (std::is_same<T, f16>::value) d[u][i] *= up;
                 }
                 if (a.dz.p) LnVec<T>::store((T*)a.dz.p + (r + u * down) * a.dz.stride + q, n, d[u]);
+                if constexpr (sizeof(T) == 2) {
+                    if (a.rest) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float left = d[u][i] - (float)(T)d[u][i];
+                            d[u][i] = fabsf(left) < INFINITY ? left : 0.0f;   // (infinity and NaN are in dz)
+                        }
+                        LnVec<T>::store((T*)a.rest + (r + u * down) * a.dz.stride + q, n, d[u]);
+                    }
+                }
             }
         };
         constexpr int U = 2;
@@ -1008,7 +1035,8 @@ struct LnPlan {
 
 // The form and the splits that take the least time: rounds of the workgroups of the fullest CU, and the join, which
 // reads at 6 TB/s what the splits have left in the last-level cache, one after the other.
-static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direct) {
+// `two`: a sum of two products, each by as many splits.
+static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direct, bool two) {
     if (P < 1 || Q < 1 || R < 1) return {};
     const bool f32 = dtype == TDGS_F32;
     const int chunk = f32 ? 4 : 8;
@@ -1044,6 +1072,7 @@ static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direc
             }
         }
     }
+    if (two) best.splits *= 2;
     best.part_q = (int)(ceil_div(Q, 8) * 8);
     best.bytes = best.splits > 1 ? align_up((size_t)best.splits * P * best.part_q * sizeof(float)) : 0;
     return best;
@@ -1089,7 +1118,7 @@ static int ln_product(LnArgs r, char** temp, LnJoins* joins, hipStream_t stream)
         return TDGS_OK;
     }
     const bool aligned = sizeof(T) == 2 && ln_aligned(r.a, AD, r.P) && ln_aligned(r.b, BD, r.Q);
-    const LnPlan p = ln_plan(dtype, r.P, r.Q, r.R, aligned);
+    const LnPlan p = ln_plan(dtype, r.P, r.Q, r.R, aligned, r.a2 != nullptr);
     r.tiles_p = p.tiles_p;
     r.tiles_q = p.tiles_q;
     r.splits = p.splits;
@@ -1176,16 +1205,23 @@ static LnMatrix ln_weight(const tdgs_linear* a) {
                                                   : ln_operand_rows(a->weight, a->out_features, a->in_features);
 }
 
+// Up to so many elements of dz, which 16 bits round once more than the results, its products are taken of two operands, the second
+// holding what the rounding leaves of the first. Over a large dz that rounding makes dx and dweight 1.46 times as inexact
+// as the exact result rounded once (with the rounded z), over a few values it may be more; and it is large products that
+// the second operand would cost their time again, not these.
+constexpr int64_t kLnFewSlopes = 1 << 16;
+
 // The gradient's scratch: dz, its power of two, maxima and columns' sums, then a product's partial sums.
 struct LnGradPlan {
     int64_t dz_stride;
     int blocks, shift;
+    bool two;
     size_t dz, small, sums, part, bytes;
 };
 
 // Scratch of a product, whatever its operands' alignment.
-static size_t ln_part_bytes(int32_t dtype, int64_t P, int64_t Q, int64_t R) {
-    const size_t a = ln_plan(dtype, P, Q, R, false).bytes, b = ln_plan(dtype, P, Q, R, true).bytes;
+static size_t ln_part_bytes(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool two) {
+    const size_t a = ln_plan(dtype, P, Q, R, false, two).bytes, b = ln_plan(dtype, P, Q, R, true, two).bytes;
     return a > b ? a : b;
 }
 
@@ -1193,6 +1229,7 @@ static LnGradPlan ln_grad_plan(const tdgs_linear* a) {
     LnGradPlan g;
     const bool slope = a->activation != TDGS_ACT_IDENTITY;
     g.dz_stride = ceil_div(a->out_features, 8) * 8;
+    g.two = slope && a->activation != TDGS_ACT_RELU && a->dtype != TDGS_F32 && a->rows * a->out_features <= kLnFewSlopes;
     g.dz = slope ? align_up((size_t)a->rows * g.dz_stride * dtype_size(a->dtype)) : 0;
     g.small = align_up((kLnTops + 1) * sizeof(float));
     g.shift = 0;
@@ -1203,10 +1240,10 @@ static LnGradPlan ln_grad_plan(const tdgs_linear* a) {
     g.blocks = (int)blocks;
     g.sums = align_up((size_t)g.blocks * a->out_features * sizeof(float));
     // dx and (the weight's gradient or its transpose, whichever is asked for)
-    const size_t dw = ln_part_bytes(a->dtype, a->in_features, a->out_features, a->rows);
-    const size_t t = ln_part_bytes(a->dtype, a->out_features, a->in_features, a->rows);
-    g.part = ln_part_bytes(a->dtype, a->rows, a->in_features, a->out_features) + (dw > t ? dw : t);
-    g.bytes = g.dz + g.small + g.sums + g.part;
+    const size_t dw = ln_part_bytes(a->dtype, a->in_features, a->out_features, a->rows, g.two);
+    const size_t t = ln_part_bytes(a->dtype, a->out_features, a->in_features, a->rows, g.two);
+    g.part = ln_part_bytes(a->dtype, a->rows, a->in_features, a->out_features, g.two) + (dw > t ? dw : t);
+    g.bytes = (g.two ? 2 : 1) * g.dz + g.small + g.sums + g.part;
     return g;
 }
 
@@ -1218,7 +1255,7 @@ extern "C" {
 
 size_t tdgs_linear_temp_bytes(const tdgs_linear* a, int32_t grad) {
     if (ln_check(a) != TDGS_OK) return 0;
-    size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features);
+    size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features, false);
     if (grad) {
         const size_t g = ln_grad_plan(a).bytes;
         if (g > bytes) bytes = g;
@@ -1235,7 +1272,7 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     if (a->residual.data) TDGS_TRY(ln_check_rows(a->residual, "residual", a->dtype, a->rows, a->out_features, false));
     if (a->pre.data) TDGS_TRY(ln_check_rows(a->pre, "pre", a->dtype, a->rows, a->out_features, true));
     TDGS_REQUIRE(aligned_to(a->bias, (size_t)dtype_size(a->dtype)), "linear: bias is not aligned to its element type");
-    const size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features);
+    const size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features, false);
     TDGS_REQUIRE(bytes == 0 || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
                  "linear: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, bytes);
     LnArgs r = {};
@@ -1307,6 +1344,10 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     e.pre = ln_matrix(a->pre);
     if (slope) e.dz = {at, p.dz_stride};
     at += p.dz;
+    if (p.two) {
+        e.rest = at;
+        at += p.dz;
+    }
     float* const top = (float*)at;
     at += p.small;
     e.sums = want_db ? (float*)at : nullptr;
@@ -1354,6 +1395,8 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
         if (want_dx) {
             LnArgs x = r;   // dx = dz W^T
             x.b = ln_weight(a);
+            x.a2 = e.rest;
+            if (e.rest) x.b2 = x.b.p;
             x.P = (int32_t)a->rows;
             x.Q = a->in_features;
             x.R = a->out_features;
@@ -1370,6 +1413,10 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             const LnMatrix rows_x = ln_operand_rows(a->x, a->rows, a->in_features);
             w.b = dw_in_out ? r.a : rows_x;
             w.a = dw_in_out ? rows_x : r.a;
+            if (e.rest) {
+                w.a2 = dw_in_out ? rows_x.p : e.rest;
+                w.b2 = dw_in_out ? e.rest : rows_x.p;
+            }
             TDGS_TRY((ln_product<T, false, false>(w, &at, &joins, stream)));
         }
         return ln_launch_joins<T>(joins, stream);
