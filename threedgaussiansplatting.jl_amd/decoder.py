@@ -499,7 +499,8 @@ def linear_grad_(dx, dweight, dbias, dout, x, weight, *, activation="identity", 
     """The gradients of sum(dout * out) for linear_'s x, weight and bias (tdgs_linear_grad), from its pre; any of them may
     be None. dweight lies either way round, whatever weight does. The residual's gradient is dout.
 
-    dout act'(pre) is an operand of two matrix products and rounded to the type for them; dbias is summed before."""
+    With 16-bit types, silu and gelu, dout act'(pre) is rounded to the type for its two matrix products where it has more than
+    65536 elements, and keeps twice its bits otherwise (tdgs_linear_grad); dbias is summed before that."""
     if pre is None and activation != "identity":
         raise ValueError("the gradient needs the forward call's pre")
     a, b, shape, device = _linear(x, weight, None, activation, pre)
