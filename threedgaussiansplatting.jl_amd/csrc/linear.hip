@@ -878,6 +878,7 @@ struct LnGradArgs {
     int64_t rows;
     int32_t n, act, blocks, shift;
     float* sums;                // blocks x n; null: not wanted
+    void* dbias;                // with one block: they are dbias
     const float* top;           // float16: partial maxima of |dout|; null: dz is not scaled
     int32_t tops;
     float* scale;               // what undoes dz's power of two
@@ -995,7 +996,8 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
         if (col >= a.n) break;
         float x = 0.0f;
         for (int w = 0; w < down; ++w) x += s[w * across * 8 + c];
-        a.sums[(int64_t)blockIdx.y * a.n + col] = x;
+        if (a.dbias) ((T*)a.dbias)[col] = (T)x;
+        else a.sums[(int64_t)blockIdx.y * a.n + col] = x;
     }
 }
 
@@ -1085,8 +1087,10 @@ static bool ln_aligned(const LnMatrix& m, bool depth, int64_t items) {
 
 // Whether a product of few rows goes by vectors. float: 1 to 8 rows x 4096 x 4096 take 22 to 28 us so, 30 by tiles; 512 x 2048
 // 10 and 13 (9.5 of them the call). 16-bit types have tiles that are read faster than this: 1 and 4 rows x 2048 x 512 11
-// and 13 us, 15 and 13 by tiles; but 8 rows 18 and 14, one row x 4096 x 4096 20 and 14.
-static bool ln_few(int64_t size, int64_t P, int64_t Q, int64_t R) {
+// and 13 us, 15 and 13 by tiles; but 8 rows 18 and 14, one row x 4096 x 4096 20 and 14. Where the items are contiguous, a thread
+// takes its depths 512 at a time one after the other, and few columns make few workgroups: tiles split the depth then.
+static bool ln_few(int64_t size, bool depth, int64_t P, int64_t Q, int64_t R) {
+    if (!depth && R > 2048 && (size == 2 || Q < 1024)) return false;
     return size == 4 ? P <= kLsRows : P <= 4 && Q * R <= (1 << 21);
 }
 
@@ -1104,7 +1108,7 @@ static int ln_launch_joins(const LnJoins& j, hipStream_t stream) {
 template <class T, bool AD, bool BD>
 static int ln_product(LnArgs r, char** temp, LnJoins* joins, hipStream_t stream) {
     const int32_t dtype = sizeof(T) == 4 ? TDGS_F32 : std::is_same<T, bf16>::value ? TDGS_BF16 : TDGS_F16;
-    if (AD && ln_few(sizeof(T), r.P, r.Q, r.R)) {
+    if (AD && ln_few(sizeof(T), BD, r.P, r.Q, r.R)) {
         auto few = [&](auto rows) {
             constexpr int ROWS = decltype(rows)::value;
             const int64_t cols = BD ? kLsThreads / kWave * 2 : 4 * ln_chunk<T>();
@@ -1236,7 +1240,9 @@ static LnGradPlan ln_grad_plan(const tdgs_linear* a) {
     while (g.shift < 6 && (8 << g.shift) < a->out_features) ++g.shift;
     const int64_t down = kLnThreads >> g.shift;
     int64_t blocks = ceil_div(1024, ceil_div(a->out_features, 8 << g.shift));
-    if (blocks > ceil_div(a->rows, 2 * down)) blocks = ceil_div(a->rows, 2 * down);
+    // (a block of eight turns is as quick as the join of several)
+    const int64_t turns = ceil_div(a->rows, 2 * down);
+    if (blocks > turns) blocks = turns <= 8 ? 1 : turns;
     g.blocks = (int)blocks;
     g.sums = align_up((size_t)g.blocks * a->out_features * sizeof(float));
     // dx and (the weight's gradient or its transpose, whichever is asked for)
@@ -1351,6 +1357,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     float* const top = (float*)at;
     at += p.small;
     e.sums = want_db ? (float*)at : nullptr;
+    e.dbias = p.blocks == 1 ? g->dbias : nullptr;
     at += p.sums;
     e.rows = a->rows;
     e.n = a->out_features;
@@ -1385,7 +1392,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             TDGS_LAUNCHED();
         }
         LnJoins joins = {};
-        if (want_db) {
+        if (want_db && !e.dbias) {
             joins.sums = e.sums;
             joins.sum_blocks = p.blocks;
             joins.n = a->out_features;
