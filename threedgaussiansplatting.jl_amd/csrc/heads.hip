@@ -64,19 +64,21 @@ struct HnPlaces {
 // The places of `count` tokens from `first` on, and cosine and sine of their pairs.
 template <bool GRAD>
 __device__ __forceinline__ void hn_tokens(const HnArgs& a, int64_t first, int count, HnPlaces& at, float2* s) {
-    for (int i = threadIdx.x; i < 2 * count; i += kHnThreads) {
-        const int token = i >> 1, k = i & 1;
-        const HnTensor& t = a.t[k];
+    // (arguments are indexed by constants: a lane's own index would load them from memory, one wait after the other)
+    for (int token = threadIdx.x; token < count; token += kHnThreads) {
         const uint32_t row = (uint32_t)(first + token), b = a.by_length.div(row), l = row - b * a.by_length.d;
-        at.x[k][token] = b * t.xb + l * t.xl;
-        at.out[k][token] = b * t.ob + l * t.ol;
-        if (GRAD) at.dout[k][token] = b * t.db + l * t.dl;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const HnTensor& t = a.t[k];
+            at.x[k][token] = b * t.xb + l * t.xl;
+            at.out[k][token] = b * t.ob + l * t.ol;
+            if (GRAD) at.dout[k][token] = b * t.db + l * t.dl;
+        }
     }
     for (int i = threadIdx.x; i < count * a.pairs; i += kHnThreads) {
         const int token = (int)a.by_pairs.div((uint32_t)i), p = i - token * a.pairs;
         const uint32_t row = (uint32_t)(first + token), b = a.by_length.div(row), l = row - b * a.by_length.d;
-        int axis = 0;
-        while (p >= a.ends[axis]) ++axis;
+        const int axis = (p >= a.ends[0]) + (p >= a.ends[1]) + (p >= a.ends[2]);   // (unused axes end with the last one)
         const double t = hn_position(a, b * a.position_batch + (int64_t)l * a.axes + axis) * a.turns[p];
         float sn, cs;
         sincospif(2.0f * (float)(t - rint(t)), &sn, &cs);
@@ -155,26 +157,43 @@ __device__ __forceinline__ void hn_store(T* __restrict__ p, const HnUnit<V, KIND
     }
 }
 
-// A lane's weights, of queries and of keys: they stay in registers.
+// A lane's weights, of queries and of keys: they stay in registers. All of them are loaded at once, from elements that exist (one
+// load behind a branch after the other took a workgroup longer than its rows).
 template <class T, int V, int N, int KIND>
 struct HnWeights {
     float x[2][N][V], y[2][N][V];
+    template <class W>
+    __device__ __forceinline__ void load(const W* w, const HnArgs& a, int k, int lane) {
+        W first[N][V], second[N][V];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const HnUnit<V, KIND, N == 1> u(a, lane + n * a.lanes);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int f = u.first + i * u.step, s = u.second + i * u.step;
+                first[n][i] = w[f < a.d ? f : a.d - 1];
+                second[n][i] = w[s < a.d ? s : a.d - 1];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                x[k][n][i] = (float)first[n][i];
+                y[k][n][i] = (float)second[n][i];
+            }
+    }
     __device__ __forceinline__ HnWeights(const HnArgs& a, int lane) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < 2; ++k) {
+            const void* const w = a.t[k].weight;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const HnUnit<V, KIND, N == 1> u(a, lane + n * a.lanes);
-                const void* const w = a.t[k].weight;
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[k][n][i] = y[k][n][i] = 1.0f;
-                    if (!w || !u.on) continue;
-                    const int f = u.first + i * u.step, s = u.second + i * u.step;
-                    x[k][n][i] = a.param_f32 ? ((const float*)w)[f] : (float)((const T*)w)[f];
-                    if (s < a.d) y[k][n][i] = a.param_f32 ? ((const float*)w)[s] : (float)((const T*)w)[s];
-                }
-            }
+                for (int i = 0; i < V; ++i) x[k][n][i] = y[k][n][i] = 1.0f;
+            if (w && a.param_f32) load((const float*)w, a, k, lane);
+            else if (w) load((const T*)w, a, k, lane);
+        }
     }
 };
 
