@@ -15,7 +15,7 @@
 // wanted, applies the activation and adds the residual, all in 32 bits; only what is stored is rounded.
 //
 // What bounds the products: for 16-bit types the vector operations of the epilogue next to the matrix cores (32400 x 1024 ->
-// 4096 bfloat16 with GELU, 335 us: matrix cores busy for 44%, vector issue for 65%; 8192^3 without an activation 870 us,
+// 4096 bfloat16 with GELU, 322 us: matrix cores busy for 44%, vector issue for 65%; 8192^3 without an activation 870 us,
 // 1260 TFLOP/s); for float the matrix cores (66 to 70% busy over 7503 x 387 x 1029, 79 us, of which some ten are the
 // first tiles' way from memory and the last ones' back); for 34230 x 320 -> 320 memory (66 MB in 19 us); for few rows
 // the call.
@@ -1014,7 +1014,7 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_zero(T* p, int64_t rows, 
 // workgroup's start and end, a step of one alone on its CU, and a step's share where the CU is full. 256x256 needs the fewest
 // bytes from LDS per product (1.93 us a step are 1110 TFLOP/s), but fills a CU alone, so that nothing is multiplied
 // while it ends; two workgroups of 128x256, with half the registers, end beside each other (64800 x 512 -> 2048 bfloat16 with
-// GELU: 223 us, 247 by 256x256; at a depth of 1024 they are even, at 8192 it is 1440 and 980). Small tiles leave fewer
+// GELU: 223 us, 247 by 256x256; at a depth of 1024 they are nearly even, at 8192^3 it is 919 and 870). Small tiles leave fewer
 // CUs idle (34230 x 320 -> 320 float16 with a residual: 20 us by 128x64, 25 by 128x128, 43 by 256x256).
 struct LnForm {
     int bp, bq, bk, per_cu;
