@@ -709,7 +709,7 @@ int tdgs_linear_forward(void* stream, const tdgs_linear* a);
  * dout to 2^14), but up to 65536 elements of it keep twice the type's bits; dbias is summed before that. act'(z) comes from the
  * rounded z of pre. With 16-bit types and SiLU or GELU the relative error of dx and dweight over a tensor is
  * so 1.46 times that of the exact gradient rounded once (bfloat16 0.0024, 0.0017), with up to 65536 elements of dz 1.06
- * times. The gradients overlap nothing else. */
+ * times. The gradients overlap nothing else (not dout either). */
 int tdgs_linear_grad(void* stream, const tdgs_linear* a, const tdgs_linear_grads* g);
 
 enum { TDGS_PAIRS_HALVES = 0, TDGS_PAIRS_INTERLEAVED = 1 };

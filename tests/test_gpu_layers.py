@@ -236,6 +236,38 @@ def test_streams_and_graphs(gpu):
                 assert torch.equal(a, c)
 
 
+def test_two_calls_at_once(gpu):
+    """Layers of different sizes on two streams, each with its scratch, in flight together: the bits of one after the other."""
+    def layer(seed, m, k, n, t, act):
+        x, w, dout = rand(m, k, seed=seed, t=t), rand(k, n, seed=seed + 1, t=t) / k ** 0.5, rand(m, n, seed=seed + 2, t=t)
+        out, pre, dx, dw, db = torch.empty_like(dout), torch.empty_like(dout), torch.empty_like(x), torch.empty_like(w), dout[0].clone()
+        q, dq, temp = out.reshape(1, m, -1, 8), torch.empty_like(out).reshape(1, m, -1, 8), decoder.linear_temp(x, w, grad=True)
+
+        def run():
+            decoder.linear_(out, x, w, activation=act, pre=pre, temp=temp)
+            decoder.linear_grad_(dx, dw, db, dout, x, w, activation=act, pre=pre, temp=temp)
+            decoder.rotate_(dq, None, q, None, rotary, places[:m])
+            decoder.dropout_(out, out, 0.3, seed)
+        return run, (out, dx, dw, db, dq)
+
+    rotary, places = decoder.Rotary((4,)), torch.arange(20000, device="cuda")[:, None]
+    layers = [layer(0, 9000, 256, 512, torch.bfloat16, "gelu"), layer(5, 20000, 64, 40, torch.float32, "silu")]
+    wants = []
+    for run, results in layers:
+        run()
+        wants.append([r.clone() for r in results])
+    streams = [torch.cuda.Stream() for _ in layers]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for stream, (run, _) in zip(streams, layers):
+            with torch.cuda.stream(stream):
+                run()
+    torch.cuda.synchronize()
+    for (_, results), want in zip(layers, wants):
+        for a, b in zip(results, want):
+            assert torch.equal(a, b)
+
+
 def test_offsets_past_32_bits(gpu):
     """Tensors of more than 2^31 elements: the last rows are those of a small call."""
     t = torch.bfloat16

@@ -73,8 +73,8 @@ def fill(s, **kw):
 
 
 def linear(**kw):
-    given = dict(dtype=abi.TDGS_BF16, rows=8, in_features=16, out_features=24, x=(64, 16), weight=(64, 24), out=(64, 24), temp=64,
-                 temp_bytes=1 << 30, pre=(64, 24))
+    given = dict(dtype=abi.TDGS_BF16, rows=8, in_features=16, out_features=24, x=(64, 16), weight=(128, 24), out=(192, 24), temp=64,
+                 temp_bytes=1 << 30, pre=(256, 24))
     return fill(abi.LinearC(), **{**given, **kw})
 
 
@@ -83,8 +83,10 @@ def linear(**kw):
     ({"rows": -1}, b"rows"), ({"rows": 2 ** 31}, b"rows"), ({"in_features": 0}, b"weight matrix"),
     ({"out_features": 2 ** 21}, b"weight matrix"), ({"in_features": 2 ** 20, "out_features": 2 ** 20}, b"weight matrix"),
     ({"weight_layout": 2}, b"weight layout"), ({"x": (0, 16)}, b"x is null"), ({"x": (65, 16)}, b"x is not aligned"),
-    ({"weight": (0, 24)}, b"the weight is null"), ({"out": (0, 24)}, b"out is null"), ({"out": (64, 23)}, b"rows of out overlap"),
-    ({"out": (64, -24)}, b"negative stride"), ({"pre": (64, 5)}, b"rows of pre overlap"), ({"residual": (65, 24)}, b"residual"),
+    ({"weight": (0, 24)}, b"the weight is null"), ({"out": (0, 24)}, b"out is null"), ({"out": (192, 23)}, b"rows of out overlap"),
+    ({"out": (192, -24)}, b"negative stride"), ({"pre": (256, 5)}, b"rows of pre overlap"), ({"residual": (65, 24)}, b"residual"),
+    ({"out": (64, 24)}, b"out is also an operand"), ({"out": (128, 24)}, b"out is also an operand"),
+    ({"pre": (192, 24)}, b"pre is also"), ({"pre": (64, 24)}, b"pre is also"), ({"residual": (256, 24)}, b"pre is also"),
     ({"bias": 65}, b"bias"), ({"x": (64, 2 ** 24)}, b"too far apart"), ({"weight": (64, 2 ** 24)}, b"too far apart"),
     ({"rows": 64, "in_features": 4096, "weight": (64, 24), "x": (64, 4096), "temp_bytes": 0}, b"scratch"),
 ])
@@ -95,13 +97,16 @@ def test_linear_refusals(lib, kw, text):
 
 
 @pytest.mark.parametrize("kw,grads,text", [
-    ({}, {"dout": (0, 24)}, b"dout is null"), ({}, {"dx": (64, 15)}, b"rows of dx overlap"),
-    ({}, {"dweight": (64, 24), "dweight_layout": 5}, b"weight layout"), ({}, {"dweight": (64, 23)}, b"rows of dweight"),
+    ({}, {"dout": (0, 24)}, b"dout is null"), ({}, {"dx": (384, 15)}, b"rows of dx overlap"),
+    ({}, {"dweight_layout": 5}, b"weight layout"), ({}, {"dweight": (448, 23)}, b"rows of dweight"),
     ({}, {"dbias": 65}, b"dbias"), ({"activation": 1, "pre": (0, 24)}, {}, b"pre is null"), ({"x": (0, 16)}, {"dx": (0, 0)}, b"x is null"),
-    ({"temp_bytes": 16}, {}, b"scratch"), ({"temp": 8}, {}, b"scratch"), ({}, {"dout": (64, 2 ** 24)}, b"too far apart"),
+    ({"temp_bytes": 16}, {}, b"scratch"), ({"temp": 8}, {}, b"scratch"), ({}, {"dout": (320, 2 ** 24)}, b"too far apart"),
+    ({}, {"dx": (320, 24)}, b"dx is also"), ({}, {"dx": (64, 16)}, b"dx is also"), ({"activation": 1}, {"dx": (256, 24)}, b"dx is also"),
+    ({}, {"dx": (448, 24)}, b"dx is also"), ({}, {"dweight": (320, 24)}, b"dweight is also"), ({}, {"dweight": (64, 24)}, b"dweight is also"),
+    ({}, {"dweight": (128, 24)}, b"dweight is also"),
 ])
 def test_linear_gradient_refusals(lib, kw, grads, text):
-    g = fill(abi.LinearGradsC(), **{**dict(dout=(64, 24), dx=(64, 16), dweight=(64, 24), dbias=64), **grads})
+    g = fill(abi.LinearGradsC(), **{**dict(dout=(320, 24), dx=(384, 16), dweight=(448, 24), dbias=64), **grads})
     assert lib.tdgs_linear_grad(None, C.byref(linear(**kw)), C.byref(g)) == abi.TDGS_ERR_INVALID
     assert text in lib.tdgs_last_error(), lib.tdgs_last_error()
     assert lib.tdgs_linear_grad(None, C.byref(linear()), None) == abi.TDGS_ERR_INVALID

@@ -1278,6 +1278,11 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     if (a->residual.data) TDGS_TRY(ln_check_rows(a->residual, "residual", a->dtype, a->rows, a->out_features, false));
     if (a->pre.data) TDGS_TRY(ln_check_rows(a->pre, "pre", a->dtype, a->rows, a->out_features, true));
     TDGS_REQUIRE(aligned_to(a->bias, (size_t)dtype_size(a->dtype)), "linear: bias is not aligned to its element type");
+    // (tiles of x and of the weight are read while others of the results are written)
+    TDGS_REQUIRE(a->out.data != a->x.data && a->out.data != a->weight.data, "linear: out is also an operand");
+    TDGS_REQUIRE(!a->pre.data || (a->pre.data != a->out.data && a->pre.data != a->x.data && a->pre.data != a->weight.data &&
+                                  a->pre.data != a->residual.data),
+                 "linear: pre is also another tensor of the call");
     const size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features, false);
     TDGS_REQUIRE(bytes == 0 || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
                  "linear: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, bytes);
@@ -1324,6 +1329,14 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
         TDGS_TRY(ln_check_weight(g->dweight, "dweight", a, g->dweight_layout, true));
     }
     TDGS_REQUIRE(aligned_to(g->dbias, (size_t)dtype_size(a->dtype)), "linear: dbias is not aligned to its element type");
+    if (rows) {   // (the products follow one another)
+        TDGS_REQUIRE(!want_dx || (g->dx.data != g->dout.data && g->dx.data != a->weight.data && (!slope || g->dx.data != a->pre.data) &&
+                                  (!want_dw || (g->dx.data != a->x.data && g->dx.data != g->dweight.data))),
+                     "linear: dx is also another tensor of the call");
+        TDGS_REQUIRE(!want_dw || (g->dweight.data != g->dout.data && g->dweight.data != a->x.data &&
+                                  (!want_dx || g->dweight.data != a->weight.data) && (!slope || g->dweight.data != a->pre.data)),
+                     "linear: dweight is also another tensor of the call");
+    }
     LnGradPlan p = ln_grad_plan(a);
     TDGS_REQUIRE(!rows || (a->temp && a->temp_bytes >= p.bytes && aligned_to(a->temp, 16)),
                  "linear: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0, p.bytes);
