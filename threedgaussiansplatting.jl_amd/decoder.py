@@ -550,8 +550,8 @@ class Rotary:
         f = torch.as_tensor(frequencies, dtype=torch.float64)
         if f.shape != (self.pairs,):
             raise ValueError(f"{tuple(f.shape)} frequencies of {self.pairs} pairs")
+        # (a call asks this tensor for its address: a copy or an unpickled rotation has one of its own)
         self.turns = (f / (2 * math.pi)).to(_dev(device))
-        self.device, self.pointer = self.turns.get_device(), self.turns.data_ptr()
         self._fields = (self.pairs, _PAIRS[pairs], self.axes, *self.sections, *(0,) * (4 - self.axes))
 
 
@@ -587,7 +587,7 @@ def _head_norm(q, k, q_weight, k_weight, norm, eps, rotary, positions, inverse):
             raise ValueError("positions without a rotary")
         rotation, place = _NO_ROTATION, _NO_PLACE
     else:
-        if not isinstance(positions, torch.Tensor) or not device == positions.get_device() == rotary.device:
+        if not isinstance(positions, torch.Tensor) or not device == positions.get_device() == rotary.turns.get_device():
             _check_tensor(rotary.turns, "the rotary", q)
             _check_tensor(positions, "positions", q)
         kind = _POSITIONS.get(positions.dtype)
@@ -598,7 +598,7 @@ def _head_norm(q, k, q_weight, k_weight, norm, eps, rotary, positions, inverse):
         if n != ((b, l, axes) if batched else (l, axes)) or not positions.is_contiguous():
             raise ValueError(f"positions must be contiguous, ({l}, {axes}) or ({b}, {l}, {axes})")
         rotation = rotary._fields
-        place = (kind, rotary.pointer, positions.data_ptr(), l * axes if batched else 0)
+        place = (kind, rotary.turns.data_ptr(), positions.data_ptr(), l * axes if batched else 0)
     return ((dtype, param, b, l, h, hk, d, 1 if norm else 0, eps, *rotation, 1 if inverse else 0, *place), (wq, wk))
 
 
