@@ -20,7 +20,9 @@ __device__ __forceinline__ float act_value(float z, float* slope) {
     } else if constexpr (ACT == TDGS_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
         const float y = z * s;
-        if (SLOPE) *slope = __builtin_fmaf(y, 1.0f - s, s);
+        // (infinities, as which float16 keeps a z past its range, have slopes of 0 and 1: at both ends a factor is zero,
+        // which the largest magnitudes that are taken leave zero; NaN is s's)
+        if (SLOPE) *slope = __builtin_fmaf(__builtin_amdgcn_fmed3f(z, -1e30f, 1e30f) * s, 1.0f - s, s);
         return y;
     } else {
         const float ax = fabsf(z) * 0.70710678118654752f;
