@@ -70,14 +70,11 @@ class AppearanceDecoder:
             p.requires_grad_(True)
         self.dropout, self.seed = dropout, seed
         self.passes = torch.zeros(1, dtype=torch.int64, device=d)   # training passes, whose masks differ
-        self._places = {}
 
     def _patch_places(self, pw, ph):
-        """Column and row of each of pw x ph patches."""
-        if (pw, ph) not in self._places:
-            at = torch.arange(pw * ph, dtype=torch.int32, device=self.device)
-            self._places[pw, ph] = torch.stack([at // ph, at % ph], dim=1)
-        return self._places[pw, ph]
+        """Column and row of each of pw x ph patches, made on the call's own stream or in its own graph."""
+        at = (torch.arange(n, dtype=torch.int32, device=self.device) for n in (pw, ph))
+        return torch.stack(torch.meshgrid(*at, indexing="ij"), dim=2).reshape(pw * ph, 2)
 
     def _add(self, x, y, weight, bias, layer, train):
         """x + y weight + bias, the sum's second part dropped in training."""
