@@ -88,9 +88,15 @@ class AppearanceDecoder:
     def __call__(self, rgb, image, states=None, *, states_positions=None, train=False):
         """The corrected (w, h, 3) float32 image of the rendered one, as photograph `image` of the collection
         shows it; states (length, states_dim) are an encoder's, states_positions (length, 2; with rotary) their
-        columns and rows, in patches. train: with dropout. Differentiable for rgb and the parameters."""
+        columns and rows, in patches (without them all at 0, as the tokens). train: with dropout. Differentiable for rgb and
+        the parameters."""
         if not isinstance(image, torch.Tensor) and not 0 <= image < self.nb_images:
             raise ValueError(f"photograph {image} of a collection of {self.nb_images}")
+        if states_positions is not None:
+            if self.rotary is None or states is None:
+                raise ValueError(f"states_positions without {'rotary' if self.rotary is None else 'states'}")
+            if states_positions.shape != (states.shape[0], 2):
+                raise ValueError(f"states_positions have shape {tuple(states_positions.shape)}, not ({states.shape[0]}, 2)")
         p, s, c = self.parameters, self.patch, self.channels
         w, h, _ = rgb.shape
         pw, ph = -(-w // s), -(-h // s)
@@ -147,13 +153,16 @@ class AppearanceLoss:
         self.sums = torch.zeros(2, dtype=torch.float64, device=d)
         self.temp = torch.empty(int(lib().tdgs_loss_temp_bytes(width, height)), dtype=torch.uint8, device=d)
 
-    def step_(self, decoder_, optimizer, rgb, image, photograph, states=None):
-        """One step of the decoder's parameters on a rendered image; returns the loss's gradient for that
-        image, from which the render's backward pass goes on. The loss's sums stay on the device (value())."""
+    def step_(self, decoder_, optimizer, rgb, image, photograph, states=None, states_positions=None):
+        """One step of the decoder's parameters on a rendered image, with states and their positions as the decoder takes
+        them; returns the loss's gradient for that image, from which the render's backward pass goes on. The loss's sums
+        stay on the device (value())."""
         rgb = rgb.detach().requires_grad_(True)
         optimizer.zero_grad(set_to_none=True)
-        train = {"train": True} if getattr(decoder_, "dropout", 0.0) else {}
-        corrected = decoder_(rgb, image, states, **train).contiguous()
+        options = {"train": True} if getattr(decoder_, "dropout", 0.0) else {}
+        if states_positions is not None:
+            options["states_positions"] = states_positions
+        corrected = decoder_(rgb, image, states, **options).contiguous()
         grad = torch.empty_like(corrected)
         self.sums.zero_()
         loss_grad_(corrected.detach(), photograph, grad, self.dssim_weight, self.sums, self.temp)
