@@ -675,7 +675,7 @@ enum { TDGS_WEIGHT_IN_OUT = 0, TDGS_WEIGHT_OUT_IN = 1 };
 /* Linear layer: with z = x W + bias, out = residual + act(z); x is rows x in_features, the others rows x
  * out_features, act as in tdgs_norm. Sums are held in 32 bits; z is rounded on its way to pre, and residual + act(z), from
  * the z that is not, on its way to out. Rows of x, weight, residual, pre (in the gradient) and dout are at most 2^24 bytes
- * apart. out and pre overlap nothing else, but that residual may be out. */
+ * apart. out and pre overlap nothing else, but that residual may be out (its stride too). */
 typedef struct tdgs_linear {
     int32_t dtype;              /* of every tensor */
     int32_t activation;
@@ -738,15 +738,17 @@ typedef struct tdgs_head_norm {
     const double* turns;        /* pairs entries: frequency / (2 pi), turns for a step of one */
     const void* positions;      /* element position_batch_stride b + axes l + axis */
     int64_t position_batch_stride;   /* 0: the same for every batch */
-    tdgs_heads q, k, q_out, k_out;   /* q_out may be q and k_out k; the gradient does not read them */
+    tdgs_heads q, k, q_out, k_out;   /* q_out may be q and k_out k (the same strides too), and they overlap nothing else; each
+                                        stride of a result reaches past all that its smaller ones cover. The gradient does not
+                                        read q_out and k_out */
     const void* q_weight;       /* head_dim; null: 1 */
     const void* k_weight;
     void* temp;                 /* scratch of the gradient, tdgs_head_norm_temp_bytes() bytes */
     size_t temp_bytes;
 } tdgs_head_norm;
 
-/* The results' gradients; dq and dk (dq may be dq_out, dk dk_out), and those of the weights, of their type (null: not
- * wanted). */
+/* The results' gradients; dq and dk (dq may be dq_out, dk dk_out, as q_out q), and those of the weights, of their type (null:
+ * not wanted). */
 typedef struct tdgs_head_norm_grads {
     tdgs_heads dq_out, dk_out, dq, dk;
     void* dq_weight;
@@ -764,7 +766,8 @@ int tdgs_head_norm_grad(void* stream, const tdgs_head_norm* a, const tdgs_head_n
  * (low and high word of i / 4, low and high word of call) is at least floor(p 2^32), p in [0, 1]; what x holds where it is
  * dropped does not matter. call_dev, where not null, is one int64 on the device that is read instead of `call` (a
  * captured call so takes another mask at each replay). The gradient for x is the same call on dout without a
- * residual: the mask is made again and never stored. out may be x or residual. */
+ * residual: the mask is made again and never stored. out may be x or residual, their stride too, and overlaps them in no other
+ * way. */
 typedef struct tdgs_dropout {
     int32_t dtype;
     int32_t reserved;

@@ -17,6 +17,7 @@
 // the rotation alone 57, gradients 85; few tokens by the latency of their positions, rows and stores.
 #include "internal.hpp"
 #include "elem.hpp"
+#include "overlap.hpp"
 
 namespace tdgs {
 
@@ -452,14 +453,39 @@ static int hn_check(const tdgs_head_norm* a) {
     return TDGS_OK;
 }
 
+static ByteDims hn_bytes(const tdgs_heads& v, const tdgs_head_norm* a, int heads) {
+    const int64_t size = (int64_t)dtype_size(a->dtype);
+    return ByteDims(v.data, {a->batch, a->length, heads}, {v.stride_b * size, v.stride_l * size, v.stride_h * size}, a->head_dim * size);
+}
+
 static int hn_check_view(const tdgs_heads* v, const char* name, const tdgs_head_norm* a, int heads, bool written) {
     TDGS_REQUIRE(v->data != nullptr, "head norm: %s is null", name);
     TDGS_REQUIRE(aligned_to(v->data, (size_t)dtype_size(a->dtype)), "head norm: %s is not aligned to its element type", name);
     TDGS_REQUIRE(v->stride_b >= 0 && v->stride_l >= 0 && v->stride_h >= 0, "head norm: %s has a negative stride", name);
     if (written)
-        TDGS_REQUIRE((a->batch <= 1 || v->stride_b >= a->head_dim) && (a->length <= 1 || v->stride_l >= a->head_dim) &&
-                         (heads <= 1 || v->stride_h >= a->head_dim),
-                     "head norm: rows of %s overlap", name);
+        TDGS_REQUIRE(hn_bytes(*v, a, heads).nested, "head norm: rows of %s overlap", name);
+    return TDGS_OK;
+}
+
+// A result may be what it is computed from (a head is read by the lanes that write it), and overlaps nothing else: the other result,
+// what that is computed from. `read`: x, and dout or null, of queries and keys, `written` their results; null without heads.
+static int hn_check_apart(const tdgs_head_norm* a, const tdgs_heads* const (&read)[2][2], const tdgs_heads* const (&written)[2],
+                          const char* const (&names)[2][3]) {
+    const int heads[2] = {a->heads, a->kv_heads};
+    for (int i = 0; i < 2; ++i) {
+        if (!written[i]) continue;
+        const ByteDims w = hn_bytes(*written[i], a, heads[i]);
+        for (int j = 0; j < 2; ++j) {
+            for (int n = 0; n < 2; ++n) {
+                if (!written[j] || !read[j][n]) continue;
+                const ByteDims r = hn_bytes(*read[j][n], a, heads[j]);
+                TDGS_REQUIRE(!dims_overlap(w, r) || (i == j && w.same(r)), "head norm: %s overlaps %s%s", names[i][2], names[j][n],
+                             i == j ? " without being it" : "");
+            }
+            if (j > i && written[j])
+                TDGS_REQUIRE(!dims_overlap(w, hn_bytes(*written[j], a, heads[j])), "head norm: %s overlaps %s", names[i][2], names[j][2]);
+        }
+    }
     return TDGS_OK;
 }
 
@@ -584,6 +610,8 @@ int tdgs_head_norm_forward(void* stream_, const tdgs_head_norm* a) {
         TDGS_TRY(hn_check_view(&a->k_out, "k_out", a, a->kv_heads, true));
         hn_out(&r.t[1], a->k_out);
     }
+    TDGS_TRY(hn_check_apart(a, {{&a->q, nullptr}, {&a->k, nullptr}}, {a->heads > 0 ? &a->q_out : nullptr, a->kv_heads > 0 ? &a->k_out : nullptr},
+                            {{"q", "", "q_out"}, {"k", "", "k_out"}}));
     const HnPlan p = hn_plan(a, &r, false);
     hipStream_t stream = (hipStream_t)stream_;
     return hn_dispatch(a, p, [&](auto t, auto v, auto n, auto kind) -> int {
@@ -624,6 +652,9 @@ int tdgs_head_norm_grad(void* stream_, const tdgs_head_norm* a, const tdgs_head_
     const size_t bytes = (size_t)p.blocks * 2 * a->head_dim * sizeof(float);
     TDGS_REQUIRE(!weights || empty || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
                  "head norm: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0, bytes);
+    if (!empty)
+        TDGS_TRY(hn_check_apart(a, {{&a->q, &g->dq_out}, {&a->k, &g->dk_out}},
+                                {a->heads > 0 ? &g->dq : nullptr, a->kv_heads > 0 ? &g->dk : nullptr}, kNames));
     hipStream_t stream = (hipStream_t)stream_;
     r.part = weights ? (float*)a->temp : nullptr;
     if (empty) p.blocks = 0;   // (the weights' gradients are zero)

@@ -22,6 +22,7 @@
 #include "internal.hpp"
 #include "elem.hpp"
 #include "activation.hpp"
+#include "overlap.hpp"
 
 namespace tdgs {
 
@@ -1204,6 +1205,28 @@ static LnMatrix ln_matrix(const tdgs_rows& v) { return {v.data, v.stride}; }
 // An operand: the stride of a single row means nothing, and must not be calculated with.
 static LnMatrix ln_operand_rows(const tdgs_rows& v, int64_t rows, int64_t cols) { return {v.data, rows > 1 ? v.stride : cols}; }
 
+// What a matrix, or (layout) a weight matrix, or a vector covers.
+static ByteRows ln_bytes(const tdgs_rows& v, const tdgs_linear* a, int64_t rows, int64_t cols) {
+    const int64_t size = (int64_t)dtype_size(a->dtype);
+    return ByteRows(v.data, v.data ? rows : 0, rows > 1 ? v.stride * size : 0, cols * size);
+}
+static ByteRows ln_weight_bytes(const tdgs_rows& v, const tdgs_linear* a, int32_t layout) {
+    return layout == TDGS_WEIGHT_IN_OUT ? ln_bytes(v, a, a->in_features, a->out_features)
+                                        : ln_bytes(v, a, a->out_features, a->in_features);
+}
+static ByteRows ln_vector_bytes(const void* v, const tdgs_linear* a) { return ln_bytes({(void*)v, 0}, a, 1, a->out_features); }
+
+// Refuses `written` where it shares memory with one of the others: tiles of those are read, or written, at any time.
+struct LnNamed {
+    ByteRows rows;
+    const char* name;
+};
+static int ln_check_apart(const LnNamed& written, std::initializer_list<LnNamed> others) {
+    for (const LnNamed& o : others)
+        TDGS_REQUIRE(!rows_overlap(written.rows, o.rows), "linear: %s overlaps %s", written.name, o.name);
+    return TDGS_OK;
+}
+
 static LnMatrix ln_weight(const tdgs_linear* a) {
     return a->weight_layout == TDGS_WEIGHT_IN_OUT ? ln_operand_rows(a->weight, a->in_features, a->out_features)
                                                   : ln_operand_rows(a->weight, a->out_features, a->in_features);
@@ -1286,6 +1309,13 @@ int tdgs_linear_forward(void* stream_, const tdgs_linear* a) {
     const size_t bytes = ln_part_bytes(a->dtype, a->rows, a->out_features, a->in_features, false);
     TDGS_REQUIRE(bytes == 0 || (a->temp && a->temp_bytes >= bytes && aligned_to(a->temp, 16)),
                  "linear: scratch of %zu bytes, %zu needed", a->temp ? a->temp_bytes : (size_t)0, bytes);
+    const LnNamed x = {ln_bytes(a->x, a, a->rows, a->in_features), "x"}, w = {ln_weight_bytes(a->weight, a, a->weight_layout), "the weight"},
+                  bias = {ln_vector_bytes(a->bias, a), "the bias"}, out = {ln_bytes(a->out, a, a->rows, a->out_features), "out"},
+                  residual = {ln_bytes(a->residual, a, a->rows, a->out_features), "the residual"},
+                  pre = {ln_bytes(a->pre, a, a->rows, a->out_features), "pre"};
+    TDGS_TRY(ln_check_apart(out, {x, w, bias}));
+    TDGS_REQUIRE(same_or_apart(out.rows, residual.rows), "linear: out overlaps the residual without being it");
+    TDGS_TRY(ln_check_apart(pre, {x, w, bias, residual, out}));
     LnArgs r = {};
     r.a = ln_operand_rows(a->x, a->rows, a->in_features);
     r.b = ln_weight(a);
@@ -1340,8 +1370,20 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
     LnGradPlan p = ln_grad_plan(a);
     TDGS_REQUIRE(!rows || (a->temp && a->temp_bytes >= p.bytes && aligned_to(a->temp, 16)),
                  "linear: scratch of %zu bytes, the gradient needs %zu", a->temp ? a->temp_bytes : (size_t)0, p.bytes);
-    hipStream_t stream = (hipStream_t)stream_;
     const bool dw_in_out = g->dweight_layout == TDGS_WEIGHT_IN_OUT;
+    if (rows) {   // (of the operands those that are read)
+        const tdgs_rows none = {};
+        const LnNamed dout = {ln_bytes(g->dout, a, a->rows, a->out_features), "dout"},
+                      pre = {ln_bytes(slope ? a->pre : none, a, a->rows, a->out_features), "pre"},
+                      x = {ln_bytes(want_dw ? a->x : none, a, a->rows, a->in_features), "x"},
+                      w = {ln_weight_bytes(want_dx ? a->weight : none, a, a->weight_layout), "the weight"},
+                      dx = {ln_bytes(g->dx, a, a->rows, a->in_features), "dx"},
+                      dw = {ln_weight_bytes(g->dweight, a, g->dweight_layout), "dweight"}, db = {ln_vector_bytes(g->dbias, a), "dbias"};
+        TDGS_TRY(ln_check_apart(dx, {dout, pre, x, w, dw}));
+        TDGS_TRY(ln_check_apart(dw, {dout, pre, x, w}));
+        TDGS_TRY(ln_check_apart(db, {dout, pre, x, w, dx, dw}));
+    }
+    hipStream_t stream = (hipStream_t)stream_;
     if (!rows) {
         return with_dtype(a->dtype, [&](auto t) -> int {
             using T = decltype(t);
