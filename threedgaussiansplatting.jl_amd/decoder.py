@@ -909,12 +909,16 @@ class _HeadNorm(torch.autograd.Function):
     @_once
     def backward(ctx, *douts):
         q, k, q_weight, k_weight, positions = ctx.saved_tensors
-        dq, dk = (None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
-        weights = [torch.empty_like(w) if want else None for w, want in zip((q_weight, k_weight), ctx.needs_input_grad[2:4])]
-        douts = [_rows_contiguous(d) for d in douts] + [None] * (k is None)
-        head_norm_grad_(dq, dk, *weights, *douts, q, k, q_weight, k_weight, eps=ctx.eps, rotary=ctx.rotary,
-                        positions=positions)
-        return dq, dk, *weights, None, None, None
+        grads = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if want else None
+                 for x, want in zip((q, k, q_weight, k_weight), ctx.needs_input_grad)]
+        # queries or keys of which nothing is wanted are left out of the call; weights are summed on the way to dx
+        sides = [(torch.empty_like(d) if dx is None else dx, dw, d, x, w) for dx, dw, d, x, w in
+                 zip(grads[:2], grads[2:], map(_rows_contiguous, douts), (q, k), (q_weight, k_weight))
+                 if dx is not None or dw is not None]
+        if sides:
+            dx, dw, dout, x, w = zip(*sides, *[(None,) * 5] * (2 - len(sides)))
+            head_norm_grad_(*dx, *dw, *dout, *x, *w, eps=ctx.eps, rotary=ctx.rotary, positions=positions)
+        return *grads, None, None, None
 
 
 def head_norm(q, k=None, q_weight=None, k_weight=None, *, eps=1e-6, rotary=None, positions=None):
@@ -938,11 +942,13 @@ class _Rotate(torch.autograd.Function):
     @_once
     def backward(ctx, *douts):
         positions, = ctx.saved_tensors
-        douts = [_rows_contiguous(d) for d in douts]
-        grads = [torch.empty(d.shape, dtype=d.dtype, device=d.device) for d in douts]
-        rotate_(grads[0], grads[1] if len(grads) > 1 else None, douts[0], douts[1] if len(douts) > 1 else None, ctx.rotary,
-                positions, inverse=not ctx.inverse)
-        return grads[0], grads[1] if len(grads) > 1 else None, None, None, None
+        grads = [torch.empty(d.shape, dtype=d.dtype, device=d.device) if want else None
+                 for d, want in zip(douts, ctx.needs_input_grad)] + [None] * (2 - len(douts))
+        sides = [(dx, d) for dx, d in zip(grads, map(_rows_contiguous, douts)) if dx is not None]
+        if sides:
+            dx, dout = zip(*sides, *[(None, None)] * (2 - len(sides)))
+            rotate_(*dx, *dout, ctx.rotary, positions, inverse=not ctx.inverse)
+        return *grads, None, None, None
 
 
 def rotate(q, k, rotary, positions, *, inverse=False):
