@@ -343,8 +343,10 @@ struct LnPlace {
 };
 
 // Two stages: while a step is multiplied, the next one's tiles are stored to LDS and the loads of the one after are in flight.
-// float by 64x64, eight workgroups a CU: 8192 x 4096 x 4096 in 2.2 ms by 128x128 (124 TFLOP/s; a library product 145),
-// 7503 x 387 x 1029 with SiLU 79 us by 64x64 (a plain library product 69), 107 by 128x128, which leaves CUs idle.
+// float by 128x128, three workgroups a CU, or 64x64, eight: forward 8192 x 4096 x 4096 2222 us (124 TFLOP/s; a library product
+// 1822) and 2327, 32400 x 512 x 2048 588 and 624, its weight's gradient 569 and 776; 7503 x 387 x 1029 97 (CUs idle) and
+// 66 (a library product 61), 64800 x 64 x 512 63 and 56. Of 135 products, forward and weights' gradients, that were timed by
+// both, ln_plan takes the faster one, or one within 2% of it, in 125, and loses 26% at most (64x64 always: 36%).
 template <class S>
 __global__ __launch_bounds__(S::TH) void k_linear(LnArgs a) {
     using T = typename S::T;
@@ -1024,7 +1026,7 @@ struct LnForm {
 enum { kLnStaged64, kLnStaged128, kLnDirect64, kLnDirect128x64, kLnDirect128, kLnDirect128x256, kLnDirect256, kLnForms };
 template <class T>
 constexpr int ln_depth() { return sizeof(T) == 4 ? 16 : 32; }
-constexpr LnForm kLnF32[2] = {{64, 64, ln_depth<float>(), 8, 3.0f, 0.5f, 0.3f}, {128, 128, ln_depth<float>(), 3, 5.0f, 1.3f, 1.2f}};
+constexpr LnForm kLnF32[2] = {{64, 64, ln_depth<float>(), 8, 3.0f, 0.5f, 0.3f}, {128, 128, ln_depth<float>(), 3, 5.0f, 1.3f, 1.12f}};
 constexpr LnForm kLn16[kLnForms] = {{64, 64, ln_depth<bf16>(), 6, 3.0f, 0.5f, 0.25f}, {128, 128, ln_depth<bf16>(), 3, 5.0f, 0.8f, 0.42f},
                                     {64, 64, 64, 4, 3.0f, 0.46f, 0.206f},  {128, 64, 64, 3, 4.0f, 0.6f, 0.34f},
                                     {128, 128, 64, 2, 5.0f, 0.85f, 0.59f}, {128, 256, 32, 2, 3.0f, 0.8f, 0.62f}, {256, 256, 64, 1, 12.0f, 1.93f, 1.93f}};
@@ -1037,7 +1039,9 @@ struct LnPlan {
 };
 
 // The form and the splits that take the least time: rounds of the workgroups of the fullest CU, and the join, which
-// reads at 6 TB/s what the splits have left in the last-level cache, one after the other.
+// reads at 6 TB/s what the splits have left in the last-level cache, one after the other. A last round of float is counted by the
+// workgroups that are in it (128x128 puts three on a CU: eight are two rounds and two thirds, not three); the figures of the
+// 16-bit forms were fitted to rounds that count whole.
 // `two`: a sum of two products, each by as many splits.
 static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direct, bool two) {
     if (P < 1 || Q < 1 || R < 1) return {};
@@ -1061,9 +1065,12 @@ static LnPlan ln_plan(int32_t dtype, int64_t P, int64_t Q, int64_t R, bool direc
             }
             const int64_t per = ceil_div(steps, splits);
             splits = ceil_div(steps, per);
-            const int64_t on = ceil_div(tiles * splits, kLnCus), together = on < f.per_cu ? on : f.per_cu;
-            const float step = f.full * together > f.alone ? f.full * together : f.alone;
-            float time = (float)ceil_div(on, f.per_cu) * (f.ends + per * step);
+            const int64_t on = ceil_div(tiles * splits, kLnCus), whole = on / f.per_cu, rest = on % f.per_cu;
+            auto round = [&](int64_t together) {
+                return f.ends + per * (f.full * together > f.alone ? f.full * together : f.alone);
+            };
+            float time = whole ? (float)whole * round(f.per_cu) : 0.0f;
+            if (rest) time += round(whole && !f32 ? f.per_cu : rest);
             if (splits > 1) time += 3.0f + 0.012f * splits + (float)splits * P * Q * 4.0f / 6e6f;
             if (time < least) {
                 least = time;
