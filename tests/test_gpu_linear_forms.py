@@ -15,6 +15,7 @@ HALF = {
     "256x256 128x64 128x128": (6000, 1544, 2056),      # 24 steps and 8 more; 6000 rows: 93 steps and 48 in two splits
     "128x64 256x256 128x128": (6000, 2056, 1544),
     "128x64 128x64 256x256": (4100, 2056, 2056),       # 64 steps and 4 more, in three splits
+    "64x64 64x64 128x256": (140, 1032, 4104),          # four steps of 32 and 12 more
 }
 FLOAT = {
     "128x128 64x64 64x64": (5001, 133, 2052),          # eight steps of 16 and 5 more
