@@ -24,6 +24,7 @@ namespace tdgs {
 constexpr int kHnThreads = 256;
 constexpr int kHnAngles = 4096;     // of a workgroup's tokens, in LDS: 32 KB
 constexpr int kHnBlocks = 1024;     // workgroups of the gradient, which leave one partial sum of dw each
+constexpr int kHnMostBlocks = 1 << 23;   // of any launch, which has fewer than 2^32 threads
 constexpr int kHnMaxDim = 256;
 constexpr int kHnTokens = 64;       // of a workgroup at a time, at most
 
@@ -516,7 +517,8 @@ static HnPlan hn_plan(const tdgs_head_norm* a, HnArgs* r, bool grad) {
     if (per < 1) per = 1;
     r->per = (int32_t)per;
     const int64_t blocks = ceil_div(tokens, per);
-    p.blocks = (int)(grad && blocks > kHnBlocks ? kHnBlocks : blocks);
+    const int64_t most = grad ? kHnBlocks : kHnMostBlocks;
+    p.blocks = (int)(blocks < most ? blocks : most);
     p.lds = (size_t)(per * a->pairs * (int64_t)sizeof(float2));
     return p;
 }

@@ -1007,8 +1007,8 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
 // What is zero without rows (dweight and dbias).
 template <class T>
 __global__ __launch_bounds__(kLnThreads) void k_linear_zero(T* p, int64_t rows, int cols, int64_t stride) {
-    const int64_t i = (int64_t)blockIdx.x * kLnThreads + threadIdx.x;
-    if (i < rows * cols) p[i / cols * stride + i % cols] = (T)0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * kLnThreads + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * kLnThreads)
+        p[i / cols * stride + i % cols] = (T)0.0f;
 }
 
 // ---- host ----------------------------------------------------------------------------------
@@ -1139,7 +1139,9 @@ static int ln_product(LnArgs r, char** temp, LnJoins* joins, hipStream_t stream)
     r.part = p.splits > 1 ? (float*)*temp : nullptr;
     *temp += p.bytes;
     const int64_t grid = (int64_t)p.tiles_p * p.tiles_q * p.splits;
-    TDGS_REQUIRE(grid <= INT32_MAX, "linear: too many tiles");
+    // (a launch has fewer than 2^32 threads)
+    TDGS_REQUIRE(grid * (p.form == kLnDirect128x256 || p.form == kLnDirect256 ? 512 : 256) <= UINT32_MAX,
+                 "linear: %lld x %lld results are too many tiles for one call", (long long)r.P, (long long)r.Q);
     constexpr int C = ln_chunk<T>(), D = ln_depth<T>();
     auto staged = [&](auto shape) {
         using S = decltype(shape);
@@ -1397,7 +1399,7 @@ int tdgs_linear_grad(void* stream_, const tdgs_linear* a, const tdgs_linear_grad
             const int64_t n = (int64_t)a->in_features * a->out_features;
             const int cols = dw_in_out ? a->out_features : a->in_features;
             if (want_dw)
-                k_linear_zero<T><<<(unsigned)ceil_div(n, kLnThreads), kLnThreads, 0, stream>>>(
+                k_linear_zero<T><<<(unsigned)std::min<int64_t>(ceil_div(n, kLnThreads), 1 << 16), kLnThreads, 0, stream>>>(
                     (T*)g->dweight.data, n / cols, cols, g->dweight.stride);
             if (want_db)
                 k_linear_zero<T><<<(unsigned)ceil_div(a->out_features, kLnThreads), kLnThreads, 0, stream>>>(
