@@ -426,6 +426,8 @@ static int hn_check(const tdgs_head_norm* a) {
     TDGS_REQUIRE(known_dtype(a->dtype), "head norm: unknown element type %d", a->dtype);
     TDGS_REQUIRE(a->param_dtype == a->dtype || a->param_dtype == TDGS_F32,
                  "head norm: weights must be float32 or of the input's type");
+    TDGS_REQUIRE(aligned_to(a->q_weight, (size_t)dtype_size(a->param_dtype)) && aligned_to(a->k_weight, (size_t)dtype_size(a->param_dtype)),
+                 "head norm: the weights are not aligned to their element type");
     TDGS_REQUIRE(a->batch >= 0 && a->length >= 0 && a->heads >= 0 && a->kv_heads >= 0, "head norm: negative size");
     TDGS_REQUIRE(a->heads <= 65536 && a->kv_heads <= 65536, "head norm: %d and %d heads", a->heads, a->kv_heads);
     TDGS_REQUIRE((int64_t)a->batch * a->length <= INT32_MAX - 65536, "head norm: too many tokens");
@@ -633,6 +635,8 @@ int tdgs_head_norm_grad(void* stream_, const tdgs_head_norm* a, const tdgs_head_
     TDGS_TRY(hn_check(a));
     TDGS_REQUIRE(g != nullptr, "head norm: null gradients");
     TDGS_REQUIRE(a->norm, "head norm: the gradient of a rotation alone is the inverse rotation");
+    TDGS_REQUIRE(aligned_to(g->dq_weight, (size_t)dtype_size(a->param_dtype)) && aligned_to(g->dk_weight, (size_t)dtype_size(a->param_dtype)),
+                 "head norm: the weights' gradients are not aligned to their element type");
     HnArgs r = hn_args(a);
     const bool empty = a->batch == 0 || a->length == 0 || a->heads + a->kv_heads == 0;
     auto view = [&](int i, const tdgs_heads& x, const tdgs_heads& d, const tdgs_heads& dx, int heads, const char* const* names) -> int {
