@@ -709,7 +709,8 @@ int tdgs_linear_forward(void* stream, const tdgs_linear* a);
  * dout to 2^14), but up to 65536 elements of it keep twice the type's bits; dbias is summed before that. act'(z) comes from the
  * rounded z of pre. With 16-bit types and SiLU or GELU the relative error of dx and dweight over a tensor is
  * so 1.46 times that of the exact gradient rounded once (bfloat16 0.0024, 0.0017), with up to 65536 elements of dz 1.06
- * times. The gradients overlap nothing else (not dout either). */
+ * times (where an element of x or the weight is then infinite, what it reaches may be NaN instead of an infinity). The gradients
+ * overlap nothing else (not dout either). */
 int tdgs_linear_grad(void* stream, const tdgs_linear* a, const tdgs_linear_grads* g);
 
 enum { TDGS_PAIRS_HALVES = 0, TDGS_PAIRS_INTERLEAVED = 1 };
@@ -719,8 +720,9 @@ enum { TDGS_POSITION_I32 = 0, TDGS_POSITION_I64 = 1, TDGS_POSITION_F32 = 2 };
  * y_i = x_i weight_i / sqrt(mean x^2 + eps) over the head's elements (norm 0: y = x), then with t = position * frequency the
  * pair (y_a, y_b) becomes (y_a cos t - y_b sin t, y_a sin t + y_b cos t). Pair p < pairs is elements (p, p + pairs)
  * (TDGS_PAIRS_HALVES) or (2 p, 2 p + 1) (TDGS_PAIRS_INTERLEAVED); elements from 2 pairs on are not rotated. Its axis is
- * the one in whose section of sections[0], sections[1], .. neighbouring pairs it lies. Angles are made in 64 bits. Queries
- * and keys are of the same positions; a call may be for one of them (heads or kv_heads 0). */
+ * the one in whose section of sections[0], sections[1], .. neighbouring pairs it lies. Angles are made in 64 bits, as turns;
+ * sine and cosine are taken, in 32, of what is left without whole turns, rounded to 2^-26 of a turn or less, however far the
+ * position. Queries and keys are of the same positions; a call may be for one of them (heads or kv_heads 0). */
 typedef struct tdgs_head_norm {
     int32_t dtype;              /* of q, k, their results and gradients */
     int32_t param_dtype;        /* of the weights and their gradients: TDGS_F32 or dtype */

@@ -1242,9 +1242,10 @@ static LnMatrix ln_weight(const tdgs_linear* a) {
 }
 
 // Up to so many elements of dz, which 16 bits round once more than the results, its products are taken of two operands, the second
-// holding what the rounding leaves of the first. Over a large dz that rounding makes dx and dweight 1.46 times as inexact
-// as the exact result rounded once (with the rounded z), over a few values it may be more; and it is large products that
-// the second operand would cost their time again, not these.
+// holding what the rounding leaves of the first: the errors of dx and dweight are 1.00 times those of the exact result rounded
+// once instead of 1.40 to 1.42, for every size. What it costs decides: these calls are mostly latency (the whole gradient with
+// GELU, one operand and two, in a graph: 256 x 256 -> 256 bfloat16 12 and 15 us, 64 x 1024 -> 1024 24 and 31, 128 x 2048 -> 512 13
+// and 21, 32 x 1024 -> 2048 19 and 35), large ones would take both products' time again (64800 x 512 -> 2048: 284 of 432 us).
 constexpr int64_t kLnFewSlopes = 1 << 16;
 
 // The gradient's scratch: dz, its power of two, maxima and columns' sums, then a product's partial sums.

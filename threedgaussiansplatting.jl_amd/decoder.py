@@ -640,7 +640,9 @@ def head_norm_(q_out, k_out, q, k=None, q_weight=None, k_weight=None, *, eps=1e-
 
     q and k are (batch, length, heads, head_dim), of any strides with the last dimension contiguous, head_dim up to 256; k (and
     k_out) may be None. weights are head_dim values, float32 or of q's type; None: ones. positions are (length, axes) or
-    (batch, length, axes), int32, int64 or float32; their angles are made in 64 bits. q_out may be q and k_out k."""
+    (batch, length, axes), int32, int64 or float32; their angles are made in 64 bits, and what is left of them
+    without whole turns is rounded to 2^-26 of a turn. q_out may be q and k_out k (the same strides too), and they overlap
+    nothing else."""
     a, w = _head_norm(q, k, q_weight, k_weight, True, eps, rotary, positions, False)
     x = _head_views(("q", "k"), (q, k), (q, k))
     o = _head_views(("q_out", "k_out"), (q_out, k_out), (q, k))
