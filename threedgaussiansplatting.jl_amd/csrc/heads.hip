@@ -387,12 +387,15 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
                 if (u.second + i * u.step < a.d) s_sums[lane.sub * a.d + u.second + i * u.step] = db[k][n][i];
             }
         }
-        __syncthreads();
-        for (int c = threadIdx.x; c < a.d; c += kHnThreads) {
-            float x = 0.0f;
-            for (int r = 0; r < lane.rows; ++r) x += s_sums[r * a.d + c];
-            a.part[((int64_t)blockIdx.x * 2 + k) * a.d + c] = x;
+        // by halves: one after the other, the 128 rows of heads of 16 left twice the error
+        for (int rows = lane.rows; rows > 1;) {
+            const int half = (rows + 1) / 2;
+            __syncthreads();
+            for (int c = threadIdx.x; c < (rows - half) * a.d; c += kHnThreads) s_sums[c] += s_sums[half * a.d + c];
+            rows = half;
         }
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.d; c += kHnThreads) a.part[((int64_t)blockIdx.x * 2 + k) * a.d + c] = s_sums[c];
     }
 }
 
@@ -409,9 +412,12 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_join(const float* __re
         for (int b = y; b < blocks; b += kHnThreads / kHnJoinCols) x += part[(int64_t)b * 2 * d + c];
     }
     s[y][threadIdx.x % kHnJoinCols] = x;
-    __syncthreads();
+    for (int w = kHnThreads / kHnJoinCols / 2; w > 0; w >>= 1) {
+        __syncthreads();
+        if (y < w) s[y][threadIdx.x % kHnJoinCols] += s[y + w][threadIdx.x % kHnJoinCols];
+    }
     if (y != 0 || c >= 2 * d) return;
-    for (int i = 1; i < kHnThreads / kHnJoinCols; ++i) x += s[i][threadIdx.x];
+    x = s[0][threadIdx.x];
     void* const p = c < d ? dq : dk;
     if (!p) return;
     const int e = c < d ? c : c - d;

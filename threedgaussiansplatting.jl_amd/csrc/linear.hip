@@ -696,10 +696,11 @@ __device__ __forceinline__ void ln_dbias(const float* __restrict__ sums, int blo
         for (int b = y; b < blocks; b += kLnThreads / kLnBiasCols) v += sums[(int64_t)b * n + c];
     }
     s[y * (kLnBiasCols + 1) + x] = v;
-    __syncthreads();
-    if (y != 0 || c >= n) return;
-    for (int i = 1; i < kLnThreads / kLnBiasCols; ++i) v += s[i * (kLnBiasCols + 1) + x];
-    dbias[c] = (T)v;
+    for (int w = kLnThreads / kLnBiasCols / 2; w > 0; w >>= 1) {   // by halves, as k_linear_dz
+        __syncthreads();
+        if (y < w) s[y * (kLnBiasCols + 1) + x] += s[(y + w) * (kLnBiasCols + 1) + x];
+    }
+    if (y == 0 && c < n) dbias[c] = (T)s[x];
 }
 
 // What a call has to join, in one launch at its end: up to two products, and dbias.
@@ -991,16 +992,22 @@ __global__ __launch_bounds__(kLnThreads) void k_linear_dz(LnGradArgs a) {
         }
     }
     if (!a.sums) return;
+    // The threads of a column by halves: one after the other, the 256 of a narrow layer left 2.5 to 3 times the error.
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[t * 8 + i] = sum[i];
+    for (int w = down / 2; w > 0; w >>= 1) {
+        __syncthreads();
+        if (t < w * across) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[t * 8 + i] += s[(t + w * across) * 8 + i];
+        }
+    }
     __syncthreads();
     for (int c = t; c < across * 8; c += kLnThreads) {
         const int col = (int)blockIdx.x * across * 8 + c;
         if (col >= a.n) break;
-        float x = 0.0f;
-        for (int w = 0; w < down; ++w) x += s[w * across * 8 + c];
-        if (a.dbias) ((T*)a.dbias)[col] = (T)x;
-        else a.sums[(int64_t)blockIdx.y * a.n + col] = x;
+        if (a.dbias) ((T*)a.dbias)[col] = (T)s[c];
+        else a.sums[(int64_t)blockIdx.y * a.n + col] = s[c];
     }
 }
 
