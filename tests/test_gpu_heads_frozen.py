@@ -72,3 +72,12 @@ def test_one_sided_calls(gpu):
     decoder.head_norm(q, None, w).square().sum().backward()
     decoder.head_norm(full, None, fw).square().sum().backward()
     assert torch.equal(w.grad, fw.grad)
+
+
+def test_weight_of_no_keys(gpu):
+    """Its gradient is zero, alone and with q's."""
+    for wants_q in (False, True):
+        q, w = rand(2, 5, 4, 8).requires_grad_(wants_q), (1 + rand(8, seed=2) / 4).requires_grad_(True)
+        torch.full((8,), 5.0, device="cuda")   # (what a gradient left unwritten would likely hold)
+        (decoder.head_norm(q, None, None, w).sum() + 0 * w.sum()).backward()
+        assert w.grad is not None and not w.grad.any() and (q.grad is not None) == wants_q

@@ -920,6 +920,8 @@ class _HeadNorm(torch.autograd.Function):
         if sides:
             dx, dw, dout, x, w = zip(*sides, *[(None,) * 5] * (2 - len(sides)))
             head_norm_grad_(*dx, *dw, *dout, *x, *w, eps=ctx.eps, rotary=ctx.rotary, positions=positions)
+        if k is None and grads[3] is not None:   # (a weight of no keys)
+            grads[3].zero_()
         return *grads, None, None, None
 
 
