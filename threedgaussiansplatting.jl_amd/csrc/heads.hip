@@ -455,7 +455,9 @@ static int hn_check(const tdgs_head_norm* a) {
         TDGS_REQUIRE(a->position_type >= TDGS_POSITION_I32 && a->position_type <= TDGS_POSITION_F32,
                      "head norm: unknown type of positions %d", a->position_type);
         TDGS_REQUIRE(a->turns && aligned_to(a->turns, 8), "head norm: the frequencies are null or not aligned");
-        TDGS_REQUIRE(a->positions && aligned_to(a->positions, a->position_type == TDGS_POSITION_I64 ? 8 : 4),
+        // (an empty tensor has no address)
+        TDGS_REQUIRE((a->positions || a->batch == 0 || a->length == 0) &&
+                         aligned_to(a->positions, a->position_type == TDGS_POSITION_I64 ? 8 : 4),
                      "head norm: the positions are null or not aligned");
         TDGS_REQUIRE(a->position_batch_stride >= 0, "head norm: positions have a negative stride");
     }
