@@ -35,9 +35,10 @@ def test_bias(gpu, rows, n):
 
 @pytest.mark.parametrize("size", [(1, 300, 4, 64), (3, 2501, 8, 64), (1, 64800, 4, 16), (1, 30000, 1, 10), (2, 9000, 4, 128)], ids=str)
 def test_head_weights(gpu, size):
-    """Up to four rows to a thread (2.5), 256 by halves (8), 1024 workgroups, 32 to a thread (16.5), and 32 by halves (5):
-    0.42 sqrt(32) = 2.4; and each term's own error, of a root and three products (0.42 sqrt(4) of the root of their
-    sum of squares): 2.5 together, a quarter more for few values. One after the other, 128 rows make 3.4 alone."""
+    """Up to four rows to a thread (2.5), eight threads to a thread (4.5), those in turn or by halves (5), 1024 workgroups, 32 to a
+    thread (16.5), and 32 by halves (5): 0.42 sqrt(33) = 2.4; and each term's own error, of a root and three products
+    (0.42 sqrt(4) of the root of their sum of squares): 2.6 together, a fifth more for few values. One after the other, 128 rows
+    make 3.4 alone."""
     gen = torch.Generator(device="cuda").manual_seed(sum(size))
     errors = []
     for _ in range(-(-128 // size[-1])):

@@ -374,8 +374,14 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
     if (!a.part) return;
     // over the rows that were taken at once: every thread's 2 N V elements
     __shared__ float s_sums[kHnThreads * 2 * V * N];
+    const int across = kHnThreads / a.d, y = (int)threadIdx.x / a.d, c = (int)threadIdx.x - y * a.d;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
+        float* const part = a.part + ((int64_t)blockIdx.x * 2 + k) * a.d;
+        if (a.heads[k] == 0) {
+            if (y == 0) part[c] = 0.0f;
+            continue;
+        }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -387,15 +393,26 @@ __global__ __launch_bounds__(kHnThreads) void k_head_norm_grad(HnArgs a) {
                 if (u.second + i * u.step < a.d) s_sums[lane.sub * a.d + u.second + i * u.step] = db[k][n][i];
             }
         }
-        // by halves: one after the other, the 128 rows of heads of 16 left twice the error
-        for (int rows = lane.rows; rows > 1;) {
-            const int half = (rows + 1) / 2;
+        // a column by as many threads as there are for it, up to eight rows each, whose sums are joined in turn or, if they are
+        // many, by halves: all rows one after the other, the 128 of heads of 16 left twice the error
+        float x = 0.0f;
+        __syncthreads();
+        if (y < across)
+            for (int r = y; r < lane.rows; r += across) x += s_sums[r * a.d + c];
+        __syncthreads();
+        if (y < across) s_sums[threadIdx.x] = x;
+        int left = across;
+        for (; left > 8; left = (left + 1) / 2) {
             __syncthreads();
-            for (int c = threadIdx.x; c < (rows - half) * a.d; c += kHnThreads) s_sums[c] += s_sums[half * a.d + c];
-            rows = half;
+            const int half = (left + 1) / 2;
+            if (y < left - half) s_sums[threadIdx.x] += s_sums[threadIdx.x + half * a.d];
         }
         __syncthreads();
-        for (int c = threadIdx.x; c < a.d; c += kHnThreads) a.part[((int64_t)blockIdx.x * 2 + k) * a.d + c] = s_sums[c];
+        if (y == 0) {
+            x = s_sums[c];
+            for (int i = 1; i < left; ++i) x += s_sums[i * a.d + c];
+            part[c] = x;
+        }
     }
 }
 
