@@ -15,9 +15,9 @@
 // wanted, applies the activation and adds the residual, all in 32 bits; only what is stored is rounded.
 //
 // What bounds the products: for 16-bit types the vector operations of the epilogue next to the matrix cores (32400 x 1024 ->
-// 4096 bfloat16 with GELU, 322 us: matrix cores busy for 44%, vector issue for 65%; 8192^3 without an activation 870 us,
+// 4096 bfloat16 with GELU, 314 to 340 us by card: matrix cores busy for 44%, vector issue for 65%; 8192^3 without an activation 870 us,
 // 1260 TFLOP/s); for float the matrix cores (66 to 70% busy over 7503 x 387 x 1029, 79 us, of which some ten are the
-// first tiles' way from memory and the last ones' back); for 34230 x 320 -> 320 memory (66 MB in 19 us); for few rows
+// first tiles' way from memory and the last ones' back); for 34230 x 320 -> 320 memory (66 MB in 18 to 22 us); for few rows
 // the call.
 #include "internal.hpp"
 #include "elem.hpp"
@@ -1252,7 +1252,7 @@ static LnMatrix ln_weight(const tdgs_linear* a) {
 // holding what the rounding leaves of the first: the errors of dx and dweight are 1.00 times those of the exact result rounded
 // once instead of 1.40 to 1.42, for every size. What it costs decides: these calls are mostly latency (the whole gradient with
 // GELU, one operand and two, in a graph: 256 x 256 -> 256 bfloat16 12 and 15 us, 64 x 1024 -> 1024 24 and 31, 128 x 2048 -> 512 13
-// and 21, 32 x 1024 -> 2048 19 and 35), large ones would take both products' time again (64800 x 512 -> 2048: 284 of 432 us).
+// and 21, 32 x 1024 -> 2048 19 and 35), large ones would take both products' time again (64800 x 512 -> 2048: 293 of 468 us).
 constexpr int64_t kLnFewSlopes = 1 << 16;
 
 // The gradient's scratch: dz, its power of two, maxima and columns' sums, then a product's partial sums.
